@@ -15,10 +15,10 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 OUT = os.path.join(HERE, "dfa3d_b200", "libdfa3d_b200.so")
 SOURCES = ["dfa3d_forward.cu", "dfa3d_forward_packed.cu", "dfa3d_backward.cu", "dfa3d_backward_packed.cu", "dfa3d_rebatch.cu", "dfa3d_dist_producer.cu",
-           "dfa3d_fp64.cu", "dfa3d_layer_ops.cu", "dfa3d_capi.cu"]
+           "dfa3d_fp64.cu", "dfa3d_layer_ops.cu", "dfa3d_dropout.cu", "dfa3d_group_norm.cu", "dfa3d_capi.cu"]
 RATES_SRC = os.path.join(CSRC, "rates", "dfa3d_rates.cu")
 RATES_OUT = os.path.join(HERE, "dfa3d_b200", "libdfa3d_rates.so")
-NATIVE_SRC = [os.path.join(CSRC, "binding", f) for f in ("dfa3d_torch.cpp", "dfa3d_torch_layers.cpp")]
+NATIVE_SRC = [os.path.join(CSRC, "binding", f) for f in ("dfa3d_torch.cpp", "dfa3d_torch_layers.cpp", "dfa3d_torch_rows.cpp")]
 NATIVE_OUT = os.path.join(HERE, "dfa3d_b200", "_native.so")
 INCLUDE = os.path.join(HERE, "..", "include")
 NVCC_FLAGS = ["-O3", "-I", INCLUDE, "-std=c++17", "-lineinfo", "-gencode", "arch=compute_100a,code=sm_100a",

@@ -652,7 +652,7 @@ PyModuleDef module = {PyModuleDef_HEAD_INIT, "_native", nullptr, -1, methods, nu
 PyMODINIT_FUNC PyInit__native(void) {
   PyObject *m = PyModule_Create(&module);
   // the headers this was compiled against: another torch may lay its classes out differently
-  if (m && (PyModule_AddFunctions(m, dfa3d_torch::layer_methods) != 0 ||
+  if (m && (PyModule_AddFunctions(m, dfa3d_torch::layer_methods) != 0 || PyModule_AddFunctions(m, dfa3d_torch::row_methods) != 0 ||
             PyModule_AddStringConstant(m, "built_for", DFA3D_BUILT_FOR) != 0 ||
             PyModule_AddIntConstant(m, "split_rows", kSplitRows) != 0 || PyModule_AddIntConstant(m, "splits", kSplits) != 0)) {
     Py_DECREF(m);

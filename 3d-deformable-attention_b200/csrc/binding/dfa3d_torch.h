@@ -1,5 +1,5 @@
-// What the two halves of the native host path share: the C ABI's entry points, argument checks and small helpers
-// (dfa3d_torch.cpp: the operator; dfa3d_torch_layers.cpp: the layer around it).
+// What the parts of the native host path share: the C ABI's entry points, argument checks and small helpers
+// (dfa3d_torch.cpp: the operator; dfa3d_torch_layers.cpp: the layer around it; dfa3d_torch_rows.cpp: dropout and group norm).
 #pragma once
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
@@ -38,7 +38,10 @@ using torch::autograd::variable_list;
   X(dfa3d_zero_two) X(dfa3d_convert_two) X(dfa3d_attn2d_supported) X(dfa3d_attn2d_forward) X(dfa3d_attn2d_backward)           \
   X(dfa3d_rebatch_gather) X(dfa3d_rebatch_combine) X(dfa3d_add_layer_norm_forward)                       \
   X(dfa3d_add_layer_norm_infer) X(dfa3d_layer_norm_backward) X(dfa3d_column_sum)                         \
-  X(dfa3d_relu_backward_column_sum) X(dfa3d_slice_sum) X(dfa3d_copy_segments)
+  X(dfa3d_relu_backward_column_sum) X(dfa3d_slice_sum) X(dfa3d_copy_segments)                               \
+  X(dfa3d_dropout_forward) X(dfa3d_dropout_backward) X(dfa3d_dropout_add_layer_norm_forward)             \
+  X(dfa3d_dropout_add_layer_norm_workspace) X(dfa3d_dropout_add_layer_norm_backward)                     \
+  X(dfa3d_group_norm_workspace) X(dfa3d_group_norm_forward) X(dfa3d_group_norm_backward)
 
 struct Abi {
 #define X(name) decltype(&::name) name = nullptr;
@@ -287,5 +290,6 @@ inline PyObject *not_plain() { Py_RETURN_NOTIMPLEMENTED; }
 constexpr int64_t kSplitRows = 16384, kSplits = 16;
 
 extern PyMethodDef layer_methods[];      // dfa3d_torch_layers.cpp, ends in a null entry
+extern PyMethodDef row_methods[];        // dfa3d_torch_rows.cpp, likewise
 
 }  // namespace dfa3d_torch

@@ -4,6 +4,8 @@
 #include <stdio.h>
 #include <string.h>
 
+#include <initializer_list>
+
 #include "dfa3d_b200.h"
 #include "dfa3d_common.cuh"
 #include "dfa3d_launch.h"
@@ -716,6 +718,199 @@ int dfa3d_zero_two(float *a, int64_t na, float *b, int64_t nb, void *stream) {
   if (na > 0) { REQUIRE_PTR(a); REQUIRE_ALIGNED(a); }
   if (nb > 0) { REQUIRE_PTR(b); REQUIRE_ALIGNED(b); }
   return finish(dfa3d::launch_zero_two(a, na, b, nb, (cudaStream_t)stream), "dfa3d_zero_two launch");
+}
+
+// ---- dropout without a stored mask -------------------------------------------------------------
+static int element_bytes(int32_t dtype) {
+  return dtype == DFA3D_DTYPE_F32 ? 4 : dtype == DFA3D_DTYPE_BF16 || dtype == DFA3D_DTYPE_F16 ? 2 : 0;
+}
+static int check_elements(int32_t dtype, std::initializer_list<const void *> tensors) {
+  const int e = element_bytes(dtype);
+  if (!e) return fail(DFA3D_ERR_INVALID_ARGUMENT, "dtype %d is not DFA3D_DTYPE_F32, _BF16 or _F16", dtype);
+  for (const void *t : tensors)
+    if (reinterpret_cast<uintptr_t>(t) % e != 0)
+      return fail(DFA3D_ERR_INVALID_ARGUMENT, "a tensor is not aligned to its elements of %d bytes", e);
+  return DFA3D_OK;
+}
+static int check_drop(double p, const int64_t *seed, int32_t site) {
+  if (!(p >= 0.0 && p <= 1.0)) return fail(DFA3D_ERR_INVALID_ARGUMENT, "p must be in [0, 1] (got %g)", p);
+  if (site < 0) return fail(DFA3D_ERR_INVALID_ARGUMENT, "site must be >= 0 (got %d)", site);
+  if (p > 0.0) {
+    REQUIRE_PTR(seed);
+    if (!aligned8(seed)) return fail(DFA3D_ERR_INVALID_ARGUMENT, "seed must be 8-byte aligned");
+  }
+  return DFA3D_OK;
+}
+static int check_wide_rows(int64_t rows, int32_t E) {
+  if (rows < 0) return fail(DFA3D_ERR_INVALID_ARGUMENT, "rows must be >= 0 (got %lld)", (long long)rows);
+  if (E <= 0) return fail(DFA3D_ERR_INVALID_ARGUMENT, "E must be positive (got %d)", E);
+  if (E > dfa3d::layer_norm_max_columns())
+    return fail(DFA3D_ERR_UNSUPPORTED, "E=%d: rows of up to %d columns are covered", E, dfa3d::layer_norm_max_columns());
+  return DFA3D_OK;
+}
+
+int dfa3d_dropout_forward(const void *x, const void *residual, int32_t dtype, int64_t n, int32_t activation, double p,
+                          const int64_t *seed, int32_t site, void *y, void *stream) {
+  if (int rc = check_elements(dtype, {x, residual, y})) return rc;
+  if (int rc = check_drop(p, n > 0 ? seed : reinterpret_cast<const int64_t *>(16), site)) return rc;
+  if (n < 0) return fail(DFA3D_ERR_INVALID_ARGUMENT, "n must be >= 0 (got %lld)", (long long)n);
+  if (activation != DFA3D_ROW_NONE && activation != DFA3D_ROW_RELU)
+    return fail(DFA3D_ERR_INVALID_ARGUMENT, "activation %d is not DFA3D_ROW_NONE or _RELU", activation);
+  if (n == 0) return DFA3D_OK;
+  REQUIRE_PTR(x); REQUIRE_PTR(y);
+  return finish(dfa3d::launch_dropout_forward(x, residual, dtype, n, activation == DFA3D_ROW_RELU, p, seed, (uint32_t)site, y,
+                                              (cudaStream_t)stream),
+                "dfa3d_dropout_forward launch");
+}
+
+int dfa3d_dropout_backward(const void *grad_y, const void *ref, int32_t ref_is_result, int32_t dtype, int64_t n, double p,
+                           const int64_t *seed, int32_t site, void *grad_x, void *stream) {
+  if (int rc = check_elements(dtype, {grad_y, ref, grad_x})) return rc;
+  if (ref_is_result && !ref) return fail(DFA3D_ERR_INVALID_ARGUMENT, "ref_is_result without ref");
+  if (int rc = check_drop(p, n > 0 ? seed : reinterpret_cast<const int64_t *>(16), site)) return rc;
+  if (n < 0) return fail(DFA3D_ERR_INVALID_ARGUMENT, "n must be >= 0 (got %lld)", (long long)n);
+  if (n == 0) return DFA3D_OK;
+  REQUIRE_PTR(grad_y); REQUIRE_PTR(grad_x);
+  return finish(dfa3d::launch_dropout_backward(grad_y, ref, ref_is_result != 0, dtype, n, p, seed, (uint32_t)site, grad_x,
+                                               (cudaStream_t)stream),
+                "dfa3d_dropout_backward launch");
+}
+
+int dfa3d_dropout_add_layer_norm_forward(const void *x, const void *residual, const float *gamma, const float *beta,
+                                         int32_t dtype, int64_t rows, int32_t E, double p, const int64_t *seed, int32_t site,
+                                         float eps, void *y, float *mean, float *rstd, void *stream) {
+  if (int rc = check_wide_rows(rows, E)) return rc;
+  if (int rc = check_elements(dtype, {x, residual, y})) return rc;
+  if (int rc = check_elements(DFA3D_DTYPE_F32, {gamma, beta, mean, rstd})) return rc;
+  if (int rc = check_drop(p, rows > 0 ? seed : reinterpret_cast<const int64_t *>(16), site)) return rc;
+  if (!(eps >= 0.f)) return fail(DFA3D_ERR_INVALID_ARGUMENT, "eps must be >= 0");
+  if ((mean == nullptr) != (rstd == nullptr))
+    return fail(DFA3D_ERR_INVALID_ARGUMENT, "mean and rstd must be given together or not at all");
+  if (rows == 0) return DFA3D_OK;
+  REQUIRE_PTR(x); REQUIRE_PTR(residual); REQUIRE_PTR(gamma); REQUIRE_PTR(beta); REQUIRE_PTR(y);
+  return finish(dfa3d::launch_dropout_add_layer_norm(x, residual, gamma, beta, dtype, rows, E, p, seed, (uint32_t)site, eps, y,
+                                                     mean, rstd, (cudaStream_t)stream),
+                "dfa3d_dropout_add_layer_norm_forward launch");
+}
+
+int64_t dfa3d_dropout_add_layer_norm_workspace(int64_t rows, int32_t E) {
+  if (int rc = check_wide_rows(rows, E)) return rc;
+  return dfa3d::dropout_layer_norm_workspace(rows, E);
+}
+
+int dfa3d_dropout_add_layer_norm_backward(const void *grad_y, const void *x, const void *residual, const float *gamma,
+                                          const float *mean, const float *rstd, int32_t dtype, int64_t rows, int32_t E,
+                                          double p, const int64_t *seed, int32_t site, void *grad_x, void *grad_residual,
+                                          float *grad_gamma, float *grad_beta, void *workspace, int64_t workspace_bytes,
+                                          void *stream) {
+  if (int rc = check_wide_rows(rows, E)) return rc;
+  if (int rc = check_elements(dtype, {grad_y, x, residual, grad_x, grad_residual})) return rc;
+  if (int rc = check_elements(DFA3D_DTYPE_F32, {gamma, mean, rstd, grad_gamma, grad_beta})) return rc;
+  if (int rc = check_drop(p, rows > 0 ? seed : reinterpret_cast<const int64_t *>(16), site)) return rc;
+  if ((grad_gamma == nullptr) != (grad_beta == nullptr))
+    return fail(DFA3D_ERR_INVALID_ARGUMENT, "grad_gamma and grad_beta must be given together or not at all");
+  if (rows == 0) {      // sums over no rows
+    if (!grad_gamma) return DFA3D_OK;
+    REQUIRE_ALIGNED(grad_gamma); REQUIRE_ALIGNED(grad_beta);
+    return finish(dfa3d::launch_zero_two(grad_gamma, E, grad_beta, E, (cudaStream_t)stream),
+                  "dfa3d_dropout_add_layer_norm_backward launch");
+  }
+  REQUIRE_PTR(grad_y); REQUIRE_PTR(x); REQUIRE_PTR(residual); REQUIRE_PTR(gamma); REQUIRE_PTR(mean); REQUIRE_PTR(rstd);
+  if (grad_gamma) {
+    REQUIRE_PTR(workspace); REQUIRE_ALIGNED(workspace);
+    const long long need = dfa3d::dropout_layer_norm_workspace(rows, E);
+    if (workspace_bytes < need)
+      return fail(DFA3D_ERR_INVALID_ARGUMENT, "workspace of %lld bytes is smaller than the %lld needed",
+                  (long long)workspace_bytes, need);
+  }
+  if (!grad_x && !grad_residual && !grad_gamma) return DFA3D_OK;
+  return finish(dfa3d::launch_dropout_layer_norm_backward(grad_y, x, residual, gamma, mean, rstd, dtype, rows, E, p, seed,
+                                                          (uint32_t)site, grad_x, grad_residual, grad_gamma, grad_beta,
+                                                          static_cast<float *>(workspace), (cudaStream_t)stream),
+                "dfa3d_dropout_add_layer_norm_backward launch");
+}
+
+// ---- group norm ---------------------------------------------------------------------------------
+static int check_group_norm_sizes(int32_t B, int32_t N, int32_t C, int32_t G, int32_t L) {
+  if (B < 0 || N < 0) return fail(DFA3D_ERR_INVALID_ARGUMENT, "B and N must be >= 0 (got %d, %d)", B, N);
+  if (C <= 0 || G <= 0 || C % G != 0)
+    return fail(DFA3D_ERR_INVALID_ARGUMENT, "C=%d channels do not make G=%d groups", C, G);
+  if (C > DFA3D_MAX_CHANNELS) return fail(DFA3D_ERR_UNSUPPORTED, "C=%d exceeds %d", C, DFA3D_MAX_CHANNELS);
+  if (L <= 0) return fail(DFA3D_ERR_INVALID_ARGUMENT, "L must be positive (got %d)", L);
+  if (L > DFA3D_MAX_LEVELS) return fail(DFA3D_ERR_UNSUPPORTED, "L=%d exceeds DFA3D_MAX_LEVELS=%d", L, DFA3D_MAX_LEVELS);
+  if (N >= (1 << 30) || B >= (1 << 24)) return fail(DFA3D_ERR_UNSUPPORTED, "B=%d images of N=%d rows are too many", B, N);
+  return DFA3D_OK;
+}
+static int check_group_norm(int32_t B, int32_t N, int32_t C, int32_t G, const int64_t *spatial_shapes, int32_t shape_stride,
+                            const int64_t *level_start, int32_t L, int32_t weight_rows, int32_t activation) {
+  if (int rc = check_group_norm_sizes(B, N, C, G, L)) return rc;
+  if ((spatial_shapes == nullptr) != (level_start == nullptr))
+    return fail(DFA3D_ERR_INVALID_ARGUMENT, "spatial_shapes and level_start must be given together or not at all");
+  if (!spatial_shapes && L != 1) return fail(DFA3D_ERR_INVALID_ARGUMENT, "L=%d levels without a level table", L);
+  if (spatial_shapes && shape_stride < 2)
+    return fail(DFA3D_ERR_INVALID_ARGUMENT, "shape_stride must be at least 2 (got %d)", shape_stride);
+  if (weight_rows != 1 && weight_rows != L)
+    return fail(DFA3D_ERR_INVALID_ARGUMENT, "weight_rows=%d is neither 1 nor the L=%d levels", weight_rows, L);
+  if (activation != DFA3D_ROW_NONE && activation != DFA3D_ROW_RELU && activation != DFA3D_ROW_SILU)
+    return fail(DFA3D_ERR_INVALID_ARGUMENT, "activation %d is not a DFA3D_ROW_*", activation);
+  return DFA3D_OK;
+}
+static int check_group_norm_workspace(const void *workspace, int64_t have, long long need) {
+  REQUIRE_PTR(workspace); REQUIRE_ALIGNED(workspace);
+  if (have < need)
+    return fail(DFA3D_ERR_INVALID_ARGUMENT, "workspace of %lld bytes is smaller than the %lld needed", (long long)have, need);
+  return DFA3D_OK;
+}
+
+int64_t dfa3d_group_norm_workspace(int32_t B, int32_t N, int32_t C, int32_t G, int32_t L, int32_t backward) {
+  if (int rc = check_group_norm_sizes(B, N, C, G, L)) return rc;
+  return dfa3d::group_norm_workspace(B, N, C, G, L, backward != 0);
+}
+
+int dfa3d_group_norm_forward(const void *x, int32_t dtype, int32_t B, int32_t N, int32_t C, int32_t G,
+                             const int64_t *spatial_shapes, int32_t shape_stride, const int64_t *level_start, int32_t L,
+                             const float *weight, const float *bias, int32_t weight_rows, float eps, int32_t activation,
+                             void *y, float *mean, float *rstd, void *workspace, int64_t workspace_bytes, void *stream) {
+  if (int rc = check_group_norm(B, N, C, G, spatial_shapes, shape_stride, level_start, L, weight_rows, activation)) return rc;
+  if (int rc = check_elements(dtype, {x, y})) return rc;
+  if (int rc = check_elements(DFA3D_DTYPE_F32, {weight, bias, mean, rstd})) return rc;
+  if (!(eps >= 0.f)) return fail(DFA3D_ERR_INVALID_ARGUMENT, "eps must be >= 0");
+  if ((mean == nullptr) != (rstd == nullptr))
+    return fail(DFA3D_ERR_INVALID_ARGUMENT, "mean and rstd must be given together or not at all");
+  if (B == 0 || N == 0) return DFA3D_OK;
+  REQUIRE_PTR(x); REQUIRE_PTR(weight); REQUIRE_PTR(bias); REQUIRE_PTR(y);
+  if (int rc = check_group_norm_workspace(workspace, workspace_bytes, dfa3d::group_norm_workspace(B, N, C, G, L, false)))
+    return rc;
+  return finish(dfa3d::launch_group_norm_forward(x, dtype, B, N, C, G, spatial_shapes, shape_stride, level_start, L, weight, bias,
+                                                 weight_rows, eps, activation, y, mean, rstd, workspace, (cudaStream_t)stream),
+                "dfa3d_group_norm_forward launch");
+}
+
+int dfa3d_group_norm_backward(const void *grad_y, const void *x, int32_t dtype, int32_t B, int32_t N, int32_t C, int32_t G,
+                              const int64_t *spatial_shapes, int32_t shape_stride, const int64_t *level_start, int32_t L,
+                              const float *weight, const float *bias, int32_t weight_rows, int32_t activation,
+                              const float *mean, const float *rstd, void *grad_x, float *grad_weight, float *grad_bias,
+                              void *workspace, int64_t workspace_bytes, void *stream) {
+  if (int rc = check_group_norm(B, N, C, G, spatial_shapes, shape_stride, level_start, L, weight_rows, activation)) return rc;
+  if (int rc = check_elements(dtype, {grad_y, x, grad_x})) return rc;
+  if (int rc = check_elements(DFA3D_DTYPE_F32, {weight, bias, mean, rstd, grad_weight, grad_bias})) return rc;
+  if ((grad_weight == nullptr) != (grad_bias == nullptr))
+    return fail(DFA3D_ERR_INVALID_ARGUMENT, "grad_weight and grad_bias must be given together or not at all");
+  if (B == 0 || N == 0) {
+    if (!grad_weight) return DFA3D_OK;
+    REQUIRE_ALIGNED(grad_weight); REQUIRE_ALIGNED(grad_bias);
+    return finish(dfa3d::launch_zero_two(grad_weight, (int64_t)weight_rows * C, grad_bias, (int64_t)weight_rows * C,
+                                         (cudaStream_t)stream),
+                  "dfa3d_group_norm_backward launch");
+  }
+  REQUIRE_PTR(grad_y); REQUIRE_PTR(x); REQUIRE_PTR(weight); REQUIRE_PTR(bias); REQUIRE_PTR(mean); REQUIRE_PTR(rstd);
+  if (int rc = check_group_norm_workspace(workspace, workspace_bytes, dfa3d::group_norm_workspace(B, N, C, G, L, true)))
+    return rc;
+  if (!grad_x && !grad_weight) return DFA3D_OK;
+  return finish(dfa3d::launch_group_norm_backward(grad_y, x, dtype, B, N, C, G, spatial_shapes, shape_stride, level_start, L,
+                                                  weight, bias, weight_rows, mean, rstd, activation, grad_x, grad_weight,
+                                                  grad_bias, workspace, (cudaStream_t)stream),
+                "dfa3d_group_norm_backward launch");
 }
 
 // ---- double precision -------------------------------------------------------------------------

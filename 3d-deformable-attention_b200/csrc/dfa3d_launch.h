@@ -79,4 +79,27 @@ cudaError_t launch_copy_segments(const float *const *src, float *const *dst, con
 cudaError_t launch_convert_two(bool half, bool widen, void *n0, void *w0, long long c0, void *n1, void *w1, long long c1,
                                cudaStream_t s);
 cudaError_t launch_zero_two(float *a, long long na, float *b, long long nb, cudaStream_t s);
+// dropout without a stored mask (dfa3d_dropout.cu); p in [0, 1], dtype DFA3D_DTYPE_F32, _BF16 or _F16
+cudaError_t launch_dropout_forward(const void *x, const void *residual, int dtype, long long n, bool relu, double p,
+                                   const int64_t *seed, uint32_t site, void *y, cudaStream_t s);
+cudaError_t launch_dropout_backward(const void *grad_y, const void *ref, bool ref_is_result, int dtype, long long n, double p,
+                                    const int64_t *seed, uint32_t site, void *grad_x, cudaStream_t s);
+cudaError_t launch_dropout_add_layer_norm(const void *x, const void *residual, const float *gamma, const float *beta, int dtype,
+                                          long long rows, int E, double p, const int64_t *seed, uint32_t site, float eps, void *y,
+                                          float *mean, float *rstd, cudaStream_t s);
+long long dropout_layer_norm_workspace(long long rows, int E);
+cudaError_t launch_dropout_layer_norm_backward(const void *grad_y, const void *x, const void *residual, const float *gamma,
+                                               const float *mean, const float *rstd, int dtype, long long rows, int E, double p,
+                                               const int64_t *seed, uint32_t site, void *grad_x, void *grad_residual,
+                                               float *grad_gamma, float *grad_beta, float *partial, cudaStream_t s);
+// group norm over the levels of a feature pyramid (dfa3d_group_norm.cu); act: DFA3D_ROW_*
+long long group_norm_workspace(int B, int N, int C, int G, int L, bool backward);
+cudaError_t launch_group_norm_forward(const void *x, int dtype, int B, int N, int C, int G, const int64_t *shapes,
+                                      int shape_stride, const int64_t *start, int L, const float *weight, const float *bias,
+                                      int weight_rows, float eps, int act, void *y, float *mean, float *rstd, void *workspace,
+                                      cudaStream_t s);
+cudaError_t launch_group_norm_backward(const void *grad_y, const void *x, int dtype, int B, int N, int C, int G,
+                                       const int64_t *shapes, int shape_stride, const int64_t *start, int L, const float *weight,
+                                       const float *bias, int weight_rows, const float *mean, const float *rstd, int act,
+                                       void *grad_x, float *grad_weight, float *grad_bias, void *workspace, cudaStream_t s);
 }  // namespace dfa3d

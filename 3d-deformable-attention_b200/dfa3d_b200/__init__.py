@@ -6,6 +6,8 @@ this package is the PyTorch-facing host side: ``ext`` mirrors the reference's ex
 operators raise.
 """
 from . import _lib, ext  # noqa: F401
+from .dropout_ops import CounterDropout, draw_seed, dropout, dropout_add_layer_norm  # noqa: F401
+from .group_norm_ops import LevelGroupNorm, group_norm  # noqa: F401
 from .host import HostPipeline  # noqa: F401
 from .functions import (  # noqa: F401
     DeformableAttn3DFromOffsetsFunction,
@@ -26,6 +28,7 @@ from .functions import (  # noqa: F401
 
 __all__ = [
     "ext", "HostPipeline",
+    "CounterDropout", "draw_seed", "dropout", "dropout_add_layer_norm", "LevelGroupNorm", "group_norm",
     "MultiScaleDepthScoreSampleFunction", "WeightedMultiScaleDeformableAttnFunction",
     "MultiScale3DDeformableAttnFunction",
     "MultiScaleDepthScoreSampleFunction_fp32", "WeightedMultiScaleDeformableAttnFunction_fp32",

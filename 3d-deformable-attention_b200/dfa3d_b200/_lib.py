@@ -90,9 +90,21 @@ PLAIN_ENTRY_POINTS = {
     "dfa3d_slice_sum": [ctypes.c_void_p] + [_I32] * 3 + [ctypes.c_void_p] * 2 + [_I32] + [ctypes.c_void_p] * 3,
     "dfa3d_copy_segments": [ctypes.c_void_p] * 3 + [_I32, ctypes.c_void_p],
     "dfa3d_convert_two": [_I32, _I32, _V, _V, _I64, _V, _V, _I64, _V],
+    "dfa3d_dropout_forward": [_V, _V, _I32, _I64, _I32, ctypes.c_double, _V, _I32, _V, _V],
+    "dfa3d_dropout_backward": [_V, _V, _I32, _I32, _I64, ctypes.c_double, _V, _I32, _V, _V],
+    "dfa3d_dropout_add_layer_norm_forward": [_V] * 4 + [_I32, _I64, _I32, ctypes.c_double, _V, _I32, ctypes.c_float] + [_V] * 4,
+    "dfa3d_dropout_add_layer_norm_backward": [_V] * 6 + [_I32, _I64, _I32, ctypes.c_double, _V, _I32] + [_V] * 5 + [_I64, _V],
+    "dfa3d_group_norm_forward": [_V] + [_I32] * 5 + [_V, _I32, _V, _I32, _V, _V, _I32, ctypes.c_float, _I32] + [_V] * 4
+                                + [_I64, _V],
+    "dfa3d_group_norm_backward": [_V, _V] + [_I32] * 5 + [_V, _I32, _V, _I32, _V, _V, _I32, _I32] + [_V] * 6 + [_I64, _V],
+    "dfa3d_dropout_add_layer_norm_workspace": [_I64, _I32],
+    "dfa3d_group_norm_workspace": [_I32] * 6,
     "dfa3d_zero_two": [ctypes.c_void_p, _I64, ctypes.c_void_p, _I64, ctypes.c_void_p],
 }
+# of these the ones that answer with a number of bytes (or a negative error code)
+SIZE_ENTRY_POINTS = ("dfa3d_dropout_add_layer_norm_workspace", "dfa3d_group_norm_workspace")
 ACT_SOFTMAX, ACT_SIGMOID = 0, 1
+ROW_NONE, ROW_RELU, ROW_SILU = 0, 1, 2
 
 _lib = None
 _native = None
@@ -133,6 +145,8 @@ def load():
         fn = getattr(lib, name)
         fn.restype = ctypes.c_int
         fn.argtypes = argtypes
+    for name in SIZE_ENTRY_POINTS:
+        getattr(lib, name).restype = _I64
     got = lib.dfa3d_abi_version()
     if got != ABI_VERSION:
         raise ImportError(f"libdfa3d_b200.so has ABI version {got}, this package expects {ABI_VERSION}")
@@ -183,6 +197,16 @@ def native_apply(name):
         return cls
 
     return wrap
+
+
+def size(name, *args):
+    """Bytes of workspace that an entry point asks for."""
+    lib = load()
+    n = getattr(lib, name)(*args)
+    if n < 0:
+        msg = lib.dfa3d_last_error().decode("utf-8", "replace")
+        raise RuntimeError(f"{name} failed ({ERROR_NAMES.get(n, n)}): {msg}")
+    return n
 
 
 def call_plain(name, *args):

@@ -397,6 +397,68 @@ int dfa3d_zero_two(float *a, int64_t na, float *b, int64_t nb, void *stream);
 int dfa3d_convert_two(int32_t narrow_dtype, int32_t widen, void *narrow0, void *wide0, int64_t count0, void *narrow1,
                       void *wide1, int64_t count1, void *stream);
 
+/* ---- dropout without a stored mask -------------------------------------------------------------
+ * Element i of the tensor in row-major order takes word i mod 4 of Philox4x32 with 7 rounds (Salmon et al., SC 2011) at
+ * counter (i / 4 low, i / 4 high, site, 0) under the key (seed low, seed high) and is kept where word >= p * 2^32; kept
+ * elements are scaled by 1 / (1 - p), a dropped one is 0 whatever it was.  The mask is a function of (seed, site, element
+ * number) alone: a backward gets the same three and forms it again.  seed: ONE int64 in DEVICE memory (a captured graph
+ * reads the value of each replay), not looked at where p < 2^-33.  0 <= p <= 1, site >= 0 tells the calls of one pass
+ * apart.  dtype of x, residual, results and gradients: DFA3D_DTYPE_F32, _BF16 or _F16; arithmetic is fp32.  Addresses off
+ * the 16-byte grid are taken, more slowly. */
+#define DFA3D_ROW_NONE 0
+#define DFA3D_ROW_RELU 1
+#define DFA3D_ROW_SILU 2
+
+/* y = [residual +] keep * act(x) / (1 - p), n elements; activation DFA3D_ROW_NONE or _RELU; residual may be null.  y may be x. */
+int dfa3d_dropout_forward(const void *x, const void *residual, int32_t dtype, int64_t n, int32_t activation, double p,
+                          const int64_t *seed, int32_t site, void *y, void *stream);
+
+/* grad_x = keep * grad_y / (1 - p), and 0 where the ReLU had cut (ref <= 0).  ref: null without an activation; the forward's
+ * x; or (ref_is_result != 0, only if there was no residual) the forward's y, whose zeros are the dropped elements too, so
+ * that no mask is formed.  The gradient of residual is grad_y. */
+int dfa3d_dropout_backward(const void *grad_y, const void *ref, int32_t ref_is_result, int32_t dtype, int64_t n, double p,
+                           const int64_t *seed, int32_t site, void *grad_x, void *stream);
+
+/* y = LayerNorm(residual + keep * x / (1 - p)) * gamma + beta over rows of E columns (any E up to 1024), the end of a residual
+ * block that is trained with dropout.  gamma, beta, mean, rstd fp32; mean and rstd (rows) may be null together. */
+int dfa3d_dropout_add_layer_norm_forward(const void *x, const void *residual, const float *gamma, const float *beta,
+                                         int32_t dtype, int64_t rows, int32_t E, double p, const int64_t *seed, int32_t site,
+                                         float eps, void *y, float *mean, float *rstd, void *stream);
+
+/* Bytes that its backward needs at `workspace` (device, 16-byte aligned, contents irrelevant), or a negative error code. */
+int64_t dfa3d_dropout_add_layer_norm_workspace(int64_t rows, int32_t E);
+
+/* Its backward.  grad_x, grad_residual (rows, E) and grad_gamma, grad_beta (E) are overwritten; each of the first two, and
+ * the last two together, may be null.  The sums over rows are added up in a fixed order: same bits in every run. */
+int dfa3d_dropout_add_layer_norm_backward(const void *grad_y, const void *x, const void *residual, const float *gamma,
+                                          const float *mean, const float *rstd, int32_t dtype, int64_t rows, int32_t E,
+                                          double p, const int64_t *seed, int32_t site, void *grad_x, void *grad_residual,
+                                          float *grad_gamma, float *grad_beta, void *workspace, int64_t workspace_bytes,
+                                          void *stream);
+
+/* ---- group norm of channels-last feature pyramids -----------------------------------------------
+ * x (B, N, C): the layout of the operator's value.  Every (image, level, group of C / G channels) is normalised by itself
+ * (biased variance, eps inside the square root), y = act(xhat * weight + bias), activation DFA3D_ROW_NONE, _RELU or _SILU.
+ * spatial_shapes (L, shape_stride) int64 with height and width first, level_start (L) int64, device, levels ascending; both
+ * null with L = 1: the N rows are one level.  A table that points outside of the N rows or overlaps is cut to disjoint
+ * levels; rows of no level become 0 in y and in grad_x.  weight, bias fp32 (weight_rows, C) with weight_rows 1 (shared by
+ * the levels) or L.  C <= 1024, G divides C.  dtype (of x, y and their gradients): DFA3D_DTYPE_F32, _BF16 or _F16.
+ * mean, rstd (B, L, G) fp32 for the backward; may be null together in the forward. */
+int64_t dfa3d_group_norm_workspace(int32_t B, int32_t N, int32_t C, int32_t G, int32_t L, int32_t backward);
+
+int dfa3d_group_norm_forward(const void *x, int32_t dtype, int32_t B, int32_t N, int32_t C, int32_t G,
+                             const int64_t *spatial_shapes, int32_t shape_stride, const int64_t *level_start, int32_t L,
+                             const float *weight, const float *bias, int32_t weight_rows, float eps, int32_t activation,
+                             void *y, float *mean, float *rstd, void *workspace, int64_t workspace_bytes, void *stream);
+
+/* grad_x may be null, grad_weight and grad_bias (weight_rows, C) together; all are overwritten, with the same bits in every
+ * run. */
+int dfa3d_group_norm_backward(const void *grad_y, const void *x, int32_t dtype, int32_t B, int32_t N, int32_t C, int32_t G,
+                              const int64_t *spatial_shapes, int32_t shape_stride, const int64_t *level_start, int32_t L,
+                              const float *weight, const float *bias, int32_t weight_rows, int32_t activation,
+                              const float *mean, const float *rstd, void *grad_x, float *grad_weight, float *grad_bias,
+                              void *workspace, int64_t workspace_bytes, void *stream);
+
 #ifdef __cplusplus
 }
 #endif
