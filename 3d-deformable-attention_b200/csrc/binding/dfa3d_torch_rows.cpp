@@ -252,7 +252,7 @@ PyObject *run_group_norm(PyObject *const *a, Py_ssize_t n) {
     return not_plain();
   auto s = c10::make_intrusive<Levels>();
   const int64_t B = x.size(0), C = x.size(-1), N = x.numel() / B / C, L = table ? shapes.size(0) : 1;
-  if (B >= (1 << 24) || N >= (1 << 30) || C > 1024 || G <= 0 || C % G != 0 || L < 1 || L > DFA3D_MAX_LEVELS ||
+  if (B * std::max(std::min<int64_t>(N, 2052), L * C) >= (int64_t(1) << 31) || N >= (1 << 30) || C > 1024 || G <= 0 || C % G != 0 || L < 1 || L > DFA3D_MAX_LEVELS ||
       w.sizes() != b.sizes() || !one_device(x, w, b))
     return not_plain();
   if (table && (!one_device(x, shapes, lsi) || (shapes.size(1) != 2 && shapes.size(1) != 3) || lsi.numel() != L)) return not_plain();

@@ -838,7 +838,8 @@ static int check_group_norm_sizes(int32_t B, int32_t N, int32_t C, int32_t G, in
   if (C > DFA3D_MAX_CHANNELS) return fail(DFA3D_ERR_UNSUPPORTED, "C=%d exceeds %d", C, DFA3D_MAX_CHANNELS);
   if (L <= 0) return fail(DFA3D_ERR_INVALID_ARGUMENT, "L must be positive (got %d)", L);
   if (L > DFA3D_MAX_LEVELS) return fail(DFA3D_ERR_UNSUPPORTED, "L=%d exceeds DFA3D_MAX_LEVELS=%d", L, DFA3D_MAX_LEVELS);
-  if (N >= (1 << 30) || B >= (1 << 24)) return fail(DFA3D_ERR_UNSUPPORTED, "B=%d images of N=%d rows are too many", B, N);
+  if (N >= (1 << 30) || (int64_t)B * (N < 2052 ? N : 2052) >= (1LL << 31) || (int64_t)B * L * C >= (1LL << 31))
+    return fail(DFA3D_ERR_UNSUPPORTED, "B=%d images of N=%d rows are too many", B, N);
   return DFA3D_OK;
 }
 static int check_group_norm(int32_t B, int32_t N, int32_t C, int32_t G, const int64_t *spatial_shapes, int32_t shape_stride,

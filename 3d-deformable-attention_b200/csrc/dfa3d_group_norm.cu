@@ -9,8 +9,18 @@
 // Statistics: a thread keeps, for each of its V channels, the number of values, their mean and the sum of squares around it; eight
 // rows at a time are reduced in registers around their own mean and merged by
 //   M2 = M2a + M2b + (mb - ma)^2 na nb / (na + nb)                      (Chan, Golub, LeVeque 1979),
-// so that nothing is lost where the mean is large against the spread.  Threads, warps and CTAs are merged in a fixed order: a
+// so that nothing is lost where the mean is large against the spread.  Threads, warps and tiles are merged in a fixed order: a
 // result is the same bits in every run.
+//
+// Three launches each way: statistics of tiles of rows; a warp for every group of a level of an image merges its tiles' parts;
+// the result.  They follow one another as programmatic dependent launches, so that the third has its rows on the way while the
+// second runs, and the third walks the tiles from the last one back, whose rows the first has left in L2.  What bounds them is HBM:
+// x is read once and a second time as far as it has left L2 (126 MB), y written once.
+//
+// 6 x 30 825 x 256, 32 groups, 4 levels: fp32 (189 MB) forward 99 us, backward 158; bf16 58 and 97; 6 x 920 x 256 fp32 10 and 12.
+// Measured against it, fp32 forward / backward: one launch that walks the images in batches with a barrier of the grid after each
+// 257 / 287 (each barrier leaves every SM waiting through the merge); launches that form the statistics of one batch and the
+// results of the one before 129 to 270; merges by every CTA of the third launch instead of a second one 144 / 249.
 #include <algorithm>
 
 #include "dfa3d_launch.h"
@@ -22,14 +32,25 @@ namespace {
 
 enum Act { kNone = 0, kRelu = 1, kSilu = 2 };
 
+// Threads of a CTA: at least as many as a row has words of V channels.
+template <int V> constexpr int kThreads = V == 4 ? 256 : 1024 / V;
+// CTAs an SM: what the registers of a thread's rows leave.
+template <typename T, int V> constexpr int kResident = V == 4 ? (sizeof(T) == 4 ? 3 : 4) : V;
+// Words of a thread in flight, and of each of two tensors.
+constexpr int kAhead = 8, kGradAhead = 4;
+
 struct GnArgs {
   const int64_t *shapes, *start;     // level table, or null: one level
   int shape_stride;
-  int N, C, G, L, S, act;            // S runs of rows an image
+  int B, N, C, G, L, act;
   int weight_rows;                   // 1, or L: weights of each level's own
   const float *weight, *bias;
   float eps;
-  int cpg, nv, RL;                   // channels a group, vectors a row, rows a CTA reads at a time
+  int cpg, V, nv, RL;                // channels a group, a word; words a row, rows a CTA reads at a time
+  int R, tiles, entries;             // rows of a tile; tiles and pieces of an image
+  Divisor by_r, by_tiles, by_nv, by_per, by_groups, by_levels;
+  bool whole;                        // a word's channels are of one group: by_per divides by its words, else by its channels
+  bool wide_params;                  // four weights at a time
 };
 
 __device__ __forceinline__ float warp_sum(float v) {
@@ -37,463 +58,696 @@ __device__ __forceinline__ float warp_sum(float v) {
   for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
   return v;
 }
+// over eight lanes
+__device__ __forceinline__ float sum8(float v) {
+  v += __shfl_xor_sync(0xffffffffu, v, 1);
+  v += __shfl_xor_sync(0xffffffffu, v, 2);
+  return v + __shfl_xor_sync(0xffffffffu, v, 4);
+}
 
-__device__ __forceinline__ int pieces(const GnArgs &a) { return a.S + 2 * a.L + 1; }
-
-// Rows that row lane rl of RL takes of a piece of n.
-__device__ __forceinline__ int lane_rows(int n, int rl, int RL) { return n > rl ? (n - rl + RL - 1) / RL : 0; }
-
+__device__ __forceinline__ float sigmoid(float z) { return __fdividef(1.f, 1.f + __expf(-z)); }
+template <bool ACT>
 __device__ __forceinline__ float activate(float z, int act) {
+  if (!ACT) return z;
   if (act == kRelu) return z <= 0.f ? 0.f : z;                       // a NaN passes, as in torch
-  if (act == kSilu) return z / (1.f + __expf(-z));
-  return z;
+  return z * sigmoid(z);
 }
 // dz of dy
+template <bool ACT>
 __device__ __forceinline__ float activate_grad(float g, float z, int act) {
+  if (!ACT) return g;
   if (act == kRelu) return z <= 0.f ? 0.f : g;
-  if (act == kSilu) {
-    const float s = 1.f / (1.f + __expf(-z));
-    return g * s * (1.f + z * (1.f - s));
-  }
-  return g;
+  const float s = sigmoid(z);
+  return g * s * fmaf(z, 1.f - s, 1.f);
 }
 
-constexpr int kRows = 8;      // rows of a thread in flight
+// The launches of a call follow one another closely: each lets the next begin as its CTAs leave, and waits for the one before it
+// with launch_wait() before it reads what that wrote.
+__device__ __forceinline__ void launch_next() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void launch_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 
-// Threads of a CTA: 256, or as many as a row of up to 1024 channels has vectors.
-constexpr int max_threads(int V) { return V >= 4 ? 256 : 1024 / V; }
+// Every thread returns with the table complete.
+__device__ __forceinline__ void make_table(SegmentTable &seg, const GnArgs &a) {
+  if (threadIdx.x < 32) make_segments_warp(seg, a.shapes, a.shape_stride, a.start, a.L, a.N);
+  __syncthreads();
+}
+
+// A thread's place in a CTA's rows: row lane rl, word cv; `at` elements behind the first word of a row of lane 0.
+struct Place {
+  int rl, cv;
+  unsigned at;
+  __device__ __forceinline__ Place(const GnArgs &a) {
+    rl = quotient(threadIdx.x, a.by_nv);
+    cv = threadIdx.x - rl * a.nv;
+    at = (unsigned)(rl * a.C + cv * a.V);
+  }
+};
+
+// The tile of a CTA: rows [r0, r1) of image b, the first of its segments.
+struct Tile {
+  int b, t, r0, r1, i;
+  __device__ __forceinline__ Tile(const GnArgs &a, const SegmentTable &seg, int index) {
+    b = quotient(index, a.by_tiles);
+    t = index - b * a.tiles;
+    r0 = t * a.R;
+    r1 = min(a.N, r0 + a.R);
+    i = 0;
+    while (seg.end[i] <= r0) ++i;
+  }
+};
+
+// A thread's next U words, RL rows (`step` elements) apart.  base, the row r of lane 0 and the row `end` are the same for the
+// CTA; ALL: no lane's last word lies at or beyond `end`.
+template <typename T, int V, int U, bool ONCE, bool ALL>
+__device__ __forceinline__ void load_rows(const T *base, unsigned at, int r, int end, int RL, long long step, Word<T, V> (&w)[U]) {
+#pragma unroll
+  for (int u = 0; u < U; ++u)
+    if (ALL || r + u * RL < end) w[u] = ONCE ? load_once<T, V>(base + u * step + at) : load_word<T, V>(base + u * step + at);
+}
+
+template <typename T, int V>
+__device__ __forceinline__ void zero_rows(T *base, unsigned at, int r, int end, int RL, long long step) {
+  const float zero[V] = {};
+  for (; r < end; r += RL, base += step) store_word<T, V>(base + at, zero);
+}
+
+// The groups of a thread's channels; their weights.
+template <int V>
+__device__ __forceinline__ void groups_of(const GnArgs &a, int cv, int (&g)[V]) {
+#pragma unroll
+  for (int c = 0; c < V; ++c) g[c] = a.whole ? (c == 0 ? quotient(cv, a.by_per) : g[0]) : quotient(cv * V + c, a.by_per);
+}
+template <int V>
+__device__ __forceinline__ void params_of(const GnArgs &a, const float *p, float (&f)[V]) {
+  if constexpr (V == 4) {
+    if (a.wide_params) {
+      const float4 t = __ldg(reinterpret_cast<const float4 *>(p));
+      f[0] = t.x; f[1] = t.y; f[2] = t.z; f[3] = t.w;
+      return;
+    }
+  }
+#pragma unroll
+  for (int c = 0; c < V; ++c) f[c] = __ldg(p + c);
+}
 
 // ------------------------------------------------------------------------------------------------
 // forward
 // ------------------------------------------------------------------------------------------------
-// partial (B, pieces, G): mean and sum of squares around it, of the piece's values of the group.
-template <typename T, int V>
-__global__ void __launch_bounds__(max_threads(V))
-gn_stats_kernel(const T *__restrict__ x, GnArgs a, float2 *__restrict__ partial) {
-  extern __shared__ float2 chan[];       // (RL, C): a thread's mean and M2 of its channels
-  __shared__ SegmentTable seg;
-  if (threadIdx.x == 0) make_segments(seg, a.shapes, a.shape_stride, a.start, a.L, a.N);
-  __syncthreads();
-  const int b = blockIdx.x / a.S, run = blockIdx.x % a.S;
-  const int r0 = run_begin(run, a.S, a.N), r1 = run_begin(run + 1, a.S, a.N);
-  const int cv = threadIdx.x % a.nv, rl = threadIdx.x / a.nv;
-  const bool active = rl < a.RL;
-  const T *base = x + ((long long)b * a.N) * a.C + cv * V;
-  for (int i = 1; i < seg.count; i += 2) {
-    const int lo = max(r0, seg.end[i - 1]), hi = min(r1, seg.end[i]);
-    if (lo >= hi) continue;
-    float n = 0.f, mean[V] = {}, m2[V] = {};
-    if (active) {
-      for (int r = lo + rl; r < hi; r += a.RL * kRows) {
-        Word<T, V> w[kRows];
+// Number, mean and sum of squares around it, of a thread's values of each of its channels.
+template <int V>
+struct Moments {
+  float n = 0.f, mean[V] = {}, m2[V] = {};
+  // U rows more, of which those before `have` count (all of them if ALL)
+  template <typename T, int U, bool ALL>
+  __device__ __forceinline__ void add(const Word<T, V> (&w)[U], int have) {
+    float s[V] = {}, q[V] = {}, f[V];
 #pragma unroll
-        for (int u = 0; u < kRows; ++u)
-          if (r + u * a.RL < hi) w[u] = load_word<T, V>(base + (long long)(r + u * a.RL) * a.C);
-        const int cnt = min(kRows, (hi - r + a.RL - 1) / a.RL);
-        float f[kRows][V];
+    for (int u = 0; u < U; ++u)
+      if (ALL || u < have) {
+        widen_word<T, V>(w[u], f);
 #pragma unroll
-        for (int u = 0; u < kRows; ++u) widen_word<T, V>(w[u], f[u]);
-        const float nc = (float)cnt, inv = 1.f / nc, total = n + nc, part = nc / total, cross = n * part;
+        for (int c = 0; c < V; ++c) s[c] += f[c];
+      }
+    const float nc = ALL ? (float)U : (float)have, inv = ALL ? 1.f / U : __fdividef(1.f, nc);
+    const float total = n + nc, part = __fdividef(nc, total), cross = n * part;
+#pragma unroll
+    for (int c = 0; c < V; ++c) s[c] *= inv;
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (ALL || u < have) {
+        widen_word<T, V>(w[u], f);
 #pragma unroll
         for (int c = 0; c < V; ++c) {
-          float s = 0.f, q = 0.f;
-#pragma unroll
-          for (int u = 0; u < kRows; ++u)
-            if (u < cnt) s += f[u][c];
-          s *= inv;
-#pragma unroll
-          for (int u = 0; u < kRows; ++u)
-            if (u < cnt) q = fmaf(f[u][c] - s, f[u][c] - s, q);
-          const float delta = s - mean[c];
-          mean[c] = fmaf(delta, part, mean[c]);
-          m2[c] += fmaf(delta * delta, cross, q);
+          f[c] -= s[c];
+          q[c] = fmaf(f[c], f[c], q[c]);
         }
-        n = total;
       }
 #pragma unroll
-      for (int c = 0; c < V; ++c) chan[rl * a.C + cv * V + c] = make_float2(mean[c], m2[c]);
+    for (int c = 0; c < V; ++c) {
+      const float delta = s[c] - mean[c];
+      mean[c] = fmaf(delta, part, mean[c]);
+      m2[c] += fmaf(delta * delta, cross, q[c]);
     }
-    __syncthreads();
-    const int lane = threadIdx.x & 31, warps = blockDim.x >> 5, all = a.RL * a.cpg;
-    const float inv_n = 1.f / ((float)(hi - lo) * (float)a.cpg);
-    for (int g = threadIdx.x >> 5; g < a.G; g += warps) {
-      float s = 0.f, q = 0.f;
-      for (int e = lane; e < all; e += 32) {
-        const int l = e / a.cpg;
-        s = fmaf((float)lane_rows(hi - lo, l, a.RL), chan[l * a.C + g * a.cpg + e - l * a.cpg].x, s);
-      }
-      const float m = warp_sum(s) * inv_n;
-      for (int e = lane; e < all; e += 32) {
-        const int l = e / a.cpg;
-        const float2 t = chan[l * a.C + g * a.cpg + e - l * a.cpg];
-        const float d = t.x - m;
-        q += fmaf(d * d, (float)lane_rows(hi - lo, l, a.RL), t.y);
-      }
-      q = warp_sum(q);
-      if (lane == 0) partial[((long long)b * pieces(a) + run + i) * a.G + g] = make_float2(m, q);
-    }
-    __syncthreads();
+    n = total;
   }
-}
+};
 
-// Merges the pieces of segment i of image b; every thread returns when stats[g] = (mean, rstd) is in shared memory.
-__device__ __forceinline__ void merge_stats(const GnArgs &a, const SegmentTable &seg, const float2 *partial, int b, int i,
-                                            float2 *stats) {
-  const int lane = threadIdx.x & 31, warps = blockDim.x >> 5;
-  const int lo = seg.end[i - 1], hi = seg.end[i], first = run_of(lo, a.S, a.N), last = run_of(hi - 1, a.S, a.N);
-  const float2 *p = partial + ((long long)b * pieces(a) + i) * a.G;
-  for (int g = threadIdx.x >> 5; g < a.G; g += warps) {
-    float s = 0.f, q = 0.f;
-    for (int r = first + lane; r <= last; r += 32) {
-      const float n = (float)(min(hi, run_begin(r + 1, a.S, a.N)) - max(lo, run_begin(r, a.S, a.N)));
-      s = fmaf(n, p[(long long)r * a.G + g].x, s);
-    }
-    const float m = warp_sum(s) / (float)(hi - lo);
-    for (int r = first + lane; r <= last; r += 32) {
-      const float n = (float)(min(hi, run_begin(r + 1, a.S, a.N)) - max(lo, run_begin(r, a.S, a.N)));
-      const float2 t = p[(long long)r * a.G + g];
-      const float d = t.x - m;
-      q += fmaf(d * d, n * (float)a.cpg, t.y);
-    }
-    q = warp_sum(q);
-    if (lane == 0) stats[g] = make_float2(m, rsqrtf(q / ((float)(hi - lo) * (float)a.cpg) + a.eps));
-  }
-  __syncthreads();
-}
-
+// A tile's statistics into partial (B, entries, G): mean and sum of squares around it, of each piece's values of a group.
 template <typename T, int V>
-__device__ __forceinline__ void zero_rows(T *base, const GnArgs &a, int lo, int hi, int rl) {
-  const float zero[V] = {};
-  if (rl < a.RL)
-    for (int r = lo + rl; r < hi; r += a.RL) store_word<T, V>(base + (long long)r * a.C, zero);
-}
-
-template <typename T, int V>
-__global__ void __launch_bounds__(max_threads(V))
-gn_apply_kernel(const T *__restrict__ x, GnArgs a, const float2 *__restrict__ partial, T *__restrict__ y,
-                                float *__restrict__ mean_out, float *__restrict__ rstd_out) {
-  extern __shared__ float2 stats[];      // (G): mean, rstd
+__global__ void __launch_bounds__(kThreads<V>, kResident<T, V>)
+group_stats_kernel(const T *__restrict__ x, const GnArgs a, float2 *__restrict__ partial) {
+  constexpr int U = kAhead;
+  extern __shared__ float2 chan[];                       // a thread's channels
+  __shared__ float count[kThreads<V>];                   // values that an entry of a row lane stands for
   __shared__ SegmentTable seg;
-  if (threadIdx.x == 0) make_segments(seg, a.shapes, a.shape_stride, a.start, a.L, a.N);
-  __syncthreads();
-  const int b = blockIdx.x / a.S, run = blockIdx.x % a.S;
-  const int r0 = run_begin(run, a.S, a.N), r1 = run_begin(run + 1, a.S, a.N);
-  const int cv = threadIdx.x % a.nv, rl = threadIdx.x / a.nv;
-  const long long base = ((long long)b * a.N) * a.C + cv * V;
-  for (int i = 0; i < seg.count; ++i) {
-    const int begin = segment_begin(seg, i), lo = max(r0, begin), hi = min(r1, seg.end[i]);
-    if (lo >= hi) continue;
-    if ((i & 1) == 0) {
-      zero_rows<T, V>(y + base, a, lo, hi, rl);
+  launch_next();
+  make_table(seg, a);
+  Tile tile(a, seg, blockIdx.x);
+  const Place at(a);
+  const long long step = (long long)a.RL * a.C;
+  // a thread's channels are of one group where V divides it: one entry for all of them, or one for each
+  const int lane = threadIdx.x & 31, sub = lane & 7, width = a.whole ? a.nv : a.C, per = (int)a.by_per.d;
+  for (int lo = tile.r0; lo < tile.r1; ++tile.i) {
+    const int hi = min(tile.r1, seg.end[tile.i]), rows = hi - lo, from = lo;
+    lo = hi;
+    if (rows <= 0 || (tile.i & 1) == 0) continue;
+    if (at.rl < a.RL) {
+      const T *base = x + ((long long)tile.b * a.N + from) * a.C;
+      Moments<V> k;
+      Word<T, V> w[U];
+      int r = 0;
+      for (; r + U * a.RL <= rows; r += U * a.RL, base += U * step) {
+        load_rows<T, V, U, false, true>(base, at.at, r, rows, a.RL, step, w);
+        k.template add<T, U, true>(w, U);
+      }
+      if (r + at.rl < rows) {
+        load_rows<T, V, U, false, false>(base, at.at, r + at.rl, rows, a.RL, step, w);
+        int have = 0;
+#pragma unroll
+        for (int u = 0; u < U; ++u) have += r + at.rl + u * a.RL < rows;
+        k.template add<T, U, false>(w, have);
+      }
+      if (a.whole) {
+        float m = 0.f, q = 0.f;
+#pragma unroll
+        for (int c = 0; c < V; ++c) m += k.mean[c];
+        m *= 1.f / V;
+#pragma unroll
+        for (int c = 0; c < V; ++c) q += fmaf((k.mean[c] - m) * (k.mean[c] - m), k.n, k.m2[c]);
+        chan[at.rl * width + at.cv] = make_float2(m, q);
+      } else {
+#pragma unroll
+        for (int c = 0; c < V; ++c) chan[at.rl * width + at.cv * V + c] = make_float2(k.mean[c], k.m2[c]);
+      }
+      if (at.cv == 0) count[at.rl] = a.whole ? k.n * V : k.n;
+    }
+    __syncthreads();
+    // eight lanes have a group
+    const float inv_n = __fdividef(1.f, (float)rows * (float)a.cpg);
+    const int l0 = quotient(sub, a.by_per), j0 = sub - l0 * per, dl = quotient(8, a.by_per), dj = 8 - dl * per;
+    for (int g0 = (threadIdx.x >> 5) * 4; g0 < a.G; g0 += kThreads<V> / 8) {
+      const int g = g0 + (lane >> 3), RL = g < a.G ? a.RL : 0;
+      const float2 *entries = chan + g * per;
+      float s = 0.f, q = 0.f;
+#pragma unroll 1
+      for (int l = l0, j = j0; l < RL; l += dl) {
+        s = fmaf(count[l], entries[l * width + j].x, s);
+        j += dj;
+        if (j >= per) j -= per, ++l;
+      }
+      const float m = sum8(s) * inv_n;
+#pragma unroll 1
+      for (int l = l0, j = j0; l < RL; l += dl) {
+        const float2 v = entries[l * width + j];
+        q += fmaf((v.x - m) * (v.x - m), count[l], v.y);
+        j += dj;
+        if (j >= per) j -= per, ++l;
+      }
+      q = sum8(q);
+      if (sub == 0 && RL) partial[((long long)tile.b * a.entries + tile.t + tile.i) * a.G + g] = make_float2(m, q);
+    }
+    __syncthreads();
+  }
+}
+
+// A segment of an image, and the tiles that have a piece of it.
+struct Span {
+  int begin, end, from, to;
+  __device__ __forceinline__ Span(const GnArgs &a, const SegmentTable &seg, int i) {
+    begin = segment_begin(seg, i);
+    end = seg.end[i];
+    from = quotient(begin, a.by_r);
+    to = end > begin ? quotient(end - 1, a.by_r) : from - 1;
+  }
+};
+
+constexpr int kMergeThreads = 256;
+
+// The group of a level of an image that a warp merges.
+struct MergeTask {
+  int b, l, g;
+  bool mine;
+  __device__ __forceinline__ MergeTask(const GnArgs &a, int task) {
+    mine = task < a.B * a.L * a.G;
+    const int q = quotient(task, a.by_groups);
+    g = task - q * a.G;
+    b = quotient(q, a.by_levels);
+    l = q - b * a.L;
+  }
+};
+
+// Merges the tiles' parts: mean, rstd (B, L, G).
+__global__ void __launch_bounds__(kMergeThreads)
+group_merge_kernel(const GnArgs a, const float2 *partial, float *__restrict__ mean_out, float *__restrict__ rstd_out) {
+  constexpr int U = 8;
+  __shared__ SegmentTable seg;
+  launch_next();
+  make_table(seg, a);
+  const int task = blockIdx.x * (kMergeThreads / 32) + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+  const MergeTask k(a, task);
+  launch_wait();
+  if (!k.mine) return;
+  const Span s(a, seg, 2 * k.l + 1);
+  const float2 *src = partial + ((long long)k.b * a.entries + 2 * k.l + 1) * a.G + k.g;
+  float n = 0.f, mean = 0.f, m2 = 0.f;
+  for (int t = s.from + lane; t <= s.to; t += 32 * U) {
+    float2 v[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (t + 32 * u <= s.to) v[u] = __ldcg(src + (long long)(t + 32 * u) * a.G);
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int tu = t + 32 * u;
+      if (tu > s.to) break;
+      const float nb = (float)(min(s.end, (tu + 1) * a.R) - max(s.begin, tu * a.R)) * (float)a.cpg, total = n + nb;
+      const float part = __fdividef(nb, total), delta = v[u].x - mean;
+      mean = fmaf(delta, part, mean);
+      m2 += fmaf(delta * delta, n * part, v[u].y);
+      n = total;
+    }
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    const float nb = __shfl_down_sync(0xffffffffu, n, o), mb = __shfl_down_sync(0xffffffffu, mean, o);
+    const float qb = __shfl_down_sync(0xffffffffu, m2, o), total = n + nb, delta = mb - mean;
+    const float part = total > 0.f ? __fdividef(nb, total) : 0.f;
+    mean = fmaf(delta, part, mean);
+    m2 += fmaf(delta * delta, n * part, qb);
+    n = total;
+  }
+  if (lane == 0) {
+    mean_out[task] = mean;
+    rstd_out[task] = n > 0.f ? rsqrtf(__fdividef(m2, n) + a.eps) : 0.f;
+  }
+}
+
+// y = act((x - mean) * rstd * weight + bias).  Tiles are taken from the last one on: what the statistics read last is still in L2.
+template <typename T, int V, bool ACT>
+__global__ void __launch_bounds__(kThreads<V>, kResident<T, V>)
+group_apply_kernel(const T *__restrict__ x, const GnArgs a, const float *mean_in, const float *rstd_in, T *__restrict__ y) {
+  constexpr int U = kAhead;
+  __shared__ SegmentTable seg;
+  launch_next();
+  make_table(seg, a);
+  Tile tile(a, seg, (int)(gridDim.x - 1 - blockIdx.x));
+  const Place at(a);
+  const long long step = (long long)a.RL * a.C;
+  int group[V];
+  groups_of<V>(a, at.cv, group);
+  bool waited = false;
+  for (int lo = tile.r0; lo < tile.r1; ++tile.i) {
+    const int hi = min(tile.r1, seg.end[tile.i]), rows = at.rl < a.RL ? hi - lo : 0, l = tile.i >> 1;
+    const long long first = ((long long)tile.b * a.N + lo) * a.C;
+    const T *in = x + first;
+    T *out = y + first;
+    lo = max(lo, hi);
+    Word<T, V> w[U];
+    // on its way before the statistics are there
+    if (tile.i & 1) load_rows<T, V, U, true, false>(in, at.at, at.rl, rows, a.RL, step, w);
+    if (!waited) launch_wait();
+    waited = true;
+    if (rows <= 0) continue;
+    if ((tile.i & 1) == 0) {
+      zero_rows<T, V>(out, at.at, at.rl, rows, a.RL, step);
       continue;
     }
-    merge_stats(a, seg, partial, b, i, stats);
-    const int l = i >> 1;
-    if (mean_out && lo == begin)
-      for (int g = threadIdx.x; g < a.G; g += blockDim.x) {
-        mean_out[((long long)b * a.L + l) * a.G + g] = stats[g].x;
-        rstd_out[((long long)b * a.L + l) * a.G + g] = stats[g].y;
-      }
-    if (rl < a.RL) {
-      float mean[V], scale[V], shift[V];
-      const int wrow = a.weight_rows == 1 ? 0 : l;
+    float mean[V], scale[V], shift[V];
+    const int w0 = (a.weight_rows == 1 ? 0 : l) * a.C + at.cv * V;
+    const long long g0 = ((long long)tile.b * a.L + l) * a.G;
+    params_of<V>(a, a.weight + w0, scale);
+    params_of<V>(a, a.bias + w0, shift);
 #pragma unroll
-      for (int c = 0; c < V; ++c) {
-        const float2 s = stats[(cv * V + c) / a.cpg];
-        mean[c] = s.x;
-        scale[c] = s.y * __ldg(a.weight + wrow * a.C + cv * V + c);
-        shift[c] = __ldg(a.bias + wrow * a.C + cv * V + c);
-      }
-      for (int r = lo + rl; r < hi; r += a.RL * kRows) {
-        Word<T, V> w[kRows];
-#pragma unroll
-        for (int u = 0; u < kRows; ++u)
-          if (r + u * a.RL < hi) w[u] = load_once<T, V>(x + base + (long long)(r + u * a.RL) * a.C);
-#pragma unroll
-        for (int u = 0; u < kRows; ++u) {
-          if (r + u * a.RL >= hi) break;
-          float f[V];
-          widen_word<T, V>(w[u], f);
-#pragma unroll
-          for (int c = 0; c < V; ++c) f[c] = activate(fmaf(f[c] - mean[c], scale[c], shift[c]), a.act);
-          store_word<T, V>(y + base + (long long)(r + u * a.RL) * a.C, f);
-        }
-      }
+    for (int c = 0; c < V; ++c) {
+      mean[c] = __ldcg(mean_in + g0 + group[c]);
+      scale[c] *= __ldcg(rstd_in + g0 + group[c]);
     }
-    __syncthreads();      // stats are overwritten for the next piece
+    auto store = [&](int u) {
+      float f[V];
+      widen_word<T, V>(w[u], f);
+#pragma unroll
+      for (int c = 0; c < V; ++c) f[c] = activate<ACT>(fmaf(f[c] - mean[c], scale[c], shift[c]), a.act);
+      store_word<T, V>(out + u * step + at.at, f);
+    };
+    int r = 0;
+    for (; r + U * a.RL <= rows; r += U * a.RL, in += U * step, out += U * step) {
+      if (r > 0) load_rows<T, V, U, true, true>(in, at.at, r, rows, a.RL, step, w);
+#pragma unroll
+      for (int u = 0; u < U; ++u) store(u);
+    }
+    if (r > 0) load_rows<T, V, U, true, false>(in, at.at, r + at.rl, rows, a.RL, step, w);
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (r + at.rl + u * a.RL < rows) store(u);
   }
 }
 
 // ------------------------------------------------------------------------------------------------
 // backward
 // ------------------------------------------------------------------------------------------------
-// What a thread knows of its channels.
-template <int V>
-struct Channels {
-  float mean[V], rstd[V], gamma[V], beta[V];
-  __device__ __forceinline__ void load(const GnArgs &a, const float *mean_in, const float *rstd_in, int b, int l, int cv) {
-    const int wrow = a.weight_rows == 1 ? 0 : l;
-#pragma unroll
-    for (int c = 0; c < V; ++c) {
-      const long long g = ((long long)b * a.L + l) * a.G + (cv * V + c) / a.cpg;
-      mean[c] = __ldg(mean_in + g);
-      rstd[c] = __ldg(rstd_in + g);
-      gamma[c] = __ldg(a.weight + wrow * a.C + cv * V + c);
-      beta[c] = __ldg(a.bias + wrow * a.C + cv * V + c);
-    }
-  }
-  // xhat and dz; z as the forward forms it, so that a ReLU's border falls the same way
-  __device__ __forceinline__ void one(float x, float g, int c, int act, float &hat, float &dz) const {
-    hat = (x - mean[c]) * rstd[c];
-    dz = act == kNone ? g : activate_grad(g, fmaf(x - mean[c], rstd[c] * gamma[c], beta[c]), act);
-  }
-};
-
-constexpr int kGradRows = 4;
-
-// by_channel (B, pieces, C): sums of dz and of dz * xhat over the piece's rows; by_group (B, pieces, G): the same times gamma,
-// over the group's channels.
-template <typename T, int V>
-__global__ void __launch_bounds__(max_threads(V))
-gn_grad_stats_kernel(const T *__restrict__ grad_y, const T *__restrict__ x, GnArgs a,
-                                     const float *__restrict__ mean_in, const float *__restrict__ rstd_in,
-                                     float2 *__restrict__ by_channel, float2 *__restrict__ by_group) {
-  extern __shared__ float2 chan[];       // (RL, C)
+// Sums of dz and of dz * xhat over a tile's pieces: by_channel (B, entries, C), and times gamma over a group's channels: by_group
+// (B, entries, G).
+template <typename T, int V, bool ACT>
+__global__ void __launch_bounds__(kThreads<V>, kResident<T, V>)
+group_grad_stats_kernel(const T *__restrict__ grad_y, const T *__restrict__ x, const GnArgs a, const float *__restrict__ mean_in,
+                        const float *__restrict__ rstd_in, float2 *__restrict__ by_channel, float2 *__restrict__ by_group) {
+  constexpr int U = kGradAhead;
+  extern __shared__ float2 chan[];                       // (RL, C)
   __shared__ SegmentTable seg;
-  if (threadIdx.x == 0) make_segments(seg, a.shapes, a.shape_stride, a.start, a.L, a.N);
-  __syncthreads();
-  const int b = blockIdx.x / a.S, run = blockIdx.x % a.S;
-  const int r0 = run_begin(run, a.S, a.N), r1 = run_begin(run + 1, a.S, a.N);
-  const int cv = threadIdx.x % a.nv, rl = threadIdx.x / a.nv;
-  const long long base = ((long long)b * a.N) * a.C + cv * V;
-  for (int i = 1; i < seg.count; i += 2) {
-    const int lo = max(r0, seg.end[i - 1]), hi = min(r1, seg.end[i]);
-    if (lo >= hi) continue;
-    const int l = i >> 1, wrow = a.weight_rows == 1 ? 0 : l;
-    if (rl < a.RL) {
-      Channels<V> ch;
-      ch.load(a, mean_in, rstd_in, b, l, cv);
-      float s1[V] = {}, s2[V] = {};
-      for (int r = lo + rl; r < hi; r += a.RL * kGradRows) {
-        Word<T, V> xw[kGradRows], gw[kGradRows];
-#pragma unroll
-        for (int u = 0; u < kGradRows; ++u)
-          if (r + u * a.RL < hi) {
-            xw[u] = load_word<T, V>(x + base + (long long)(r + u * a.RL) * a.C);
-            gw[u] = load_word<T, V>(grad_y + base + (long long)(r + u * a.RL) * a.C);
-          }
-#pragma unroll
-        for (int u = 0; u < kGradRows; ++u) {
-          if (r + u * a.RL >= hi) break;
-          float xf[V], gf[V];
-          widen_word<T, V>(xw[u], xf);
-          widen_word<T, V>(gw[u], gf);
-#pragma unroll
-          for (int c = 0; c < V; ++c) {
-            float hat, dz;
-            ch.one(xf[c], gf[c], c, a.act, hat, dz);
-            s1[c] += dz;
-            s2[c] = fmaf(dz, hat, s2[c]);
-          }
-        }
+  launch_next();
+  make_table(seg, a);
+  Tile tile(a, seg, blockIdx.x);
+  const Place at(a);
+  const long long step = (long long)a.RL * a.C;
+  int group[V];
+  groups_of<V>(a, at.cv, group);
+  for (int lo = tile.r0; lo < tile.r1; ++tile.i) {
+    const int hi = min(tile.r1, seg.end[tile.i]), rows = hi - lo, from = lo, l = tile.i >> 1;
+    lo = max(lo, hi);
+    if (rows <= 0 || (tile.i & 1) == 0) continue;
+    const float *gamma = a.weight + (a.weight_rows == 1 ? 0 : l) * a.C, *beta = a.bias + (gamma - a.weight);
+    const long long g0 = ((long long)tile.b * a.L + l) * a.G;
+    if (at.rl < a.RL) {
+      const long long first = ((long long)tile.b * a.N + from) * a.C;
+      const T *xin = x + first, *gin = grad_y + first;
+      float mean[V], scale[V], shift[V], s1[V] = {}, s2[V] = {};
+      if (ACT) {
+        params_of<V>(a, gamma + at.cv * V, scale);
+        params_of<V>(a, beta + at.cv * V, shift);
       }
-#pragma unroll
-      for (int c = 0; c < V; ++c) chan[rl * a.C + cv * V + c] = make_float2(s1[c], s2[c]);
-    }
-    __syncthreads();
-    const long long piece = (long long)b * pieces(a) + run + i;
-    for (int c = threadIdx.x; c < a.C; c += blockDim.x) {
-      float2 t = chan[c];
-      for (int k = 1; k < a.RL; ++k) {
-        t.x += chan[k * a.C + c].x;
-        t.y += chan[k * a.C + c].y;
-      }
-      by_channel[piece * a.C + c] = t;
-      const float w = __ldg(a.weight + wrow * a.C + c);
-      chan[c] = make_float2(t.x * w, t.y * w);
-    }
-    __syncthreads();
-    const int lane = threadIdx.x & 31, warps = blockDim.x >> 5;
-    for (int g = threadIdx.x >> 5; g < a.G; g += warps) {
-      float u = 0.f, v = 0.f;
-      for (int e = lane; e < a.cpg; e += 32) {
-        u += chan[g * a.cpg + e].x;
-        v += chan[g * a.cpg + e].y;
-      }
-      u = warp_sum(u);
-      v = warp_sum(v);
-      if (lane == 0) by_group[piece * a.G + g] = make_float2(u, v);
-    }
-    __syncthreads();
-  }
-}
-
-// grad_x = rstd * (d - mean(d) - xhat * mean(d * xhat)), d = dz * gamma, means over the group.
-template <typename T, int V>
-__global__ void __launch_bounds__(max_threads(V))
-gn_grad_apply_kernel(const T *__restrict__ grad_y, const T *__restrict__ x, GnArgs a,
-                                     const float *__restrict__ mean_in, const float *__restrict__ rstd_in,
-                                     const float2 *__restrict__ by_group, T *__restrict__ grad_x) {
-  extern __shared__ float2 means[];      // (G)
-  __shared__ SegmentTable seg;
-  if (threadIdx.x == 0) make_segments(seg, a.shapes, a.shape_stride, a.start, a.L, a.N);
-  __syncthreads();
-  const int b = blockIdx.x / a.S, run = blockIdx.x % a.S;
-  const int r0 = run_begin(run, a.S, a.N), r1 = run_begin(run + 1, a.S, a.N);
-  const int cv = threadIdx.x % a.nv, rl = threadIdx.x / a.nv, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
-  const long long base = ((long long)b * a.N) * a.C + cv * V;
-  for (int i = 0; i < seg.count; ++i) {
-    const int begin = segment_begin(seg, i), lo = max(r0, begin), hi = min(r1, seg.end[i]);
-    if (lo >= hi) continue;
-    if ((i & 1) == 0) {
-      zero_rows<T, V>(grad_x + base, a, lo, hi, rl);
-      continue;
-    }
-    const int first = run_of(begin, a.S, a.N), last = run_of(seg.end[i] - 1, a.S, a.N);
-    const float inv = 1.f / ((float)(seg.end[i] - begin) * (float)a.cpg);
-    const float2 *p = by_group + ((long long)b * pieces(a) + i) * a.G;
-    for (int g = threadIdx.x >> 5; g < a.G; g += warps) {
-      float u = 0.f, v = 0.f;
-      for (int r = first + lane; r <= last; r += 32) {
-        u += p[(long long)r * a.G + g].x;
-        v += p[(long long)r * a.G + g].y;
-      }
-      u = warp_sum(u);
-      v = warp_sum(v);
-      if (lane == 0) means[g] = make_float2(u * inv, v * inv);
-    }
-    __syncthreads();
-    if (rl < a.RL) {
-      Channels<V> ch;
-      ch.load(a, mean_in, rstd_in, b, i >> 1, cv);
-      float c1[V], c2[V];
 #pragma unroll
       for (int c = 0; c < V; ++c) {
-        c1[c] = means[(cv * V + c) / a.cpg].x;
-        c2[c] = means[(cv * V + c) / a.cpg].y;
+        mean[c] = __ldg(mean_in + g0 + group[c]);
+        if (ACT) scale[c] *= __ldg(rstd_in + g0 + group[c]);      // as the forward forms it
       }
-      for (int r = lo + rl; r < hi; r += a.RL * kGradRows) {
-        Word<T, V> xw[kGradRows], gw[kGradRows];
+      Word<T, V> xw[U], gw[U];
+      auto add = [&](int u) {
+        float xf[V], gf[V];
+        widen_word<T, V>(xw[u], xf);
+        widen_word<T, V>(gw[u], gf);
 #pragma unroll
-        for (int u = 0; u < kGradRows; ++u)
-          if (r + u * a.RL < hi) {
-            xw[u] = load_once<T, V>(x + base + (long long)(r + u * a.RL) * a.C);
-            gw[u] = load_once<T, V>(grad_y + base + (long long)(r + u * a.RL) * a.C);
-          }
-#pragma unroll
-        for (int u = 0; u < kGradRows; ++u) {
-          if (r + u * a.RL >= hi) break;
-          float xf[V], gf[V];
-          widen_word<T, V>(xw[u], xf);
-          widen_word<T, V>(gw[u], gf);
-#pragma unroll
-          for (int c = 0; c < V; ++c) {
-            float hat, dz;
-            ch.one(xf[c], gf[c], c, a.act, hat, dz);
-            xf[c] = ch.rstd[c] * (dz * ch.gamma[c] - c1[c] - hat * c2[c]);
-          }
-          store_word<T, V>(grad_x + base + (long long)(r + u * a.RL) * a.C, xf);
+        for (int c = 0; c < V; ++c) {
+          const float centred = xf[c] - mean[c];
+          const float dz = ACT ? activate_grad<ACT>(gf[c], fmaf(centred, scale[c], shift[c]), a.act) : gf[c];
+          s1[c] += dz;
+          s2[c] = fmaf(dz, centred, s2[c]);
         }
+      };
+      int r = 0;
+      for (; r + U * a.RL <= rows; r += U * a.RL, xin += U * step, gin += U * step) {
+        load_rows<T, V, U, false, true>(xin, at.at, r, rows, a.RL, step, xw);
+        load_rows<T, V, U, false, true>(gin, at.at, r, rows, a.RL, step, gw);
+#pragma unroll
+        for (int u = 0; u < U; ++u) add(u);
       }
+      load_rows<T, V, U, false, false>(xin, at.at, r + at.rl, rows, a.RL, step, xw);
+      load_rows<T, V, U, false, false>(gin, at.at, r + at.rl, rows, a.RL, step, gw);
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (r + at.rl + u * a.RL < rows) add(u);
+#pragma unroll
+      for (int c = 0; c < V; ++c) chan[at.rl * a.C + at.cv * V + c] = make_float2(s1[c], s2[c]);
+    }
+    __syncthreads();
+    const long long entry = (long long)tile.b * a.entries + tile.t + tile.i;
+    for (int c = threadIdx.x; c < a.C; c += kThreads<V>) {
+      float2 s = chan[c];
+      for (int j = 1; j < a.RL; ++j) {
+        s.x += chan[j * a.C + c].x;
+        s.y += chan[j * a.C + c].y;
+      }
+      s.y *= __ldg(rstd_in + g0 + c / a.cpg);
+      by_channel[entry * a.C + c] = s;
+      const float w = __ldg(gamma + c);
+      chan[c] = make_float2(s.x * w, s.y * w);
+    }
+    __syncthreads();
+    const int lane = threadIdx.x & 31, sub = lane & 7;
+    for (int q0 = (threadIdx.x >> 5) * 4; q0 < a.G; q0 += kThreads<V> / 8) {      // eight lanes have a group
+      const int g = q0 + (lane >> 3);
+      float u = 0.f, v = 0.f;
+      if (g < a.G)
+        for (int c = g * a.cpg + sub; c < (g + 1) * a.cpg; c += 8) {
+          u += chan[c].x;
+          v += chan[c].y;
+        }
+      u = sum8(u);
+      v = sum8(v);
+      if (sub == 0 && g < a.G) by_group[entry * a.G + g] = make_float2(u, v);
     }
     __syncthreads();
   }
 }
 
-// grad_weight, grad_bias (weight_rows, C): the sums of by_channel over images and pieces, and over levels where they share the
-// weights, in a fixed order.  32 channels and 8 lanes over the pieces a CTA.
-__global__ void __launch_bounds__(256)
-gn_param_kernel(const float2 *__restrict__ by_channel, GnArgs a, int B, float *__restrict__ grad_weight, float *__restrict__ grad_bias) {
+// The first `merges` CTAs: means over a group of a level of an image, by a warp: means (B, L, G).  The others: by_channel summed over
+// a level's tiles into by_level (B, L, C), 32 channels a CTA, a warp every eighth tile.
+__global__ void __launch_bounds__(kMergeThreads)
+group_grad_merge_kernel(const GnArgs a, int merges, const float2 *by_group, const float2 *by_channel, float2 *__restrict__ means,
+                        float2 *__restrict__ by_level) {
+  constexpr int U = 8, kWarps = kMergeThreads / 32;
   __shared__ SegmentTable seg;
-  __shared__ float2 part[8][32];
-  if (threadIdx.x == 0) make_segments(seg, a.shapes, a.shape_stride, a.start, a.L, a.N);
-  __syncthreads();
-  const int lane = threadIdx.x & 31, k = threadIdx.x >> 5, c = blockIdx.x * 32 + lane;
-  const int l0 = a.weight_rows == 1 ? 0 : blockIdx.y, l1 = a.weight_rows == 1 ? a.L : l0 + 1;
-  float2 t = make_float2(0.f, 0.f);
-  if (c < a.C)
-    for (int l = l0; l < l1; ++l) {
-      const int lo = seg.end[2 * l], hi = seg.end[2 * l + 1];
-      if (lo >= hi) continue;
-      const int first = run_of(lo, a.S, a.N), n = run_of(hi - 1, a.S, a.N) - first + 1;
-      const long long all = (long long)n * B;
-#pragma unroll 4
-      for (long long e = k; e < all; e += 8) {
-        const int b = (int)(e / n), r = first + (int)(e - (long long)b * n);
-        const float2 v = __ldg(by_channel + ((long long)b * pieces(a) + r + 2 * l + 1) * a.C + c);
-        t.x += v.x;
-        t.y += v.y;
-      }
-    }
-  part[k][lane] = t;
-  __syncthreads();
-  if (k != 0 || c >= a.C) return;
+  __shared__ float2 part[kMergeThreads];
+  launch_next();
+  make_table(seg, a);
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  launch_wait();
+  const bool channels = (int)blockIdx.x >= merges;
+  const int chunk = ((int)blockIdx.x - merges) % ((a.C + 31) / 32), c = chunk * 32 + lane;
+  const int level = channels ? ((int)blockIdx.x - merges) / ((a.C + 31) / 32) : 0;      // of the B * L
+  const MergeTask k(a, channels ? level * a.G : (int)blockIdx.x * kWarps + warp);
+  float u = 0.f, v = 0.f;
+  if (k.mine) {
+    const Span s(a, seg, 2 * k.l + 1);
+    const long long entry = (long long)k.b * a.entries + 2 * k.l + 1;
+    const float2 *src = channels ? by_channel + entry * a.C + c : by_group + entry * a.G + k.g;
+    const int first = channels ? warp : lane, every = channels ? kWarps : 32, width = channels ? a.C : a.G;
+    if (!channels || c < a.C)
+      for (int t = s.from + first; t <= s.to; t += every * U) {
+        float2 p[U];
 #pragma unroll
-  for (int i = 1; i < 8; ++i) {
-    t.x += part[i][lane].x;
-    t.y += part[i][lane].y;
+        for (int j = 0; j < U; ++j)
+          if (t + every * j <= s.to) p[j] = __ldcg(src + (long long)(t + every * j) * width);
+#pragma unroll
+        for (int j = 0; j < U; ++j)
+          if (t + every * j <= s.to) {
+            u += p[j].x;
+            v += p[j].y;
+          }
+      }
+    if (!channels) {
+      u = warp_sum(u);
+      v = warp_sum(v);
+      const float n = (float)(s.end - s.begin) * (float)a.cpg;
+      if (lane == 0) means[(k.b * a.L + k.l) * a.G + k.g] = n > 0.f ? make_float2(__fdividef(u, n), __fdividef(v, n)) : make_float2(0.f, 0.f);
+    }
   }
-  grad_bias[blockIdx.y * a.C + c] = t.x;
-  grad_weight[blockIdx.y * a.C + c] = t.y;
+  if (!channels) return;
+  part[threadIdx.x] = make_float2(u, v);
+  __syncthreads();
+  if (warp == 0 && c < a.C) {
+#pragma unroll
+    for (int j = 1; j < kWarps; ++j) {
+      u += part[j * 32 + lane].x;
+      v += part[j * 32 + lane].y;
+    }
+    by_level[(long long)level * a.C + c] = make_float2(u, v);
+  }
+}
+
+// grad_weight, grad_bias (weight_rows, C): by_level summed over images, and over levels where they share the weights.
+__device__ __forceinline__ void parameter_sums(const GnArgs &a, const float2 *by_level, int column, float *grad_weight,
+                                               float *grad_bias) {
+  if (column >= a.weight_rows * a.C) return;
+  const int row = column / a.C, c = column - row * a.C, levels = a.weight_rows == 1 ? a.L : 1;
+  float2 s = make_float2(0.f, 0.f);
+  for (int l = row; l < row + levels; ++l)
+#pragma unroll 8
+    for (int b = 0; b < a.B; ++b) {
+      const float2 v = __ldcg(by_level + ((long long)b * a.L + l) * a.C + c);
+      s.x += v.x;
+      s.y += v.y;
+    }
+  grad_bias[column] = s.x;
+  grad_weight[column] = s.y;
+}
+
+// grad_x = rstd * (d - mean(d) - xhat * mean(d * xhat)), d = dz * gamma, means over the group; the first `sums` CTAs form the
+// parameters' gradients instead, beside the others.
+template <typename T, int V, bool ACT>
+__global__ void __launch_bounds__(kThreads<V>, kResident<T, V>)
+group_grad_apply_kernel(const T *__restrict__ grad_y, const T *__restrict__ x, const GnArgs a, int sums,
+                        const float *__restrict__ mean_in, const float *__restrict__ rstd_in, const float2 *means,
+                        const float2 *by_level, T *__restrict__ grad_x, float *grad_weight, float *grad_bias) {
+  constexpr int U = kGradAhead;
+  __shared__ SegmentTable seg;
+  if ((int)blockIdx.x < sums) {
+    launch_wait();
+    parameter_sums(a, by_level, blockIdx.x * kThreads<V> + threadIdx.x, grad_weight, grad_bias);
+    return;
+  }
+  make_table(seg, a);
+  Tile tile(a, seg, (int)(gridDim.x - 1 - blockIdx.x));
+  const Place at(a);
+  const long long step = (long long)a.RL * a.C;
+  int group[V];
+  groups_of<V>(a, at.cv, group);
+  bool waited = false;
+  for (int lo = tile.r0; lo < tile.r1; ++tile.i) {
+    const int hi = min(tile.r1, seg.end[tile.i]), rows = at.rl < a.RL ? hi - lo : 0, l = tile.i >> 1;
+    const long long first = ((long long)tile.b * a.N + lo) * a.C;
+    const T *xin = x + first, *gin = grad_y + first;
+    T *out = grad_x + first;
+    lo = max(lo, hi);
+    Word<T, V> xw[U], gw[U];
+    if (tile.i & 1) {
+      load_rows<T, V, U, true, false>(xin, at.at, at.rl, rows, a.RL, step, xw);
+      load_rows<T, V, U, true, false>(gin, at.at, at.rl, rows, a.RL, step, gw);
+    }
+    if (!waited) launch_wait();
+    waited = true;
+    if (rows <= 0) continue;
+    if ((tile.i & 1) == 0) {
+      zero_rows<T, V>(out, at.at, at.rl, rows, a.RL, step);
+      continue;
+    }
+    // grad_x = dz * scale - (k1 + (x - mean) * k2)
+    float mean[V], scale[V], shift[V], k1[V], k2[V];
+    const int w0 = (a.weight_rows == 1 ? 0 : l) * a.C + at.cv * V;
+    const long long g0 = ((long long)tile.b * a.L + l) * a.G;
+    params_of<V>(a, a.weight + w0, scale);
+    if (ACT) params_of<V>(a, a.bias + w0, shift);
+#pragma unroll
+    for (int c = 0; c < V; ++c) {
+      const float rstd = __ldg(rstd_in + g0 + group[c]);
+      const float2 m = __ldcg(means + g0 + group[c]);
+      mean[c] = __ldg(mean_in + g0 + group[c]);
+      scale[c] *= rstd;
+      k1[c] = rstd * m.x;
+      k2[c] = rstd * rstd * m.y;
+    }
+    auto store = [&](int u) {
+      float xf[V], gf[V];
+      widen_word<T, V>(xw[u], xf);
+      widen_word<T, V>(gw[u], gf);
+#pragma unroll
+      for (int c = 0; c < V; ++c) {
+        const float centred = xf[c] - mean[c];
+        const float dz = ACT ? activate_grad<ACT>(gf[c], fmaf(centred, scale[c], shift[c]), a.act) : gf[c];
+        xf[c] = fmaf(dz, scale[c], -fmaf(centred, k2[c], k1[c]));
+      }
+      store_word<T, V>(out + u * step + at.at, xf);
+    };
+    int r = 0;
+    for (; r + U * a.RL <= rows; r += U * a.RL, xin += U * step, gin += U * step, out += U * step) {
+      if (r > 0) {
+        load_rows<T, V, U, true, true>(xin, at.at, r, rows, a.RL, step, xw);
+        load_rows<T, V, U, true, true>(gin, at.at, r, rows, a.RL, step, gw);
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u) store(u);
+    }
+    if (r > 0) {
+      load_rows<T, V, U, true, false>(xin, at.at, r + at.rl, rows, a.RL, step, xw);
+      load_rows<T, V, U, true, false>(gin, at.at, r + at.rl, rows, a.RL, step, gw);
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (r + at.rl + u * a.RL < rows) store(u);
+  }
 }
 
 // ------------------------------------------------------------------------------------------------
 // host
 // ------------------------------------------------------------------------------------------------
-constexpr int kCtas = 148 * 4;
+int threads_of(int V) { return V == 4 ? kThreads<4> : V == 2 ? kThreads<2> : kThreads<1>; }
 
-int runs_of(int B, int N, int C) {
-  const int rows_at_once = std::max(1, 256 * 4 / C);                          // about what a CTA reads at a time
-  const long long most = std::max(1, N / (rows_at_once * 4));
-  return (int)std::max(1LL, std::min<long long>({(kCtas + B - 1) / B, most, N}));
+// Rows of a tile: 4 to 32 of a thread, so that a small call spreads over the device and a large one has long-lived CTAs; more where
+// an image would have more than 2048 tiles to merge.
+int tile_rows(int B, int N, int C, int V) {
+  const int RL = threads_of(V) / (C / V);
+  const long long even = ((long long)B * N + 148 * 5 * RL - 1) / (148 * 5 * RL);
+  long long rows = RL * std::max(4LL, std::min(32LL, even));
+  rows = std::max(rows, ((long long)N + 2047) / 2048);
+  return (int)std::min<long long>(rows, N);
 }
 
-struct Shape {
-  GnArgs a;
-  unsigned grid, threads;
-  size_t chan_bytes;
-};
-
-template <int V>
-Shape shape_of(GnArgs a, int B) {
-  Shape s;
+void complete(GnArgs &a, int V) {
   a.cpg = a.C / a.G;
+  a.V = V;
   a.nv = a.C / V;
-  s.threads = a.nv <= 256 ? 256u : (unsigned)((a.nv + 31) / 32 * 32);
-  a.RL = std::max(1, (int)s.threads / a.nv);
-  a.S = runs_of(B, a.N, a.C);
-  s.grid = (unsigned)(a.S * B);
-  s.chan_bytes = (size_t)a.RL * a.C * sizeof(float2);
-  s.a = a;
-  return s;
+  a.RL = threads_of(V) / a.nv;
+  a.R = tile_rows(a.B, a.N, a.C, V);
+  a.tiles = (a.N + a.R - 1) / a.R;
+  a.entries = a.tiles + 2 * a.L + 1;
+  a.whole = a.cpg % V == 0;
+  a.by_r = make_divisor(a.R);
+  a.by_tiles = make_divisor(a.tiles);
+  a.by_nv = make_divisor(a.nv);
+  a.by_groups = make_divisor(a.G);
+  a.by_levels = make_divisor(a.L);
+  a.by_per = make_divisor(a.whole ? a.cpg / V : a.cpg);
+  a.wide_params = a.C % 4 == 0 && ((reinterpret_cast<uintptr_t>(a.weight) | reinterpret_cast<uintptr_t>(a.bias)) & 15) == 0;
+}
+
+// A launch that may begin while the one before it in the sequence runs (`follows`).
+template <typename... P, typename... A>
+cudaError_t launch(void (*kernel)(P...), unsigned grid, int threads, size_t shared, bool follows, cudaStream_t st, A... args) {
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(grid);
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = shared;
+  cfg.stream = st;
+  cfg.attrs = at;
+  cfg.numAttrs = follows ? 1 : 0;
+  return cudaLaunchKernelEx(&cfg, kernel, static_cast<P>(args)...);
+}
+
+#define DFA3D_TRY(call) do { const cudaError_t rc_ = (call); if (rc_ != cudaSuccess) return rc_; } while (0)
+
+unsigned merge_grid(const GnArgs &a) {
+  return (unsigned)(((long long)a.B * a.L * a.G + kMergeThreads / 32 - 1) / (kMergeThreads / 32));
 }
 
 template <typename T, int V>
-cudaError_t forward(const T *x, GnArgs args, int B, T *y, float *mean, float *rstd, void *workspace, cudaStream_t st) {
-  const Shape s = shape_of<V>(args, B);
+cudaError_t forward(const T *x, GnArgs a, T *y, float *mean, float *rstd, void *workspace, cudaStream_t st) {
+  complete(a, V);
   float2 *partial = static_cast<float2 *>(workspace);
-  gn_stats_kernel<T, V><<<s.grid, s.threads, s.chan_bytes, st>>>(x, s.a, partial);
-  gn_apply_kernel<T, V><<<s.grid, s.threads, s.a.G * sizeof(float2), st>>>(x, s.a, partial, y, mean, rstd);
-  return cudaGetLastError();
+  if (!mean) {                                           // nobody keeps them: behind the tiles' parts
+    mean = reinterpret_cast<float *>(partial + (long long)a.B * a.entries * a.G);
+    rstd = mean + (long long)a.B * a.L * a.G;
+  }
+  const unsigned grid = (unsigned)(a.B * a.tiles);
+  DFA3D_TRY(launch(group_stats_kernel<T, V>, grid, kThreads<V>, sizeof(float2) * kThreads<V> * V, false, st, x, a, partial));
+  DFA3D_TRY(launch(group_merge_kernel, merge_grid(a), kMergeThreads, 0, true, st, a, partial, mean, rstd));
+  auto apply = a.act == kNone ? group_apply_kernel<T, V, false> : group_apply_kernel<T, V, true>;
+  return launch(apply, grid, kThreads<V>, 0, true, st, x, a, mean, rstd, y);
 }
 
 template <typename T, int V>
-cudaError_t backward(const T *grad_y, const T *x, GnArgs args, int B, const float *mean, const float *rstd, T *grad_x,
+cudaError_t backward(const T *grad_y, const T *x, GnArgs a, const float *mean, const float *rstd, T *grad_x,
                      float *grad_weight, float *grad_bias, void *workspace, cudaStream_t st) {
-  const Shape s = shape_of<V>(args, B);
-  float2 *by_channel = static_cast<float2 *>(workspace);
-  float2 *by_group = by_channel + (long long)B * (s.a.S + 2 * s.a.L + 1) * s.a.C;
-  gn_grad_stats_kernel<T, V><<<s.grid, s.threads, s.chan_bytes, st>>>(grad_y, x, s.a, mean, rstd, by_channel, by_group);
-  if (grad_x)
-    gn_grad_apply_kernel<T, V><<<s.grid, s.threads, s.a.G * sizeof(float2), st>>>(grad_y, x, s.a, mean, rstd, by_group, grad_x);
-  if (grad_weight)
-    gn_param_kernel<<<dim3((s.a.C + 31) / 32, s.a.weight_rows), 256, 0, st>>>(by_channel, s.a, B, grad_weight, grad_bias);
-  return cudaGetLastError();
+  complete(a, V);
+  const long long pieces = (long long)a.B * a.entries;
+  float2 *by_channel = static_cast<float2 *>(workspace), *by_group = by_channel + pieces * a.C, *means = by_group + pieces * a.G,
+         *by_level = means + (long long)a.B * a.L * a.G;
+  const unsigned grid = (unsigned)(a.B * a.tiles);
+  auto stats = a.act == kNone ? group_grad_stats_kernel<T, V, false> : group_grad_stats_kernel<T, V, true>;
+  auto apply = a.act == kNone ? group_grad_apply_kernel<T, V, false> : group_grad_apply_kernel<T, V, true>;
+  DFA3D_TRY(launch(stats, grid, kThreads<V>, sizeof(float2) * kThreads<V> * V, false, st, grad_y, x, a, mean, rstd, by_channel,
+                   by_group));
+  const unsigned merges = merge_grid(a), channels = grad_weight ? (unsigned)(a.B * a.L * ((a.C + 31) / 32)) : 0;
+  DFA3D_TRY(launch(group_grad_merge_kernel, merges + channels, kMergeThreads, 0, true, st, a, merges, by_group, by_channel, means,
+                   by_level));
+  const int sums = grad_weight ? (a.C * a.weight_rows + kThreads<V> - 1) / kThreads<V> : 0;
+  return launch(apply, sums + (grad_x ? grid : 0), kThreads<V>, 0, true, st, grad_y, x, a, sums, mean, rstd, means, by_level, grad_x,
+                grad_weight, grad_bias);
 }
 
-// Elements a thread reads at a time: as many as divide the channels and as every address is aligned for, up to 16 bytes.
+// Elements a thread reads at a time: as many as divide the channels and as every address is aligned for, up to four.
 int vector_width(int C, size_t size, std::initializer_list<const void *> addresses) {
-  int v = 16 / (int)size;
+  int v = 4;
   while (v > 1) {
     bool ok = C % v == 0;
     for (const void *p : addresses) ok = ok && reinterpret_cast<uintptr_t>(p) % (v * size) == 0;
@@ -503,21 +757,27 @@ int vector_width(int C, size_t size, std::initializer_list<const void *> address
   return v;
 }
 
-GnArgs arguments(int N, int C, int G, const int64_t *shapes, int shape_stride, const int64_t *start, int L, const float *weight,
+GnArgs arguments(int B, int N, int C, int G, const int64_t *shapes, int shape_stride, const int64_t *start, int L, const float *weight,
                  const float *bias, int weight_rows, float eps, int act) {
   GnArgs a = {};
   a.shapes = shapes; a.start = start; a.shape_stride = shape_stride;
-  a.N = N; a.C = C; a.G = G; a.L = L; a.act = act;
+  a.B = B; a.N = N; a.C = C; a.G = G; a.L = L; a.act = act;
   a.weight_rows = weight_rows; a.weight = weight; a.bias = bias; a.eps = eps;
   return a;
 }
 
 }  // namespace
 
+// For any word that a launch may read by.
 long long group_norm_workspace(int B, int N, int C, int G, int L, bool backward) {
   if (B == 0 || N == 0) return 0;
-  const long long pieces = (long long)B * (runs_of(B, N, C) + 2 * L + 1);
-  return pieces * (backward ? C + G : G) * (long long)sizeof(float2);
+  long long pieces = 0;
+  for (int V = 4; V >= 1; V /= 2)
+    if (C % V == 0) {
+      const int R = tile_rows(B, N, C, V);
+      pieces = std::max<long long>(pieces, (long long)B * ((N + R - 1) / R + 2 * L + 1));
+    }
+  return (pieces * (backward ? C + G : G) + (long long)B * L * (backward ? C + G : G)) * (long long)sizeof(float2);
 }
 
 #define DFA3D_GN(fn, v, ...)                                            \
@@ -528,13 +788,11 @@ long long group_norm_workspace(int B, int N, int C, int G, int L, bool backward)
     return fn<T, 1>(__VA_ARGS__);                                       \
   } else if (dtype == 1) {                                              \
     using T = __nv_bfloat16;                                            \
-    if (v == 8) return fn<T, 8>(__VA_ARGS__);                           \
     if (v == 4) return fn<T, 4>(__VA_ARGS__);                           \
     if (v == 2) return fn<T, 2>(__VA_ARGS__);                           \
     return fn<T, 1>(__VA_ARGS__);                                       \
   } else {                                                              \
     using T = __half;                                                   \
-    if (v == 8) return fn<T, 8>(__VA_ARGS__);                           \
     if (v == 4) return fn<T, 4>(__VA_ARGS__);                           \
     if (v == 2) return fn<T, 2>(__VA_ARGS__);                           \
     return fn<T, 1>(__VA_ARGS__);                                       \
@@ -544,18 +802,18 @@ cudaError_t launch_group_norm_forward(const void *x, int dtype, int B, int N, in
                                       int shape_stride, const int64_t *start, int L, const float *weight, const float *bias,
                                       int weight_rows, float eps, int act, void *y, float *mean, float *rstd, void *workspace,
                                       cudaStream_t s) {
-  const GnArgs a = arguments(N, C, G, shapes, shape_stride, start, L, weight, bias, weight_rows, eps, act);
+  const GnArgs a = arguments(B, N, C, G, shapes, shape_stride, start, L, weight, bias, weight_rows, eps, act);
   const int v = vector_width(C, dtype == 0 ? 4 : 2, {x, y});
-  DFA3D_GN(forward, v, (const T *)x, a, B, (T *)y, mean, rstd, workspace, s)
+  DFA3D_GN(forward, v, (const T *)x, a, (T *)y, mean, rstd, workspace, s)
 }
 
 cudaError_t launch_group_norm_backward(const void *grad_y, const void *x, int dtype, int B, int N, int C, int G,
                                        const int64_t *shapes, int shape_stride, const int64_t *start, int L, const float *weight,
                                        const float *bias, int weight_rows, const float *mean, const float *rstd, int act,
                                        void *grad_x, float *grad_weight, float *grad_bias, void *workspace, cudaStream_t s) {
-  const GnArgs a = arguments(N, C, G, shapes, shape_stride, start, L, weight, bias, weight_rows, 0.f, act);
+  const GnArgs a = arguments(B, N, C, G, shapes, shape_stride, start, L, weight, bias, weight_rows, 0.f, act);
   const int v = vector_width(C, dtype == 0 ? 4 : 2, {x, grad_y, grad_x ? grad_x : x});
-  DFA3D_GN(backward, v, (const T *)grad_y, (const T *)x, a, B, mean, rstd, (T *)grad_x, grad_weight, grad_bias, workspace, s)
+  DFA3D_GN(backward, v, (const T *)grad_y, (const T *)x, a, mean, rstd, (T *)grad_x, grad_weight, grad_bias, workspace, s)
 }
 
 }  // namespace dfa3d

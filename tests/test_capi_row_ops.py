@@ -90,6 +90,9 @@ def test_sizes_are_checked(lib):
         refused(lib, call(lib, name, L=0), b"L must be positive")
         refused(lib, call(lib, name, B=-1), b"B and N")
         refused(lib, call(lib, name, N=1 << 30), b"too many", -2)
+        refused(lib, call(lib, name, N=3000, B=1 << 21), b"too many", -2)
+        refused(lib, call(lib, name, N=1, B=1 << 28), b"too many", -2)
+        refused(lib, call(lib, name, N=1, B=1 << 26, workspace=None), b"workspace")
         refused(lib, call(lib, name, weight_rows=3), b"weight_rows")
         refused(lib, call(lib, name, stride=1), b"shape_stride")
         refused(lib, call(lib, name, start=None), b"together")

@@ -153,6 +153,13 @@ def test_larger_calls_and_the_same_bits_again(lib_built, B, N, C, G, dtype):
     assert all(torch.equal(a, b) for a, b in zip(got, again))
 
 
+@pytest.mark.parametrize("B,N,C,G", [(2, 70000, 256, 32), (1, 90000, 200, 25), (1, 150000, 96, 3)])
+def test_images_that_are_cut_into_slabs_of_channels(lib_built, B, N, C, G):
+    """Images too large for one batch of work; the last slab is narrower than the others in one of the directions."""
+    tensors, g = inputs(B, N, C, torch.float32)
+    check(True, tensors, g, G)
+
+
 @BOTH
 @pytest.mark.parametrize("dtype", R.DTYPES, ids=str)
 def test_addresses_off_the_grid_and_strides(lib_built, dtype, native):

@@ -1,5 +1,5 @@
 """How the rows of a feature pyramid are cut up for the group norm (csrc/dfa3d_segments.h), on the CPU: whatever the level table says,
-the segments are disjoint and cover the rows; every row has one run; pieces have numbers of their own."""
+the segments are disjoint and cover the rows, pieces have numbers of their own."""
 import ctypes
 import os
 import random
@@ -18,8 +18,7 @@ extern "C" int segments(const int64_t *shapes, int stride, const int64_t *start,
   for (int i = 0; i < t.count; ++i) end[i] = t.end[i];
   return t.count;
 }
-extern "C" int begin(int s, int S, int N) { return run_begin(s, S, N); }
-extern "C" int run(int r, int S, int N) { return run_of(r, S, N); }
+extern "C" int divided(int n, uint32_t d) { return quotient(n, make_divisor(d)); }
 """
 
 
@@ -78,20 +77,22 @@ def test_any_table_gives_disjoint_ascending_segments(lib):
         assert all(0 <= a <= b for a, b in zip([0] + end, end)) and end[-1] == N
 
 
-def test_runs_cover_the_rows_and_pieces_have_their_own_numbers(lib):
+def test_pieces_have_their_own_numbers(lib):
     rng = random.Random(4)
     for _ in range(300):
-        N = rng.randint(1, 200)
-        S = rng.randint(1, N)
-        for s in range(S):
-            rows = range(lib.begin(s, S, N), lib.begin(s + 1, S, N))
-            assert all(lib.run(r, S, N) == s for r in rows)
-        assert lib.begin(0, S, N) == 0 and lib.begin(S, S, N) == N
-        cuts = sorted(rng.randint(0, N) for _ in range(6))
-        segment = [sum(r >= c for c in cuts) for r in range(N)]
-        pieces = [(lib.run(r, S, N), segment[r]) for r in range(N)]
+        n, R = rng.randint(1, 200), rng.randint(1, 60)
+        cuts = sorted(rng.randint(0, n) for _ in range(6))
+        segment = [sum(r >= c for c in cuts) for r in range(n)]
         numbers = {}
-        for run, seg in pieces:
-            assert numbers.setdefault(run + seg, (run, seg)) == (run, seg)
-            assert run + seg < S + 7
-    assert lib.run((1 << 30) - 2, 592, (1 << 30) - 1) == 591
+        for r in range(n):
+            piece = (lib.divided(r, R), segment[r])
+            assert numbers.setdefault(sum(piece), piece) == piece
+            assert sum(piece) < -(-n // R) + 7
+
+
+def test_division_by_a_number_of_the_host(lib):
+    rng = random.Random(6)
+    numbers = [1, 2, 3, 5, 7, 10, 375, 920, 30825, 2 ** 30 - 1, 2 ** 30, 2 ** 31 - 1]
+    for d in numbers + [rng.randint(1, 2 ** 31 - 1) for _ in range(200)] + [rng.randint(1, 1000) for _ in range(200)]:
+        for n in [0, 1, d - 1, d, min(2 * d - 1, 2 ** 31 - 1), 2 ** 31 - 1] + [rng.randint(0, 2 ** 31 - 1) for _ in range(50)]:
+            assert lib.divided(n, d) == n // d
