@@ -16,6 +16,24 @@ namespace {
 
 constexpr int kThreads = 256;
 
+// Words of elements base + e ... + V - 1, where base is a multiple of 2048 and e below 4096 is one of 4.
+template <int V>
+__device__ __forceinline__ void words_from(const DropRule &d, DropKey k, long long base, unsigned e, uint32_t (&words)[V]) {
+  const unsigned long long block = (unsigned long long)base >> 2;
+  if (!d.rng) {
+#pragma unroll
+    for (int i = 0; i < V; ++i) words[i] = ~0u;
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < V; i += 4) {
+    // no carry: the upper half is the same for the whole CTA, and so is what the first round makes of it
+    const unsigned long long at = (block & 0xffffffff00000000ull) | (uint32_t)((uint32_t)block + ((e + i) >> 2));
+    const PhiloxWords w = philox_words(at, d.site, k);
+    words[i] = w.x; words[i + 1] = w.y; words[i + 2] = w.z; words[i + 3] = w.w;
+  }
+}
+
 // ------------------------------------------------------------------------------------------------
 // elementwise
 // ------------------------------------------------------------------------------------------------
@@ -27,49 +45,50 @@ __device__ __forceinline__ float drop_one(float x, float r, bool kept, float sca
   return kept ? x * scale : 0.f;
 }
 
-// Threads take 16-byte words of every tensor, U of them a CTA width apart, all loads first.  VEC = false: an address is off the
-// 16-byte grid, elements are read and written one by one (same mask, same result).
+// Threads take 16-byte words of every tensor, U of them a CTA width apart, all loads first.  A CTA's elements begin at a multiple of
+// 4096 or 2048, so that the upper half of their block numbers is one value.  VEC = false: an address is off the 16-byte grid,
+// elements are read and written one by one (same mask, same result).
+constexpr int kUnroll = 2;
+
 template <typename T, bool RELU, bool RES, bool VEC>
 __global__ void __launch_bounds__(kThreads)
 dropout_forward_kernel(const T *x, const T *__restrict__ residual, long long n, DropRule d,
                        T *y) {      // y may be x
-  constexpr int V = 16 / sizeof(T), U = 2;
+  constexpr int V = 16 / sizeof(T), U = kUnroll;
   const DropKey key = drop_key(d);
-  const long long words = n / V, first = (long long)blockIdx.x * kThreads * U + threadIdx.x;
-  if (VEC) {
+  const long long base = (long long)blockIdx.x * (kThreads * U * V);
+  if (VEC && base + kThreads * U * V <= n) {
     Word<T, V> xw[U], rw[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const long long w = first + u * kThreads;
-      if (w < words) {
-        xw[u] = load_once<T, V>(x + w * V);
-        if (RES) rw[u] = load_once<T, V>(residual + w * V);
-      }
+      const unsigned e = (u * kThreads + threadIdx.x) * V;
+      xw[u] = load_once<T, V>(x + base + e);
+      if (RES) rw[u] = load_once<T, V>(residual + base + e);
     }
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const long long w = first + u * kThreads;
-      if (w >= words) break;
-      const uint32_t kept = kept_bits<V, true>(d, key, (unsigned long long)w * V);
+      const unsigned e = (u * kThreads + threadIdx.x) * V;
       float f[V], r[V] = {};
       widen_word<T, V>(xw[u], f);
       if (RES) widen_word<T, V>(rw[u], r);
+      uint32_t words[V];
+      words_from<V>(d, key, base, e, words);
 #pragma unroll
-      for (int i = 0; i < V; ++i) f[i] = drop_one<RELU, RES>(f[i], r[i], kept >> i & 1u, d.scale);
-      store_word<T, V>(y + w * V, f);
+      for (int i = 0; i < V; ++i) f[i] = drop_one<RELU, RES>(f[i], r[i], words[i] > d.last, d.scale);
+      store_word<T, V>(y + base + e, f);
     }
+    return;
   }
-  // all elements where VEC is false, the few behind the last word otherwise (by the first CTA)
-  const long long from = VEC ? words * V : 0;
-  if (VEC && blockIdx.x != 0) return;
-  const long long groups = (n - from + 3) / 4, step = VEC ? kThreads : (long long)gridDim.x * kThreads;
-  for (long long q = VEC ? threadIdx.x : (long long)blockIdx.x * kThreads + threadIdx.x; q < groups; q += step) {
-    const long long at = from + q * 4;
-    const uint32_t kept = kept_bits<4, true>(d, key, (unsigned long long)at);
+  for (int q = threadIdx.x; q < kThreads * U * V / 4; q += kThreads) {      // the last CTA, or all of them
+    const long long at = base + q * 4;
+    if (at >= n) return;
+    uint32_t words[4];
+    words_of<4>(d, key, (unsigned long long)at, words);
 #pragma unroll
     for (int i = 0; i < 4; ++i)
       if (at + i < n)
-        y[at + i] = narrow<T>(drop_one<RELU, RES>(wide(x[at + i]), RES ? wide(residual[at + i]) : 0.f, kept >> i & 1u, d.scale));
+        y[at + i] = narrow<T>(drop_one<RELU, RES>(wide(x[at + i]), RES ? wide(residual[at + i]) : 0.f,
+                                                  words[i] > d.last, d.scale));
   }
 }
 
@@ -79,42 +98,41 @@ dropout_forward_kernel(const T *x, const T *__restrict__ residual, long long n, 
 template <typename T, bool REF, bool RNG, bool VEC>
 __global__ void __launch_bounds__(kThreads)
 dropout_backward_kernel(const T *__restrict__ grad_y, const T *__restrict__ ref, long long n, DropRule d, T *__restrict__ grad_x) {
-  constexpr int V = 16 / sizeof(T), U = 2;
+  constexpr int V = 16 / sizeof(T), U = kUnroll;
   const DropKey key = RNG ? drop_key(d) : DropKey{0u, 0u};
   auto one = [&](float g, float v, bool kept) { return !kept || (REF && v <= 0.f) ? 0.f : g * d.scale; };
-  const long long words = n / V, first = (long long)blockIdx.x * kThreads * U + threadIdx.x;
-  if (VEC) {
+  const long long base = (long long)blockIdx.x * (kThreads * U * V);
+  if (VEC && base + kThreads * U * V <= n) {
     Word<T, V> gw[U], vw[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const long long w = first + u * kThreads;
-      if (w < words) {
-        gw[u] = load_once<T, V>(grad_y + w * V);
-        if (REF) vw[u] = load_once<T, V>(ref + w * V);
-      }
+      const unsigned e = (u * kThreads + threadIdx.x) * V;
+      gw[u] = load_once<T, V>(grad_y + base + e);
+      if (REF) vw[u] = load_once<T, V>(ref + base + e);
     }
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const long long w = first + u * kThreads;
-      if (w >= words) break;
-      const uint32_t kept = RNG ? kept_bits<V, true>(d, key, (unsigned long long)w * V) : ~0u;
+      const unsigned e = (u * kThreads + threadIdx.x) * V;
       float g[V], v[V] = {};
       widen_word<T, V>(gw[u], g);
       if (REF) widen_word<T, V>(vw[u], v);
+      uint32_t words[V];
+      if (RNG) words_from<V>(d, key, base, e, words);
 #pragma unroll
-      for (int i = 0; i < V; ++i) g[i] = one(g[i], v[i], kept >> i & 1u);
-      store_word<T, V>(grad_x + w * V, g);
+      for (int i = 0; i < V; ++i) g[i] = one(g[i], v[i], !RNG || words[i] > d.last);
+      store_word<T, V>(grad_x + base + e, g);
     }
+    return;
   }
-  const long long from = VEC ? words * V : 0;
-  if (VEC && blockIdx.x != 0) return;
-  const long long groups = (n - from + 3) / 4, step = VEC ? kThreads : (long long)gridDim.x * kThreads;
-  for (long long q = VEC ? threadIdx.x : (long long)blockIdx.x * kThreads + threadIdx.x; q < groups; q += step) {
-    const long long at = from + q * 4;
-    const uint32_t kept = RNG ? kept_bits<4, true>(d, key, (unsigned long long)at) : ~0u;
+  for (int q = threadIdx.x; q < kThreads * U * V / 4; q += kThreads) {
+    const long long at = base + q * 4;
+    if (at >= n) return;
+    uint32_t words[4];
+    if (RNG) words_of<4>(d, key, (unsigned long long)at, words);
 #pragma unroll
     for (int i = 0; i < 4; ++i)
-      if (at + i < n) grad_x[at + i] = narrow<T>(one(wide(grad_y[at + i]), REF ? wide(ref[at + i]) : 0.f, kept >> i & 1u));
+      if (at + i < n)
+        grad_x[at + i] = narrow<T>(one(wide(grad_y[at + i]), REF ? wide(ref[at + i]) : 0.f, !RNG || words[i] > d.last));
   }
 }
 
@@ -122,12 +140,6 @@ dropout_backward_kernel(const T *__restrict__ grad_y, const T *__restrict__ ref,
 // LayerNorm(residual + dropout(x))
 // ------------------------------------------------------------------------------------------------
 constexpr int kWarps = 8;
-
-__device__ __forceinline__ float warp_sum(float v) {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-  return v;
-}
 
 // V elements from `c` on of a row of E.  VEC: V divides E and the row is aligned for words of V; else one by one, zeros behind
 // the row's end.
@@ -164,59 +176,83 @@ __device__ __forceinline__ void load_param(const float *p, int c, int E, bool wh
   }
 }
 
-// A warp owns a row; lane l holds the groups of V columns l, l + 32, ... (K of them).  The sum is normalised as it stands in
-// 32 bits and is not written: the backward forms it again from the same x and residual, so that storage in 16 bits rounds
-// nothing but y.
-template <typename T, int V, int K, bool VEC>
+// Which of V elements from `first` on are kept.
+template <int V, bool VEC>
+__device__ __forceinline__ void words_at(const DropRule &d, DropKey k, unsigned long long first, uint32_t (&words)[V]) {
+  if constexpr (VEC) words_of<V>(d, k, first, words);
+  else words_of_any(d, k, first, words);
+}
+
+// Sum over the LANES lanes that share a row.
+template <int LANES>
+__device__ __forceinline__ float row_sum(float v) {
+#pragma unroll
+  for (int o = LANES / 2; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+
+// LANES lanes have a row, 32 / LANES rows a warp at a time: lane l holds the groups of V columns l, l + LANES, ... (K of them, 16
+// elements in most widths: enough for the sums over lanes and the loads of weights not to count).  The sum is normalised as it
+// stands in 32 bits and is not written: the backward forms it again from the same x and residual, so that storage in 16 bits
+// rounds nothing but y.
+template <typename T, int V, int K, int LANES, bool VEC>
 __global__ void __launch_bounds__(kWarps * 32)
 dropout_add_layer_norm_kernel(const T *__restrict__ x, const T *__restrict__ residual, const float *__restrict__ gamma,
                               const float *__restrict__ beta, long long rows, int E, DropRule d, float eps, T *__restrict__ y,
                               float *__restrict__ mean_out, float *__restrict__ rstd_out) {
+  constexpr int kRowsAtOnce = 32 / LANES;
   const DropKey key = drop_key(d);
   const float inv_e = 1.f / (float)E;
-  const int lane = threadIdx.x & 31;
-  const long long stride = (long long)gridDim.x * kWarps;
-  for (long long row = (long long)blockIdx.x * kWarps + (threadIdx.x >> 5); row < rows; row += stride) {
+  const int lane = threadIdx.x & (LANES - 1), slot = (threadIdx.x & 31) / LANES;
+  const long long stride = (long long)gridDim.x * kWarps * kRowsAtOnce;
+  for (long long row0 = ((long long)blockIdx.x * kWarps + (threadIdx.x >> 5)) * kRowsAtOnce; row0 < rows; row0 += stride) {
+    const long long row = row0 + slot;
+    const bool live = row < rows;
+    const long long at = (live ? row : row0) * E;
     float v[K][V];
     float s = 0.f;
 #pragma unroll
     for (int j = 0; j < K; ++j) {
-      const int c = (lane + 32 * j) * V;
+      const int c = (lane + LANES * j) * V;
 #pragma unroll
       for (int i = 0; i < V; ++i) v[j][i] = 0.f;
       if (c >= E) continue;
       float xf[V];
-      load_group<T, V, VEC>(x + row * E, c, E, xf);
-      load_group<T, V, VEC>(residual + row * E, c, E, v[j]);
-      const uint32_t kept = kept_bits<V, VEC>(d, key, (unsigned long long)(row * E + c));
+      load_group<T, V, VEC>(x + at, c, E, xf);
+      load_group<T, V, VEC>(residual + at, c, E, v[j]);
+      uint32_t words[V];
+      words_at<V, VEC>(d, key, (unsigned long long)(at + c), words);
 #pragma unroll
       for (int i = 0; i < V; ++i) {
-        v[j][i] = kept >> i & 1u ? fmaf(xf[i], d.scale, v[j][i]) : v[j][i];
+        const float sum = fmaf(xf[i], d.scale, v[j][i]);
+        v[j][i] = words[i] > d.last ? sum : v[j][i];
         s += v[j][i];
       }
     }
-    const float mean = warp_sum(s) * inv_e;
+    const float mean = row_sum<LANES>(s) * inv_e;
     float q = 0.f;
 #pragma unroll
     for (int j = 0; j < K; ++j) {
-      const int c = (lane + 32 * j) * V;
+      const int c = (lane + LANES * j) * V;
 #pragma unroll
       for (int i = 0; i < V; ++i) {
-        const float t = c + i < E ? v[j][i] - mean : 0.f;
+        v[j][i] -= mean;
+        const float t = VEC ? (c < E ? v[j][i] : 0.f) : (c + i < E ? v[j][i] : 0.f);
         q = fmaf(t, t, q);
       }
     }
-    const float rstd = rsqrtf(warp_sum(q) * inv_e + eps);
+    const float rstd = rsqrtf(row_sum<LANES>(q) * inv_e + eps);
+    if (!live) continue;
 #pragma unroll
     for (int j = 0; j < K; ++j) {
-      const int c = (lane + 32 * j) * V;
+      const int c = (lane + LANES * j) * V;
       if (c >= E) continue;
       float g[V], b[V];
       load_param<V>(gamma, c, E, VEC, g);
       load_param<V>(beta, c, E, VEC, b);
 #pragma unroll
-      for (int i = 0; i < V; ++i) g[i] = (v[j][i] - mean) * rstd * g[i] + b[i];
-      store_group<T, V, VEC>(y + row * E, c, E, g);
+      for (int i = 0; i < V; ++i) g[i] = fmaf(v[j][i] * rstd, g[i], b[i]);
+      store_group<T, V, VEC>(y + at, c, E, g);
     }
     if (lane == 0 && mean_out) {
       mean_out[row] = mean;
@@ -225,44 +261,51 @@ dropout_add_layer_norm_kernel(const T *__restrict__ x, const T *__restrict__ res
   }
 }
 
+__device__ __forceinline__ void launch_next() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void launch_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
 // grad_residual = rstd * (d - mean(d) - xhat * mean(d * xhat)) with d = grad_y * gamma; grad_x = keep * grad_residual / (1 - p).
-// grad_gamma (sum of grad_y * xhat) and grad_beta (sum of grad_y) are summed over a warp's rows in registers, over the CTA's
-// warps in shared memory, and written as the CTA's own row of `partial` (ctas, 2, E): the second kernel adds these up in a
-// fixed order, so that a gradient is the same bits in every run.
-template <typename T, int V, int K, bool VEC>
+// grad_gamma (sum of grad_y * xhat) and grad_beta (sum of grad_y) are summed over a lane's rows in registers, over the CTA in
+// shared memory, and written as the CTA's own row of `partial` (ctas, 2, E): the second kernel adds these up in a fixed order, so
+// that a gradient is the same bits in every run.
+template <typename T, int V, int K, int LANES, bool VEC>
 __global__ void __launch_bounds__(kWarps * 32)
 dropout_layer_norm_backward_kernel(const T *__restrict__ grad_y, const T *__restrict__ x, const T *__restrict__ residual,
                                    const float *__restrict__ gamma, const float *__restrict__ mean_in,
                                    const float *__restrict__ rstd_in, long long rows, int E, DropRule d, T *__restrict__ grad_x,
                                    T *__restrict__ grad_residual, float *__restrict__ partial) {
-  __shared__ float part[kWarps][32 * V * K];
+  constexpr int kRowsAtOnce = 32 / LANES, kSlots = kWarps * kRowsAtOnce;
+  __shared__ float part[kSlots * LANES * V * K];
+  launch_next();
   const DropKey key = drop_key(d);
   const float inv_e = 1.f / (float)E;
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const long long stride = (long long)gridDim.x * kWarps;
+  const int lane = threadIdx.x & (LANES - 1), slot = (threadIdx.x & 31) / LANES, warp = threadIdx.x >> 5;
+  const long long stride = (long long)gridDim.x * kSlots;
   float dg[K][V] = {}, db[K][V] = {};
-  for (long long row = (long long)blockIdx.x * kWarps + warp; row < rows; row += stride) {
-    const float mean = __ldg(mean_in + row), rstd = __ldg(rstd_in + row);
+  for (long long row0 = ((long long)blockIdx.x * kWarps + warp) * kRowsAtOnce; row0 < rows; row0 += stride) {
+    const long long row = row0 + slot;
+    const bool live = row < rows;
+    const long long at = (live ? row : row0) * E;
+    const float mean = __ldg(mean_in + (live ? row : row0)), rstd = __ldg(rstd_in + (live ? row : row0));
     float g[K][V], h[K][V];
-    uint32_t kept[K];
+    uint32_t words[K][V];
     float s1 = 0.f, s2 = 0.f;
 #pragma unroll
     for (int j = 0; j < K; ++j) {
-      const int c = (lane + 32 * j) * V;
-      kept[j] = 0;
+      const int c = (lane + LANES * j) * V;
 #pragma unroll
       for (int i = 0; i < V; ++i) g[j][i] = h[j][i] = 0.f;
-      if (c >= E) continue;
+      if (c >= E || !live) continue;
       float xf[V], w[V];
-      load_group<T, V, VEC>(grad_y + row * E, c, E, g[j]);
-      load_group<T, V, VEC>(x + row * E, c, E, xf);
-      load_group<T, V, VEC>(residual + row * E, c, E, h[j]);
+      load_group<T, V, VEC>(grad_y + at, c, E, g[j]);
+      load_group<T, V, VEC>(x + at, c, E, xf);
+      load_group<T, V, VEC>(residual + at, c, E, h[j]);
       load_param<V>(gamma, c, E, VEC, w);
-      kept[j] = kept_bits<V, VEC>(d, key, (unsigned long long)(row * E + c));
+      words_at<V, VEC>(d, key, (unsigned long long)(at + c), words[j]);
 #pragma unroll
       for (int i = 0; i < V; ++i) {
-        const float sum = kept[j] >> i & 1u ? fmaf(xf[i], d.scale, h[j][i]) : h[j][i];
-        h[j][i] = (sum - mean) * rstd;
+        const float sum = fmaf(xf[i], d.scale, h[j][i]);
+        h[j][i] = ((words[j][i] > d.last ? sum : h[j][i]) - mean) * rstd;
         if (!VEC && c + i >= E) h[j][i] = 0.f;
         dg[j][i] = fmaf(g[j][i], h[j][i], dg[j][i]);
         db[j][i] += g[j][i];
@@ -271,62 +314,71 @@ dropout_layer_norm_backward_kernel(const T *__restrict__ grad_y, const T *__rest
         s2 = fmaf(g[j][i], h[j][i], s2);
       }
     }
-    const float c1 = warp_sum(s1) * inv_e, c2 = warp_sum(s2) * inv_e;
+    // by rstd already
+    const float c1 = row_sum<LANES>(s1) * inv_e * rstd, c2 = row_sum<LANES>(s2) * inv_e * rstd;
+    if (!live) continue;
 #pragma unroll
     for (int j = 0; j < K; ++j) {
-      const int c = (lane + 32 * j) * V;
+      const int c = (lane + LANES * j) * V;
       if (c >= E) continue;
 #pragma unroll
-      for (int i = 0; i < V; ++i) g[j][i] = rstd * (g[j][i] - c1 - h[j][i] * c2);
-      if (grad_residual) store_group<T, V, VEC>(grad_residual + row * E, c, E, g[j]);
+      for (int i = 0; i < V; ++i) g[j][i] = fmaf(g[j][i], rstd, -fmaf(h[j][i], c2, c1));
+      if (grad_residual) store_group<T, V, VEC>(grad_residual + at, c, E, g[j]);
 #pragma unroll
-      for (int i = 0; i < V; ++i) g[j][i] = kept[j] >> i & 1u ? g[j][i] * d.scale : 0.f;
-      if (grad_x) store_group<T, V, VEC>(grad_x + row * E, c, E, g[j]);
+      for (int i = 0; i < V; ++i) g[j][i] = words[j][i] > d.last ? g[j][i] * d.scale : 0.f;
+      if (grad_x) store_group<T, V, VEC>(grad_x + at, c, E, g[j]);
     }
   }
   if (!partial) return;
+  constexpr int kWidth = LANES * V * K;
+  float *mine = part + (warp * kRowsAtOnce + slot) * kWidth + lane * V;
 #pragma unroll
   for (int pass = 0; pass < 2; ++pass) {
 #pragma unroll
     for (int j = 0; j < K; ++j)
 #pragma unroll
-      for (int i = 0; i < V; ++i) part[warp][(lane + 32 * j) * V + i] = pass == 0 ? dg[j][i] : db[j][i];
+      for (int i = 0; i < V; ++i) mine[j * LANES * V + i] = pass == 0 ? dg[j][i] : db[j][i];
     __syncthreads();
     for (int c = threadIdx.x; c < E; c += kWarps * 32) {
-      float t = part[0][c];
-#pragma unroll
-      for (int w = 1; w < kWarps; ++w) t += part[w][c];
+      float t = part[c];
+#pragma unroll 8
+      for (int w = 1; w < kSlots; ++w) t += part[w * kWidth + c];
       partial[((long long)blockIdx.x * 2 + pass) * E + c] = t;
     }
     __syncthreads();
   }
 }
 
-// Sums of the CTAs' rows: columns [0, E) of `partial` are grad_gamma, [E, 2E) grad_beta.  32 columns and 8 row lanes a CTA.
-__global__ void __launch_bounds__(256)
-partial_sum_kernel(const float *__restrict__ partial, int ctas, int E, float *__restrict__ grad_gamma, float *__restrict__ grad_beta) {
-  __shared__ float part[8][32];
+// Sums of the CTAs' rows: columns [0, E) of `partial` are grad_gamma, [E, 2E) grad_beta.  32 columns and 32 row lanes a CTA.
+__global__ void __launch_bounds__(1024)
+partial_sum_kernel(const float *partial, int ctas, int E, float *__restrict__ grad_gamma, float *__restrict__ grad_beta) {
+  __shared__ float part[32][32];
   const int lane = threadIdx.x & 31, rl = threadIdx.x >> 5, col = blockIdx.x * 32 + lane;
+  launch_wait();
   float t = 0.f;
   if (col < 2 * E)
 #pragma unroll 8
-    for (int i = rl; i < ctas; i += 8) t += __ldg(partial + (long long)i * 2 * E + col);
+    for (int i = rl; i < ctas; i += 32) t += __ldcg(partial + (long long)i * 2 * E + col);
   part[rl][lane] = t;
   __syncthreads();
   if (rl != 0 || col >= 2 * E) return;
 #pragma unroll
-  for (int i = 1; i < 8; ++i) t += part[i][lane];
+  for (int i = 1; i < 32; ++i) t += part[i][lane];
   (col < E ? grad_gamma + col : grad_beta + col - E)[0] = t;
 }
 
 bool on_grid(const void *p, size_t bytes) { return reinterpret_cast<uintptr_t>(p) % bytes == 0; }
 
 template <typename T>
+unsigned elementwise_grid(long long n) {
+  const long long per_cta = kThreads * kUnroll * (16 / (int)sizeof(T));
+  return (unsigned)((n + per_cta - 1) / per_cta);
+}
+
+template <typename T>
 cudaError_t forward(const T *x, const T *residual, long long n, bool relu, const DropRule &d, T *y, cudaStream_t s) {
-  constexpr int V = 16 / sizeof(T), U = 2;
   const bool vec = on_grid(x, 16) && on_grid(y, 16) && (!residual || on_grid(residual, 16));
-  const long long per_cta = (long long)kThreads * U * V;
-  const unsigned grid = (unsigned)std::min((n + per_cta - 1) / per_cta, (1LL << 31) - 1);
+  const unsigned grid = elementwise_grid<T>(n);
 #define DFA3D_GO(RELU, RES)                                                                                        \
   (vec ? dropout_forward_kernel<T, RELU, RES, true><<<grid, kThreads, 0, s>>>(x, residual, n, d, y)                 \
        : dropout_forward_kernel<T, RELU, RES, false><<<grid, kThreads, 0, s>>>(x, residual, n, d, y))
@@ -343,10 +395,8 @@ cudaError_t forward(const T *x, const T *residual, long long n, bool relu, const
 
 template <typename T>
 cudaError_t backward(const T *grad_y, const T *ref, long long n, bool rng, const DropRule &d, T *grad_x, cudaStream_t s) {
-  constexpr int V = 16 / sizeof(T), U = 2;
   const bool vec = on_grid(grad_y, 16) && on_grid(grad_x, 16) && (!ref || on_grid(ref, 16));
-  const long long per_cta = (long long)kThreads * U * V;
-  const unsigned grid = (unsigned)std::min((n + per_cta - 1) / per_cta, (1LL << 31) - 1);
+  const unsigned grid = elementwise_grid<T>(n);
 #define DFA3D_GO(REF, RNG)                                                                                       \
   (vec ? dropout_backward_kernel<T, REF, RNG, true><<<grid, kThreads, 0, s>>>(grad_y, ref, n, d, grad_x)          \
        : dropout_backward_kernel<T, REF, RNG, false><<<grid, kThreads, 0, s>>>(grad_y, ref, n, d, grad_x))
@@ -361,63 +411,96 @@ cudaError_t backward(const T *grad_y, const T *ref, long long n, bool rng, const
   return cudaGetLastError();
 }
 
-long long row_ctas(long long rows, long long rows_a_warp, long long cap) {
-  return std::max(1LL, std::min((rows + kWarps * rows_a_warp - 1) / (kWarps * rows_a_warp), cap));
+// How a row of E is laid out over lanes: words of V elements, K words a lane.
+struct RowShape {
+  int lanes, K;
+  bool vec;
+};
+template <typename T>
+RowShape row_shape(int E, bool aligned) {
+  constexpr int V = 16 / (int)sizeof(T);
+  if (!aligned || E % V != 0) return {32, E <= 256 ? 2 : 8, false};
+  const int words = E / V, want = 16 / V;            // 16 elements a lane
+  if (words <= 8 * want) return {8, words <= 8 ? 1 : words <= 16 ? 2 : 4, true};
+  if (words <= 16 * want) return {16, want, true};
+  const int K = (words + 31) / 32;
+  return {32, V == 8 || K <= 4 ? K : K <= 6 ? 6 : 8, true};
+}
+// Calls GO(V, K, LANES, VEC) with what `r` says; the K that occur are 1, 2, 4 (fp32) or 1, 2 (16 bits) for 8 lanes, 4 or 2 for 16,
+// 2 to 8 for 32.
+#define DFA3D_ROWS(T, r, GO)                                                                     \
+  if (!r.vec) {                                                                                  \
+    if (r.K == 2) GO(4, 2, 32, false);                                                           \
+    else GO(4, 8, 32, false);                                                                    \
+  } else if constexpr (sizeof(T) == 4) {                                                         \
+    if (r.lanes == 8) {                                                                          \
+      if (r.K == 1) GO(4, 1, 8, true);                                                           \
+      else if (r.K == 2) GO(4, 2, 8, true);                                                      \
+      else GO(4, 4, 8, true);                                                                    \
+    } else if (r.lanes == 16) GO(4, 4, 16, true);                                                \
+    else if (r.K <= 3) GO(4, 3, 32, true);                                                       \
+    else if (r.K == 4) GO(4, 4, 32, true);                                                       \
+    else if (r.K == 6) GO(4, 6, 32, true);                                                       \
+    else GO(4, 8, 32, true);                                                                     \
+  } else {                                                                                       \
+    if (r.lanes == 8) {                                                                          \
+      if (r.K == 1) GO(8, 1, 8, true);                                                           \
+      else GO(8, 2, 8, true);                                                                    \
+    } else if (r.lanes == 16) GO(8, 2, 16, true);                                                \
+    else if (r.K <= 2) GO(8, 2, 32, true);                                                       \
+    else if (r.K == 3) GO(8, 3, 32, true);                                                       \
+    else GO(8, 4, 32, true);                                                                     \
+  }
+
+// CTAs for `rows` rows, a lane group of which takes `each` one after the other, at most `cap`.
+long long row_ctas(long long rows, int lanes, long long each, long long cap) {
+  const long long at_once = kWarps * (32 / lanes) * each;
+  return std::max(1LL, std::min((rows + at_once - 1) / at_once, cap));
 }
 
 template <typename T>
 cudaError_t norm_forward(const T *x, const T *residual, const float *gamma, const float *beta, long long rows, int E,
                          const DropRule &d, float eps, T *y, float *mean, float *rstd, cudaStream_t s) {
-  const bool vec = E % 4 == 0 && on_grid(x, 4 * sizeof(T)) && on_grid(residual, 4 * sizeof(T)) && on_grid(y, 4 * sizeof(T)) &&
-                   on_grid(gamma, 16) && on_grid(beta, 16);
-  const unsigned grid = (unsigned)row_ctas(rows, 1, 148 * 4);
-#define DFA3D_GO(K, VEC)                                                                                                 \
-  dropout_add_layer_norm_kernel<T, 4, K, VEC><<<grid, kWarps * 32, 0, s>>>(x, residual, gamma, beta, rows, E, d, eps, y, \
-                                                                           mean, rstd)
-  const int k = (E + 127) / 128;
-  if (!vec) {
-    if (k <= 2) DFA3D_GO(2, false);
-    else DFA3D_GO(8, false);
-  } else switch (k) {
-    case 1: DFA3D_GO(1, true); break;
-    case 2: DFA3D_GO(2, true); break;
-    case 3: DFA3D_GO(3, true); break;
-    case 4: DFA3D_GO(4, true); break;
-    case 5: case 6: DFA3D_GO(6, true); break;
-    default: DFA3D_GO(8, true);
-  }
+  const RowShape r = row_shape<T>(E, on_grid(x, 16) && on_grid(residual, 16) && on_grid(y, 16) && on_grid(gamma, 16) &&
+                                         on_grid(beta, 16));
+  const unsigned grid = (unsigned)row_ctas(rows, r.lanes, 1, 148 * 8);
+#define DFA3D_GO(V, K, LANES, VEC)                                                                          \
+  dropout_add_layer_norm_kernel<T, V, K, LANES, VEC><<<grid, kWarps * 32, 0, s>>>(x, residual, gamma, beta, rows, E, d, eps, y, \
+                                                                                  mean, rstd)
+  DFA3D_ROWS(T, r, DFA3D_GO)
 #undef DFA3D_GO
   return cudaGetLastError();
 }
 
-long long backward_ctas(long long rows) { return row_ctas(rows, 4, 148 * 3); }
+// Every CTA leaves a row of `partial` to be added up.
+long long backward_ctas(long long rows, int lanes) { return row_ctas(rows, lanes, 1, 148 * 2); }
 
 template <typename T>
 cudaError_t norm_backward(const T *grad_y, const T *x, const T *residual, const float *gamma, const float *mean,
                           const float *rstd, long long rows, int E, const DropRule &d, T *grad_x, T *grad_residual,
                           float *grad_gamma, float *grad_beta, float *partial, cudaStream_t s) {
-  const bool vec = E % 4 == 0 && on_grid(x, 4 * sizeof(T)) && on_grid(residual, 4 * sizeof(T)) &&
-                   on_grid(grad_y, 4 * sizeof(T)) && (!grad_x || on_grid(grad_x, 4 * sizeof(T))) &&
-                   (!grad_residual || on_grid(grad_residual, 4 * sizeof(T))) && on_grid(gamma, 16);
-  const unsigned grid = (unsigned)backward_ctas(rows);
-#define DFA3D_GO(K, VEC)                                                                                        \
-  dropout_layer_norm_backward_kernel<T, 4, K, VEC><<<grid, kWarps * 32, 0, s>>>(                                 \
-      grad_y, x, residual, gamma, mean, rstd, rows, E, d, grad_x, grad_residual, grad_gamma ? partial : nullptr)
-  const int k = (E + 127) / 128;
-  if (!vec) {
-    if (k <= 2) DFA3D_GO(2, false);
-    else DFA3D_GO(8, false);
-  } else switch (k) {
-    case 1: DFA3D_GO(1, true); break;
-    case 2: DFA3D_GO(2, true); break;
-    case 3: DFA3D_GO(3, true); break;
-    case 4: DFA3D_GO(4, true); break;
-    case 5: case 6: DFA3D_GO(6, true); break;
-    default: DFA3D_GO(8, true);
-  }
+  const RowShape r = row_shape<T>(E, on_grid(x, 16) && on_grid(residual, 16) && on_grid(grad_y, 16) && on_grid(gamma, 16) &&
+                                         on_grid(grad_x, 16) && on_grid(grad_residual, 16));      // null is on the grid
+  const unsigned grid = (unsigned)backward_ctas(rows, r.lanes);
+  if (!grad_gamma) partial = nullptr;
+#define DFA3D_GO(V, K, LANES, VEC)                                                                      \
+  dropout_layer_norm_backward_kernel<T, V, K, LANES, VEC><<<grid, kWarps * 32, 0, s>>>(                  \
+      grad_y, x, residual, gamma, mean, rstd, rows, E, d, grad_x, grad_residual, partial)
+  DFA3D_ROWS(T, r, DFA3D_GO)
 #undef DFA3D_GO
-  if (grad_gamma) partial_sum_kernel<<<(2 * E + 31) / 32, 256, 0, s>>>(partial, (int)grid, E, grad_gamma, grad_beta);
-  return cudaGetLastError();
+  cudaError_t rc = cudaGetLastError();
+  if (rc != cudaSuccess || !partial) return rc;
+  // begins while the other's CTAs leave
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((2 * E + 31) / 32);
+  cfg.blockDim = dim3(1024);
+  cfg.stream = s;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, partial_sum_kernel, (const float *)partial, (int)grid, E, grad_gamma, grad_beta);
 }
 
 }  // namespace
@@ -447,7 +530,8 @@ cudaError_t launch_dropout_add_layer_norm(const void *x, const void *residual, c
   DFA3D_TYPED(norm_forward<T>((const T *)x, (const T *)residual, gamma, beta, rows, E, d, eps, (T *)y, mean, rstd, s))
 }
 
-long long dropout_layer_norm_workspace(long long rows, int E) { return rows > 0 ? backward_ctas(rows) * 2 * E * 4 : 0; }
+// For the layout with the fewest rows at a time.
+long long dropout_layer_norm_workspace(long long rows, int E) { return rows > 0 ? backward_ctas(rows, 32) * 2 * E * 4 : 0; }
 
 cudaError_t launch_dropout_layer_norm_backward(const void *grad_y, const void *x, const void *residual, const float *gamma,
                                                const float *mean, const float *rstd, int dtype, long long rows, int E, double p,

@@ -3,8 +3,7 @@
 // Element i of a tensor in row-major order takes word i mod 4 of Philox4x32 at counter (i / 4 low, i / 4 high, site, 0) under the
 // key (seed low, seed high), and is kept where word >= p * 2^32.  The generator is Philox4x32 of Salmon, Moraes, Dror and Shaw,
 // "Parallel random numbers: as easy as 1, 2, 3" (SC 2011), with 7 rounds, the fewest that the authors found to pass all of
-// TestU01's BigCrush: a word costs about 12 instructions of the integer pipes, which keeps a 16-bit dropout at the speed of HBM
-// (with 10 rounds its arithmetic would take as long as its memory traffic).
+// TestU01's BigCrush: a word then costs eight instructions of the integer pipes, and a 16-bit dropout stays near the speed of HBM.
 #pragma once
 #include <stdint.h>
 
@@ -27,7 +26,7 @@ inline DropRule drop_rule(double p, const int64_t *seed, uint32_t site) {
   r.seed = seed;
   r.site = site;
   r.rng = dropped > 0;
-  r.last = (uint32_t)(dropped - 1);
+  r.last = dropped > 0 ? (uint32_t)(dropped - 1) : 0u;
   r.scale = p < 1.0 ? (float)(1.0 / (1.0 - p)) : 0.f;
   return r;
 }
@@ -72,26 +71,32 @@ __device__ __forceinline__ DropKey drop_key(const DropRule &d) {
   return k;
 }
 
-// Which of the elements 4 * block ... 4 * block + 3 are kept, one bit each.
-__device__ __forceinline__ uint32_t kept_of_block(const DropRule &d, DropKey k, unsigned long long block) {
-  const PhiloxWords w = philox_words(block, d.site, k);
-  return (w.x > d.last ? 1u : 0u) | (w.y > d.last ? 2u : 0u) | (w.z > d.last ? 4u : 0u) | (w.w > d.last ? 8u : 0u);
-}
-
-// Which of V consecutive elements from `first` on are kept (V = 4 or 8); `first` a multiple of 4 if ALIGNED.
-template <int V, bool ALIGNED>
-__device__ __forceinline__ uint32_t kept_bits(const DropRule &d, DropKey k, unsigned long long first) {
-  if (!d.rng) return (1u << V) - 1u;
-  const unsigned long long block = first >> 2;
-  uint32_t bits = 0;
+// words[i] is that of element `first` + i, a multiple of 4; above `last` where nothing is dropped.
+template <int V>
+__device__ __forceinline__ void words_of(const DropRule &d, DropKey k, unsigned long long first, uint32_t (&words)[V]) {
+  if (!d.rng) {
 #pragma unroll
-  for (int i = 0; i < V / 4; ++i) bits |= kept_of_block(d, k, block + i) << (4 * i);
-  if (!ALIGNED) {
-    const uint32_t skip = (uint32_t)first & 3u;
-    if (skip) bits |= kept_of_block(d, k, block + V / 4) << V;
-    bits = (bits >> skip) & ((1u << V) - 1u);
+    for (int i = 0; i < V; ++i) words[i] = ~0u;
+    return;
   }
-  return bits;
+#pragma unroll
+  for (int i = 0; i < V; i += 4) {
+    const PhiloxWords w = philox_words((first >> 2) + i / 4, d.site, k);
+    words[i] = w.x; words[i + 1] = w.y; words[i + 2] = w.z; words[i + 3] = w.w;
+  }
+}
+// The same for any `first`; V = 4.
+__device__ __forceinline__ void words_of_any(const DropRule &d, DropKey k, unsigned long long first, uint32_t (&words)[4]) {
+  if (!d.rng) {
+    words[0] = words[1] = words[2] = words[3] = ~0u;
+    return;
+  }
+  const PhiloxWords a = philox_words(first >> 2, d.site, k), b = philox_words((first >> 2) + 1, d.site, k);
+  const uint32_t skip = (uint32_t)first & 3u;
+  words[0] = skip == 0 ? a.x : skip == 1 ? a.y : skip == 2 ? a.z : a.w;
+  words[1] = skip == 0 ? a.y : skip == 1 ? a.z : skip == 2 ? a.w : b.x;
+  words[2] = skip == 0 ? a.z : skip == 1 ? a.w : skip == 2 ? b.x : b.y;
+  words[3] = skip == 0 ? a.w : skip == 1 ? b.x : skip == 2 ? b.y : b.z;
 }
 #endif
 
