@@ -4,7 +4,14 @@
 //   y = LayerNorm(residual + keep * x / (1 - p))                  rows of up to 1024 columns
 //
 // with their backward passes, which form the mask again from (seed, site, element).  Every tensor is read once and written once;
-// what bounds them is HBM, with the integer pipes next: a Philox block for four elements is about 50 instructions.
+// what bounds them is HBM, with the instructions next: a Philox block for four elements is about 30 of them, twelve of which are
+// 32 x 32 -> 64 bit products at half rate.
+//
+// Measured (HBM copy 6528 GB/s): 40 000 x 512 fp32 with ReLU 26 us forward, 38 backward (6.2, 6.5 TB/s); 184 950 x 256 bf16 33.8
+// and 33.7 (5.6 TB/s; 41 before the upper counter word was made one value for a CTA and the kept bits were compared in place).
+// Norm of 40 000 x 256 fp32 23.6 forward, 38.6 backward (5.2, 5.3 TB/s), of 80 000 x 256 bf16 28.3 and 41.6 (4.3, 4.9 TB/s: 30 and
+// 40 instructions an element); 900 x 256 fp32 3.2 and 5.5.  Rows loaded into registers instead of one ahead through shared memory:
+// 26 and 46, 1024 columns 66 and 138 for 49 and 80; a warp a row of four elements a lane 25 and 56, bf16 39 and 86.
 #include <algorithm>
 
 #include "dfa3d_launch.h"
@@ -140,6 +147,8 @@ dropout_backward_kernel(const T *__restrict__ grad_y, const T *__restrict__ ref,
 // LayerNorm(residual + dropout(x))
 // ------------------------------------------------------------------------------------------------
 constexpr int kWarps = 8;
+// CTAs of the forward on an SM.  40 000 x 256 fp32: 23.6 us at three, 25.6 at four, 29.1 at five (spills).
+constexpr int kForwardResident = 3;
 
 // V elements from `c` on of a row of E.  VEC: V divides E and the row is aligned for words of V; else one by one, zeros behind
 // the row's end.
@@ -191,24 +200,59 @@ __device__ __forceinline__ float row_sum(float v) {
   return v;
 }
 
+// A row's words of NT tensors, asked for one row ahead by asynchronous copies: a thread's own words, so that no barrier is
+// needed and the loads of a row take no registers while the row before it is worked on.
+template <typename T, int V, int K, int LANES, int NT>
+struct RowsAhead {
+  static constexpr unsigned kWord = kWarps * 32 * 16, kStage = K * NT * kWord;
+  unsigned mine, stage = 0;
+  __device__ __forceinline__ explicit RowsAhead(void *ring)
+      : mine((unsigned)__cvta_generic_to_shared(ring) + threadIdx.x * 16) {}
+  // `at` elements behind the pointers begins the row; nothing if it is not `live`
+  __device__ __forceinline__ void ask(const T *const (&p)[NT], long long at, int lane, int E, bool live) {
+#pragma unroll
+    for (int j = 0; j < K; ++j) {
+      const int c = (lane + LANES * j) * V;
+      if (live && c < E) {
+#pragma unroll
+        for (int t = 0; t < NT; ++t) copy_async16(mine + stage * kStage + (j * NT + t) * kWord, p[t] + at + c);
+      }
+    }
+    copies_asked();
+    stage ^= 1;
+  }
+  // word j of tensor t of the row that was asked for before the last one
+  __device__ __forceinline__ void read(int j, int t, float (&f)[V]) const {
+    widen_word<T, V>(read_shared16(mine + stage * kStage + (j * NT + t) * kWord), f);
+  }
+};
+
 // LANES lanes have a row, 32 / LANES rows a warp at a time: lane l holds the groups of V columns l, l + LANES, ... (K of them, 16
 // elements in most widths: enough for the sums over lanes and the loads of weights not to count).  The sum is normalised as it
 // stands in 32 bits and is not written: the backward forms it again from the same x and residual, so that storage in 16 bits
 // rounds nothing but y.
 template <typename T, int V, int K, int LANES, bool VEC>
-__global__ void __launch_bounds__(kWarps * 32)
+__global__ void __launch_bounds__(kWarps * 32, K * V <= 16 ? kForwardResident : 1)
 dropout_add_layer_norm_kernel(const T *__restrict__ x, const T *__restrict__ residual, const float *__restrict__ gamma,
                               const float *__restrict__ beta, long long rows, int E, DropRule d, float eps, T *__restrict__ y,
                               float *__restrict__ mean_out, float *__restrict__ rstd_out) {
   constexpr int kRowsAtOnce = 32 / LANES;
-  const DropKey key = drop_key(d);
+  extern __shared__ __align__(16) unsigned char ring[];
   const float inv_e = 1.f / (float)E;
   const int lane = threadIdx.x & (LANES - 1), slot = (threadIdx.x & 31) / LANES;
   const long long stride = (long long)gridDim.x * kWarps * kRowsAtOnce;
-  for (long long row0 = ((long long)blockIdx.x * kWarps + (threadIdx.x >> 5)) * kRowsAtOnce; row0 < rows; row0 += stride) {
-    const long long row = row0 + slot;
+  long long row = ((long long)blockIdx.x * kWarps + (threadIdx.x >> 5)) * kRowsAtOnce + slot;
+  const T *const in[2] = {x, residual};
+  RowsAhead<T, V, K, LANES, 2> ahead(ring);
+  if constexpr (VEC) ahead.ask(in, row * E, lane, E, row < rows);
+  const DropKey key = drop_key(d);
+  for (; row - slot < rows; row += stride) {
     const bool live = row < rows;
-    const long long at = (live ? row : row0) * E;
+    const long long at = row * E;
+    if constexpr (VEC) {
+      ahead.ask(in, at + stride * E, lane, E, row + stride < rows);
+      copies_wait<1>();
+    }
     float v[K][V];
     float s = 0.f;
 #pragma unroll
@@ -216,10 +260,15 @@ dropout_add_layer_norm_kernel(const T *__restrict__ x, const T *__restrict__ res
       const int c = (lane + LANES * j) * V;
 #pragma unroll
       for (int i = 0; i < V; ++i) v[j][i] = 0.f;
-      if (c >= E) continue;
+      if (c >= E || !live) continue;
       float xf[V];
-      load_group<T, V, VEC>(x + at, c, E, xf);
-      load_group<T, V, VEC>(residual + at, c, E, v[j]);
+      if constexpr (VEC) {
+        ahead.read(j, 0, xf);
+        ahead.read(j, 1, v[j]);
+      } else {
+        load_group<T, V, VEC>(x + at, c, E, xf);
+        load_group<T, V, VEC>(residual + at, c, E, v[j]);
+      }
       uint32_t words[V];
       words_at<V, VEC>(d, key, (unsigned long long)(at + c), words);
 #pragma unroll
@@ -259,6 +308,7 @@ dropout_add_layer_norm_kernel(const T *__restrict__ x, const T *__restrict__ res
       rstd_out[row] = rstd;
     }
   }
+  copies_wait<0>();
 }
 
 __device__ __forceinline__ void launch_next() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
@@ -275,18 +325,23 @@ dropout_layer_norm_backward_kernel(const T *__restrict__ grad_y, const T *__rest
                                    const float *__restrict__ rstd_in, long long rows, int E, DropRule d, T *__restrict__ grad_x,
                                    T *__restrict__ grad_residual, float *__restrict__ partial) {
   constexpr int kRowsAtOnce = 32 / LANES, kSlots = kWarps * kRowsAtOnce;
-  __shared__ float part[kSlots * LANES * V * K];
+  extern __shared__ __align__(16) unsigned char ring[];
   launch_next();
-  const DropKey key = drop_key(d);
   const float inv_e = 1.f / (float)E;
   const int lane = threadIdx.x & (LANES - 1), slot = (threadIdx.x & 31) / LANES, warp = threadIdx.x >> 5;
   const long long stride = (long long)gridDim.x * kSlots;
+  long long row = ((long long)blockIdx.x * kWarps + warp) * kRowsAtOnce + slot;
+  const T *const in[3] = {grad_y, x, residual};
+  RowsAhead<T, V, K, LANES, 3> ahead(ring);
+  if constexpr (VEC) ahead.ask(in, row * E, lane, E, row < rows);
+  const DropKey key = drop_key(d);
   float dg[K][V] = {}, db[K][V] = {};
-  for (long long row0 = ((long long)blockIdx.x * kWarps + warp) * kRowsAtOnce; row0 < rows; row0 += stride) {
-    const long long row = row0 + slot;
+  for (; row - slot < rows; row += stride) {
     const bool live = row < rows;
-    const long long at = (live ? row : row0) * E;
-    const float mean = __ldg(mean_in + (live ? row : row0)), rstd = __ldg(rstd_in + (live ? row : row0));
+    const long long at = row * E;
+    if constexpr (VEC) ahead.ask(in, at + stride * E, lane, E, row + stride < rows);
+    const float mean = live ? __ldg(mean_in + row) : 0.f, rstd = live ? __ldg(rstd_in + row) : 0.f;
+    if constexpr (VEC) copies_wait<1>();
     float g[K][V], h[K][V];
     uint32_t words[K][V];
     float s1 = 0.f, s2 = 0.f;
@@ -297,9 +352,15 @@ dropout_layer_norm_backward_kernel(const T *__restrict__ grad_y, const T *__rest
       for (int i = 0; i < V; ++i) g[j][i] = h[j][i] = 0.f;
       if (c >= E || !live) continue;
       float xf[V], w[V];
-      load_group<T, V, VEC>(grad_y + at, c, E, g[j]);
-      load_group<T, V, VEC>(x + at, c, E, xf);
-      load_group<T, V, VEC>(residual + at, c, E, h[j]);
+      if constexpr (VEC) {
+        ahead.read(j, 0, g[j]);
+        ahead.read(j, 1, xf);
+        ahead.read(j, 2, h[j]);
+      } else {
+        load_group<T, V, VEC>(grad_y + at, c, E, g[j]);
+        load_group<T, V, VEC>(x + at, c, E, xf);
+        load_group<T, V, VEC>(residual + at, c, E, h[j]);
+      }
       load_param<V>(gamma, c, E, VEC, w);
       words_at<V, VEC>(d, key, (unsigned long long)(at + c), words[j]);
 #pragma unroll
@@ -330,8 +391,10 @@ dropout_layer_norm_backward_kernel(const T *__restrict__ grad_y, const T *__rest
     }
   }
   if (!partial) return;
+  copies_wait<0>();
+  __syncthreads();                                       // the ring becomes the lanes' sums
   constexpr int kWidth = LANES * V * K;
-  float *mine = part + (warp * kRowsAtOnce + slot) * kWidth + lane * V;
+  float *part = reinterpret_cast<float *>(ring), *mine = part + (warp * kRowsAtOnce + slot) * kWidth + lane * V;
 #pragma unroll
   for (int pass = 0; pass < 2; ++pass) {
 #pragma unroll
@@ -458,18 +521,32 @@ long long row_ctas(long long rows, int lanes, long long each, long long cap) {
   return std::max(1LL, std::min((rows + at_once - 1) / at_once, cap));
 }
 
+// Two rows of a thread's words of `tensors` tensors, or its columns' sums.
+size_t ring_bytes(const RowShape &r, int tensors) { return r.vec ? 2u * r.K * tensors * kWarps * 32 * 16 : 0u; }
+
+// Launches a kernel that may need more shared memory than it gets by itself (a setting of the kernel on the current device).
+template <typename... P, typename... A>
+cudaError_t launch_rows(void (*kernel)(P...), unsigned grid, size_t shared, cudaStream_t s, A... args) {
+  if (shared > 48 * 1024) {
+    const cudaError_t rc = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)shared);
+    if (rc != cudaSuccess) return rc;
+  }
+  kernel<<<grid, kWarps * 32, shared, s>>>(static_cast<P>(args)...);
+  return cudaGetLastError();
+}
+
 template <typename T>
 cudaError_t norm_forward(const T *x, const T *residual, const float *gamma, const float *beta, long long rows, int E,
                          const DropRule &d, float eps, T *y, float *mean, float *rstd, cudaStream_t s) {
   const RowShape r = row_shape<T>(E, on_grid(x, 16) && on_grid(residual, 16) && on_grid(y, 16) && on_grid(gamma, 16) &&
                                          on_grid(beta, 16));
-  const unsigned grid = (unsigned)row_ctas(rows, r.lanes, 1, 148 * 8);
-#define DFA3D_GO(V, K, LANES, VEC)                                                                          \
-  dropout_add_layer_norm_kernel<T, V, K, LANES, VEC><<<grid, kWarps * 32, 0, s>>>(x, residual, gamma, beta, rows, E, d, eps, y, \
-                                                                                  mean, rstd)
+  const unsigned grid = (unsigned)row_ctas(rows, r.lanes, 1, 148 * kForwardResident);
+  const size_t shared = ring_bytes(r, 2);
+#define DFA3D_GO(V, K, LANES, VEC)                                                                                      \
+  return launch_rows(dropout_add_layer_norm_kernel<T, V, K, LANES, VEC>, grid, shared, s, x, residual, gamma, beta, rows, E, d, \
+                     eps, y, mean, rstd)
   DFA3D_ROWS(T, r, DFA3D_GO)
 #undef DFA3D_GO
-  return cudaGetLastError();
 }
 
 // Every CTA leaves a row of `partial` to be added up.
@@ -483,12 +560,13 @@ cudaError_t norm_backward(const T *grad_y, const T *x, const T *residual, const 
                                          on_grid(grad_x, 16) && on_grid(grad_residual, 16));      // null is on the grid
   const unsigned grid = (unsigned)backward_ctas(rows, r.lanes);
   if (!grad_gamma) partial = nullptr;
-#define DFA3D_GO(V, K, LANES, VEC)                                                                      \
-  dropout_layer_norm_backward_kernel<T, V, K, LANES, VEC><<<grid, kWarps * 32, 0, s>>>(                  \
-      grad_y, x, residual, gamma, mean, rstd, rows, E, d, grad_x, grad_residual, partial)
+  cudaError_t rc = cudaSuccess;
+#define DFA3D_GO(V, K, LANES, VEC)                                                                                            \
+  rc = launch_rows(dropout_layer_norm_backward_kernel<T, V, K, LANES, VEC>, grid,                                             \
+                   std::max(ring_bytes(r, 3), sizeof(float) * kWarps * 32 * V * K), s, grad_y, x, residual, gamma, mean, rstd, \
+                   rows, E, d, grad_x, grad_residual, partial)
   DFA3D_ROWS(T, r, DFA3D_GO)
 #undef DFA3D_GO
-  cudaError_t rc = cudaGetLastError();
   if (rc != cudaSuccess || !partial) return rc;
   // begins while the other's CTAs leave
   cudaLaunchAttribute at[1];

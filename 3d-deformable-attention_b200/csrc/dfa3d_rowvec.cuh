@@ -88,4 +88,19 @@ __device__ __forceinline__ void store_word(T *p, const float (&f)[V]) {
   *reinterpret_cast<Word<T, V> *>(p) = narrow_word<T, V>(f);
 }
 
+// A 16-byte copy into shared memory that nobody waits for yet; the thread that asked for it may read it after copies_wait().
+__device__ __forceinline__ void copy_async16(unsigned shared, const void *global) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(shared), "l"(global) : "memory");
+}
+__device__ __forceinline__ void copies_asked() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int LEFT>
+__device__ __forceinline__ void copies_wait() {      // all but the last LEFT groups are there
+  asm volatile("cp.async.wait_group %0;" ::"n"(LEFT) : "memory");
+}
+__device__ __forceinline__ uint4 read_shared16(unsigned shared) {
+  uint4 w;
+  asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(w.x), "=r"(w.y), "=r"(w.z), "=r"(w.w) : "r"(shared) : "memory");
+  return w;
+}
+
 }  // namespace dfa3d
