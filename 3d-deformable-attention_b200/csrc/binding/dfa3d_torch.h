@@ -41,7 +41,8 @@ using torch::autograd::variable_list;
   X(dfa3d_relu_backward_column_sum) X(dfa3d_slice_sum) X(dfa3d_copy_segments)                               \
   X(dfa3d_dropout_forward) X(dfa3d_dropout_backward) X(dfa3d_dropout_add_layer_norm_forward)             \
   X(dfa3d_dropout_add_layer_norm_workspace) X(dfa3d_dropout_add_layer_norm_backward)                     \
-  X(dfa3d_group_norm_workspace) X(dfa3d_group_norm_forward) X(dfa3d_group_norm_backward)
+  X(dfa3d_group_norm_workspace) X(dfa3d_group_norm_forward) X(dfa3d_group_norm_backward)                 \
+  X(dfa3d_relu_dropout_backward_column_sum)
 
 struct Abi {
 #define X(name) decltype(&::name) name = nullptr;
@@ -247,6 +248,30 @@ c10::intrusive_ptr<X> kept(AutogradContext *ctx, variable_list &tensors) {
   }
   return x;
 }
+
+inline const void *vp(const Tensor &t) { return t.defined() ? t.const_data_ptr() : nullptr; }
+inline void *vpm(const Tensor &t) { return t.defined() ? t.mutable_data_ptr() : nullptr; }
+
+inline bool number(PyObject *o, double &v) {
+  if (!PyFloat_CheckExact(o)) return false;
+  v = PyFloat_AS_DOUBLE(o);
+  return true;
+}
+
+// A dropout's seed (one int64 on the device, or None where p is 0), rate and site.
+struct Rule : Kept {
+  double p = 0;
+  int64_t site = 0;
+  bool by_result = false, residual = false;
+  at::ScalarType type = at::kFloat;
+};
+inline bool rule_arguments(PyObject *seed_o, PyObject *p_o, PyObject *site_o, const Tensor &x, Tensor &seed, Rule &r) {
+  if (!number(p_o, r.p) || !(r.p >= 0 && r.p <= 1) || !integer(site_o, r.site) || r.site < 0 || r.site >= (int64_t(1) << 31))
+    return false;
+  if (seed_o == Py_None) return r.p == 0;
+  return plain_tensor(seed_o, seed) && seed.scalar_type() == at::kLong && seed.numel() == 1 && one_device(x, seed);
+}
+inline const int64_t *seed_of(const Tensor &seed) { return static_cast<const int64_t *>(vp(seed)); }
 
 // Gradients of a backward that must not be differentiated again: with create_graph the results get a node that
 // says so when it is reached (torch.autograd.function.once_differentiable does the same).

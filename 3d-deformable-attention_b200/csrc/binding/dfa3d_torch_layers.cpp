@@ -84,6 +84,39 @@ struct LinearFn : torch::autograd::Function<LinearFn> {
   }
 };
 
+// dropout(relu(x W^T + b)): the product with its ReLU, the dropout in place; the sign of the result is both masks in the backward.
+struct LinearReluDropoutFn : torch::autograd::Function<LinearReluDropoutFn> {
+  static Tensor forward(AutogradContext *ctx, const Tensor &x, const Tensor &w, const Tensor &b, const Tensor &seed,
+                        const c10::intrusive_ptr<Rule> &r) {
+    c10::cuda::CUDAGuard guard(x.device());
+    Tensor y = linear_forward(x, w, b, true);
+    check(lib.dfa3d_dropout_forward(vp(y), nullptr, DFA3D_DTYPE_F32, y.numel(), DFA3D_ROW_NONE, r->p, seed_of(seed),
+                                    (int32_t)r->site, vpm(y), stream_of(x)),
+          "dfa3d_dropout_forward");
+    keep(ctx, r, {x, w, y});
+    return y;
+  }
+  static variable_list backward(AutogradContext *ctx, variable_list grads) {
+    const NoAutocast no_autocast(c10::autocast_dispatch_keyset);
+    variable_list v;
+    const auto r = kept<Rule>(ctx, v);
+    const Tensor &x = v[0], &w = v[1], &y = v[2];
+    c10::cuda::CUDAGuard guard(x.device());
+    Tensor g = rows_of(f32(grads[0])), gx, gw, none;
+    if (!aligned(g, 16)) g = g.clone();
+    const Tensor kept_y = aligned(y, 16) ? y : y.clone();
+    void *s = stream_of(g);
+    Tensor masked = at::empty_like(g), gb = empty_f32({g.size(1)}, g);
+    zero_two(gb, Tensor(), s);
+    check(lib.dfa3d_relu_dropout_backward_column_sum(fp(g), fp(kept_y), g.size(0), (int32_t)g.size(1), r->p, fpm(masked), fpm(gb),
+                                                     s),
+          "dfa3d_relu_dropout_backward_column_sum");
+    if (ctx->needs_input_grad(0)) gx = at::mm(masked, w).view(x.sizes());
+    parameter_gradients(masked, rows_of(x), ctx->needs_input_grad(1), false, gw, none);
+    return once({gx, gw, gb, Tensor(), Tensor()}, grads);
+  }
+};
+
 // Two or three Linear layers of one input, run as one with their weights one below the other: y = [y0 | y1 | y2].  One
 // product instead of three each way, one pass over y's gradient for the bias, and the input's gradient is not summed up
 // from parts.
@@ -157,6 +190,22 @@ PyObject *run_linear(PyObject *const *a, Py_ssize_t n, bool relu) {
       c10::cuda::CUDAGuard guard(x.device());
       y = linear_forward(x, w, b, relu);
     }
+  }
+  return THPVariable_Wrap(y);
+}
+
+PyObject *run_linear_relu_dropout(PyObject *const *a, Py_ssize_t n) {
+  // x, weight, bias, seed, p, site
+  if (n != 6 || !plain_mode()) return not_plain();
+  Tensor x, w, b, seed;
+  auto r = c10::make_intrusive<Rule>();
+  if (!float_tensor(a[0], x, -1) || x.dim() < 1 || x.numel() == 0 || !linear_arguments(a + 1, x, w, b) ||
+      !rule_arguments(a[3], a[4], a[5], x, seed, *r) || !seed.defined())
+    return not_plain();
+  Tensor y;
+  {
+    pybind11::gil_scoped_release nogil;
+    y = LinearReluDropoutFn::apply(x, w, b, seed, r);
   }
   return THPVariable_Wrap(y);
 }
@@ -452,6 +501,7 @@ PyObject *run_attn2d(PyObject *const *a, Py_ssize_t n) {
   }
 FAST(linear, run_linear(a, n, false))
 FAST(linear_relu, run_linear(a, n, true))
+FAST(linear_relu_dropout, run_linear_relu_dropout(a, n))
 FAST(joint_linear, run_joint_linear(a, n))
 FAST(add_layer_norm, run_add_layer_norm(a, n))
 FAST(gather_queries, run_gather(a, n))
@@ -465,7 +515,7 @@ FAST(attn2d, run_attn2d(a, n))
 namespace dfa3d_torch {
 #define FAST(name) {#name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_##name)), METH_FASTCALL, nullptr}
 PyMethodDef layer_methods[] = {
-    FAST(linear), FAST(linear_relu), FAST(joint_linear), FAST(add_layer_norm), FAST(gather_queries), FAST(combine_cameras),
+    FAST(linear), FAST(linear_relu), FAST(linear_relu_dropout), FAST(joint_linear), FAST(add_layer_norm), FAST(gather_queries), FAST(combine_cameras),
     FAST(gather_per_camera), FAST(attn2d), {nullptr, nullptr, 0, nullptr},
 };
 #undef FAST

@@ -6,9 +6,6 @@ using namespace dfa3d_torch;
 
 namespace {
 
-const void *vp(const Tensor &t) { return t.defined() ? t.const_data_ptr() : nullptr; }
-void *vpm(const Tensor &t) { return t.defined() ? t.mutable_data_ptr() : nullptr; }
-
 // a gradient as the kernels take it: of the forward's type, contiguous
 Tensor like_forward(const Tensor &g, at::ScalarType type) {
   if (g.scalar_type() == type) return g.contiguous();
@@ -21,27 +18,6 @@ bool stored_tensor(PyObject *o, Tensor &t) { return plain_tensor(o, t) && storag
 bool same_kind(const Tensor &a, const Tensor &b) {
   return a.scalar_type() == b.scalar_type() && a.sizes() == b.sizes() && a.device() == b.device();
 }
-
-bool number(PyObject *o, double &v) {
-  if (!PyFloat_CheckExact(o)) return false;
-  v = PyFloat_AS_DOUBLE(o);
-  return true;
-}
-
-// seed (one int64 on the device, or None where p is 0), p, site
-struct Rule : Kept {
-  double p = 0;
-  int64_t site = 0;
-  bool by_result = false, residual = false;
-  at::ScalarType type = at::kFloat;
-};
-bool rule_arguments(PyObject *seed_o, PyObject *p_o, PyObject *site_o, const Tensor &x, Tensor &seed, Rule &r) {
-  if (!number(p_o, r.p) || !(r.p >= 0 && r.p <= 1) || !integer(site_o, r.site) || r.site < 0 || r.site >= (int64_t(1) << 31))
-    return false;
-  if (seed_o == Py_None) return r.p == 0;
-  return plain_tensor(seed_o, seed) && seed.scalar_type() == at::kLong && seed.numel() == 1 && one_device(x, seed);
-}
-const int64_t *seed_of(const Tensor &seed) { return static_cast<const int64_t *>(vp(seed)); }
 
 // ------------------------------------------------------------------------------------------------
 // dropout

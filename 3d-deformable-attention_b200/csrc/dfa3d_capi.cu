@@ -661,16 +661,27 @@ int dfa3d_add_layer_norm_infer(const float *x, const float *residual, const floa
                 "dfa3d_add_layer_norm_infer launch");
 }
 
-int dfa3d_relu_backward_column_sum(const float *grad_y, const float *y, int64_t rows, int32_t cols, float *grad_in,
-                                   float *dst, void *stream) {
+static int relu_backward(const float *grad_y, const float *y, int64_t rows, int32_t cols, double p, float *grad_in, float *dst,
+                         void *stream, const char *what) {
   if (rows < 0 || cols < 0)
     return fail(DFA3D_ERR_INVALID_ARGUMENT, "rows and cols must be >= 0 (got %lld, %d)", (long long)rows, cols);
   if (cols % 4 != 0) return fail(DFA3D_ERR_UNSUPPORTED, "cols=%d must be a multiple of 4", cols);
+  if (!(p >= 0.0 && p <= 1.0)) return fail(DFA3D_ERR_INVALID_ARGUMENT, "p must be in [0, 1] (got %g)", p);
   if (rows == 0 || cols == 0) return DFA3D_OK;
   REQUIRE_PTR(grad_y); REQUIRE_PTR(y); REQUIRE_PTR(grad_in); REQUIRE_PTR(dst);
   REQUIRE_ALIGNED(grad_y); REQUIRE_ALIGNED(y); REQUIRE_ALIGNED(grad_in); REQUIRE_ALIGNED(dst);
-  return finish(dfa3d::launch_relu_backward(grad_y, y, rows, cols, grad_in, dst, (cudaStream_t)stream),
-                "dfa3d_relu_backward_column_sum launch");
+  const float scale = p < 1.0 ? (float)(1.0 / (1.0 - p)) : 0.f;
+  return finish(dfa3d::launch_relu_backward(grad_y, y, rows, cols, scale, grad_in, dst, (cudaStream_t)stream), what);
+}
+
+int dfa3d_relu_backward_column_sum(const float *grad_y, const float *y, int64_t rows, int32_t cols, float *grad_in,
+                                   float *dst, void *stream) {
+  return relu_backward(grad_y, y, rows, cols, 0.0, grad_in, dst, stream, "dfa3d_relu_backward_column_sum launch");
+}
+
+int dfa3d_relu_dropout_backward_column_sum(const float *grad_y, const float *y, int64_t rows, int32_t cols, double p,
+                                           float *grad_in, float *dst, void *stream) {
+  return relu_backward(grad_y, y, rows, cols, p, grad_in, dst, stream, "dfa3d_relu_dropout_backward_column_sum launch");
 }
 
 int dfa3d_slice_sum(const float *partial, int32_t slices, int32_t out, int32_t in, const float *grad_tail,

@@ -242,8 +242,9 @@ column_sum_kernel(const float *__restrict__ src, long long rows, int cols, float
 
 // Backward of relu(x W^T + b) up to the products: grad_in = y <= 0 ? 0 : grad_y (a NaN lets its gradient pass, as in
 // torch) and its column sums (the bias gradient) in one pass over both operands.  Split and accumulation as in column_sum_kernel.
+// With a dropout behind the ReLU, y is its result, whose zeros are the dropped elements too, and `scale` is 1 / (1 - p).
 __global__ void __launch_bounds__(kCsThreads)
-relu_backward_kernel(const float *grad_y, const float *__restrict__ y, long long rows, int cols,
+relu_backward_kernel(const float *grad_y, const float *__restrict__ y, long long rows, int cols, float scale,
                      float *grad_in, float *__restrict__ dst) {
   __shared__ float4 part[kCsLanes][kCsGroups];
   const int grp = threadIdx.x % kCsGroups, rl = threadIdx.x / kCsGroups;
@@ -263,8 +264,8 @@ relu_backward_kernel(const float *grad_y, const float *__restrict__ y, long long
 #pragma unroll
       for (int u = 0; u < U; ++u)
         if (r + u * step < rows) {
-          const float4 t = make_float4(v[u].x <= 0.f ? 0.f : g[u].x, v[u].y <= 0.f ? 0.f : g[u].y,
-                                       v[u].z <= 0.f ? 0.f : g[u].z, v[u].w <= 0.f ? 0.f : g[u].w);
+          const float4 t = make_float4(v[u].x <= 0.f ? 0.f : g[u].x * scale, v[u].y <= 0.f ? 0.f : g[u].y * scale,
+                                       v[u].z <= 0.f ? 0.f : g[u].z * scale, v[u].w <= 0.f ? 0.f : g[u].w * scale);
           st4(grad_in + (r + u * step) * cols + col, t);
           acc.x += t.x; acc.y += t.y; acc.z += t.z; acc.w += t.w;
         }
@@ -456,15 +457,15 @@ cudaError_t launch_column_sum(const float *src, long long rows, int cols, float 
   return cudaGetLastError();
 }
 
-cudaError_t launch_relu_backward(const float *grad_y, const float *y, long long rows, int cols, float *grad_in, float *dst,
-                                 cudaStream_t s) {
+cudaError_t launch_relu_backward(const float *grad_y, const float *y, long long rows, int cols, float scale, float *grad_in,
+                                 float *dst, cudaStream_t s) {
   if (rows == 0 || cols == 0) return cudaSuccess;
   const unsigned bands = (unsigned)((cols / 4 + kCsGroups - 1) / kCsGroups);
   long long gx = (long long)kSms * 2 / bands;                            // as launch_column_sum
   const long long most = (rows + kCsLanes * 8 - 1) / (kCsLanes * 8);
   if (gx > most) gx = most;
   if (gx < 1) gx = 1;
-  relu_backward_kernel<<<dim3((unsigned)gx, bands, 1), kCsThreads, 0, s>>>(grad_y, y, rows, cols, grad_in, dst);
+  relu_backward_kernel<<<dim3((unsigned)gx, bands, 1), kCsThreads, 0, s>>>(grad_y, y, rows, cols, scale, grad_in, dst);
   return cudaGetLastError();
 }
 

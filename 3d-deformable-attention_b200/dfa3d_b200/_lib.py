@@ -87,6 +87,7 @@ PLAIN_ENTRY_POINTS = {
     "dfa3d_column_sum": [ctypes.c_void_p, _I64, _I32, ctypes.c_void_p, ctypes.c_void_p],
     "dfa3d_add_layer_norm_infer": [ctypes.c_void_p] * 4 + [_I64, _I32, ctypes.c_float] + [ctypes.c_void_p] * 2,
     "dfa3d_relu_backward_column_sum": [ctypes.c_void_p] * 2 + [_I64, _I32] + [ctypes.c_void_p] * 3,
+    "dfa3d_relu_dropout_backward_column_sum": [ctypes.c_void_p] * 2 + [_I64, _I32, ctypes.c_double] + [ctypes.c_void_p] * 3,
     "dfa3d_slice_sum": [ctypes.c_void_p] + [_I32] * 3 + [ctypes.c_void_p] * 2 + [_I32] + [ctypes.c_void_p] * 3,
     "dfa3d_copy_segments": [ctypes.c_void_p] * 3 + [_I32, ctypes.c_void_p],
     "dfa3d_convert_two": [_I32, _I32, _V, _V, _I64, _V, _V, _I64, _V],

@@ -20,6 +20,8 @@ import torch.nn.modules.module as _module
 from torch.autograd.function import Function, once_differentiable
 
 from . import _lib
+from .dropout_ops import CounterDropout, draw_seed, dropout_add_layer_norm
+from .dropout_ops import dropout as _dropout
 
 
 def _stream(t):
@@ -193,6 +195,52 @@ def linear_relu(x, linear, relu):
         if out is not NotImplemented:
             return out
     return relu(linear(x))
+
+
+def _counts(dropout):
+    """Whether a call of `dropout` is the library's dropout at work and nothing else."""
+    return type(dropout) is CounterDropout and dropout.training and dropout.p > 0.0 and runs_forward_only(dropout)
+
+
+def linear_relu_dropout(x, linear, relu, dropout, seed, site):
+    """dropout(relu(linear(x))); as one operation where all three are plain and `dropout` is a CounterDropout: no mask is stored, and
+    the backward has it from the signs of the result.  seed(): the seed of this pass."""
+    if not _counts(dropout):
+        return dropout(linear_relu(x, linear, relu))
+    if _plain_linear(linear) and type(relu) is nn.ReLU and runs_forward_only(relu):
+        out = _lib.native().linear_relu_dropout(x, linear.weight, linear.bias, seed(x.device), float(dropout.p), site)
+        if out is not NotImplemented:
+            return out
+    return _dropout(linear_relu(x, linear, relu), dropout.p, seed(x.device), site)
+
+
+def dropout_sum(x, residual, dropout):
+    """dropout(x) + residual; as one operation where `dropout` is a CounterDropout and both are of one kind."""
+    if _counts(dropout) and x.is_cuda and x.shape == residual.shape and x.dtype == residual.dtype and x.device == residual.device:
+        return _dropout(x, dropout.p, draw_seed(x.device), residual=residual)
+    return dropout(x) + residual
+
+
+def dropout_norm(x, residual, dropout, norm, seed, site):
+    """norm(dropout(x), residual) for an AddLayerNorm; as one operation where `dropout` is a CounterDropout.  seed(): the seed of
+    this pass."""
+    if not _counts(dropout):
+        return norm(dropout(x), residual)
+    if type(norm) is AddLayerNorm and runs_forward_only(norm) and x.shape == residual.shape and x.dtype == residual.dtype:
+        return dropout_add_layer_norm(x, residual, norm.weight, norm.bias, dropout.p, seed(x.device), site, norm.eps)
+    return norm(_dropout(x, dropout.p, seed(x.device), site), residual)
+
+
+class PassSeed:
+    """One seed for the dropouts of a pass, drawn when the first of them asks for it."""
+
+    def __init__(self):
+        self.value = None
+
+    def __call__(self, device):
+        if self.value is None:
+            self.value = draw_seed(device)
+        return self.value
 
 
 def _time_ms(fn, launches=200):

@@ -22,6 +22,8 @@ visible, as packed rows moved by kernels (``rebatch.RebatchPlan``), instead of P
 padded to the longest camera, and the operator is called once for all cameras with their row offsets.
 The layers' norms are ``layer_ops.AddLayerNorm`` (torch LayerNorm parameters; the residual add happens
 inside the norm kernel) and the projections ``layer_ops.Linear`` (bias gradient by a column-sum kernel).
+``counter_dropout=True`` builds the layers with ``CounterDropout`` instead of ``torch.nn.Dropout`` (no stored masks; another
+sequence of them for one torch seed), which the layers then run inside the norm and the feed-forward kernels.
 """
 import math
 
@@ -34,9 +36,15 @@ from .functions import (MultiScaleDeformableAttnFunction_fp32,
                         MultiScale3DDeformableAttnFunction_fp32,
                         MultiScale3DDeformableAttnRaggedFunction_fp32)
 from . import _lib
-from .layer_ops import AddLayerNorm, Linear, joint_linear, linear_relu, runs_forward_only
+from .dropout_ops import CounterDropout
+from .layer_ops import (AddLayerNorm, Linear, PassSeed, dropout_norm, dropout_sum, joint_linear, linear_relu,
+                        linear_relu_dropout, runs_forward_only)
 from .rebatch import (CombineCamerasFunction, GatherQueriesFunction, GatherSharedRowsFunction, RebatchPlan,
                       gather_per_camera)
+
+
+def _dropout_module(p, counter):
+    return CounterDropout(p) if counter else nn.Dropout(p)
 
 
 def bev_reference_points(bev_h, bev_w, pillar_height=8, num_points_in_pillar=4, dim="3d", bs=1,
@@ -244,7 +252,7 @@ class SpatialCrossAttention_DFA3D(nn.Module):
     """BEV queries attend to the cameras that see them (spatial_cross_attention.py:616-751)."""
 
     def __init__(self, embed_dims=256, num_cams=6, dropout=0.1, deformable_attention=None,
-                 bev_h=200, bev_w=200, num_head=8, use_empty=False):
+                 bev_h=200, bev_w=200, num_head=8, use_empty=False, counter_dropout=False):
         super().__init__()
         self.embed_dims, self.num_cams = embed_dims, num_cams
         self.bev_h, self.bev_w, self.num_head, self.use_empty = bev_h, bev_w, num_head, use_empty
@@ -252,7 +260,7 @@ class SpatialCrossAttention_DFA3D(nn.Module):
         if not use_empty:
             self.deformable_attention.compute_weight_update = False
         self.output_proj = Linear(embed_dims, embed_dims)
-        self.dropout = nn.Dropout(dropout)
+        self.dropout = _dropout_module(dropout, counter_dropout)
         if use_empty:
             self.empty_query = nn.Embedding(bev_h * bev_w * num_head, embed_dims)
         nn.init.xavier_uniform_(self.output_proj.weight)
@@ -269,7 +277,7 @@ class SpatialCrossAttention_DFA3D(nn.Module):
         row count back from the device once.  ``dist_map=(h, w)``: value_dpt_dist is one h x w map per
         camera, (num_cams, h*w, bs, D), read by all levels with nearest indexing.  Returns (bs, Q, E);
         with ``return_residual`` the two summands (attention branch, residual) separately, for a norm that
-        adds them itself."""
+        adds them itself (``return_residual="undropped"``: the branch before its dropout)."""
         inp_residual = query if residual is None else residual
         if query_pos is not None:
             query = query + query_pos
@@ -304,8 +312,10 @@ class SpatialCrossAttention_DFA3D(nn.Module):
                 self.empty_query.weight.view(self.bev_h * self.bev_w, self.num_head * E), plan)
             out_rows = out_rows + ((1 - update_weight) * empty.view(-1, self.num_head, E)).mean(-2)
         slots = CombineCamerasFunction.apply(out_rows, plan)                      # sum over cameras / count
-        slots = self.dropout(self.output_proj(slots))
-        return (slots, inp_residual) if return_residual else slots + inp_residual
+        slots = self.output_proj(slots)
+        if return_residual == "undropped":
+            return slots, inp_residual
+        return (self.dropout(slots), inp_residual) if return_residual else dropout_sum(slots, inp_residual, self.dropout)
 
 
 def _attention_2d(value, query, module, reference_points, spatial_shapes, level_start_index, maps):
@@ -332,7 +342,7 @@ class TemporalSelfAttention(nn.Module):
     (``MultiScaleDeformableAttnFunction_fp32``); the reference takes it from the mmcv extension."""
 
     def __init__(self, embed_dims=256, num_heads=8, num_levels=4, num_points=4, num_bev_queue=2,
-                 im2col_step=64, dropout=0.1, batch_first=True):
+                 im2col_step=64, dropout=0.1, batch_first=True, counter_dropout=False):
         super().__init__()
         if embed_dims % num_heads != 0:
             raise ValueError(f"embed_dims must be divisible by num_heads, but got {embed_dims} and "
@@ -340,7 +350,7 @@ class TemporalSelfAttention(nn.Module):
         self.embed_dims, self.num_heads = embed_dims, num_heads
         self.num_levels, self.num_points, self.num_bev_queue = num_levels, num_points, num_bev_queue
         self.im2col_step, self.batch_first = im2col_step, batch_first
-        self.dropout = nn.Dropout(dropout)
+        self.dropout = _dropout_module(dropout, counter_dropout)
         self.sampling_offsets = Linear(embed_dims * num_bev_queue,
                                           num_bev_queue * num_heads * num_levels * num_points * 2)
         self.attention_weights = Linear(embed_dims * num_bev_queue,
@@ -371,7 +381,7 @@ class TemporalSelfAttention(nn.Module):
         element, or None (then the current queries stand for both, :180-184); reference_points
         (bs*num_bev_queue, Q, num_levels, 2); spatial_shapes (L, 2); level_start_index (L).
         Returns (bs, Q, E)  -- :130-272; with ``return_residual`` the attention branch and the identity
-        separately."""
+        separately (``return_residual="undropped"``: the branch before its dropout)."""
         if self.num_bev_queue != 2:
             raise ValueError("the BEV queue holds the previous and the current BEV: num_bev_queue == 2")
         if value is None:
@@ -400,8 +410,9 @@ class TemporalSelfAttention(nn.Module):
         out = self.output_proj(out)
         if not self.batch_first:
             out = out.permute(1, 0, 2)
-        out = self.dropout(out)
-        return (out, identity) if return_residual else out + identity
+        if return_residual == "undropped":
+            return out, identity
+        return (self.dropout(out), identity) if return_residual else dropout_sum(out, identity, self.dropout)
 
     def _attention_in_steps(self, value, offsets, logits, reference_points, spatial_shapes, level_start_index):
         """:205-262 one operation after the other, for what `_attention_2d` does not cover."""
@@ -438,24 +449,48 @@ def _run_ffn(ffn, x):
     return x
 
 
+def _ffn_norm(ffn, norm, x, seed):
+    """``norm(ffn(x), x)``; where the block is the layers' own with CounterDropouts, the first dropout is run with the first
+    product and the second one inside the norm."""
+    if type(ffn) is not nn.Sequential or len(ffn) != 5 or not runs_forward_only(ffn) or type(ffn[2]) is not CounterDropout \
+            or type(ffn[4]) is not CounterDropout:
+        return norm(_run_ffn(ffn, x), x)
+    h = linear_relu_dropout(x, ffn[0], ffn[1], ffn[2], seed, 2)
+    return dropout_norm(ffn[3](h), x, ffn[4], norm, seed, 3)
+
+
+def _attention_norm(attention, norm, own, seed, site, query, **kw):
+    """``norm(*attention(query, return_residual=True))``; where the attention is the class `own` with a CounterDropout, its dropout
+    is run inside the norm."""
+    if type(attention) is own and type(attention.dropout) is CounterDropout and runs_forward_only(attention):
+        branch, residual = attention(query, return_residual="undropped", **kw)
+        return dropout_norm(branch, residual, attention.dropout, norm, seed, site)
+    return norm(*attention(query, return_residual=True, **kw))
+
+
+def _ffn(embed_dims, ffn_dims, dropout, counter_dropout):
+    return nn.Sequential(Linear(embed_dims, ffn_dims), nn.ReLU(inplace=True), _dropout_module(dropout, counter_dropout),
+                         Linear(ffn_dims, embed_dims), _dropout_module(dropout, counter_dropout))
+
+
 class SCAEncoderLayer(nn.Module):
     """cross-attention -> LayerNorm -> FFN -> LayerNorm (encoder.py:389-411 operation order without the
     temporal self-attention, which uses a different, 2-D operator)."""
 
     def __init__(self, embed_dims=256, ffn_dims=512, num_cams=6, num_heads=8, num_levels=4, num_points=8,
-                 dropout=0.1):
+                 dropout=0.1, counter_dropout=False):
         super().__init__()
         self.cross_attn = SpatialCrossAttention_DFA3D(
             embed_dims, num_cams, dropout,
-            MSDeformableAttention3D_DFA3D(embed_dims, num_heads, num_levels, num_points))
+            MSDeformableAttention3D_DFA3D(embed_dims, num_heads, num_levels, num_points), counter_dropout=counter_dropout)
         self.norm1 = AddLayerNorm(embed_dims)
-        self.ffn = nn.Sequential(Linear(embed_dims, ffn_dims), nn.ReLU(inplace=True), nn.Dropout(dropout),
-                                 Linear(ffn_dims, embed_dims), nn.Dropout(dropout))
+        self.ffn = _ffn(embed_dims, ffn_dims, dropout, counter_dropout)
         self.norm2 = AddLayerNorm(embed_dims)
 
     def forward(self, query, **kw):
-        query = self.norm1(*self.cross_attn(query, return_residual=True, **kw))     # norm(branch + residual)
-        return self.norm2(_run_ffn(self.ffn, query), query)
+        seed = PassSeed()
+        query = _attention_norm(self.cross_attn, self.norm1, SpatialCrossAttention_DFA3D, seed, 1, query, **kw)
+        return _ffn_norm(self.ffn, self.norm2, query, seed)
 
 
 class CustomMSDeformableAttention(nn.Module):
@@ -464,7 +499,7 @@ class CustomMSDeformableAttention(nn.Module):
     the reference: query (Q, bs, E), value (N, bs, E)."""
 
     def __init__(self, embed_dims=256, num_heads=8, num_levels=4, num_points=4, im2col_step=64, dropout=0.1,
-                 batch_first=False):
+                 batch_first=False, counter_dropout=False):
         super().__init__()
         if embed_dims % num_heads != 0:
             raise ValueError(f"embed_dims must be divisible by num_heads, but got {embed_dims} and "
@@ -472,7 +507,7 @@ class CustomMSDeformableAttention(nn.Module):
         self.embed_dims, self.num_heads = embed_dims, num_heads
         self.num_levels, self.num_points = num_levels, num_points
         self.im2col_step, self.batch_first = im2col_step, batch_first
-        self.dropout = nn.Dropout(dropout)
+        self.dropout = _dropout_module(dropout, counter_dropout)
         self.sampling_offsets = Linear(embed_dims, num_heads * num_levels * num_points * 2)
         self.attention_weights = Linear(embed_dims, num_heads * num_levels * num_points)
         self.value_proj = Linear(embed_dims, embed_dims)
@@ -521,7 +556,7 @@ class CustomMSDeformableAttention(nn.Module):
         out = self.output_proj(out)
         if not self.batch_first:
             out = out.permute(1, 0, 2)
-        return self.dropout(out) + identity
+        return dropout_sum(out, identity, self.dropout)
 
     def _attention_in_steps(self, value, offsets, logits, reference_points, spatial_shapes, level_start_index):
         """:283-318 one operation after the other, for what `_attention_2d` does not cover."""
@@ -548,20 +583,19 @@ class BEVFormerEncoderLayer(nn.Module):
     by encoder.py:363-411; post-norm, so every block adds its own input as the residual)."""
 
     def __init__(self, embed_dims=256, ffn_dims=512, num_cams=6, num_heads=8, num_levels=4, num_points=8,
-                 bev_h=200, bev_w=200, dropout=0.1):
+                 bev_h=200, bev_w=200, dropout=0.1, counter_dropout=False):
         super().__init__()
         self.bev_h, self.bev_w = bev_h, bev_w
         self._tables = {}
         self.self_attn = TemporalSelfAttention(embed_dims, num_heads, num_levels=1, num_points=4,
-                                               dropout=dropout)
+                                               dropout=dropout, counter_dropout=counter_dropout)
         self.norm0 = AddLayerNorm(embed_dims)
         self.cross_attn = SpatialCrossAttention_DFA3D(
             embed_dims, num_cams, dropout,
             MSDeformableAttention3D_DFA3D(embed_dims, num_heads, num_levels, num_points), bev_h=bev_h,
-            bev_w=bev_w, num_head=num_heads)
+            bev_w=bev_w, num_head=num_heads, counter_dropout=counter_dropout)
         self.norm1 = AddLayerNorm(embed_dims)
-        self.ffn = nn.Sequential(Linear(embed_dims, ffn_dims), nn.ReLU(inplace=True), nn.Dropout(dropout),
-                                 Linear(ffn_dims, embed_dims), nn.Dropout(dropout))
+        self.ffn = _ffn(embed_dims, ffn_dims, dropout, counter_dropout)
         self.norm2 = AddLayerNorm(embed_dims)
 
     def _bev_tables(self, device, dtype):
@@ -596,10 +630,11 @@ class BEVFormerEncoderLayer(nn.Module):
         shapes, lsi, cells = self._bev_tables(query.device, query.dtype)
         if ref_2d is None:
             ref_2d = cells.expand(query.shape[0] * 2, -1, -1, -1)
-        query = self.norm0(*self.self_attn(query, value=prev_bev, query_pos=bev_pos, reference_points=ref_2d,
-                                           spatial_shapes=shapes, level_start_index=lsi, return_residual=True))
-        query = self.norm1(*self.cross_attn(query, return_residual=True, **cross_kw))
-        return self.norm2(_run_ffn(self.ffn, query), query)
+        seed = PassSeed()
+        query = _attention_norm(self.self_attn, self.norm0, TemporalSelfAttention, seed, 0, query, value=prev_bev,
+                                query_pos=bev_pos, reference_points=ref_2d, spatial_shapes=shapes, level_start_index=lsi)
+        query = _attention_norm(self.cross_attn, self.norm1, SpatialCrossAttention_DFA3D, seed, 1, query, **cross_kw)
+        return _ffn_norm(self.ffn, self.norm2, query, seed)
 
 
 class SCAEncoderStack(nn.Module):

@@ -378,6 +378,11 @@ int dfa3d_add_layer_norm_infer(const float *x, const float *residual, const floa
 int dfa3d_relu_backward_column_sum(const float *grad_y, const float *y, int64_t rows, int32_t cols, float *grad_in,
                                    float *dst, void *stream);
 
+/* The same behind a dropout of rate p: y = dropout(relu(x W^T + b)) (dfa3d_dropout_forward), grad_in = y <= 0 ? 0 :
+ * grad_y / (1 - p).  The zeros of y are the dropped elements too. */
+int dfa3d_relu_dropout_backward_column_sum(const float *grad_y, const float *y, int64_t rows, int32_t cols, double p,
+                                           float *grad_in, float *dst, void *stream);
+
 /* dst (out, in) = sum of `slices` partial products partial (slices, out, in) + grad_tail^T x_tail, with grad_tail
  * (tail_rows, out) and x_tail (tail_rows, in): the end of a weight gradient that was formed as a batch of row slices.
  * zeroed (out), if given, is set to 0 (a bias gradient to be accumulated next).  in a multiple of 4; partial, dst and
