@@ -103,16 +103,16 @@ struct Place {
   }
 };
 
-// The tile of a CTA: rows [r0, r1) of image b, the first of its segments.
+// The tile of a CTA: rows [r0, r1) of image b; the segment that its first row belongs to, or its last one.
 struct Tile {
   int b, t, r0, r1, i;
-  __device__ __forceinline__ Tile(const GnArgs &a, const SegmentTable &seg, int index) {
-    b = quotient(index, a.by_tiles);
-    t = index - b * a.tiles;
+  __device__ __forceinline__ Tile(const GnArgs &a, const SegmentTable &seg, bool last) {
+    b = quotient(blockIdx.x, a.by_tiles);
+    t = blockIdx.x - b * a.tiles;
     r0 = t * a.R;
     r1 = min(a.N, r0 + a.R);
     i = 0;
-    while (seg.end[i] <= r0) ++i;
+    while (seg.end[i] <= (last ? r1 - 1 : r0)) ++i;
   }
 };
 
@@ -202,7 +202,7 @@ group_stats_kernel(const T *__restrict__ x, const GnArgs a, float2 *__restrict__
   __shared__ SegmentTable seg;
   launch_next();
   make_table(seg, a);
-  Tile tile(a, seg, blockIdx.x);
+  Tile tile(a, seg, false);
   const Place at(a);
   const long long step = (long long)a.RL * a.C;
   // a thread's channels are of one group where V divides it: one entry for all of them, or one for each
@@ -341,7 +341,7 @@ group_merge_kernel(const GnArgs a, const float2 *partial, float *__restrict__ me
   }
 }
 
-// y = act((x - mean) * rstd * weight + bias).  Tiles are taken from the last one on: what the statistics read last is still in L2.
+// y = act((x - mean) * rstd * weight + bias).  A tile is walked from its end: what the statistics read last is still in L2.
 template <typename T, int V, bool ACT>
 __global__ void __launch_bounds__(kThreads<V>, kResident<T, V>)
 group_apply_kernel(const T *__restrict__ x, const GnArgs a, const float *mean_in, const float *rstd_in, T *__restrict__ y) {
@@ -349,26 +349,29 @@ group_apply_kernel(const T *__restrict__ x, const GnArgs a, const float *mean_in
   __shared__ SegmentTable seg;
   launch_next();
   make_table(seg, a);
-  Tile tile(a, seg, (int)(gridDim.x - 1 - blockIdx.x));
+  Tile tile(a, seg, true);
   const Place at(a);
   const long long step = (long long)a.RL * a.C;
+  const int chunk = U * a.RL;
   int group[V];
   groups_of<V>(a, at.cv, group);
   bool waited = false;
-  for (int lo = tile.r0; lo < tile.r1; ++tile.i) {
-    const int hi = min(tile.r1, seg.end[tile.i]), rows = at.rl < a.RL ? hi - lo : 0, l = tile.i >> 1;
-    const long long first = ((long long)tile.b * a.N + lo) * a.C;
+  for (int hi = tile.r1; hi > tile.r0; --tile.i) {
+    const int lo = max(tile.r0, segment_begin(seg, tile.i)), all = hi - lo, rows = at.rl < a.RL ? all : 0, l = tile.i >> 1;
+    if (all <= 0) continue;
+    hi = lo;
+    int r = (all - 1) / chunk * chunk;                   // the last chunk of rows, which may be a short one
+    const long long first = ((long long)tile.b * a.N + lo + r) * a.C;
     const T *in = x + first;
     T *out = y + first;
-    lo = max(lo, hi);
     Word<T, V> w[U];
     // on its way before the statistics are there
-    if (tile.i & 1) load_rows<T, V, U, true, false>(in, at.at, at.rl, rows, a.RL, step, w);
+    if (tile.i & 1) load_rows<T, V, U, true, false>(in, at.at, r + at.rl, rows, a.RL, step, w);
     if (!waited) launch_wait();
     waited = true;
     if (rows <= 0) continue;
     if ((tile.i & 1) == 0) {
-      zero_rows<T, V>(out, at.at, at.rl, rows, a.RL, step);
+      zero_rows<T, V>(out - (long long)r * a.C, at.at, at.rl, rows, a.RL, step);
       continue;
     }
     float mean[V], scale[V], shift[V];
@@ -386,18 +389,18 @@ group_apply_kernel(const T *__restrict__ x, const GnArgs a, const float *mean_in
       widen_word<T, V>(w[u], f);
 #pragma unroll
       for (int c = 0; c < V; ++c) f[c] = activate<ACT>(fmaf(f[c] - mean[c], scale[c], shift[c]), a.act);
-      store_word<T, V>(out + u * step + at.at, f);
+      store_once<T, V>(out + u * step + at.at, f);
     };
-    int r = 0;
-    for (; r + U * a.RL <= rows; r += U * a.RL, in += U * step, out += U * step) {
-      if (r > 0) load_rows<T, V, U, true, true>(in, at.at, r, rows, a.RL, step, w);
-#pragma unroll
-      for (int u = 0; u < U; ++u) store(u);
-    }
-    if (r > 0) load_rows<T, V, U, true, false>(in, at.at, r + at.rl, rows, a.RL, step, w);
 #pragma unroll
     for (int u = 0; u < U; ++u)
       if (r + at.rl + u * a.RL < rows) store(u);
+    for (r -= chunk; r >= 0; r -= chunk) {
+      in -= U * step;
+      out -= U * step;
+      load_rows<T, V, U, true, true>(in, at.at, r, rows, a.RL, step, w);
+#pragma unroll
+      for (int u = 0; u < U; ++u) store(u);
+    }
   }
 }
 
@@ -415,7 +418,7 @@ group_grad_stats_kernel(const T *__restrict__ grad_y, const T *__restrict__ x, c
   __shared__ SegmentTable seg;
   launch_next();
   make_table(seg, a);
-  Tile tile(a, seg, blockIdx.x);
+  Tile tile(a, seg, false);
   const Place at(a);
   const long long step = (long long)a.RL * a.C;
   int group[V];
@@ -570,43 +573,47 @@ __device__ __forceinline__ void parameter_sums(const GnArgs &a, const float2 *by
   grad_weight[column] = s.y;
 }
 
-// grad_x = rstd * (d - mean(d) - xhat * mean(d * xhat)), d = dz * gamma, means over the group; the first `sums` CTAs form the
-// parameters' gradients instead, beside the others.
+// grad_x = rstd * (d - mean(d) - xhat * mean(d * xhat)), d = dz * gamma, means over the group; the CTAs beyond its
+// `tiles` form the parameters' gradients.
 template <typename T, int V, bool ACT>
 __global__ void __launch_bounds__(kThreads<V>, kResident<T, V>)
-group_grad_apply_kernel(const T *__restrict__ grad_y, const T *__restrict__ x, const GnArgs a, int sums,
+group_grad_apply_kernel(const T *__restrict__ grad_y, const T *__restrict__ x, const GnArgs a, int tiles,
                         const float *__restrict__ mean_in, const float *__restrict__ rstd_in, const float2 *means,
                         const float2 *by_level, T *__restrict__ grad_x, float *grad_weight, float *grad_bias) {
   constexpr int U = kGradAhead;
   __shared__ SegmentTable seg;
-  if ((int)blockIdx.x < sums) {
+  const int beyond = (int)blockIdx.x - tiles;
+  if (beyond >= 0) {
     launch_wait();
-    parameter_sums(a, by_level, blockIdx.x * kThreads<V> + threadIdx.x, grad_weight, grad_bias);
+    parameter_sums(a, by_level, beyond * kThreads<V> + threadIdx.x, grad_weight, grad_bias);
     return;
   }
   make_table(seg, a);
-  Tile tile(a, seg, (int)(gridDim.x - 1 - blockIdx.x));
+  Tile tile(a, seg, true);
   const Place at(a);
   const long long step = (long long)a.RL * a.C;
+  const int chunk = U * a.RL;
   int group[V];
   groups_of<V>(a, at.cv, group);
   bool waited = false;
-  for (int lo = tile.r0; lo < tile.r1; ++tile.i) {
-    const int hi = min(tile.r1, seg.end[tile.i]), rows = at.rl < a.RL ? hi - lo : 0, l = tile.i >> 1;
-    const long long first = ((long long)tile.b * a.N + lo) * a.C;
+  for (int hi = tile.r1; hi > tile.r0; --tile.i) {
+    const int lo = max(tile.r0, segment_begin(seg, tile.i)), all = hi - lo, rows = at.rl < a.RL ? all : 0, l = tile.i >> 1;
+    if (all <= 0) continue;
+    hi = lo;
+    int r = (all - 1) / chunk * chunk;
+    const long long first = ((long long)tile.b * a.N + lo + r) * a.C;
     const T *xin = x + first, *gin = grad_y + first;
     T *out = grad_x + first;
-    lo = max(lo, hi);
     Word<T, V> xw[U], gw[U];
     if (tile.i & 1) {
-      load_rows<T, V, U, true, false>(xin, at.at, at.rl, rows, a.RL, step, xw);
-      load_rows<T, V, U, true, false>(gin, at.at, at.rl, rows, a.RL, step, gw);
+      load_rows<T, V, U, true, false>(xin, at.at, r + at.rl, rows, a.RL, step, xw);
+      load_rows<T, V, U, true, false>(gin, at.at, r + at.rl, rows, a.RL, step, gw);
     }
     if (!waited) launch_wait();
     waited = true;
     if (rows <= 0) continue;
     if ((tile.i & 1) == 0) {
-      zero_rows<T, V>(out, at.at, at.rl, rows, a.RL, step);
+      zero_rows<T, V>(out - (long long)r * a.C, at.at, at.rl, rows, a.RL, step);
       continue;
     }
     // grad_x = dz * scale - (k1 + (x - mean) * k2)
@@ -634,24 +641,20 @@ group_grad_apply_kernel(const T *__restrict__ grad_y, const T *__restrict__ x, c
         const float dz = ACT ? activate_grad<ACT>(gf[c], fmaf(centred, scale[c], shift[c]), a.act) : gf[c];
         xf[c] = fmaf(dz, scale[c], -fmaf(centred, k2[c], k1[c]));
       }
-      store_word<T, V>(out + u * step + at.at, xf);
+      store_once<T, V>(out + u * step + at.at, xf);
     };
-    int r = 0;
-    for (; r + U * a.RL <= rows; r += U * a.RL, xin += U * step, gin += U * step, out += U * step) {
-      if (r > 0) {
-        load_rows<T, V, U, true, true>(xin, at.at, r, rows, a.RL, step, xw);
-        load_rows<T, V, U, true, true>(gin, at.at, r, rows, a.RL, step, gw);
-      }
-#pragma unroll
-      for (int u = 0; u < U; ++u) store(u);
-    }
-    if (r > 0) {
-      load_rows<T, V, U, true, false>(xin, at.at, r + at.rl, rows, a.RL, step, xw);
-      load_rows<T, V, U, true, false>(gin, at.at, r + at.rl, rows, a.RL, step, gw);
-    }
 #pragma unroll
     for (int u = 0; u < U; ++u)
       if (r + at.rl + u * a.RL < rows) store(u);
+    for (r -= chunk; r >= 0; r -= chunk) {
+      xin -= U * step;
+      gin -= U * step;
+      out -= U * step;
+      load_rows<T, V, U, true, true>(xin, at.at, r, rows, a.RL, step, xw);
+      load_rows<T, V, U, true, true>(gin, at.at, r, rows, a.RL, step, gw);
+#pragma unroll
+      for (int u = 0; u < U; ++u) store(u);
+    }
   }
 }
 
@@ -660,22 +663,24 @@ group_grad_apply_kernel(const T *__restrict__ grad_y, const T *__restrict__ x, c
 // ------------------------------------------------------------------------------------------------
 int threads_of(int V) { return V == 4 ? kThreads<4> : V == 2 ? kThreads<2> : kThreads<1>; }
 
-// Rows of a tile: 4 to 32 of a thread, so that a small call spreads over the device and a large one has long-lived CTAs; more where
-// an image would have more than 2048 tiles to merge.
-int tile_rows(int B, int N, int C, int V) {
+int resident_of(int V, int size) { return V == 4 ? (size == 4 ? kResident<float, 4> : kResident<__half, 4>) : V; }
+
+// Rows of a tile: as many as make one full wave of CTAs of the whole call, but at least four of a thread, and at most 2048 tiles an
+// image to merge.  6 x 30 825 x 256 bf16 forward 49 us, at two waves 54, three 59; 40 000 x 256 fp32 32, 42, 49; 6 x 30 825 x 256 fp32 97,
+// 97, 100 (backward 158, 155, 159).
+int tile_rows(int B, int N, int C, int V, int size) {
   const int RL = threads_of(V) / (C / V);
-  const long long even = ((long long)B * N + 148 * 5 * RL - 1) / (148 * 5 * RL);
-  long long rows = RL * std::max(4LL, std::min(32LL, even));
-  rows = std::max(rows, ((long long)N + 2047) / 2048);
+  const long long slots = 148LL * resident_of(V, size), tiles = std::max(1LL, std::min(2048LL, slots / B));
+  const long long rows = std::max((N + tiles - 1) / tiles, 4LL * RL);
   return (int)std::min<long long>(rows, N);
 }
 
-void complete(GnArgs &a, int V) {
+void complete(GnArgs &a, int V, int size) {
   a.cpg = a.C / a.G;
   a.V = V;
   a.nv = a.C / V;
   a.RL = threads_of(V) / a.nv;
-  a.R = tile_rows(a.B, a.N, a.C, V);
+  a.R = tile_rows(a.B, a.N, a.C, V, size);
   a.tiles = (a.N + a.R - 1) / a.R;
   a.entries = a.tiles + 2 * a.L + 1;
   a.whole = a.cpg % V == 0;
@@ -712,7 +717,7 @@ unsigned merge_grid(const GnArgs &a) {
 
 template <typename T, int V>
 cudaError_t forward(const T *x, GnArgs a, T *y, float *mean, float *rstd, void *workspace, cudaStream_t st) {
-  complete(a, V);
+  complete(a, V, sizeof(T));
   float2 *partial = static_cast<float2 *>(workspace);
   if (!mean) {                                           // nobody keeps them: behind the tiles' parts
     mean = reinterpret_cast<float *>(partial + (long long)a.B * a.entries * a.G);
@@ -728,7 +733,7 @@ cudaError_t forward(const T *x, GnArgs a, T *y, float *mean, float *rstd, void *
 template <typename T, int V>
 cudaError_t backward(const T *grad_y, const T *x, GnArgs a, const float *mean, const float *rstd, T *grad_x,
                      float *grad_weight, float *grad_bias, void *workspace, cudaStream_t st) {
-  complete(a, V);
+  complete(a, V, sizeof(T));
   const long long pieces = (long long)a.B * a.entries;
   float2 *by_channel = static_cast<float2 *>(workspace), *by_group = by_channel + pieces * a.C, *means = by_group + pieces * a.G,
          *by_level = means + (long long)a.B * a.L * a.G;
@@ -741,7 +746,7 @@ cudaError_t backward(const T *grad_y, const T *x, GnArgs a, const float *mean, c
   DFA3D_TRY(launch(group_grad_merge_kernel, merges + channels, kMergeThreads, 0, true, st, a, merges, by_group, by_channel, means,
                    by_level));
   const int sums = grad_weight ? (a.C * a.weight_rows + kThreads<V> - 1) / kThreads<V> : 0;
-  return launch(apply, sums + (grad_x ? grid : 0), kThreads<V>, 0, true, st, grad_y, x, a, sums, mean, rstd, means, by_level, grad_x,
+  return launch(apply, sums + (grad_x ? grid : 0), kThreads<V>, 0, true, st, grad_y, x, a, grad_x ? (int)grid : 0, mean, rstd, means, by_level, grad_x,
                 grad_weight, grad_bias);
 }
 
@@ -768,14 +773,16 @@ GnArgs arguments(int B, int N, int C, int G, const int64_t *shapes, int shape_st
 
 }  // namespace
 
-// For any word that a launch may read by.
+// For any word that a launch may read by and either size of an element.
 long long group_norm_workspace(int B, int N, int C, int G, int L, bool backward) {
   if (B == 0 || N == 0) return 0;
   long long pieces = 0;
   for (int V = 4; V >= 1; V /= 2)
     if (C % V == 0) {
-      const int R = tile_rows(B, N, C, V);
-      pieces = std::max<long long>(pieces, (long long)B * ((N + R - 1) / R + 2 * L + 1));
+      for (int size = 2; size <= 4; size += 2) {
+        const int R = tile_rows(B, N, C, V, size);
+        pieces = std::max<long long>(pieces, (long long)B * ((N + R - 1) / R + 2 * L + 1));
+      }
     }
   return (pieces * (backward ? C + G : G) + (long long)B * L * (backward ? C + G : G)) * (long long)sizeof(float2);
 }

@@ -88,6 +88,11 @@ __device__ __forceinline__ void store_word(T *p, const float (&f)[V]) {
   *reinterpret_cast<Word<T, V> *>(p) = narrow_word<T, V>(f);
 }
 
+template <typename T, int V>
+__device__ __forceinline__ void store_once(T *p, const float (&f)[V]) {
+  __stcs(reinterpret_cast<Word<T, V> *>(p), narrow_word<T, V>(f));
+}
+
 // A 16-byte copy into shared memory that nobody waits for yet; the thread that asked for it may read it after copies_wait().
 __device__ __forceinline__ void copy_async16(unsigned shared, const void *global) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(shared), "l"(global) : "memory");
