@@ -13,6 +13,7 @@
 // 40 instructions an element); 900 x 256 fp32 3.2 and 5.5.  Rows loaded into registers instead of one ahead through shared memory:
 // 26 and 46, 1024 columns 66 and 138 for 49 and 80; a warp a row of four elements a lane 25 and 56, bf16 39 and 86.
 #include <algorithm>
+#include <atomic>
 
 #include "dfa3d_launch.h"
 #include "dfa3d_philox.cuh"
@@ -524,14 +525,23 @@ long long row_ctas(long long rows, int lanes, long long each, long long cap) {
 // Two rows of a thread's words of `tensors` tensors, or its columns' sums.
 size_t ring_bytes(const RowShape &r, int tensors) { return r.vec ? 2u * r.K * tensors * kWarps * 32 * 16 : 0u; }
 
-// Launches a kernel that may need more shared memory than it gets by itself (a setting of the kernel on the current device).
-template <typename... P, typename... A>
-cudaError_t launch_rows(void (*kernel)(P...), unsigned grid, size_t shared, cudaStream_t s, A... args) {
+// Launches a kernel that may need more shared memory than it gets by itself: a setting of the kernel on the current device, made
+// once for each of the first 64 devices.
+template <auto KERNEL, typename... A>
+cudaError_t launch_rows(unsigned grid, size_t shared, cudaStream_t s, A... args) {
   if (shared > 48 * 1024) {
-    const cudaError_t rc = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)shared);
+    static std::atomic<unsigned long long> done{0};
+    int device = 0;
+    cudaError_t rc = cudaGetDevice(&device);
     if (rc != cudaSuccess) return rc;
+    const unsigned long long bit = device < 64 ? 1ull << device : 0ull;
+    if (!(done.load(std::memory_order_relaxed) & bit)) {
+      rc = cudaFuncSetAttribute(KERNEL, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)shared);
+      if (rc != cudaSuccess) return rc;
+      done.fetch_or(bit, std::memory_order_relaxed);
+    }
   }
-  kernel<<<grid, kWarps * 32, shared, s>>>(static_cast<P>(args)...);
+  KERNEL<<<grid, kWarps * 32, shared, s>>>(args...);
   return cudaGetLastError();
 }
 
@@ -543,7 +553,7 @@ cudaError_t norm_forward(const T *x, const T *residual, const float *gamma, cons
   const unsigned grid = (unsigned)row_ctas(rows, r.lanes, 1, 148 * kForwardResident);
   const size_t shared = ring_bytes(r, 2);
 #define DFA3D_GO(V, K, LANES, VEC)                                                                                      \
-  return launch_rows(dropout_add_layer_norm_kernel<T, V, K, LANES, VEC>, grid, shared, s, x, residual, gamma, beta, rows, E, d, \
+  return launch_rows<dropout_add_layer_norm_kernel<T, V, K, LANES, VEC>>(grid, shared, s, x, residual, gamma, beta, rows, E, d, \
                      eps, y, mean, rstd)
   DFA3D_ROWS(T, r, DFA3D_GO)
 #undef DFA3D_GO
@@ -562,9 +572,9 @@ cudaError_t norm_backward(const T *grad_y, const T *x, const T *residual, const 
   if (!grad_gamma) partial = nullptr;
   cudaError_t rc = cudaSuccess;
 #define DFA3D_GO(V, K, LANES, VEC)                                                                                            \
-  rc = launch_rows(dropout_layer_norm_backward_kernel<T, V, K, LANES, VEC>, grid,                                             \
-                   std::max(ring_bytes(r, 3), sizeof(float) * kWarps * 32 * V * K), s, grad_y, x, residual, gamma, mean, rstd, \
-                   rows, E, d, grad_x, grad_residual, partial)
+  rc = launch_rows<dropout_layer_norm_backward_kernel<T, V, K, LANES, VEC>>(                                                   \
+      grid, std::max(ring_bytes(r, 3), sizeof(float) * kWarps * 32 * V * K), s, grad_y, x, residual, gamma, mean, rstd, rows,   \
+      E, d, grad_x, grad_residual, partial)
   DFA3D_ROWS(T, r, DFA3D_GO)
 #undef DFA3D_GO
   if (rc != cudaSuccess || !partial) return rc;

@@ -241,3 +241,34 @@ def test_captured_forward_and_backward(lib_built):
         y = dropout_add_layer_norm(*eager, 0.5, out[0].clone())
         for a, b in zip(out[1:], (y,) + torch.autograd.grad(y, eager, g)):
             assert torch.equal(a, b)
+
+
+def test_rows_past_two_to_the_31_elements(lib_built):
+    """The last rows of a tensor that long have the mask of their own element numbers and are normalised like any others."""
+    E, rows = 256, (1 << 23) + 11
+    last = 40
+    g = torch.Generator(device=DEV).manual_seed(3)
+    x, r, go = (torch.empty(rows, E, dtype=torch.bfloat16, device=DEV).normal_(generator=g) for _ in range(3))
+    w, b = torch.rand(E, device=DEV) + 0.5, torch.randn(E, device=DEV)
+    leaves = [x.requires_grad_(True), r.requires_grad_(True)]
+    y = apply(True, x, r, w, b, seed_tensor(5), 0.5, 9)
+    gx, gr = torch.autograd.grad(y, leaves, go)
+    first = (rows - last) * E
+    keep = torch.from_numpy(_words(first, rows * E, 5, 9) >= (1 << 31)).view(last, E)
+    xs, rs, gs = (t.detach()[-last:].cpu().double() for t in (x, r, go))
+    s = rs + torch.where(keep, xs * 2, torch.zeros_like(xs))
+    mean, var = s.mean(-1, keepdim=True), s.var(-1, keepdim=True, correction=0)
+    rstd = (var + EPS) ** -0.5
+    hat = (s - mean) * rstd
+    d = gs * w.cpu().double()
+    want = rstd * (d - d.mean(-1, keepdim=True) - hat * (d * hat).mean(-1, keepdim=True))
+    step = R.half_step(torch.bfloat16)
+    R.assert_within("y", y[-last:], hat * w.cpu().double() + b.cpu().double(), (step + 1e-5) * 8 * torch.ones(last, E).double())
+    R.assert_within("grad_residual", gr[-last:], want, (step + 1e-4) * want.abs() + 1e-4)
+    R.assert_within("grad_x", gx[-last:], torch.where(keep, want * 2, torch.zeros_like(want)), (step + 1e-4) * 2 * want.abs() + 2e-4)
+    assert not gx[-last:].cpu()[~keep].any()
+
+
+def _words(first, last, seed, site):
+    from test_gpu_dropout import _words_from
+    return _words_from(first, last, seed, site)
