@@ -112,12 +112,12 @@ struct DropNormFn : torch::autograd::Function<DropNormFn> {
     const auto r = kept<Rule>(ctx, v);
     const Tensor &x = v[0], &res = v[1], &w = v[2], &stats = v[3], &seed = v[4];
     c10::cuda::CUDAGuard guard(x.device());
-    const int64_t E = x.size(-1), rows = x.numel() / E;
+    const int64_t E = w.numel(), rows = x.numel() / E;       // counts that a saved-tensor hook cannot change, as it can a shape
     const Tensor g = like_forward(grads[0], x.scalar_type());
     const bool params = ctx->needs_input_grad(2) || ctx->needs_input_grad(3);
     Tensor gx, gr, gw, gb, work;
-    if (ctx->needs_input_grad(0)) gx = at::empty_like(x);
-    if (ctx->needs_input_grad(1)) gr = at::empty_like(x);
+    if (ctx->needs_input_grad(0)) gx = at::empty_like(g);
+    if (ctx->needs_input_grad(1)) gr = at::empty_like(g);
     if (params) {
       gw = empty_f32({E}, x);
       gb = empty_f32({E}, x);
@@ -200,7 +200,7 @@ struct GroupNormFn : torch::autograd::Function<GroupNormFn> {
     const Tensor g = like_forward(grads[0], x.scalar_type());
     const bool params = ctx->needs_input_grad(1) || ctx->needs_input_grad(2);
     Tensor gx, gw, gb, work = level_workspace(*s, x, true);
-    if (ctx->needs_input_grad(0)) gx = at::empty_like(x);
+    if (ctx->needs_input_grad(0)) gx = at::empty_like(g);
     if (params) {
       gw = at::empty_like(w);
       gb = at::empty_like(w);

@@ -58,6 +58,23 @@ def _ptr(t):
     return None if t is None else t.data_ptr()
 
 
+def keep(ctx, *tensors):
+    """Keeps tensors for the backward, and what they are beside them."""
+    ctx.save_for_backward(*tensors)
+    ctx.was = [None if t is None else (t.shape, t.dtype, t.device) for t in tensors]
+
+
+def kept(ctx):
+    """The tensors of ``keep``, contiguous.  The kernels read them by address: what a saved-tensor hook handed back instead has to be
+    of the same type, size and device."""
+    out = []
+    for t, was in zip(ctx.saved_tensors, ctx.was):
+        if (None if t is None else (t.shape, t.dtype, t.device)) != was:
+            raise RuntimeError("a saved-tensor hook returned a tensor of another type, size or device than it was given")
+        out.append(None if t is None else t.contiguous())
+    return out
+
+
 def draw_seed(device="cuda", generator=None):
     """A seed for one pass, drawn on the device from torch's generator (or the given one): follows ``torch.manual_seed``, and in
     a captured graph every replay draws another."""
@@ -83,14 +100,14 @@ class DropoutFunction(Function):
                             p, _ptr(seed), site, y.data_ptr(), _stream(x))
         # a ReLU's zeros and the dropped elements are the zeros of the result, unless a residual was added
         ctx.by_result = activation is not None and residual is None
-        ctx.save_for_backward(seed, None if activation is None else y if ctx.by_result else x)
+        keep(ctx, seed, None if activation is None else y if ctx.by_result else x)
         ctx.has_residual, ctx.p, ctx.site, ctx.dtype = residual is not None, p, site, x.dtype
         return y
 
     @staticmethod
     @once_differentiable
     def backward(ctx, grad_y):
-        seed, ref = ctx.saved_tensors
+        seed, ref = kept(ctx)
         grad_x = None
         if ctx.needs_input_grad[0]:
             g = grad_y.to(ctx.dtype).contiguous()
@@ -130,7 +147,7 @@ class DropoutAddLayerNormFunction(Function):
             _lib.call_plain("dfa3d_dropout_add_layer_norm_forward", x.data_ptr(), residual.data_ptr(), weight.data_ptr(),
                             bias.data_ptr(), _DTYPES[x.dtype], rows, E, p, _ptr(seed), site, float(eps), y.data_ptr(),
                             stats[0].data_ptr(), stats[1].data_ptr(), _stream(x))
-        ctx.save_for_backward(x, residual, weight, stats, seed)
+        keep(ctx, x, residual, weight, stats, seed)
         ctx.p, ctx.site, ctx.bias_shape = p, site, bias.shape
         return y
 
@@ -138,7 +155,7 @@ class DropoutAddLayerNormFunction(Function):
     @torch.amp.custom_bwd(device_type="cuda")
     @once_differentiable
     def backward(ctx, grad_y):
-        x, residual, weight, stats, seed = ctx.saved_tensors
+        x, residual, weight, stats, seed = kept(ctx)
         E, rows = x.shape[-1], stats.shape[1]
         g = grad_y.to(x.dtype).contiguous()
         need = ctx.needs_input_grad

@@ -14,6 +14,7 @@ import torch.nn as nn
 from torch.autograd.function import Function, once_differentiable
 
 from . import _lib
+from .dropout_ops import keep, kept
 
 _DTYPES = {torch.float32: _lib.DTYPE_F32, torch.bfloat16: _lib.DTYPE_BF16, torch.float16: _lib.DTYPE_F16}
 _ACTS = {None: _lib.ROW_NONE, "relu": _lib.ROW_RELU, "silu": _lib.ROW_SILU}
@@ -70,7 +71,7 @@ class GroupNormFunction(Function):
             _lib.call_plain("dfa3d_group_norm_forward", x.data_ptr(), _DTYPES[x.dtype], B, N, C, G, _ptr(shapes), stride, _ptr(lsi),
                             L, weight.data_ptr(), bias.data_ptr(), rows, float(eps), _ACTS[activation], y.data_ptr(),
                             stats[0].data_ptr(), stats[1].data_ptr(), work.data_ptr(), work.numel(), _stream(x))
-        ctx.save_for_backward(x, weight, bias, shapes, lsi, stats)
+        keep(ctx, x, weight, bias, shapes, lsi, stats)
         ctx.sizes, ctx.act = (B, N, C, G, stride, L, rows), _ACTS[activation]
         return y
 
@@ -78,7 +79,7 @@ class GroupNormFunction(Function):
     @torch.amp.custom_bwd(device_type="cuda")
     @once_differentiable
     def backward(ctx, grad_y):
-        x, weight, bias, shapes, lsi, stats = ctx.saved_tensors
+        x, weight, bias, shapes, lsi, stats = kept(ctx)
         B, N, C, G, stride, L, rows = ctx.sizes
         g = grad_y.to(x.dtype).contiguous()
         need = ctx.needs_input_grad

@@ -409,7 +409,7 @@ int dfa3d_convert_two(int32_t narrow_dtype, int32_t widen, void *narrow0, void *
  * number) alone: a backward gets the same three and forms it again.  seed: ONE int64 in DEVICE memory (a captured graph
  * reads the value of each replay), not looked at where p < 2^-33.  0 <= p <= 1, site >= 0 tells the calls of one pass
  * apart.  dtype of x, residual, results and gradients: DFA3D_DTYPE_F32, _BF16 or _F16; arithmetic is fp32.  Addresses off
- * the 16-byte grid are taken, more slowly. */
+ * the 16-byte grid are taken, more slowly.  Results overlap no input, but for what is allowed below. */
 #define DFA3D_ROW_NONE 0
 #define DFA3D_ROW_RELU 1
 #define DFA3D_ROW_SILU 2
@@ -448,7 +448,7 @@ int dfa3d_dropout_add_layer_norm_backward(const void *grad_y, const void *x, con
  * null with L = 1: the N rows are one level.  A table that points outside of the N rows or overlaps is cut to disjoint
  * levels; rows of no level become 0 in y and in grad_x.  weight, bias fp32 (weight_rows, C) with weight_rows 1 (shared by
  * the levels) or L.  C <= 1024, G divides C.  dtype (of x, y and their gradients): DFA3D_DTYPE_F32, _BF16 or _F16.
- * mean, rstd (B, L, G) fp32 for the backward; may be null together in the forward. */
+ * mean, rstd (B, L, G) fp32 for the backward; may be null together in the forward.  Results overlap no input. */
 int64_t dfa3d_group_norm_workspace(int32_t B, int32_t N, int32_t C, int32_t G, int32_t L, int32_t backward);
 
 int dfa3d_group_norm_forward(const void *x, int32_t dtype, int32_t B, int32_t N, int32_t C, int32_t G,
