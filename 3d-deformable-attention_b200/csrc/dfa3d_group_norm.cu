@@ -14,13 +14,16 @@
 //
 // Three launches each way: statistics of tiles of rows; a warp for every group of a level of an image merges its tiles' parts;
 // the result.  They follow one another as programmatic dependent launches, so that the third has its rows on the way while the
-// second runs, and the third walks the tiles from the last one back, whose rows the first has left in L2.  What bounds them is HBM:
-// x is read once and a second time as far as it has left L2 (126 MB), y written once.
+// second runs.  All tiles of a launch are resident at once, and the third walks each from its end, whose rows the first has left in
+// L2 (126 MB).
 //
-// 6 x 30 825 x 256, 32 groups, 4 levels: fp32 (189 MB) forward 99 us, backward 158; bf16 58 and 97; 6 x 920 x 256 fp32 10 and 12.
-// Measured against it, fp32 forward / backward: one launch that walks the images in batches with a barrier of the grid after each
-// 257 / 287 (each barrier leaves every SM waiting through the merge); launches that form the statistics of one batch and the
-// results of the one before 129 to 270; merges by every CTA of the third launch instead of a second one 144 / 249.
+// 6 x 30 825 x 256, 32 groups, 4 levels: fp32 (189 MB) forward 96 us, backward 156; bf16 52 and 86; 6 x 920 x 256 fp32 11 and 11.
+// The result's launch runs at the rate of a copy (57 us for 378 MB, the same with rows from L2 or not), the fp32 statistics at
+// 5.7 TB/s, the bf16 ones (25 us for 95 MB) at the rate of their instructions.  Measured against it, fp32 forward / backward: one
+// launch that walks the images in batches with a barrier of the grid after each 257 / 287 (each barrier leaves every SM waiting
+// through the merge); launches that form the statistics of one batch and the results of the one before 129 to 220 / 241 to 494;
+// batches that fit L2, one after the other, 102 / 178; rows one chunk ahead through shared memory 107 / 167; merges by the CTAs of
+// the third launch instead of a second one 110 / 170; two to six waves of tiles, bf16 forward 54 to 74.
 #include <algorithm>
 
 #include "dfa3d_launch.h"
