@@ -17,7 +17,7 @@
 // second runs.  All tiles of a launch are resident at once, and the third walks each from its end, whose rows the first has left in
 // L2 (126 MB).
 //
-// 6 x 30 825 x 256, 32 groups, 4 levels: fp32 (189 MB) forward 96 us, backward 156; bf16 52 and 86; 6 x 920 x 256 fp32 11 and 11.
+// 6 x 30 825 x 256, 32 groups, 4 levels: fp32 (189 MB) forward 96 us, backward 156; bf16 50 and 84; 6 x 920 x 256 fp32 11 and 11.
 // The result's launch runs at the rate of a copy (57 us for 378 MB, the same with rows from L2 or not), the fp32 statistics at
 // 5.7 TB/s, the bf16 ones (25 us for 95 MB) at the rate of their instructions.  Measured against it, fp32 forward / backward: one
 // launch that walks the images in batches with a barrier of the grid after each 257 / 287 (each barrier leaves every SM waiting
@@ -38,9 +38,11 @@ enum Act { kNone = 0, kRelu = 1, kSilu = 2 };
 // Threads of a CTA: at least as many as a row has words of V channels.
 template <int V> constexpr int kThreads = V == 4 ? 256 : 1024 / V;
 // CTAs an SM: what the registers of a thread's rows leave.
-template <typename T, int V> constexpr int kResident = V == 4 ? (sizeof(T) == 4 ? 3 : 4) : V;
+template <int V> constexpr int kResident = V == 4 ? 3 : V;
 // Words of a thread in flight, and of each of two tensors.
 constexpr int kAhead = 8, kGradAhead = 4;
+// ... of the two that are only read: 8-byte words leave registers for more (bf16 backward 84 us; four words and four CTAs an SM 86).
+template <typename T, int V> constexpr int kGradStatsAhead = V == 4 && sizeof(T) == 2 ? 8 : kGradAhead;
 
 struct GnArgs {
   const int64_t *shapes, *start;     // level table, or null: one level
@@ -197,7 +199,7 @@ struct Moments {
 
 // A tile's statistics into partial (B, entries, G): mean and sum of squares around it, of each piece's values of a group.
 template <typename T, int V>
-__global__ void __launch_bounds__(kThreads<V>, kResident<T, V>)
+__global__ void __launch_bounds__(kThreads<V>, kResident<V>)
 group_stats_kernel(const T *__restrict__ x, const GnArgs a, float2 *__restrict__ partial) {
   constexpr int U = kAhead;
   extern __shared__ float2 chan[];                       // a thread's channels
@@ -346,7 +348,7 @@ group_merge_kernel(const GnArgs a, const float2 *partial, float *__restrict__ me
 
 // y = act((x - mean) * rstd * weight + bias).  A tile is walked from its end: what the statistics read last is still in L2.
 template <typename T, int V, bool ACT>
-__global__ void __launch_bounds__(kThreads<V>, kResident<T, V>)
+__global__ void __launch_bounds__(kThreads<V>, kResident<V>)
 group_apply_kernel(const T *__restrict__ x, const GnArgs a, const float *mean_in, const float *rstd_in, T *__restrict__ y) {
   constexpr int U = kAhead;
   __shared__ SegmentTable seg;
@@ -413,10 +415,10 @@ group_apply_kernel(const T *__restrict__ x, const GnArgs a, const float *mean_in
 // Sums of dz and of dz * xhat over a tile's pieces: by_channel (B, entries, C), and times gamma over a group's channels: by_group
 // (B, entries, G).
 template <typename T, int V, bool ACT>
-__global__ void __launch_bounds__(kThreads<V>, kResident<T, V>)
+__global__ void __launch_bounds__(kThreads<V>, kResident<V>)
 group_grad_stats_kernel(const T *__restrict__ grad_y, const T *__restrict__ x, const GnArgs a, const float *__restrict__ mean_in,
                         const float *__restrict__ rstd_in, float2 *__restrict__ by_channel, float2 *__restrict__ by_group) {
-  constexpr int U = kGradAhead;
+  constexpr int U = kGradStatsAhead<T, V>;
   extern __shared__ float2 chan[];                       // (RL, C)
   __shared__ SegmentTable seg;
   launch_next();
@@ -579,7 +581,7 @@ __device__ __forceinline__ void parameter_sums(const GnArgs &a, const float2 *by
 // grad_x = rstd * (d - mean(d) - xhat * mean(d * xhat)), d = dz * gamma, means over the group; the CTAs beyond its
 // `tiles` form the parameters' gradients.
 template <typename T, int V, bool ACT>
-__global__ void __launch_bounds__(kThreads<V>, kResident<T, V>)
+__global__ void __launch_bounds__(kThreads<V>, kResident<V>)
 group_grad_apply_kernel(const T *__restrict__ grad_y, const T *__restrict__ x, const GnArgs a, int tiles,
                         const float *__restrict__ mean_in, const float *__restrict__ rstd_in, const float2 *means,
                         const float2 *by_level, T *__restrict__ grad_x, float *grad_weight, float *grad_bias) {
@@ -666,24 +668,24 @@ group_grad_apply_kernel(const T *__restrict__ grad_y, const T *__restrict__ x, c
 // ------------------------------------------------------------------------------------------------
 int threads_of(int V) { return V == 4 ? kThreads<4> : V == 2 ? kThreads<2> : kThreads<1>; }
 
-int resident_of(int V, int size) { return V == 4 ? (size == 4 ? kResident<float, 4> : kResident<__half, 4>) : V; }
+int resident_of(int V) { return V == 4 ? kResident<4> : V == 2 ? kResident<2> : kResident<1>; }
 
 // Rows of a tile: as many as make one full wave of CTAs of the whole call, but at least four of a thread, and at most 2048 tiles an
 // image to merge.  6 x 30 825 x 256 bf16 forward 49 us, at two waves 54, three 59; 40 000 x 256 fp32 32, 42, 49; 6 x 30 825 x 256 fp32 97,
 // 97, 100 (backward 158, 155, 159).
-int tile_rows(int B, int N, int C, int V, int size) {
+int tile_rows(int B, int N, int C, int V) {
   const int RL = threads_of(V) / (C / V);
-  const long long slots = 148LL * resident_of(V, size), tiles = std::max(1LL, std::min(2048LL, slots / B));
+  const long long slots = 148LL * resident_of(V), tiles = std::max(1LL, std::min(2048LL, slots / B));
   const long long rows = std::max((N + tiles - 1) / tiles, 4LL * RL);
   return (int)std::min<long long>(rows, N);
 }
 
-void complete(GnArgs &a, int V, int size) {
+void complete(GnArgs &a, int V) {
   a.cpg = a.C / a.G;
   a.V = V;
   a.nv = a.C / V;
   a.RL = threads_of(V) / a.nv;
-  a.R = tile_rows(a.B, a.N, a.C, V, size);
+  a.R = tile_rows(a.B, a.N, a.C, V);
   a.tiles = (a.N + a.R - 1) / a.R;
   a.entries = a.tiles + 2 * a.L + 1;
   a.whole = a.cpg % V == 0;
@@ -720,7 +722,7 @@ unsigned merge_grid(const GnArgs &a) {
 
 template <typename T, int V>
 cudaError_t forward(const T *x, GnArgs a, T *y, float *mean, float *rstd, void *workspace, cudaStream_t st) {
-  complete(a, V, sizeof(T));
+  complete(a, V);
   float2 *partial = static_cast<float2 *>(workspace);
   if (!mean) {                                           // nobody keeps them: behind the tiles' parts
     mean = reinterpret_cast<float *>(partial + (long long)a.B * a.entries * a.G);
@@ -736,7 +738,7 @@ cudaError_t forward(const T *x, GnArgs a, T *y, float *mean, float *rstd, void *
 template <typename T, int V>
 cudaError_t backward(const T *grad_y, const T *x, GnArgs a, const float *mean, const float *rstd, T *grad_x,
                      float *grad_weight, float *grad_bias, void *workspace, cudaStream_t st) {
-  complete(a, V, sizeof(T));
+  complete(a, V);
   const long long pieces = (long long)a.B * a.entries;
   float2 *by_channel = static_cast<float2 *>(workspace), *by_group = by_channel + pieces * a.C, *means = by_group + pieces * a.G,
          *by_level = means + (long long)a.B * a.L * a.G;
@@ -776,16 +778,14 @@ GnArgs arguments(int B, int N, int C, int G, const int64_t *shapes, int shape_st
 
 }  // namespace
 
-// For any word that a launch may read by and either size of an element.
+// For any word that a launch may read by.
 long long group_norm_workspace(int B, int N, int C, int G, int L, bool backward) {
   if (B == 0 || N == 0) return 0;
   long long pieces = 0;
   for (int V = 4; V >= 1; V /= 2)
     if (C % V == 0) {
-      for (int size = 2; size <= 4; size += 2) {
-        const int R = tile_rows(B, N, C, V, size);
-        pieces = std::max<long long>(pieces, (long long)B * ((N + R - 1) / R + 2 * L + 1));
-      }
+      const int R = tile_rows(B, N, C, V);
+      pieces = std::max<long long>(pieces, (long long)B * ((N + R - 1) / R + 2 * L + 1));
     }
   return (pieces * (backward ? C + G : G) + (long long)B * L * (backward ? C + G : G)) * (long long)sizeof(float2);
 }
