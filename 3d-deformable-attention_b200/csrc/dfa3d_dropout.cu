@@ -150,47 +150,79 @@ dropout_backward_kernel(const T *__restrict__ grad_y, const T *__restrict__ ref,
 constexpr int kWarps = 8;
 // CTAs of the forward on an SM.  40 000 x 256 fp32: 23.6 us at three, 25.6 at four, 29.1 at five (spills).
 constexpr int kForwardResident = 3;
+// ... on rows off the grid, whose words and weights stay in registers: 60 000 x 202 fp16 32.6 us at two, 36.5 at three.
+constexpr int kOddResident = 2;
 
-// V elements from `c` on of a row of E.  VEC: V divides E and the row is aligned for words of V; else one by one, zeros behind
-// the row's end.
-template <typename T, int V, bool VEC>
-__device__ __forceinline__ void load_group(const T *row, int c, int E, float (&f)[V]) {
-  if (VEC) {
-    widen_word<T, V>(load_once<T, V>(row + c), f);
-  } else {
+// A row's words of V elements.  VEC: V divides E and the tensors are on the grid of such words.  Else a word is four elements that
+// share a Philox block, whatever row they are of: a row begins `shift` elements inside of its first word, and elements of its
+// neighbours are left out (NaN and all).  A warp's rows lie a multiple of four apart, so that its shift, and with it the columns
+// of each lane, stay the same.  Against rows read one element at a time, us forward / backward: 7001 x 202 fp16 6.0 / 10.0 for
+// 6.9 / 10.6, 60 000 x 202 fp16 33 / 50 for 46 / 64, 100 000 x 61 bf16 16 / 26 for 44 / 59, 40 000 x 301 bf16 41 / 75 for 112 / 108,
+// 30 000 x 511 fp32 65 / 98 for 107 / 113, 20 000 x 1023 79 / 157 for 125 / 141.
+struct Odd {
+  int E, shift;
+  long long total;       // elements of a tensor
+  bool wide;             // words of four can be read and written at once
+  __device__ __forceinline__ bool inside(int c) const { return (unsigned)c < (unsigned)E; }
+};
+// A lane's words of NT tensors' rows, as they are stored.
+template <typename T, int K, int LANES, int NT>
+struct OddRows {
+  Word<T, 4> w[NT][K];
+  // A lane's words `first`, first + 1, ... of the row that begins `at` elements behind the pointers; nothing if it is not `live`.
+  // All loads are under way before the first is used.
+  __device__ __forceinline__ void load(const Odd &o, const T *const (&p)[NT], long long at, int lane, bool live, int first = 0) {
+    if (!live) return;
+    const bool whole = o.wide && at + o.E + 3 <= o.total;
 #pragma unroll
-    for (int i = 0; i < V; ++i) f[i] = c + i < E ? wide(row[c + i]) : 0.f;
-  }
-}
-template <typename T, int V, bool VEC>
-__device__ __forceinline__ void store_group(T *row, int c, int E, const float (&f)[V]) {
-  if (VEC) {
-    store_word<T, V>(row + c, f);
-  } else {
+    for (int j = 0; j < K; ++j) {
+      const int c = (lane + LANES * (first + j)) * 4 - o.shift;
+      if (c < o.E) {
 #pragma unroll
-    for (int i = 0; i < V; ++i)
-      if (c + i < E) row[c + i] = narrow<T>(f[i]);
+        for (int t = 0; t < NT; ++t) {
+          if (whole) {
+            w[t][j] = load_word<T, 4>(p[t] + at + c);
+          } else {
+            float f[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) f[i] = o.inside(c + i) ? wide(p[t][at + c + i]) : 0.f;
+            w[t][j] = narrow_word<T, 4>(f);
+          }
+        }
+      }
+    }
   }
+  __device__ __forceinline__ void read(const Odd &o, int j, int t, int c, float (&f)[4]) const {
+    widen_word<T, 4>(w[t][j], f);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) f[i] = o.inside(c + i) ? f[i] : 0.f;
+  }
+};
+template <typename T>
+__device__ __forceinline__ void store_odd(const Odd &o, T *p, long long at, int c, const float (&f)[4]) {
+  const bool whole = o.wide && c >= 0 && c + 4 <= o.E;
+  if (whole) store_word<T, 4>(p + at + c, f);
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    if (!whole && o.inside(c + i)) p[at + c + i] = narrow<T>(f[i]);
 }
 template <int V>
-__device__ __forceinline__ void load_param(const float *p, int c, int E, bool whole, float (&f)[V]) {
-  if (whole) {
+__device__ __forceinline__ void load_param(const float *p, int c, float (&f)[V]) {
 #pragma unroll
-    for (int i = 0; i < V; i += 4) {
-      const float4 t = __ldg(reinterpret_cast<const float4 *>(p + c + i));
-      f[i] = t.x; f[i + 1] = t.y; f[i + 2] = t.z; f[i + 3] = t.w;
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < V; ++i) f[i] = c + i < E ? __ldg(p + c + i) : 0.f;
+  for (int i = 0; i < V; i += 4) {
+    const float4 t = __ldg(reinterpret_cast<const float4 *>(p + c + i));
+    f[i] = t.x; f[i + 1] = t.y; f[i + 2] = t.z; f[i + 3] = t.w;
   }
 }
-
-// Which of V elements from `first` on are kept.
-template <int V, bool VEC>
-__device__ __forceinline__ void words_at(const DropRule &d, DropKey k, unsigned long long first, uint32_t (&words)[V]) {
-  if constexpr (VEC) words_of<V>(d, k, first, words);
-  else words_of_any(d, k, first, words);
+__device__ __forceinline__ void load_param_odd(const Odd &o, const float *p, int c, float (&f)[4]) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) f[i] = o.inside(c + i) ? __ldg(p + c + i) : 0.f;
+}
+// All of a lane's, for the rows that it will have.
+template <int K, int LANES>
+__device__ __forceinline__ void load_params_odd(const Odd &o, const float *p, int lane, float (&f)[K][4]) {
+#pragma unroll
+  for (int j = 0; j < K; ++j) load_param_odd(o, p, (lane + LANES * j) * 4 - o.shift, f[j]);
 }
 
 // Sum over the LANES lanes that share a row.
@@ -233,10 +265,10 @@ struct RowsAhead {
 // stands in 32 bits and is not written: the backward forms it again from the same x and residual, so that storage in 16 bits
 // rounds nothing but y.
 template <typename T, int V, int K, int LANES, bool VEC>
-__global__ void __launch_bounds__(kWarps * 32, K * V <= 16 ? kForwardResident : 1)
+__global__ void __launch_bounds__(kWarps * 32, K * V > 16 ? 1 : VEC ? kForwardResident : kOddResident)
 dropout_add_layer_norm_kernel(const T *__restrict__ x, const T *__restrict__ residual, const float *__restrict__ gamma,
-                              const float *__restrict__ beta, long long rows, int E, DropRule d, float eps, T *__restrict__ y,
-                              float *__restrict__ mean_out, float *__restrict__ rstd_out) {
+                              const float *__restrict__ beta, long long rows, int E, bool wide_words, DropRule d, float eps,
+                              T *__restrict__ y, float *__restrict__ mean_out, float *__restrict__ rstd_out) {
   constexpr int kRowsAtOnce = 32 / LANES;
   extern __shared__ __align__(16) unsigned char ring[];
   const float inv_e = 1.f / (float)E;
@@ -247,18 +279,32 @@ dropout_add_layer_norm_kernel(const T *__restrict__ x, const T *__restrict__ res
   RowsAhead<T, V, K, LANES, 2> ahead(ring);
   if constexpr (VEC) ahead.ask(in, row * E, lane, E, row < rows);
   const DropKey key = drop_key(d);
+  const Odd odd = {E, VEC ? 0 : (int)(row * E & 3), rows * E, wide_words};
+  constexpr bool kAhead = !VEC && K <= 2;
+  float gamma_of[VEC ? 1 : K][4], beta_of[VEC ? 1 : K][4];
+  if constexpr (!VEC) {
+    load_params_odd<K, LANES>(odd, gamma, lane, gamma_of);
+    load_params_odd<K, LANES>(odd, beta, lane, beta_of);
+  }
+  OddRows<T, VEC ? 1 : K, LANES, 2> odd_row, odd_next;
+  if constexpr (kAhead) odd_next.load(odd, in, row * E, lane, row < rows);
   for (; row - slot < rows; row += stride) {
     const bool live = row < rows;
     const long long at = row * E;
     if constexpr (VEC) {
       ahead.ask(in, at + stride * E, lane, E, row + stride < rows);
       copies_wait<1>();
+    } else if constexpr (kAhead) {
+      odd_row = odd_next;
+      odd_next.load(odd, in, at + stride * E, lane, row + stride < rows);
+    } else {
+      odd_row.load(odd, in, at, lane, live);
     }
     float v[K][V];
     float s = 0.f;
 #pragma unroll
     for (int j = 0; j < K; ++j) {
-      const int c = (lane + LANES * j) * V;
+      const int c = (lane + LANES * j) * V - odd.shift;
 #pragma unroll
       for (int i = 0; i < V; ++i) v[j][i] = 0.f;
       if (c >= E || !live) continue;
@@ -267,11 +313,11 @@ dropout_add_layer_norm_kernel(const T *__restrict__ x, const T *__restrict__ res
         ahead.read(j, 0, xf);
         ahead.read(j, 1, v[j]);
       } else {
-        load_group<T, V, VEC>(x + at, c, E, xf);
-        load_group<T, V, VEC>(residual + at, c, E, v[j]);
+        odd_row.read(odd, j, 0, c, xf);
+        odd_row.read(odd, j, 1, c, v[j]);
       }
       uint32_t words[V];
-      words_at<V, VEC>(d, key, (unsigned long long)(at + c), words);
+      words_of<V>(d, key, (unsigned long long)(at + c), words);
 #pragma unroll
       for (int i = 0; i < V; ++i) {
         const float sum = fmaf(xf[i], d.scale, v[j][i]);
@@ -283,11 +329,11 @@ dropout_add_layer_norm_kernel(const T *__restrict__ x, const T *__restrict__ res
     float q = 0.f;
 #pragma unroll
     for (int j = 0; j < K; ++j) {
-      const int c = (lane + LANES * j) * V;
+      const int c = (lane + LANES * j) * V - odd.shift;
 #pragma unroll
       for (int i = 0; i < V; ++i) {
         v[j][i] -= mean;
-        const float t = VEC ? (c < E ? v[j][i] : 0.f) : (c + i < E ? v[j][i] : 0.f);
+        const float t = (VEC ? c < E : odd.inside(c + i)) ? v[j][i] : 0.f;
         q = fmaf(t, t, q);
       }
     }
@@ -295,14 +341,20 @@ dropout_add_layer_norm_kernel(const T *__restrict__ x, const T *__restrict__ res
     if (!live) continue;
 #pragma unroll
     for (int j = 0; j < K; ++j) {
-      const int c = (lane + LANES * j) * V;
+      const int c = (lane + LANES * j) * V - odd.shift;
       if (c >= E) continue;
-      float g[V], b[V];
-      load_param<V>(gamma, c, E, VEC, g);
-      load_param<V>(beta, c, E, VEC, b);
+      if constexpr (VEC) {
+        float g[V], b[V];
+        load_param<V>(gamma, c, g);
+        load_param<V>(beta, c, b);
 #pragma unroll
-      for (int i = 0; i < V; ++i) g[i] = fmaf(v[j][i] * rstd, g[i], b[i]);
-      store_group<T, V, VEC>(y + at, c, E, g);
+        for (int i = 0; i < V; ++i) g[i] = fmaf(v[j][i] * rstd, g[i], b[i]);
+        store_word<T, V>(y + at + c, g);
+      } else {
+#pragma unroll
+        for (int i = 0; i < V; ++i) v[j][i] = fmaf(v[j][i] * rstd, gamma_of[j][i], beta_of[j][i]);
+        store_odd<T>(odd, y, at, c, v[j]);
+      }
     }
     if (lane == 0 && mean_out) {
       mean_out[row] = mean;
@@ -323,7 +375,8 @@ template <typename T, int V, int K, int LANES, bool VEC>
 __global__ void __launch_bounds__(kWarps * 32)
 dropout_layer_norm_backward_kernel(const T *__restrict__ grad_y, const T *__restrict__ x, const T *__restrict__ residual,
                                    const float *__restrict__ gamma, const float *__restrict__ mean_in,
-                                   const float *__restrict__ rstd_in, long long rows, int E, DropRule d, T *__restrict__ grad_x,
+                                   const float *__restrict__ rstd_in, long long rows, int E, bool wide_words, DropRule d,
+                                   T *__restrict__ grad_x,
                                    T *__restrict__ grad_residual, float *__restrict__ partial) {
   constexpr int kRowsAtOnce = 32 / LANES, kSlots = kWarps * kRowsAtOnce;
   extern __shared__ __align__(16) unsigned char ring[];
@@ -336,11 +389,26 @@ dropout_layer_norm_backward_kernel(const T *__restrict__ grad_y, const T *__rest
   RowsAhead<T, V, K, LANES, 3> ahead(ring);
   if constexpr (VEC) ahead.ask(in, row * E, lane, E, row < rows);
   const DropKey key = drop_key(d);
+  const Odd odd = {E, VEC ? 0 : (int)(row * E & 3), rows * E, wide_words};
+  // long rows leave no registers for the weights, the longest none for all of their words: a third of them at a time
+  constexpr bool kOnce = !VEC && K <= 4, kAhead = !VEC && K <= 2;
+  constexpr int kPart = VEC ? 1 : K <= 6 ? K : 3;
+  float gamma_of[kOnce ? K : 1][4];
+  OddRows<T, kPart, LANES, 3> odd_row, odd_next;
+  if constexpr (kOnce) load_params_odd<K, LANES>(odd, gamma, lane, gamma_of);
+  if constexpr (kAhead) odd_next.load(odd, in, row * E, lane, row < rows);
   float dg[K][V] = {}, db[K][V] = {};
   for (; row - slot < rows; row += stride) {
     const bool live = row < rows;
     const long long at = row * E;
-    if constexpr (VEC) ahead.ask(in, at + stride * E, lane, E, row + stride < rows);
+    if constexpr (VEC) {
+      ahead.ask(in, at + stride * E, lane, E, row + stride < rows);
+    } else if constexpr (kAhead) {
+      odd_row = odd_next;
+      odd_next.load(odd, in, at + stride * E, lane, row + stride < rows);
+    } else if constexpr (kOnce) {
+      odd_row.load(odd, in, at, lane, live);
+    }
     const float mean = live ? __ldg(mean_in + row) : 0.f, rstd = live ? __ldg(rstd_in + row) : 0.f;
     if constexpr (VEC) copies_wait<1>();
     float g[K][V], h[K][V];
@@ -348,7 +416,9 @@ dropout_layer_norm_backward_kernel(const T *__restrict__ grad_y, const T *__rest
     float s1 = 0.f, s2 = 0.f;
 #pragma unroll
     for (int j = 0; j < K; ++j) {
-      const int c = (lane + LANES * j) * V;
+      const int c = (lane + LANES * j) * V - odd.shift;
+      if constexpr (!VEC && !kOnce)
+        if (j % kPart == 0) odd_row.load(odd, in, at, lane, live, j);
 #pragma unroll
       for (int i = 0; i < V; ++i) g[j][i] = h[j][i] = 0.f;
       if (c >= E || !live) continue;
@@ -358,17 +428,24 @@ dropout_layer_norm_backward_kernel(const T *__restrict__ grad_y, const T *__rest
         ahead.read(j, 1, xf);
         ahead.read(j, 2, h[j]);
       } else {
-        load_group<T, V, VEC>(grad_y + at, c, E, g[j]);
-        load_group<T, V, VEC>(x + at, c, E, xf);
-        load_group<T, V, VEC>(residual + at, c, E, h[j]);
+        odd_row.read(odd, j % kPart, 0, c, g[j]);
+        odd_row.read(odd, j % kPart, 1, c, xf);
+        odd_row.read(odd, j % kPart, 2, c, h[j]);
       }
-      load_param<V>(gamma, c, E, VEC, w);
-      words_at<V, VEC>(d, key, (unsigned long long)(at + c), words[j]);
+      if constexpr (VEC) {
+        load_param<V>(gamma, c, w);
+      } else if constexpr (kOnce) {
+#pragma unroll
+        for (int i = 0; i < V; ++i) w[i] = gamma_of[j][i];
+      } else {
+        load_param_odd(odd, gamma, c, w);
+      }
+      words_of<V>(d, key, (unsigned long long)(at + c), words[j]);
 #pragma unroll
       for (int i = 0; i < V; ++i) {
         const float sum = fmaf(xf[i], d.scale, h[j][i]);
         h[j][i] = ((words[j][i] > d.last ? sum : h[j][i]) - mean) * rstd;
-        if (!VEC && c + i >= E) h[j][i] = 0.f;
+        if (!VEC && !odd.inside(c + i)) h[j][i] = 0.f;
         dg[j][i] = fmaf(g[j][i], h[j][i], dg[j][i]);
         db[j][i] += g[j][i];
         g[j][i] *= w[i];
@@ -381,27 +458,34 @@ dropout_layer_norm_backward_kernel(const T *__restrict__ grad_y, const T *__rest
     if (!live) continue;
 #pragma unroll
     for (int j = 0; j < K; ++j) {
-      const int c = (lane + LANES * j) * V;
+      const int c = (lane + LANES * j) * V - odd.shift;
       if (c >= E) continue;
 #pragma unroll
       for (int i = 0; i < V; ++i) g[j][i] = fmaf(g[j][i], rstd, -fmaf(h[j][i], c2, c1));
-      if (grad_residual) store_group<T, V, VEC>(grad_residual + at, c, E, g[j]);
+      if (grad_residual) {
+        if constexpr (VEC) store_word<T, V>(grad_residual + at + c, g[j]);
+        else store_odd<T>(odd, grad_residual, at, c, g[j]);
+      }
 #pragma unroll
       for (int i = 0; i < V; ++i) g[j][i] = words[j][i] > d.last ? g[j][i] * d.scale : 0.f;
-      if (grad_x) store_group<T, V, VEC>(grad_x + at, c, E, g[j]);
+      if (grad_x) {
+        if constexpr (VEC) store_word<T, V>(grad_x + at + c, g[j]);
+        else store_odd<T>(odd, grad_x, at, c, g[j]);
+      }
     }
   }
   if (!partial) return;
   copies_wait<0>();
   __syncthreads();                                       // the ring becomes the lanes' sums
   constexpr int kWidth = LANES * V * K;
-  float *part = reinterpret_cast<float *>(ring), *mine = part + (warp * kRowsAtOnce + slot) * kWidth + lane * V;
+  float *part = reinterpret_cast<float *>(ring), *mine = part + (warp * kRowsAtOnce + slot) * kWidth + lane * V - odd.shift;
 #pragma unroll
   for (int pass = 0; pass < 2; ++pass) {
 #pragma unroll
     for (int j = 0; j < K; ++j)
 #pragma unroll
-      for (int i = 0; i < V; ++i) mine[j * LANES * V + i] = pass == 0 ? dg[j][i] : db[j][i];
+      for (int i = 0; i < V; ++i)
+        if (VEC || odd.inside((lane + LANES * j) * V - odd.shift + i)) mine[j * LANES * V + i] = pass == 0 ? dg[j][i] : db[j][i];
     __syncthreads();
     for (int c = threadIdx.x; c < E; c += kWarps * 32) {
       float t = part[c];
@@ -475,7 +559,7 @@ cudaError_t backward(const T *grad_y, const T *ref, long long n, bool rng, const
   return cudaGetLastError();
 }
 
-// How a row of E is laid out over lanes: words of V elements, K words a lane.
+// How a row of E is laid out over lanes: words of V elements, K words a lane; off the grid words of four.
 struct RowShape {
   int lanes, K;
   bool vec;
@@ -483,7 +567,12 @@ struct RowShape {
 template <typename T>
 RowShape row_shape(int E, bool aligned) {
   constexpr int V = 16 / (int)sizeof(T);
-  if (!aligned || E % V != 0) return {32, E <= 256 ? 2 : 8, false};
+  if (!aligned || E % V != 0) {
+    const int words = (E + (E % 4 ? 3 : 0) + 3) / 4;       // that a row may have a part of
+    if (words <= 16) return {8, words <= 8 ? 1 : 2, false};
+    if (words <= 32) return {16, 2, false};
+    return {32, words <= 64 ? 2 : words <= 128 ? 4 : words <= 192 ? 6 : 9, false};
+  }
   const int words = E / V, want = 16 / V;            // 16 elements a lane
   if (words <= 8 * want) return {8, words <= 8 ? 1 : words <= 16 ? 2 : 4, true};
   if (words <= 16 * want) return {16, want, true};
@@ -494,8 +583,14 @@ RowShape row_shape(int E, bool aligned) {
 // 2 to 8 for 32.
 #define DFA3D_ROWS(T, r, GO)                                                                     \
   if (!r.vec) {                                                                                  \
-    if (r.K == 2) GO(4, 2, 32, false);                                                           \
-    else GO(4, 8, 32, false);                                                                    \
+    if (r.lanes == 8) {                                                                          \
+      if (r.K == 1) GO(4, 1, 8, false);                                                          \
+      else GO(4, 2, 8, false);                                                                   \
+    } else if (r.lanes == 16) GO(4, 2, 16, false);                                               \
+    else if (r.K == 2) GO(4, 2, 32, false);                                                      \
+    else if (r.K == 4) GO(4, 4, 32, false);                                                      \
+    else if (r.K == 6) GO(4, 6, 32, false);                                                      \
+    else GO(4, 9, 32, false);                                                                    \
   } else if constexpr (sizeof(T) == 4) {                                                         \
     if (r.lanes == 8) {                                                                          \
       if (r.K == 1) GO(4, 1, 8, true);                                                           \
@@ -550,11 +645,12 @@ cudaError_t norm_forward(const T *x, const T *residual, const float *gamma, cons
                          const DropRule &d, float eps, T *y, float *mean, float *rstd, cudaStream_t s) {
   const RowShape r = row_shape<T>(E, on_grid(x, 16) && on_grid(residual, 16) && on_grid(y, 16) && on_grid(gamma, 16) &&
                                          on_grid(beta, 16));
-  const unsigned grid = (unsigned)row_ctas(rows, r.lanes, 1, 148 * kForwardResident);
+  const bool wide = on_grid(x, 4 * sizeof(T)) && on_grid(residual, 4 * sizeof(T)) && on_grid(y, 4 * sizeof(T));
+  const unsigned grid = (unsigned)row_ctas(rows, r.lanes, 1, 148 * (r.vec ? kForwardResident : kOddResident));
   const size_t shared = ring_bytes(r, 2);
 #define DFA3D_GO(V, K, LANES, VEC)                                                                                      \
-  return launch_rows<dropout_add_layer_norm_kernel<T, V, K, LANES, VEC>>(grid, shared, s, x, residual, gamma, beta, rows, E, d, \
-                     eps, y, mean, rstd)
+  return launch_rows<dropout_add_layer_norm_kernel<T, V, K, LANES, VEC>>(grid, shared, s, x, residual, gamma, beta, rows, E, wide, \
+                     d, eps, y, mean, rstd)
   DFA3D_ROWS(T, r, DFA3D_GO)
 #undef DFA3D_GO
 }
@@ -568,13 +664,15 @@ cudaError_t norm_backward(const T *grad_y, const T *x, const T *residual, const 
                           float *grad_gamma, float *grad_beta, float *partial, cudaStream_t s) {
   const RowShape r = row_shape<T>(E, on_grid(x, 16) && on_grid(residual, 16) && on_grid(grad_y, 16) && on_grid(gamma, 16) &&
                                          on_grid(grad_x, 16) && on_grid(grad_residual, 16));      // null is on the grid
+  const bool wide = on_grid(x, 4 * sizeof(T)) && on_grid(residual, 4 * sizeof(T)) && on_grid(grad_y, 4 * sizeof(T)) &&
+                    on_grid(grad_x, 4 * sizeof(T)) && on_grid(grad_residual, 4 * sizeof(T));
   const unsigned grid = (unsigned)backward_ctas(rows, r.lanes);
   if (!grad_gamma) partial = nullptr;
   cudaError_t rc = cudaSuccess;
 #define DFA3D_GO(V, K, LANES, VEC)                                                                                            \
   rc = launch_rows<dropout_layer_norm_backward_kernel<T, V, K, LANES, VEC>>(                                                   \
       grid, std::max(ring_bytes(r, 3), sizeof(float) * kWarps * 32 * V * K), s, grad_y, x, residual, gamma, mean, rstd, rows,   \
-      E, d, grad_x, grad_residual, partial)
+      E, wide, d, grad_x, grad_residual, partial)
   DFA3D_ROWS(T, r, DFA3D_GO)
 #undef DFA3D_GO
   if (rc != cudaSuccess || !partial) return rc;

@@ -85,19 +85,6 @@ __device__ __forceinline__ void words_of(const DropRule &d, DropKey k, unsigned 
     words[i] = w.x; words[i + 1] = w.y; words[i + 2] = w.z; words[i + 3] = w.w;
   }
 }
-// The same for any `first`; V = 4.
-__device__ __forceinline__ void words_of_any(const DropRule &d, DropKey k, unsigned long long first, uint32_t (&words)[4]) {
-  if (!d.rng) {
-    words[0] = words[1] = words[2] = words[3] = ~0u;
-    return;
-  }
-  const PhiloxWords a = philox_words(first >> 2, d.site, k), b = philox_words((first >> 2) + 1, d.site, k);
-  const uint32_t skip = (uint32_t)first & 3u;
-  words[0] = skip == 0 ? a.x : skip == 1 ? a.y : skip == 2 ? a.z : a.w;
-  words[1] = skip == 0 ? a.y : skip == 1 ? a.z : skip == 2 ? a.w : b.x;
-  words[2] = skip == 0 ? a.z : skip == 1 ? a.w : skip == 2 ? b.x : b.y;
-  words[3] = skip == 0 ? a.w : skip == 1 ? b.x : skip == 2 ? b.y : b.z;
-}
 #endif
 
 }  // namespace dfa3d

@@ -269,6 +269,31 @@ def test_rows_past_two_to_the_31_elements(lib_built):
     assert not gx[-last:].cpu()[~keep].any()
 
 
+@pytest.mark.parametrize("dtype", R.DTYPES, ids=str)
+@pytest.mark.parametrize("rows,E", [(9, 2), (9, 3), (40, 5), (33, 250), (33, 253), (33, 254), (33, 255), (18, 509), (18, 510), (18, 511),
+                                    (11, 1021), (11, 1022), (5003, 6), (2500, 61)])
+def test_rows_that_begin_inside_of_a_word(lib_built, rows, E, dtype):
+    tensors, g = inputs(rows, E, dtype)
+    check(True, tensors, g, 0.2, 7, 4)
+
+
+@pytest.mark.parametrize("dtype", R.DTYPES, ids=str)
+@pytest.mark.parametrize("E", [5, 30, 202, 255, 511, 1022])
+def test_rows_without_numbers_spoil_no_neighbour(lib_built, E, dtype):
+    tensors, g = inputs(30, E, dtype)
+    results = []
+    for spoiled in (False, True):
+        x, r, w, b = [t.clone() for t in tensors]
+        go = g.clone()
+        if spoiled:
+            x[1::2], r[1::2], go[1::2] = float("nan"), float("inf"), float("nan")
+        leaves = [x.requires_grad_(True), r.requires_grad_(True)]
+        y = apply(True, x, r, w, b, seed_tensor(3), 0.3, 2)
+        results.append([t[::2] for t in (y.detach(), *torch.autograd.grad(y, leaves, go))])
+    for a, c in zip(*results):
+        assert torch.equal(a, c)
+
+
 def _words(first, last, seed, site):
     from test_gpu_dropout import _words_from
     return _words_from(first, last, seed, site)
