@@ -561,19 +561,31 @@ group_grad_merge_kernel(const GnArgs a, int merges, const float2 *by_group, cons
   }
 }
 
-// grad_weight, grad_bias (weight_rows, C): by_level summed over images, and over levels where they share the weights.
-__device__ __forceinline__ void parameter_sums(const GnArgs &a, const float2 *by_level, int column, float *grad_weight,
+// grad_weight, grad_bias (weight_rows, C): by_level summed over images, and over levels where they share the weights.  32 columns a
+// CTA, whose warps take the (image, level)s in turn.
+template <int WARPS>
+__device__ __forceinline__ void parameter_sums(const GnArgs &a, const float2 *by_level, int chunk, float *grad_weight,
                                                float *grad_bias) {
-  if (column >= a.weight_rows * a.C) return;
-  const int row = column / a.C, c = column - row * a.C, levels = a.weight_rows == 1 ? a.L : 1;
+  __shared__ float2 part[WARPS][32];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, column = chunk * 32 + lane;
+  const int row = column / a.C, c = column - row * a.C, every = a.weight_rows == 1 ? 1 : a.L, terms = a.B * a.L / every;
+  const bool mine = column < a.weight_rows * a.C;
   float2 s = make_float2(0.f, 0.f);
-  for (int l = row; l < row + levels; ++l)
-#pragma unroll 8
-    for (int b = 0; b < a.B; ++b) {
-      const float2 v = __ldcg(by_level + ((long long)b * a.L + l) * a.C + c);
+  if (mine)
+#pragma unroll 4
+    for (int t = warp; t < terms; t += WARPS) {
+      const float2 v = __ldcg(by_level + ((long long)t * every + row) * a.C + c);
       s.x += v.x;
       s.y += v.y;
     }
+  part[warp][lane] = s;
+  __syncthreads();
+  if (warp != 0 || !mine) return;
+#pragma unroll
+  for (int w = 1; w < WARPS; ++w) {
+    s.x += part[w][lane].x;
+    s.y += part[w][lane].y;
+  }
   grad_bias[column] = s.x;
   grad_weight[column] = s.y;
 }
@@ -590,7 +602,7 @@ group_grad_apply_kernel(const T *__restrict__ grad_y, const T *__restrict__ x, c
   const int beyond = (int)blockIdx.x - tiles;
   if (beyond >= 0) {
     launch_wait();
-    parameter_sums(a, by_level, beyond * kThreads<V> + threadIdx.x, grad_weight, grad_bias);
+    parameter_sums<kThreads<V> / 32>(a, by_level, beyond, grad_weight, grad_bias);
     return;
   }
   make_table(seg, a);
@@ -750,7 +762,7 @@ cudaError_t backward(const T *grad_y, const T *x, GnArgs a, const float *mean, c
   const unsigned merges = merge_grid(a), channels = grad_weight ? (unsigned)(a.B * a.L * ((a.C + 31) / 32)) : 0;
   DFA3D_TRY(launch(group_grad_merge_kernel, merges + channels, kMergeThreads, 0, true, st, a, merges, by_group, by_channel, means,
                    by_level));
-  const int sums = grad_weight ? (a.C * a.weight_rows + kThreads<V> - 1) / kThreads<V> : 0;
+  const int sums = grad_weight ? (a.C * a.weight_rows + 31) / 32 : 0;
   return launch(apply, sums + (grad_x ? grid : 0), kThreads<V>, 0, true, st, grad_y, x, a, grad_x ? (int)grid : 0, mean, rstd, means, by_level, grad_x,
                 grad_weight, grad_bias);
 }
