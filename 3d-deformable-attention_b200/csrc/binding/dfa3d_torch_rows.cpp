@@ -169,7 +169,7 @@ struct Levels : Kept {
 Tensor level_workspace(const Levels &s, const Tensor &like, bool backward) {
   const int64_t bytes = lib.dfa3d_group_norm_workspace(s.B, s.N, s.C, s.G, s.L, backward);
   TORCH_CHECK(bytes >= 0, "dfa3d_group_norm_workspace failed: ", lib.dfa3d_last_error());
-  return at::empty({bytes}, like.options().dtype(at::kByte));
+  return bytes == 0 ? Tensor() : at::empty({bytes}, like.options().dtype(at::kByte));
 }
 
 Tensor group_norm_forward(const Levels &s, const Tensor &x, const Tensor &w, const Tensor &b, const Tensor &shapes,
@@ -178,7 +178,8 @@ Tensor group_norm_forward(const Levels &s, const Tensor &x, const Tensor &w, con
   float *mean = stats.defined() ? fpm(stats) : nullptr;
   check(lib.dfa3d_group_norm_forward(vp(x), dtype_code(x), s.B, s.N, s.C, s.G, (const int64_t *)vp(shapes), s.stride,
                                      (const int64_t *)vp(lsi), s.L, fp(w), fp(b), s.rows, s.eps, s.act, vpm(y), mean,
-                                     mean ? mean + (int64_t)s.B * s.L * s.G : nullptr, vpm(work), work.numel(), stream_of(x)),
+                                     mean ? mean + (int64_t)s.B * s.L * s.G : nullptr, vpm(work), work.defined() ? work.numel() : 0,
+                                     stream_of(x)),
         "dfa3d_group_norm_forward");
   return y;
 }

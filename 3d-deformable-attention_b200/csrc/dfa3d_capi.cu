@@ -868,6 +868,7 @@ static int check_group_norm(int32_t B, int32_t N, int32_t C, int32_t G, const in
   return DFA3D_OK;
 }
 static int check_group_norm_workspace(const void *workspace, int64_t have, long long need) {
+  if (need == 0) return DFA3D_OK;
   REQUIRE_PTR(workspace); REQUIRE_ALIGNED(workspace);
   if (have < need)
     return fail(DFA3D_ERR_INVALID_ARGUMENT, "workspace of %lld bytes is smaller than the %lld needed", (long long)have, need);

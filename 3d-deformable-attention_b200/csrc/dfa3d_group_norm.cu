@@ -17,6 +17,8 @@
 // second runs.  All tiles of a launch are resident at once, and the third walks each from its end, whose rows the first has left in
 // L2 (126 MB).
 //
+// Forwards of images of up to 256 rows of 1024 channels (1024 of 256) are one launch: a cluster of CTAs has a level of an image.
+//
 // 6 x 30 825 x 256, 32 groups, 4 levels: fp32 (189 MB) forward 96 us, backward 156; bf16 50 and 84; 6 x 920 x 256 fp32 11 and 11.
 // The result's launch runs at the rate of a copy (57 us for 378 MB, the same with rows from L2 or not), the fp32 statistics at
 // 5.7 TB/s, the bf16 ones (25 us for 95 MB) at the rate of their instructions.  Measured against it, fp32 forward / backward: one
@@ -197,11 +199,75 @@ struct Moments {
   }
 };
 
-// A tile's statistics into partial (B, entries, G): mean and sum of squares around it, of each piece's values of a group.
+// Mean and sum of squares around it of a group's values in `rows` rows from `base` on (the CTA's): dst (G).  Ends with a barrier.
+template <typename T, int V>
+__device__ __forceinline__ void moments_of_piece(const T *base, int rows, const GnArgs &a, const Place &at, float2 *chan, float *count,
+                                                 float2 *dst) {
+  constexpr int U = kAhead;
+  const long long step = (long long)a.RL * a.C;
+  // a thread's channels are of one group where V divides it: one entry for all of them, or one for each
+  const int lane = threadIdx.x & 31, sub = lane & 7, width = a.whole ? a.nv : a.C, per = (int)a.by_per.d;
+  if (at.rl < a.RL) {
+    Moments<V> k;
+    Word<T, V> w[U];
+    int r = 0;
+    for (; r + U * a.RL <= rows; r += U * a.RL, base += U * step) {
+      load_rows<T, V, U, false, true>(base, at.at, r, rows, a.RL, step, w);
+      k.template add<T, U, true>(w, U);
+    }
+    if (r + at.rl < rows) {
+      load_rows<T, V, U, false, false>(base, at.at, r + at.rl, rows, a.RL, step, w);
+      int have = 0;
+#pragma unroll
+      for (int u = 0; u < U; ++u) have += r + at.rl + u * a.RL < rows;
+      k.template add<T, U, false>(w, have);
+    }
+    if (a.whole) {
+      float m = 0.f, q = 0.f;
+#pragma unroll
+      for (int c = 0; c < V; ++c) m += k.mean[c];
+      m *= 1.f / V;
+#pragma unroll
+      for (int c = 0; c < V; ++c) q += fmaf((k.mean[c] - m) * (k.mean[c] - m), k.n, k.m2[c]);
+      chan[at.rl * width + at.cv] = make_float2(m, q);
+    } else {
+#pragma unroll
+      for (int c = 0; c < V; ++c) chan[at.rl * width + at.cv * V + c] = make_float2(k.mean[c], k.m2[c]);
+    }
+    if (at.cv == 0) count[at.rl] = a.whole ? k.n * V : k.n;
+  }
+  __syncthreads();
+  // eight lanes have a group
+  const float inv_n = __fdividef(1.f, (float)rows * (float)a.cpg);
+  const int l0 = quotient(sub, a.by_per), j0 = sub - l0 * per, dl = quotient(8, a.by_per), dj = 8 - dl * per;
+  for (int g0 = (threadIdx.x >> 5) * 4; g0 < a.G; g0 += kThreads<V> / 8) {
+    const int g = g0 + (lane >> 3), RL = g < a.G ? a.RL : 0;
+    const float2 *entries = chan + g * per;
+    float s = 0.f, q = 0.f;
+#pragma unroll 1
+    for (int l = l0, j = j0; l < RL; l += dl) {
+      s = fmaf(count[l], entries[l * width + j].x, s);
+      j += dj;
+      if (j >= per) j -= per, ++l;
+    }
+    const float m = sum8(s) * inv_n;
+#pragma unroll 1
+    for (int l = l0, j = j0; l < RL; l += dl) {
+      const float2 v = entries[l * width + j];
+      q += fmaf((v.x - m) * (v.x - m), count[l], v.y);
+      j += dj;
+      if (j >= per) j -= per, ++l;
+    }
+    q = sum8(q);
+    if (sub == 0 && RL) dst[g] = make_float2(m, q);
+  }
+  __syncthreads();
+}
+
+// A tile's statistics into partial (B, entries, G), of each of its pieces.
 template <typename T, int V>
 __global__ void __launch_bounds__(kThreads<V>, kResident<V>)
 group_stats_kernel(const T *__restrict__ x, const GnArgs a, float2 *__restrict__ partial) {
-  constexpr int U = kAhead;
   extern __shared__ float2 chan[];                       // a thread's channels
   __shared__ float count[kThreads<V>];                   // values that an entry of a row lane stands for
   __shared__ SegmentTable seg;
@@ -209,69 +275,12 @@ group_stats_kernel(const T *__restrict__ x, const GnArgs a, float2 *__restrict__
   make_table(seg, a);
   Tile tile(a, seg, false);
   const Place at(a);
-  const long long step = (long long)a.RL * a.C;
-  // a thread's channels are of one group where V divides it: one entry for all of them, or one for each
-  const int lane = threadIdx.x & 31, sub = lane & 7, width = a.whole ? a.nv : a.C, per = (int)a.by_per.d;
   for (int lo = tile.r0; lo < tile.r1; ++tile.i) {
     const int hi = min(tile.r1, seg.end[tile.i]), rows = hi - lo, from = lo;
     lo = hi;
     if (rows <= 0 || (tile.i & 1) == 0) continue;
-    if (at.rl < a.RL) {
-      const T *base = x + ((long long)tile.b * a.N + from) * a.C;
-      Moments<V> k;
-      Word<T, V> w[U];
-      int r = 0;
-      for (; r + U * a.RL <= rows; r += U * a.RL, base += U * step) {
-        load_rows<T, V, U, false, true>(base, at.at, r, rows, a.RL, step, w);
-        k.template add<T, U, true>(w, U);
-      }
-      if (r + at.rl < rows) {
-        load_rows<T, V, U, false, false>(base, at.at, r + at.rl, rows, a.RL, step, w);
-        int have = 0;
-#pragma unroll
-        for (int u = 0; u < U; ++u) have += r + at.rl + u * a.RL < rows;
-        k.template add<T, U, false>(w, have);
-      }
-      if (a.whole) {
-        float m = 0.f, q = 0.f;
-#pragma unroll
-        for (int c = 0; c < V; ++c) m += k.mean[c];
-        m *= 1.f / V;
-#pragma unroll
-        for (int c = 0; c < V; ++c) q += fmaf((k.mean[c] - m) * (k.mean[c] - m), k.n, k.m2[c]);
-        chan[at.rl * width + at.cv] = make_float2(m, q);
-      } else {
-#pragma unroll
-        for (int c = 0; c < V; ++c) chan[at.rl * width + at.cv * V + c] = make_float2(k.mean[c], k.m2[c]);
-      }
-      if (at.cv == 0) count[at.rl] = a.whole ? k.n * V : k.n;
-    }
-    __syncthreads();
-    // eight lanes have a group
-    const float inv_n = __fdividef(1.f, (float)rows * (float)a.cpg);
-    const int l0 = quotient(sub, a.by_per), j0 = sub - l0 * per, dl = quotient(8, a.by_per), dj = 8 - dl * per;
-    for (int g0 = (threadIdx.x >> 5) * 4; g0 < a.G; g0 += kThreads<V> / 8) {
-      const int g = g0 + (lane >> 3), RL = g < a.G ? a.RL : 0;
-      const float2 *entries = chan + g * per;
-      float s = 0.f, q = 0.f;
-#pragma unroll 1
-      for (int l = l0, j = j0; l < RL; l += dl) {
-        s = fmaf(count[l], entries[l * width + j].x, s);
-        j += dj;
-        if (j >= per) j -= per, ++l;
-      }
-      const float m = sum8(s) * inv_n;
-#pragma unroll 1
-      for (int l = l0, j = j0; l < RL; l += dl) {
-        const float2 v = entries[l * width + j];
-        q += fmaf((v.x - m) * (v.x - m), count[l], v.y);
-        j += dj;
-        if (j >= per) j -= per, ++l;
-      }
-      q = sum8(q);
-      if (sub == 0 && RL) partial[((long long)tile.b * a.entries + tile.t + tile.i) * a.G + g] = make_float2(m, q);
-    }
-    __syncthreads();
+    moments_of_piece<T, V>(x + ((long long)tile.b * a.N + from) * a.C, rows, a, at, chan, count,
+                           partial + ((long long)tile.b * a.entries + tile.t + tile.i) * a.G);
   }
 }
 
@@ -407,6 +416,126 @@ group_apply_kernel(const T *__restrict__ x, const GnArgs a, const float *mean_in
       for (int u = 0; u < U; ++u) store(u);
     }
   }
+}
+
+// ------------------------------------------------------------------------------------------------
+// small images: one launch
+// ------------------------------------------------------------------------------------------------
+// A cluster of CTAs has a level of an image: each keeps the sums of its own rows in shared memory, reads those of the others behind a
+// barrier of the cluster, and goes through its rows, which the L1 still has, once more.
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+__device__ __forceinline__ float2 of_rank(const float2 *p, int rank) {
+  unsigned at;
+  float2 v;
+  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"((unsigned)__cvta_generic_to_shared(p)), "r"(rank));
+  asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(at) : "memory");
+  return v;
+}
+
+constexpr int kMaxCluster = 8;
+
+// A CTA's rows [r0, r1) of level l of image b: `per` rows to each of `size` CTAs, as far as the level goes.
+struct Share {
+  int b, l, rank, size, begin, end, per, r0, r1;
+  __device__ __forceinline__ Share(const GnArgs &a, const SegmentTable &seg) {
+    asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
+    asm("mov.u32 %0, %%cluster_nctaid.x;" : "=r"(size));
+    const int q = ((int)blockIdx.x - rank) / size;
+    b = quotient(q, a.by_levels);
+    l = q - b * a.L;
+    begin = segment_begin(seg, 2 * l + 1);
+    end = seg.end[2 * l + 1];
+    per = (end - begin + size - 1) / size;
+    r0 = min(begin + rank * per, end);
+    r1 = min(r0 + per, end);
+  }
+  __device__ __forceinline__ int rows_of(int j) const { return max(0, min(end - begin - j * per, per)); }
+};
+
+// The rows of no level before level l, and behind the last one.
+template <typename T, int V>
+__device__ __forceinline__ void zero_gaps(const GnArgs &a, const SegmentTable &seg, const Share &k, const Place &at, T *out) {
+  if (at.rl >= a.RL) return;
+  for (int i = 2 * k.l; i <= 2 * a.L; i += 2 * (a.L - k.l)) {
+    const int begin = segment_begin(seg, i), first = k.rank * a.RL;
+    zero_rows<T, V>(out + ((long long)k.b * a.N + begin + first) * a.C, at.at, first + at.rl, seg.end[i] - begin, k.size * a.RL,
+                    (long long)k.size * a.RL * a.C);
+    if (k.l + 1 < a.L) break;
+  }
+}
+
+template <typename T, int V, bool ACT>
+__global__ void __launch_bounds__(kThreads<V>, kResident<V>)
+group_image_kernel(const T *__restrict__ x, const GnArgs a, float *__restrict__ mean_out, float *__restrict__ rstd_out,
+                   T *__restrict__ y) {
+  constexpr int U = kAhead;
+  extern __shared__ float2 chan[];
+  __shared__ float count[kThreads<V>];
+  __shared__ SegmentTable seg;
+  float2 *own = chan + kThreads<V> * V, *merged = own + a.G;      // (G) each: of the CTA's rows; mean and rstd of the level
+  make_table(seg, a);
+  const Share k(a, seg);
+  const Place at(a);
+  const int rows = k.r1 - k.r0;
+  const long long first = ((long long)k.b * a.N + k.r0) * a.C, step = (long long)a.RL * a.C;
+  moments_of_piece<T, V>(x + first, rows, a, at, chan, count, own);
+  cluster_arrive();
+  cluster_wait();
+  for (int g = threadIdx.x; g < a.G; g += kThreads<V>) {
+    float2 v[kMaxCluster];
+#pragma unroll
+    for (int j = 0; j < kMaxCluster; ++j)
+      if (j < k.size) v[j] = of_rank(own + g, j);
+    float n = 0.f, mean = 0.f, m2 = 0.f;
+#pragma unroll
+    for (int j = 0; j < kMaxCluster; ++j)
+      if (j < k.size && k.rows_of(j) > 0) {
+        const float nb = (float)k.rows_of(j) * (float)a.cpg, total = n + nb, part = __fdividef(nb, total), delta = v[j].x - mean;
+        mean = fmaf(delta, part, mean);
+        m2 += fmaf(delta * delta, n * part, v[j].y);
+        n = total;
+      }
+    const float rstd = n > 0.f ? rsqrtf(__fdividef(m2, n) + a.eps) : 0.f;
+    merged[g] = make_float2(mean, rstd);
+    if (k.rank == 0 && mean_out) {
+      const long long to = ((long long)k.b * a.L + k.l) * a.G + g;
+      mean_out[to] = mean;
+      rstd_out[to] = rstd;
+    }
+  }
+  cluster_arrive();                                      // done with the others' shared memory
+  __syncthreads();
+  if (at.rl < a.RL) {
+    int group[V];
+    float mean[V], scale[V], shift[V];
+    groups_of<V>(a, at.cv, group);
+    const int w0 = (a.weight_rows == 1 ? 0 : k.l) * a.C + at.cv * V;
+    params_of<V>(a, a.weight + w0, scale);
+    params_of<V>(a, a.bias + w0, shift);
+#pragma unroll
+    for (int c = 0; c < V; ++c) {
+      mean[c] = merged[group[c]].x;
+      scale[c] *= merged[group[c]].y;
+    }
+    const T *in = x + first;
+    T *out = y + first;
+    for (int r = at.rl; r < rows; r += U * a.RL, in += U * step, out += U * step) {
+      Word<T, V> w[U];
+      load_rows<T, V, U, false, false>(in, at.at, r, rows, a.RL, step, w);
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        if (r + u * a.RL >= rows) break;
+        float f[V];
+        widen_word<T, V>(w[u], f);
+#pragma unroll
+        for (int c = 0; c < V; ++c) f[c] = activate<ACT>(fmaf(f[c] - mean[c], scale[c], shift[c]), a.act);
+        store_word<T, V>(out + u * step + at.at, f);
+      }
+    }
+  }
+  zero_gaps<T, V>(a, seg, k, at, y);
+  cluster_wait();
 }
 
 // ------------------------------------------------------------------------------------------------
@@ -692,6 +821,18 @@ int tile_rows(int B, int N, int C, int V) {
   return (int)std::min<long long>(rows, N);
 }
 
+// CTAs of a cluster that has a level of an image in one launch, or 0 for three launches of tiles: up to eight, while a thread would
+// have more than eight rows, and none where it would have more than 32 of eight.  us, one launch / three (host 6.4 / 11):
+// 2 x 336 x 128 fp32 5.7 / 6.2, 375 x 256 6.7 / 6.2, 200 x 40 x 64 bf16 6.1 / 7.0, 2000 x 16 x 64 fp32 25 / 30, 6 x 920 x 256 10.5 / 10.3; with
+// more rows 1600 x 256 bf16 11.0 / 8.3, 5800 x 64 15.4 / 9.1.  The backward stays with three: 23 / 12 at 6 x 920 x 256.
+int cluster_size(int N, int C) {
+  const int rows = 1024 / C;                             // that a CTA of any word reads at a time
+  if (N > kMaxCluster * 32 * rows) return 0;
+  int size = 1;
+  while (size < kMaxCluster && N > size * 8 * rows) size *= 2;
+  return size;
+}
+
 void complete(GnArgs &a, int V) {
   a.cpg = a.C / a.G;
   a.V = V;
@@ -710,22 +851,35 @@ void complete(GnArgs &a, int V) {
   a.wide_params = a.C % 4 == 0 && ((reinterpret_cast<uintptr_t>(a.weight) | reinterpret_cast<uintptr_t>(a.bias)) & 15) == 0;
 }
 
-// A launch that may begin while the one before it in the sequence runs (`follows`).
 template <typename... P, typename... A>
-cudaError_t launch(void (*kernel)(P...), unsigned grid, int threads, size_t shared, bool follows, cudaStream_t st, A... args) {
-  cudaLaunchAttribute at[1];
-  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  at[0].val.programmaticStreamSerializationAllowed = 1;
+cudaError_t launch_with(void (*kernel)(P...), unsigned grid, int threads, size_t shared, cudaLaunchAttribute *at, int count,
+                        cudaStream_t st, A... args) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(grid);
   cfg.blockDim = dim3(threads);
   cfg.dynamicSmemBytes = shared;
   cfg.stream = st;
   cfg.attrs = at;
-  cfg.numAttrs = follows ? 1 : 0;
+  cfg.numAttrs = count;
   return cudaLaunchKernelEx(&cfg, kernel, static_cast<P>(args)...);
 }
-
+// A launch that may begin while the one before it in the sequence runs (`follows`).
+template <typename... P, typename... A>
+cudaError_t launch(void (*kernel)(P...), unsigned grid, int threads, size_t shared, bool follows, cudaStream_t st, A... args) {
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  return launch_with(kernel, grid, threads, shared, at, follows ? 1 : 0, st, args...);
+}
+// ... of clusters of `size` CTAs.
+template <typename... P, typename... A>
+cudaError_t launch_clusters(void (*kernel)(P...), unsigned grid, int size, int threads, size_t shared, cudaStream_t st, A... args) {
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = size;
+  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+  return launch_with(kernel, grid, threads, shared, at, 1, st, args...);
+}
 #define DFA3D_TRY(call) do { const cudaError_t rc_ = (call); if (rc_ != cudaSuccess) return rc_; } while (0)
 
 unsigned merge_grid(const GnArgs &a) {
@@ -735,6 +889,11 @@ unsigned merge_grid(const GnArgs &a) {
 template <typename T, int V>
 cudaError_t forward(const T *x, GnArgs a, T *y, float *mean, float *rstd, void *workspace, cudaStream_t st) {
   complete(a, V);
+  if (const int size = cluster_size(a.N, a.C)) {
+    auto all = a.act == kNone ? group_image_kernel<T, V, false> : group_image_kernel<T, V, true>;
+    return launch_clusters(all, (unsigned)(a.B * a.L * size), size, kThreads<V>, sizeof(float2) * (kThreads<V> * V + 2 * a.G), st, x, a,
+                           mean, rstd, y);
+  }
   float2 *partial = static_cast<float2 *>(workspace);
   if (!mean) {                                           // nobody keeps them: behind the tiles' parts
     mean = reinterpret_cast<float *>(partial + (long long)a.B * a.entries * a.G);
@@ -792,7 +951,7 @@ GnArgs arguments(int B, int N, int C, int G, const int64_t *shapes, int shape_st
 
 // For any word that a launch may read by.
 long long group_norm_workspace(int B, int N, int C, int G, int L, bool backward) {
-  if (B == 0 || N == 0) return 0;
+  if (B == 0 || N == 0 || (!backward && cluster_size(N, C))) return 0;
   long long pieces = 0;
   for (int V = 4; V >= 1; V /= 2)
     if (C % V == 0) {

@@ -448,7 +448,8 @@ int dfa3d_dropout_add_layer_norm_backward(const void *grad_y, const void *x, con
  * null with L = 1: the N rows are one level.  A table that points outside of the N rows or overlaps is cut to disjoint
  * levels; rows of no level become 0 in y and in grad_x.  weight, bias fp32 (weight_rows, C) with weight_rows 1 (shared by
  * the levels) or L.  C <= 1024, G divides C.  dtype (of x, y and their gradients): DFA3D_DTYPE_F32, _BF16 or _F16.
- * mean, rstd (B, L, G) fp32 for the backward; may be null together in the forward.  Results overlap no input. */
+ * mean, rstd (B, L, G) fp32 for the backward; may be null together in the forward.  Results overlap no input.
+ * The workspace may be null where it has 0 bytes (forwards of small images). */
 int64_t dfa3d_group_norm_workspace(int32_t B, int32_t N, int32_t C, int32_t G, int32_t L, int32_t backward);
 
 int dfa3d_group_norm_forward(const void *x, int32_t dtype, int32_t B, int32_t N, int32_t C, int32_t G,

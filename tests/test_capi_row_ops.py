@@ -20,7 +20,7 @@ NORM = dict(x=OK, residual=OK, gamma=OK, beta=OK, dtype=0, rows=4, E=8, p=0.1, s
             stream=None)
 NORM_BACK = dict(grad_y=OK, x=OK, residual=OK, gamma=OK, mean=OK, rstd=OK, dtype=0, rows=4, E=8, p=0.1, seed=OK, site=0, grad_x=OK,
                  grad_residual=OK, grad_gamma=OK, grad_beta=OK, workspace=OK, bytes=1 << 20, stream=None)
-GROUP = dict(x=OK, dtype=0, B=2, N=10, C=8, G=2, shapes=OK, stride=2, start=OK, L=2, weight=OK, bias=OK, weight_rows=1, eps=1e-5,
+GROUP = dict(x=OK, dtype=0, B=2, N=40000, C=8, G=2, shapes=OK, stride=2, start=OK, L=2, weight=OK, bias=OK, weight_rows=1, eps=1e-5,
              activation=0, y=OK, mean=OK, rstd=OK, workspace=OK, bytes=1 << 20, stream=None)
 GROUP_BACK = dict(grad_y=OK, x=OK, dtype=0, B=2, N=10, C=8, G=2, shapes=OK, stride=2, start=OK, L=2, weight=OK, bias=OK,
                   weight_rows=1, activation=0, mean=OK, rstd=OK, grad_x=OK, grad_weight=OK, grad_bias=OK, workspace=OK,
@@ -92,7 +92,7 @@ def test_sizes_are_checked(lib):
         refused(lib, call(lib, name, N=1 << 30), b"too many", -2)
         refused(lib, call(lib, name, N=3000, B=1 << 21), b"too many", -2)
         refused(lib, call(lib, name, N=1, B=1 << 28), b"too many", -2)
-        refused(lib, call(lib, name, N=1, B=1 << 26, workspace=None), b"workspace")
+        refused(lib, call(lib, name, N=40000, B=1 << 19, workspace=None), b"workspace")
         refused(lib, call(lib, name, weight_rows=3), b"weight_rows")
         refused(lib, call(lib, name, stride=1), b"shape_stride")
         refused(lib, call(lib, name, start=None), b"together")
@@ -110,10 +110,11 @@ def test_workspaces_are_asked_for_and_checked(lib):
     assert lib.dfa3d_dropout_add_layer_norm_workspace(0, 256) == 0
     assert lib.dfa3d_dropout_add_layer_norm_workspace(5, 2000) == -2
     for backward, name in ((0, "dfa3d_group_norm_forward"), (1, "dfa3d_group_norm_backward")):
-        need = lib.dfa3d_group_norm_workspace(2, 1000, 64, 4, 2, backward)
+        need = lib.dfa3d_group_norm_workspace(2, 9000, 64, 4, 2, backward)
         assert need > 0
-        refused(lib, call(lib, name, N=1000, C=64, G=4, bytes=need - 1), b"workspace")
+        refused(lib, call(lib, name, N=9000, C=64, G=4, bytes=need - 1), b"workspace")
         refused(lib, call(lib, name, workspace=24), b"workspace")
+    assert lib.dfa3d_group_norm_workspace(2, 1000, 64, 4, 2, 0) == 0            # one launch
     assert lib.dfa3d_group_norm_workspace(2, 0, 64, 4, 2, 1) == 0
     assert lib.dfa3d_group_norm_workspace(2, 10, 64, 5, 2, 1) == -1
 

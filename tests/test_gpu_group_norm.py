@@ -145,6 +145,30 @@ def test_level_tables_that_leave_rows_out(lib_built, levels, start, N, segments,
 
 
 @pytest.mark.parametrize("dtype", R.DTYPES, ids=str)
+@pytest.mark.parametrize("B,C,G,levels,start,N", [
+    (2, 96, 12, [(60, 70), (30, 35), (8, 9), (1, 1)], [5, 4300, 5360, 5432], 5500),      # gaps and rows behind the last level
+    (1, 90, 6, [(41, 70), (0, 3), (30, 30)], [0, 2870, 2900], 3800),
+    (1, 15, 5, [(120, 130), (50, 60)], [100, 15700], 19000),
+    (3, 256, 32, [(20, 30), (20, 30)], [0, 500], 1500),                                   # the second begins inside of the first
+    (2, 256, 32, [(20, 30), (10, 15), (5, 8)], [0, 600, 750], 1024),                      # the last size of one launch, and the first
+    (2, 256, 32, [(20, 30), (10, 15), (5, 8)], [0, 600, 750], 1025),                      # of three
+])
+def test_level_tables_of_larger_images(lib_built, B, C, G, levels, start, N, dtype):
+    shapes, lsi = table(levels, start)
+    tensors, g = inputs(B, N, C, dtype, len(levels))
+    segments, at = [], 0
+    for (h, w), first in zip(levels, start):
+        lo = max(first, at)
+        at = max(lo, min(first + h * w, N))
+        segments.append((lo, at))
+    y, gx, _, _ = check(True, tensors, g, G, "silu", shapes, lsi, segments)
+    out = torch.ones(N, dtype=torch.bool)
+    for lo, hi in segments:
+        out[lo:hi] = False
+    assert not y[:, out].any() and not gx[:, out].any()
+
+
+@pytest.mark.parametrize("dtype", R.DTYPES, ids=str)
 @pytest.mark.parametrize("B,N,C,G", [(6, 5000, 256, 32), (1, 23000, 128, 16), (200, 40, 64, 8), (2, 3001, 90, 9)])
 def test_larger_calls_and_the_same_bits_again(lib_built, B, N, C, G, dtype):
     tensors, g = inputs(B, N, C, dtype)

@@ -123,12 +123,13 @@ def test_traced_calls_follow_their_inputs(lib_built):
 
 
 @pytest.mark.parametrize("bad", [float("nan"), float("inf")])
-def test_rows_of_no_level_are_not_looked_at(lib_built, bad):
+@pytest.mark.parametrize("N", [50, 12000])
+def test_rows_of_no_level_are_not_looked_at(lib_built, bad, N):
     g = torch.Generator().manual_seed(0)
-    x, go = torch.randn(2, 50, 24, generator=g).to(DEV), torch.randn(2, 50, 24, generator=g).to(DEV)
+    x, go = torch.randn(2, N, 24, generator=g).to(DEV), torch.randn(2, N, 24, generator=g).to(DEV)
     w, b = torch.rand(24, device=DEV).requires_grad_(True), torch.rand(24, device=DEV).requires_grad_(True)
     shapes, start = torch.tensor([[2, 7], [4, 4]], device=DEV), torch.tensor([3, 20], device=DEV)
-    outside = torch.ones(50, dtype=torch.bool)
+    outside = torch.ones(N, dtype=torch.bool)
     outside[3:17] = outside[20:36] = False
     results = []
     for spoiled in (False, True):
