@@ -21,11 +21,12 @@
 //
 // 6 x 30 825 x 256, 32 groups, 4 levels: fp32 (189 MB) forward 96 us, backward 156; bf16 50 and 84; 6 x 920 x 256 fp32 11 and 11.
 // The result's launch runs at the rate of a copy (57 us for 378 MB, the same with rows from L2 or not), the fp32 statistics at
-// 5.7 TB/s, the bf16 ones (25 us for 95 MB) at the rate of their instructions.  Measured against it, fp32 forward / backward: one
-// launch that walks the images in batches with a barrier of the grid after each 257 / 287 (each barrier leaves every SM waiting
-// through the merge); launches that form the statistics of one batch and the results of the one before 129 to 220 / 241 to 494;
-// batches that fit L2, one after the other, 102 / 178; rows one chunk ahead through shared memory 107 / 167; merges by the CTAs of
-// the third launch instead of a second one 110 / 170; two to six waves of tiles, bf16 forward 54 to 74.
+// 5.6 TB/s; the bf16 ones take 23 us for 95 MB, 15 at that rate and the level table, the first loads and the reduction at the end
+// (arithmetic on two values at once, or 12 and 16 words in flight: 1 %).  Measured against it, fp32 forward / backward: one launch
+// that walks the images in batches with a barrier of the grid after each 257 / 287 (each barrier leaves every SM waiting through the
+// merge); launches that form the statistics of one batch and the results of the one before 129 to 220 / 241 to 494; tiles of both
+// kinds from one queue 146 forward; batches that fit L2, one after the other, 102 / 178; rows one chunk ahead through shared memory
+// 107 / 167; merges by the CTAs of the third launch instead of a second one 110 / 170; two to six waves of tiles, bf16 forward 54 to 74.
 #include <algorithm>
 
 #include "dfa3d_launch.h"
