@@ -1,5 +1,7 @@
 // Native host path of the row operators: dropout without a stored mask, LayerNorm(residual + dropout(x)), group norm over the
 // levels of a feature pyramid.  Same contract as dfa3d_torch.cpp: NotImplemented means that the Python code has to take the call.
+#include <ATen/cuda/EmptyTensor.h>
+
 #include "dfa3d_torch.h"
 
 using namespace dfa3d_torch;
@@ -15,6 +17,12 @@ Tensor like_forward(const Tensor &g, at::ScalarType type) {
 
 bool stored_tensor(PyObject *o, Tensor &t) { return plain_tensor(o, t) && storage_type(t.scalar_type()); }
 
+// Memory for a result, on a's device: what at::empty ends in, without the way through the dispatcher (a call has up to six of them).
+Tensor fresh(at::IntArrayRef sizes, at::ScalarType type, const Tensor &a) {
+  return Tensor(at::detail::empty_cuda(sizes, type, a.device(), std::nullopt));
+}
+Tensor fresh(const Tensor &a) { return fresh(a.sizes(), a.scalar_type(), a); }
+
 bool same_kind(const Tensor &a, const Tensor &b) {
   return a.scalar_type() == b.scalar_type() && a.sizes() == b.sizes() && a.device() == b.device();
 }
@@ -23,7 +31,7 @@ bool same_kind(const Tensor &a, const Tensor &b) {
 // dropout
 // ------------------------------------------------------------------------------------------------
 Tensor dropout_forward(const Tensor &x, const Tensor &res, const Tensor &seed, const Rule &r, bool relu) {
-  Tensor y = at::empty_like(x);
+  Tensor y = fresh(x);
   check(lib.dfa3d_dropout_forward(vp(x), vp(res), dtype_code(x), x.numel(), relu ? DFA3D_ROW_RELU : DFA3D_ROW_NONE, r.p,
                                   seed_of(seed), (int32_t)r.site, vpm(y), stream_of(x)),
         "dfa3d_dropout_forward");
@@ -49,7 +57,7 @@ struct DropoutFn : torch::autograd::Function<DropoutFn> {
     if (ctx->needs_input_grad(0)) {
       const Tensor g = like_forward(grads[0], r->type);
       c10::cuda::CUDAGuard guard(g.device());
-      gx = at::empty_like(g);
+      gx = fresh(g);
       check(lib.dfa3d_dropout_backward(vp(g), vp(v[1]), r->by_result, dtype_code(g), g.numel(), r->p, seed_of(v[0]),
                                        (int32_t)r->site, vpm(gx), stream_of(g)),
             "dfa3d_dropout_backward");
@@ -88,7 +96,7 @@ PyObject *run_dropout(PyObject *const *a, Py_ssize_t n) {
 Tensor drop_norm_forward(const Tensor &x, const Tensor &res, const Tensor &w, const Tensor &b, const Tensor &seed, const Rule &r,
                          double eps, const Tensor &stats) {
   const int64_t E = x.size(-1), rows = x.numel() / E;
-  Tensor y = at::empty_like(x);
+  Tensor y = fresh(x);
   float *mean = stats.defined() ? fpm(stats) : nullptr;
   check(lib.dfa3d_dropout_add_layer_norm_forward(vp(x), vp(res), fp(w), fp(b), dtype_code(x), rows, (int32_t)E, r.p, seed_of(seed),
                                                  (int32_t)r.site, (float)eps, vpm(y), mean, mean ? mean + rows : nullptr,
@@ -102,7 +110,7 @@ struct DropNormFn : torch::autograd::Function<DropNormFn> {
                         const std::optional<Tensor> &seed, const c10::intrusive_ptr<Rule> &r, double eps) {
     c10::cuda::CUDAGuard guard(x.device());
     const Tensor s = seed ? *seed : Tensor();
-    Tensor stats = empty_f32({2, x.numel() / x.size(-1)}, x);
+    Tensor stats = fresh({2, x.numel() / x.size(-1)}, at::kFloat, x);
     Tensor y = drop_norm_forward(x, res, w, b, s, *r, eps, stats);
     keep(ctx, r, {x, res, w, stats, s});
     return y;
@@ -116,12 +124,12 @@ struct DropNormFn : torch::autograd::Function<DropNormFn> {
     const Tensor g = like_forward(grads[0], x.scalar_type());
     const bool params = ctx->needs_input_grad(2) || ctx->needs_input_grad(3);
     Tensor gx, gr, gw, gb, work;
-    if (ctx->needs_input_grad(0)) gx = at::empty_like(g);
-    if (ctx->needs_input_grad(1)) gr = at::empty_like(g);
+    if (ctx->needs_input_grad(0)) gx = fresh(g);
+    if (ctx->needs_input_grad(1)) gr = fresh(g);
     if (params) {
-      gw = empty_f32({E}, x);
-      gb = empty_f32({E}, x);
-      work = at::empty({lib.dfa3d_dropout_add_layer_norm_workspace(rows, (int32_t)E)}, x.options().dtype(at::kByte));
+      gw = fresh({E}, at::kFloat, x);
+      gb = fresh({E}, at::kFloat, x);
+      work = fresh({lib.dfa3d_dropout_add_layer_norm_workspace(rows, (int32_t)E)}, at::kByte, x);
     }
     check(lib.dfa3d_dropout_add_layer_norm_backward(vp(g), vp(x), vp(res), fp(w), fp(stats), fp(stats) + rows, dtype_code(x), rows,
                                                     (int32_t)E, r->p, seed_of(seed), (int32_t)r->site, vpm(gx), vpm(gr),
@@ -169,12 +177,12 @@ struct Levels : Kept {
 Tensor level_workspace(const Levels &s, const Tensor &like, bool backward) {
   const int64_t bytes = lib.dfa3d_group_norm_workspace(s.B, s.N, s.C, s.G, s.L, backward);
   TORCH_CHECK(bytes >= 0, "dfa3d_group_norm_workspace failed: ", lib.dfa3d_last_error());
-  return bytes == 0 ? Tensor() : at::empty({bytes}, like.options().dtype(at::kByte));
+  return bytes == 0 ? Tensor() : fresh({bytes}, at::kByte, like);
 }
 
 Tensor group_norm_forward(const Levels &s, const Tensor &x, const Tensor &w, const Tensor &b, const Tensor &shapes,
                           const Tensor &lsi, const Tensor &stats) {
-  Tensor y = at::empty_like(x), work = level_workspace(s, x, false);
+  Tensor y = fresh(x), work = level_workspace(s, x, false);
   float *mean = stats.defined() ? fpm(stats) : nullptr;
   check(lib.dfa3d_group_norm_forward(vp(x), dtype_code(x), s.B, s.N, s.C, s.G, (const int64_t *)vp(shapes), s.stride,
                                      (const int64_t *)vp(lsi), s.L, fp(w), fp(b), s.rows, s.eps, s.act, vpm(y), mean,
@@ -188,7 +196,7 @@ struct GroupNormFn : torch::autograd::Function<GroupNormFn> {
   static Tensor forward(AutogradContext *ctx, const Tensor &x, const Tensor &w, const Tensor &b, const std::optional<Tensor> &shapes,
                         const std::optional<Tensor> &lsi, const c10::intrusive_ptr<Levels> &s) {
     c10::cuda::CUDAGuard guard(x.device());
-    Tensor stats = empty_f32({2, s->B, s->L, s->G}, x), sh = shapes ? *shapes : Tensor(), st = lsi ? *lsi : Tensor();
+    Tensor stats = fresh({2, s->B, s->L, s->G}, at::kFloat, x), sh = shapes ? *shapes : Tensor(), st = lsi ? *lsi : Tensor();
     Tensor y = group_norm_forward(*s, x, w, b, sh, st, stats);
     keep(ctx, s, {x, w, b, sh, st, stats});
     return y;
@@ -201,10 +209,10 @@ struct GroupNormFn : torch::autograd::Function<GroupNormFn> {
     const Tensor g = like_forward(grads[0], x.scalar_type());
     const bool params = ctx->needs_input_grad(1) || ctx->needs_input_grad(2);
     Tensor gx, gw, gb, work = level_workspace(*s, x, true);
-    if (ctx->needs_input_grad(0)) gx = at::empty_like(g);
+    if (ctx->needs_input_grad(0)) gx = fresh(g);
     if (params) {
-      gw = at::empty_like(w);
-      gb = at::empty_like(w);
+      gw = fresh(w);
+      gb = fresh(w);
     }
     check(lib.dfa3d_group_norm_backward(vp(g), vp(x), dtype_code(x), s->B, s->N, s->C, s->G, (const int64_t *)vp(shapes), s->stride,
                                         (const int64_t *)vp(lsi), s->L, fp(w), fp(b), s->rows, s->act, fp(stats),
