@@ -60,8 +60,8 @@ def _block_by_block(layer, query, seed, kw):
 def _close(got, want):
     # products and norms of 32 to 64 elements in another order, through up to three blocks
     for i, (a, b) in enumerate(zip(got, want)):
-        scale = float(b.abs().max())
-        assert float((a - b).abs().max()) <= 2e-4 * scale + 1e-6, (i, float((a - b).abs().max()), scale)
+        scale = float(b.detach().abs().max())
+        assert float((a - b).detach().abs().max()) <= 2e-4 * scale + 1e-6, (i, float((a - b).detach().abs().max()), scale)
 
 
 @pytest.mark.parametrize("kind", ["full", "cross"])
