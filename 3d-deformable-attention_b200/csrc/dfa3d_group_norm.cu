@@ -9,8 +9,9 @@
 // Statistics: a thread keeps, for each of its V channels, the number of values, their mean and the sum of squares around it; eight
 // rows at a time are reduced in registers around their own mean and merged by
 //   M2 = M2a + M2b + (mb - ma)^2 na nb / (na + nb)                      (Chan, Golub, LeVeque 1979),
-// so that nothing is lost where the mean is large against the spread.  Threads, warps and tiles are merged in a fixed order: a
-// result is the same bits in every run.
+// so that nothing is lost where the mean is large against the spread, not even where the mean's square exceeds 32 bits; a group's
+// sum of squares has to fit them (beyond, rstd is 0 and the result act(beta), as in any 32-bit computation of the variance).
+// Threads, warps and tiles are merged in a fixed order: a result is the same bits in every run.
 //
 // Three launches each way: statistics of tiles of rows; a warp for every group of a level of an image merges its tiles' parts;
 // the result.  They follow one another as programmatic dependent launches, so that the third has its rows on the way while the
@@ -161,6 +162,12 @@ __device__ __forceinline__ void params_of(const GnArgs &a, const float *p, float
 // ------------------------------------------------------------------------------------------------
 // forward
 // ------------------------------------------------------------------------------------------------
+// m2 and what two parts' means, `delta` apart, add to it, `cross` = na nb / (na + nb).  A part without values (cross = 0) adds
+// nothing: its mean is 0 and delta the other's mean, whose square may not fit 32 bits (infinity times 0 is NaN).
+__device__ __forceinline__ float squares(float delta, float cross, float m2) {
+  return cross > 0.f ? fmaf(delta * delta, cross, m2) : m2;
+}
+
 // Number, mean and sum of squares around it, of a thread's values of each of its channels.
 template <int V>
 struct Moments {
@@ -194,7 +201,7 @@ struct Moments {
     for (int c = 0; c < V; ++c) {
       const float delta = s[c] - mean[c];
       mean[c] = fmaf(delta, part, mean[c]);
-      m2[c] += fmaf(delta * delta, cross, q[c]);
+      m2[c] += squares(delta, cross, q[c]);
     }
     n = total;
   }
@@ -255,7 +262,7 @@ __device__ __forceinline__ void moments_of_piece(const T *base, int rows, const 
 #pragma unroll 1
     for (int l = l0, j = j0; l < RL; l += dl) {
       const float2 v = entries[l * width + j];
-      q += fmaf((v.x - m) * (v.x - m), count[l], v.y);
+      q += squares(v.x - m, count[l], v.y);
       j += dj;
       if (j >= per) j -= per, ++l;
     }
@@ -337,7 +344,7 @@ group_merge_kernel(const GnArgs a, const float2 *partial, float *__restrict__ me
       const float nb = (float)(min(s.end, (tu + 1) * a.R) - max(s.begin, tu * a.R)) * (float)a.cpg, total = n + nb;
       const float part = __fdividef(nb, total), delta = v[u].x - mean;
       mean = fmaf(delta, part, mean);
-      m2 += fmaf(delta * delta, n * part, v[u].y);
+      m2 += squares(delta, n * part, v[u].y);
       n = total;
     }
   }
@@ -347,7 +354,7 @@ group_merge_kernel(const GnArgs a, const float2 *partial, float *__restrict__ me
     const float qb = __shfl_down_sync(0xffffffffu, m2, o), total = n + nb, delta = mb - mean;
     const float part = total > 0.f ? __fdividef(nb, total) : 0.f;
     mean = fmaf(delta, part, mean);
-    m2 += fmaf(delta * delta, n * part, qb);
+    m2 += squares(delta, n * part, qb);
     n = total;
   }
   if (lane == 0) {
@@ -494,7 +501,7 @@ group_image_kernel(const T *__restrict__ x, const GnArgs a, float *__restrict__ 
       if (j < k.size && k.rows_of(j) > 0) {
         const float nb = (float)k.rows_of(j) * (float)a.cpg, total = n + nb, part = __fdividef(nb, total), delta = v[j].x - mean;
         mean = fmaf(delta, part, mean);
-        m2 += fmaf(delta * delta, n * part, v[j].y);
+        m2 += squares(delta, n * part, v[j].y);
         n = total;
       }
     const float rstd = n > 0.f ? rsqrtf(__fdividef(m2, n) + a.eps) : 0.f;
