@@ -4,6 +4,7 @@ There is no CPU or pure-PyTorch fallback: if the shared library is missing or a 
 exception is raised.
 """
 import ctypes
+import operator
 import os
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
@@ -32,8 +33,20 @@ class Problem(ctypes.Structure):
         super().__init__(*args, **kw)
 
 
+class _I32:
+    """An int32 argument.  ctypes.c_int32 would pass the lower half of a number that does not fit."""
+
+    @staticmethod
+    def from_param(v):
+        v = operator.index(v)
+        if not -2 ** 31 <= v < 2 ** 31:
+            raise OverflowError(f"{v} does not fit 32 bits")
+        return ctypes.c_int32(v)
+
+
 _P = ctypes.POINTER(Problem)
 _V = ctypes.c_void_p
+_I64 = ctypes.c_int64
 
 # name -> number of pointer arguments after the problem descriptor (the stream included)
 ENTRY_POINTS = {
@@ -63,7 +76,6 @@ ENTRY_POINTS_WITH_ANCHORS = {
     "dfa3d_attn3d_forward_ragged": 11,
     "dfa3d_attn3d_backward_ragged": 16,
 }
-_I32, _I64 = ctypes.c_int32, ctypes.c_int64
 # entry points without a problem descriptor: explicit argument types
 PLAIN_ENTRY_POINTS = {
     "dfa3d_attn2d_supported": [_P, _I32],
@@ -141,7 +153,7 @@ def load():
     for name, nptr in ENTRY_POINTS_WITH_ANCHORS.items():
         fn = getattr(lib, name)
         fn.restype = ctypes.c_int
-        fn.argtypes = [_P, ctypes.c_int32] + [_V] * nptr
+        fn.argtypes = [_P, _I32] + [_V] * nptr
     for name, argtypes in PLAIN_ENTRY_POINTS.items():
         fn = getattr(lib, name)
         fn.restype = ctypes.c_int
@@ -200,22 +212,28 @@ def native_apply(name):
     return wrap
 
 
+def _invoke(name, *args):
+    """What an entry point answers; arguments that cannot be passed on raise like those that it refuses."""
+    try:
+        return getattr(load(), name)(*args)
+    except ctypes.ArgumentError as e:
+        raise RuntimeError(f"{name} failed ({ERROR_NAMES[-1]}): {e}") from None
+
+
 def size(name, *args):
     """Bytes of workspace that an entry point asks for."""
-    lib = load()
-    n = getattr(lib, name)(*args)
+    n = _invoke(name, *args)
     if n < 0:
-        msg = lib.dfa3d_last_error().decode("utf-8", "replace")
+        msg = load().dfa3d_last_error().decode("utf-8", "replace")
         raise RuntimeError(f"{name} failed ({ERROR_NAMES.get(n, n)}): {msg}")
     return n
 
 
 def call_plain(name, *args):
     """Invoke an entry point that takes no problem descriptor."""
-    lib = load()
-    rc = getattr(lib, name)(*args)
+    rc = _invoke(name, *args)
     if rc != 0:
-        msg = lib.dfa3d_last_error().decode("utf-8", "replace")
+        msg = load().dfa3d_last_error().decode("utf-8", "replace")
         raise RuntimeError(f"{name} failed ({ERROR_NAMES.get(rc, rc)}): {msg}")
     global _calls
     _calls += 1
@@ -223,10 +241,9 @@ def call_plain(name, *args):
 
 def call(name, problem, *ptrs):
     """Invoke an entry point; raise RuntimeError carrying dfa3d_last_error() on failure."""
-    lib = load()
-    rc = getattr(lib, name)(ctypes.byref(problem), *ptrs)
+    rc = _invoke(name, ctypes.byref(problem), *ptrs)
     if rc != 0:
-        msg = lib.dfa3d_last_error().decode("utf-8", "replace")
+        msg = load().dfa3d_last_error().decode("utf-8", "replace")
         raise RuntimeError(f"{name} failed ({ERROR_NAMES.get(rc, rc)}): {msg}")
     global _calls
     _calls += 1

@@ -139,8 +139,9 @@ class DropoutAddLayerNormFunction(Function):
         for t, n in ((weight, "weight"), (bias, "bias")):
             if t.dtype != torch.float32 or t.device != x.device or t.numel() != E:
                 raise RuntimeError(f"{n} must be {E} float32 elements on {x.device}, got {tuple(t.shape)} {t.dtype} on {t.device}")
-        x, residual, weight, bias = x.contiguous(), residual.contiguous(), weight.contiguous(), bias.contiguous()
         rows = x.numel() // E if E else 0
+        _lib.size("dfa3d_dropout_add_layer_norm_workspace", rows, E)          # refuses sizes before anything is copied
+        x, residual, weight, bias = x.contiguous(), residual.contiguous(), weight.contiguous(), bias.contiguous()
         y = torch.empty_like(x)
         stats = torch.empty((2, rows), dtype=torch.float32, device=x.device)
         with torch.cuda.device(x.device):

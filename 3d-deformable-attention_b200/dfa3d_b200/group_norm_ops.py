@@ -41,10 +41,6 @@ def _table(shapes, lsi, x):
     return shapes.contiguous(), lsi.contiguous(), shapes.shape[1], shapes.shape[0]
 
 
-def _workspace(B, N, C, G, L, backward, x):
-    return torch.empty(_lib.size("dfa3d_group_norm_workspace", B, N, C, G, L, int(backward)), dtype=torch.uint8, device=x.device)
-
-
 @_lib.native_apply("group_norm")
 class GroupNormFunction(Function):
     @staticmethod
@@ -62,12 +58,13 @@ class GroupNormFunction(Function):
             if t.dtype != torch.float32 or t.device != x.device or tuple(t.shape) not in ((C,), (L, C)) or t.shape != weight.shape:
                 raise RuntimeError(f"{n} must be float32 ({C}) or ({L}, {C}) on {x.device}, got {tuple(t.shape)} {t.dtype} on "
                                    f"{t.device}")
-        x, weight, bias = x.contiguous(), weight.contiguous(), bias.contiguous()
         B, N, rows = x.shape[0], x[0].numel() // C if x.numel() else 0, 1 if weight.dim() == 1 else L
+        size = _lib.size("dfa3d_group_norm_workspace", B, N, C, G, L, 0)      # refuses sizes before anything is copied
+        x, weight, bias = x.contiguous(), weight.contiguous(), bias.contiguous()
         y = torch.empty_like(x)
-        stats = torch.empty((2, B, L, max(G, 0)), dtype=torch.float32, device=x.device)
+        stats = torch.empty((2, B, L, G), dtype=torch.float32, device=x.device)
+        work = torch.empty(size, dtype=torch.uint8, device=x.device)
         with torch.cuda.device(x.device):
-            work = _workspace(B, N, C, G, L, False, x)
             _lib.call_plain("dfa3d_group_norm_forward", x.data_ptr(), _DTYPES[x.dtype], B, N, C, G, _ptr(shapes), stride, _ptr(lsi),
                             L, weight.data_ptr(), bias.data_ptr(), rows, float(eps), _ACTS[activation], y.data_ptr(),
                             stats[0].data_ptr(), stats[1].data_ptr(), work.data_ptr(), work.numel(), _stream(x))
@@ -87,8 +84,8 @@ class GroupNormFunction(Function):
         grad_wb = None
         if need[1] or need[2]:
             grad_wb = [torch.empty_like(weight), torch.empty_like(weight)]
+        work = torch.empty(_lib.size("dfa3d_group_norm_workspace", B, N, C, G, L, 1), dtype=torch.uint8, device=x.device)
         with torch.cuda.device(x.device):
-            work = _workspace(B, N, C, G, L, True, x)
             _lib.call_plain("dfa3d_group_norm_backward", g.data_ptr(), x.data_ptr(), _DTYPES[x.dtype], B, N, C, G, _ptr(shapes),
                             stride, _ptr(lsi), L, weight.data_ptr(), bias.data_ptr(), rows, ctx.act, stats[0].data_ptr(),
                             stats[1].data_ptr(), _ptr(grad_x), None if grad_wb is None else grad_wb[0].data_ptr(),
