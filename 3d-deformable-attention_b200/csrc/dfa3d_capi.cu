@@ -861,6 +861,7 @@ static int check_group_norm(int32_t B, int32_t N, int32_t C, int32_t G, const in
   if (!spatial_shapes && L != 1) return fail(DFA3D_ERR_INVALID_ARGUMENT, "L=%d levels without a level table", L);
   if (spatial_shapes && shape_stride < 2)
     return fail(DFA3D_ERR_INVALID_ARGUMENT, "shape_stride must be at least 2 (got %d)", shape_stride);
+  REQUIRE_ALIGNED8(spatial_shapes); REQUIRE_ALIGNED8(level_start);
   if (weight_rows != 1 && weight_rows != L)
     return fail(DFA3D_ERR_INVALID_ARGUMENT, "weight_rows=%d is neither 1 nor the L=%d levels", weight_rows, L);
   if (activation != DFA3D_ROW_NONE && activation != DFA3D_ROW_RELU && activation != DFA3D_ROW_SILU)
