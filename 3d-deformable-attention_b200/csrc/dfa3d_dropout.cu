@@ -25,10 +25,9 @@ namespace {
 
 constexpr int kThreads = 256;
 
-// Words of elements base + e ... + V - 1, where base is a multiple of 2048 and e below 4096 is one of 4.
+// Words of elements base + e ... + V - 1, where base is a multiple of a CTA's elements (block_of) and e below these one of 4.
 template <int V>
 __device__ __forceinline__ void words_from(const DropRule &d, DropKey k, long long base, unsigned e, uint32_t (&words)[V]) {
-  const unsigned long long block = (unsigned long long)base >> 2;
   if (!d.rng) {
 #pragma unroll
     for (int i = 0; i < V; ++i) words[i] = ~0u;
@@ -36,9 +35,7 @@ __device__ __forceinline__ void words_from(const DropRule &d, DropKey k, long lo
   }
 #pragma unroll
   for (int i = 0; i < V; i += 4) {
-    // no carry: the upper half is the same for the whole CTA, and so is what the first round makes of it
-    const unsigned long long at = (block & 0xffffffff00000000ull) | (uint32_t)((uint32_t)block + ((e + i) >> 2));
-    const PhiloxWords w = philox_words(at, d.site, k);
+    const PhiloxWords w = philox_words(block_of((unsigned long long)base, e + i), d.site, k);
     words[i] = w.x; words[i + 1] = w.y; words[i + 2] = w.z; words[i + 3] = w.w;
   }
 }

@@ -38,6 +38,18 @@ struct PhiloxWords {
   uint32_t x, y, z, w;
 };
 
+// The block of element base + e, for a base that is a multiple of `width` (2048 or 4096, the elements of a CTA) and e < width: no carry
+// leaves the lower half, so that the upper one is the same for the whole CTA, and so is what the first round makes of it.
+#ifdef __CUDACC__
+__host__ __device__ __forceinline__
+#else
+inline
+#endif
+unsigned long long block_of(unsigned long long base, uint32_t e) {
+  const unsigned long long block = base >> 2;
+  return (block & 0xffffffff00000000ull) | (uint32_t)((uint32_t)block + (e >> 2));
+}
+
 #ifdef __CUDACC__
 __host__ __device__ __forceinline__
 #else
