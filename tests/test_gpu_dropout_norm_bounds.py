@@ -12,20 +12,20 @@ from test_gpu_dropout_norm import DEV, EPS, apply, inputs, seed_tensor
 from test_gpu_native_path import _python
 
 pytestmark = pytest.mark.gpu
-P, SEED, SITE = 0.2, 41, 4
+SEED, SITE = 41, 4
 
 
-def check(tensors, g):
+def check(tensors, g, p=0.2):
     from dfa3d_b200.dropout_ops import DropoutAddLayerNormFunction
     dtype = tensors[0].dtype
     rows, E = tensors[0].shape
     h = 0 if dtype == torch.float32 else R.half_step(dtype)
     leaves = [t.detach().clone().requires_grad_(True) for t in tensors]
-    y = _python(DropoutAddLayerNormFunction).apply(*leaves, seed_tensor(SEED), P, SITE, EPS)
+    y = _python(DropoutAddLayerNormFunction).apply(*leaves, seed_tensor(SEED), p, SITE, EPS)
     stats = y.grad_fn.saved_tensors[3].clone()
     got = dict(zip(("gx", "gr", "gw", "gb"), torch.autograd.grad(y, leaves, g)), y=y.detach())
 
-    f = Bo.norm_forward(*tensors, P, SEED, SITE, EPS)
+    f = Bo.norm_forward(*tensors, p, SEED, SITE, EPS)
     mean, off, rstd, rho = Bo.norm_stats(f, EPS)
     R.assert_within("mean", stats[0], mean, off)
     R.assert_within("rstd", stats[1], rstd, rho * rstd)
@@ -38,11 +38,12 @@ def check(tensors, g):
     # a normalisation that was lost, and gradients that were, would not pass
     if E > 1:
         Bo.assert_refutes("y", tensors[3].cpu().double().expand(rows, E), k["y"][0], stored("y"))
-        Bo.assert_refutes("gr", torch.zeros(rows, E).double(), k["gr"][0], stored("gr"))
         Bo.assert_refutes("gw", torch.zeros(E).double(), *k["gw"])
+    if E > 2:      # two elements are normalised to -1 and 1 whatever they are: there is next to no gradient
+        Bo.assert_refutes("gr", torch.zeros(rows, E).double(), k["gr"][0], stored("gr"))
 
     leaves = [t.detach().clone().requires_grad_(True) for t in tensors]
-    y = apply(True, *leaves, seed_tensor(SEED), P, SITE)
+    y = apply(True, *leaves, seed_tensor(SEED), p, SITE)
     native = dict(zip(("gx", "gr", "gw", "gb"), torch.autograd.grad(y, leaves, g)), y=y.detach())
     assert all(torch.equal(native[n], got[n]) for n in got)
 
@@ -76,3 +77,11 @@ def test_several_rows_that_begin_at_even_places(lib_built, rows, E):
 @pytest.mark.parametrize("rows,E", [(29003, 32), (15001, 128), (15001, 256), (7411, 512), (7411, 1024)])
 def test_several_rows_a_lane_group_on_the_grid(lib_built, rows, E, dtype):
     check(*inputs(rows, E, dtype))
+
+
+@pytest.mark.parametrize("p", [0.1, 0.2])
+@pytest.mark.parametrize("rows,E", [(300007, 2), (200003, 3), (150001, 4)])
+def test_many_narrow_rows(lib_built, rows, E, p):
+    """Among so many rows of two or three there are some where residual and dropped part cancel and some that have next to no spread: what
+    the sum is off by is a rounding of its parts, times rstd.  1 / 0.9 is rounded too, 1 / 0.8 is not."""
+    check(*inputs(rows, E, torch.float32), p=p)
