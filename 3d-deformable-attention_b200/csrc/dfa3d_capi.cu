@@ -849,6 +849,8 @@ static int check_group_norm_sizes(int32_t B, int32_t N, int32_t C, int32_t G, in
   if (C > DFA3D_MAX_CHANNELS) return fail(DFA3D_ERR_UNSUPPORTED, "C=%d exceeds %d", C, DFA3D_MAX_CHANNELS);
   if (L <= 0) return fail(DFA3D_ERR_INVALID_ARGUMENT, "L must be positive (got %d)", L);
   if (L > DFA3D_MAX_LEVELS) return fail(DFA3D_ERR_UNSUPPORTED, "L=%d exceeds DFA3D_MAX_LEVELS=%d", L, DFA3D_MAX_LEVELS);
+  // tasks are numbered in 32 bits: (image, level, channel) and rows of an image; the middle one is a limit of the interface, which no
+  // kernel needs
   if (N >= (1 << 30) || (int64_t)B * (N < 2052 ? N : 2052) >= (1LL << 31) || (int64_t)B * L * C >= (1LL << 31))
     return fail(DFA3D_ERR_UNSUPPORTED, "B=%d images of N=%d rows are too many", B, N);
   return DFA3D_OK;

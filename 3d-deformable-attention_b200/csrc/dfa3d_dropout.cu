@@ -4,12 +4,13 @@
 //   y = LayerNorm(residual + keep * x / (1 - p))                  rows of up to 1024 columns
 //
 // with their backward passes, which form the mask again from (seed, site, element).  Every tensor is read once and written once;
-// what bounds them is HBM, with the instructions next: a Philox block for four elements is about 30 of them, twelve of which are
-// 32 x 32 -> 64 bit products at half rate.
+// what bounds them is HBM, with the instructions next: a Philox block for four elements is 43 of them, twelve of which are
+// 32 x 32 -> 64 bit products at half rate.  An element of a forward without activation costs 18.0 instructions in fp32 and 16.8 in 16 bits, 7.3
+// and 6.1 where nothing is dropped.
 //
-// Measured (HBM copy 6528 GB/s): 40 000 x 512 fp32 with ReLU 26 us forward, 38 backward (6.2, 6.5 TB/s); 184 950 x 256 bf16 33.8
-// and 33.7 (5.6 TB/s; 41 before the upper counter word was made one value for a CTA and the kept bits were compared in place; four
-// words a thread 35, CTAs that stay and ask one step ahead 36).
+// Measured (HBM copy 6528 GB/s): 40 000 x 512 fp32 with ReLU 28.4 us forward, 39.2 backward (5.8, 6.3 TB/s), 60.6 for both one after
+// the other; 184 950 x 256 bf16 35.0 and 34.9 (5.4 TB/s, 33.8 on another device; there 41 before the upper counter word was made one value
+// for a CTA and the kept bits were compared in place; four words a thread 35, CTAs that stay and ask one step ahead 36).
 // Norm of 40 000 x 256 fp32 23.6 forward, 38.6 backward (5.2, 5.3 TB/s), of 80 000 x 256 bf16 28.3 and 41.6 (4.3, 4.9 TB/s: 30 and
 // 40 instructions an element); 900 x 256 fp32 3.2 and 5.5.  Rows loaded into registers instead of one ahead through shared memory:
 // 26 and 46, 1024 columns 66 and 138 for 49 and 80; a warp a row of four elements a lane 25 and 56, bf16 39 and 86.

@@ -15,8 +15,8 @@
 //
 // Three launches each way: statistics of tiles of rows; a warp for every group of a level of an image merges its tiles' parts;
 // the result.  They follow one another as programmatic dependent launches, so that the third has its rows on the way while the
-// second runs.  All tiles of a launch are resident at once, and the third walks each from its end, whose rows the first has left in
-// L2 (126 MB).
+// second runs.  All tiles of a launch are resident at once (with up to 444 images; 296 or 148 for words of two channels or one), and
+// the third walks each from its end, whose rows the first has left in L2 (126 MB).  Beyond, a tile is an image.
 //
 // Forwards of images of up to 256 rows of 1024 channels (1024 of 256) are one launch: a cluster of CTAs has a level of an image.
 //
@@ -819,12 +819,12 @@ int threads_of(int V) { return V == 4 ? kThreads<4> : V == 2 ? kThreads<2> : kTh
 
 int resident_of(int V) { return V == 4 ? kResident<4> : V == 2 ? kResident<2> : kResident<1>; }
 
-// Rows of a tile: as many as make one full wave of CTAs of the whole call, but at least four of a thread, and at most 2048 tiles an
-// image to merge.  6 x 30 825 x 256 bf16 forward 49 us, at two waves 54, three 59; 40 000 x 256 fp32 32, 42, 49; 6 x 30 825 x 256 fp32 97,
+// Rows of a tile: as many as make one full wave of CTAs of the whole call, but at least four of a thread, and one tile an image where
+// there are more images than CTAs in a wave.  6 x 30 825 x 256 bf16 forward 49 us, at two waves 54, three 59; 40 000 x 256 fp32 32, 42, 49; 6 x 30 825 x 256 fp32 97,
 // 97, 100 (backward 158, 155, 159).
 int tile_rows(int B, int N, int C, int V) {
   const int RL = threads_of(V) / (C / V);
-  const long long slots = 148LL * resident_of(V), tiles = std::max(1LL, std::min(2048LL, slots / B));
+  const long long slots = 148LL * resident_of(V), tiles = std::max(1LL, slots / B);
   const long long rows = std::max((N + tiles - 1) / tiles, 4LL * RL);
   return (int)std::min<long long>(rows, N);
 }

@@ -3,7 +3,9 @@
 // Element i of a tensor in row-major order takes word i mod 4 of Philox4x32 at counter (i / 4 low, i / 4 high, site, 0) under the
 // key (seed low, seed high), and is kept where word >= p * 2^32.  The generator is Philox4x32 of Salmon, Moraes, Dror and Shaw,
 // "Parallel random numbers: as easy as 1, 2, 3" (SC 2011), with 7 rounds, the fewest that the authors found to pass all of
-// TestU01's BigCrush: a word then costs eight instructions of the integer pipes, and a 16-bit dropout stays near the speed of HBM.
+// TestU01's BigCrush: a block of four words then costs 43 instructions, counted on the device (25 are the 12 products and 13 logic
+// operations that the rounds take where the counter's upper half and the site are the CTA's; the rest forms round keys and counters), and
+// a 16-bit dropout stays near the speed of HBM.
 #pragma once
 #include <stdint.h>
 

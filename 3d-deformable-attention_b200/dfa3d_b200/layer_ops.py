@@ -222,8 +222,9 @@ def dropout_sum(x, residual, dropout):
 
 
 def dropout_norm(x, residual, dropout, norm, seed, site):
-    """norm(dropout(x), residual) for an AddLayerNorm; as one operation where `dropout` is a CounterDropout.  seed(): the seed of
-    this pass."""
+    """norm(dropout(x), residual) for an AddLayerNorm; as one operation where `dropout` is a CounterDropout and x and residual are of one
+    type and shape (under autocast the package's Linear returns float32: a 16-bit residual takes two operations).  seed(): the seed
+    of this pass."""
     if not _counts(dropout):
         return norm(dropout(x), residual)
     if type(norm) is AddLayerNorm and runs_forward_only(norm) and x.shape == residual.shape and x.dtype == residual.dtype:
