@@ -29,6 +29,7 @@
 // kinds from one queue 146 forward; batches that fit L2, one after the other, 102 / 178; rows one chunk ahead through shared memory
 // 107 / 167; merges by the CTAs of the third launch instead of a second one 110 / 170; two to six waves of tiles, bf16 forward 54 to 74.
 #include <algorithm>
+#include <cfloat>
 
 #include "dfa3d_launch.h"
 #include "dfa3d_rowvec.cuh"
@@ -45,6 +46,8 @@ template <int V> constexpr int kThreads = V == 4 ? 256 : 1024 / V;
 template <int V> constexpr int kResident = V == 4 ? 3 : V;
 // Words of a thread in flight, and of each of two tensors.
 constexpr int kAhead = 8, kGradAhead = 4;
+// Below it a factor of the gradient has lost some of its 24 bits, or is about to: 2^24 times the smallest normal number.
+constexpr float kSmallestFactor = FLT_MIN * 16777216.f;
 // ... of the two that are only read: 8-byte words leave registers for more (bf16 backward 84 us; four words and four CTAs an SM 86).
 template <typename T, int V> constexpr int kGradStatsAhead = V == 4 && sizeof(T) == 2 ? 8 : kGradAhead;
 
@@ -727,11 +730,30 @@ __device__ __forceinline__ void parameter_sums(const GnArgs &a, const float2 *by
   grad_weight[column] = s.y;
 }
 
+// A thread's channels of a piece's rows, one by one, where rstd^2 mean(d * xhat) does not fit a normal number: xhat is formed first.
+template <typename T, bool ACT>
+__device__ __noinline__ void grad_in_steps(const T *grad_y, const T *x, T *grad_x, const GnArgs &a, long long first, int rl, int rows,
+                                           int channel, int count, int w0, long long g0, const float *mean_in, const float *rstd_in,
+                                           const float2 *means) {
+  for (int c = 0; c < count; ++c) {
+    const long long g = g0 + (channel + c) / a.cpg;
+    const float mean = __ldg(mean_in + g), rstd = __ldg(rstd_in + g), scale = __ldg(a.weight + w0 + c) * rstd;
+    const float shift = ACT ? __ldg(a.bias + w0 + c) : 0.f;
+    const float2 m = __ldcg(means + g);
+    for (int r = rl; r < rows; r += a.RL) {
+      const long long at = first + (long long)r * a.C + channel + c;
+      const float centred = wide(x[at]) - mean, dy = wide(grad_y[at]);
+      const float dz = ACT ? activate_grad<ACT>(dy, fmaf(centred, scale, shift), a.act) : dy;
+      grad_x[at] = narrow<T>(fmaf(dz, scale, -fmaf(centred * rstd, rstd * m.y, rstd * m.x)));
+    }
+  }
+}
+
 // grad_x = rstd * (d - mean(d) - xhat * mean(d * xhat)), d = dz * gamma, means over the group; the CTAs beyond its
 // `tiles` form the parameters' gradients.
 template <typename T, int V, bool ACT>
 __global__ void __launch_bounds__(kThreads<V>, kResident<V>)
-group_grad_apply_kernel(const T *__restrict__ grad_y, const T *__restrict__ x, const GnArgs a, int tiles,
+group_grad_apply_kernel(const T *__restrict__ grad_y, const T *__restrict__ x, const __grid_constant__ GnArgs a, int tiles,
                         const float *__restrict__ mean_in, const float *__restrict__ rstd_in, const float2 *means,
                         const float2 *by_level, T *__restrict__ grad_x, float *grad_weight, float *grad_bias) {
   constexpr int U = kGradAhead;
@@ -770,7 +792,9 @@ group_grad_apply_kernel(const T *__restrict__ grad_y, const T *__restrict__ x, c
       zero_rows<T, V>(out - (long long)r * a.C, at.at, at.rl, rows, a.RL, step);
       continue;
     }
-    // grad_x = dz * scale - (k1 + (x - mean) * k2)
+    // grad_x = dz * scale - (k1 + (x - mean) * k2).  With eps = 0 and next to no spread, or a wide one and small gradients,
+    // k2 = rstd^2 mean(d * xhat) may not fit a normal number.
+    bool fits = true;
     float mean[V], scale[V], shift[V], k1[V], k2[V];
     const int w0 = (a.weight_rows == 1 ? 0 : l) * a.C + at.cv * V;
     const long long g0 = ((long long)tile.b * a.L + l) * a.G;
@@ -784,6 +808,13 @@ group_grad_apply_kernel(const T *__restrict__ grad_y, const T *__restrict__ x, c
       scale[c] *= rstd;
       k1[c] = rstd * m.x;
       k2[c] = rstd * rstd * m.y;
+      const float y = fabsf(m.y), k = fabsf(k2[c]);
+      if (y > 0.f && y <= FLT_MAX && !(k >= kSmallestFactor && k <= FLT_MAX)) fits = false;
+    }
+    if (!fits) {
+      grad_in_steps<T, ACT>(grad_y, x, grad_x, a, ((long long)tile.b * a.N + lo) * a.C, at.rl, rows, at.cv * V, V, w0, g0, mean_in, rstd_in,
+                            means);
+      continue;
     }
     auto store = [&](int u) {
       float xf[V], gf[V];
