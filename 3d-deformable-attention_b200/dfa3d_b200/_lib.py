@@ -41,7 +41,7 @@ class _I32:
         v = operator.index(v)
         if not -2 ** 31 <= v < 2 ** 31:
             raise OverflowError(f"{v} does not fit 32 bits")
-        return ctypes.c_int32(v)
+        return v                       # ctypes passes a Python integer as a C int
 
 
 _P = ctypes.POINTER(Problem)
