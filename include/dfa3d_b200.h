@@ -445,9 +445,10 @@ int dfa3d_dropout_add_layer_norm_backward(const void *grad_y, const void *x, con
  * x (B, N, C): the layout of the operator's value.  Every (image, level, group of C / G channels) is normalised by itself
  * (biased variance, eps inside the square root), y = act(xhat * weight + bias), activation DFA3D_ROW_NONE, _RELU or _SILU.
  * spatial_shapes (L, shape_stride) int64 with height and width first, level_start (L) int64, device, 8-byte aligned, levels
- * ascending; both null with L = 1: the N rows are one level.  A table that points outside of the N rows or overlaps is cut to disjoint
- * levels; rows of no level become 0 in y and in grad_x.  weight, bias fp32 (weight_rows, C) with weight_rows 1 (shared by
- * the levels) or L.  C <= 1024, G divides C, N < 2^30, B * L * C < 2^31, B * min(N, 2052) < 2^31.  dtype (of x, y and their gradients): DFA3D_DTYPE_F32, _BF16 or _F16.
+ * ascending; both null with L = 1: the N rows are one level.  A table that points outside of the N rows or overlaps is cut to
+ * disjoint levels; rows of no level become 0 in y and in grad_x.  weight, bias fp32 (weight_rows, C) with weight_rows 1
+ * (shared by the levels) or L.  C <= 1024, G divides C, N < 2^30, B * L * C < 2^31, B * min(N, 2052) < 2^31.  dtype (of x,
+ * y and their gradients): DFA3D_DTYPE_F32, _BF16 or _F16.
  * mean, rstd (B, L, G) fp32 for the backward; may be null together in the forward.  Results overlap no input.
  * The workspace may be null where it has 0 bytes (forwards of small images). */
 int64_t dfa3d_group_norm_workspace(int32_t B, int32_t N, int32_t C, int32_t G, int32_t L, int32_t backward);
