@@ -9,6 +9,7 @@
 #include "dfa3d_b200.h"
 #include "dfa3d_common.cuh"
 #include "dfa3d_launch.h"
+#include "dfa3d_product.h"
 
 namespace {
 
@@ -927,6 +928,297 @@ int dfa3d_group_norm_backward(const void *grad_y, const void *x, int32_t dtype, 
                                                   weight, bias, weight_rows, mean, rstd, activation, grad_x, grad_weight,
                                                   grad_bias, workspace, (cudaStream_t)stream),
                 "dfa3d_group_norm_backward launch");
+}
+
+// ---- products of a feed-forward block ------------------------------------------------------------
+static int check_product(int32_t dtype, int64_t rows, std::initializer_list<int32_t> widths, int32_t activation) {
+  if (dtype != DFA3D_DTYPE_BF16 && dtype != DFA3D_DTYPE_F16)
+    return fail(DFA3D_ERR_INVALID_ARGUMENT, "dtype %d is neither DFA3D_DTYPE_BF16 nor DFA3D_DTYPE_F16", dtype);
+  if (rows < 0) return fail(DFA3D_ERR_INVALID_ARGUMENT, "rows must be >= 0 (got %lld)", (long long)rows);
+  if (rows >= (1LL << 31) - 128) return fail(DFA3D_ERR_UNSUPPORTED, "rows=%lld must stay below 2^31 - 128", (long long)rows);
+  for (int32_t w : widths) {
+    if (w <= 0) return fail(DFA3D_ERR_INVALID_ARGUMENT, "widths must be positive (got %d)", w);
+    // tiles of 128 rows and 64 columns are numbered in 32 bits
+    if (w > (1 << 24) || (rows + 127) / 128 * ((w + 63) / 64) >= (1LL << 31))
+      return fail(DFA3D_ERR_UNSUPPORTED, "a matrix of %lld x %d is too large", (long long)rows, w);
+  }
+  if (activation < DFA3D_ROW_NONE || activation > DFA3D_ROW_GELU)
+    return fail(DFA3D_ERR_INVALID_ARGUMENT, "activation %d is not a DFA3D_ROW_*", activation);
+  return DFA3D_OK;
+}
+static int check_operand(const char *name, const void *p, int64_t pitch, int32_t width) {
+  if (!p) return fail(DFA3D_ERR_INVALID_ARGUMENT, "argument `%s` is null", name);
+  if (!aligned16(p)) return fail(DFA3D_ERR_INVALID_ARGUMENT, "`%s` must be 16-byte aligned", name);
+  if (pitch < width || pitch % 8 != 0 || pitch >= (1LL << 38))
+    return fail(DFA3D_ERR_INVALID_ARGUMENT, "the pitch of `%s` must be a multiple of 8 and at least %d (got %lld)", name, width,
+                (long long)pitch);
+  return DFA3D_OK;
+}
+#define REQUIRE_OPERAND(ptr, pitch, width)                                   \
+  do {                                                                       \
+    if (int rc = check_operand(#ptr, ptr, pitch, width)) return rc;          \
+  } while (0)
+
+int dfa3d_linear_act_forward(const void *x, int64_t x_pitch, const void *weight, int64_t weight_pitch, const void *bias,
+                             const void *residual, int32_t dtype, int32_t out_dtype, int64_t rows, int32_t in, int32_t out,
+                             int32_t activation, void *y, void *stream) {
+  if (int rc = check_product(dtype, rows, {in, out}, activation)) return rc;
+  if (out_dtype != dtype && out_dtype != DFA3D_DTYPE_F32)
+    return fail(DFA3D_ERR_INVALID_ARGUMENT, "out_dtype %d is neither dtype nor DFA3D_DTYPE_F32", out_dtype);
+  if (int rc = check_elements(dtype, {bias})) return rc;
+  if (int rc = check_elements(out_dtype, {residual, y})) return rc;
+  if (rows == 0) return DFA3D_OK;
+  REQUIRE_OPERAND(x, x_pitch, in);
+  REQUIRE_OPERAND(weight, weight_pitch, in);
+  REQUIRE_PTR(y);
+  dfa3d::ProductArgs a;
+  a.kind = dfa3d::kLinear;
+  a.dtype = dtype;
+  a.wide_out = out_dtype == DFA3D_DTYPE_F32;
+  a.rows = rows;
+  a.n = out;
+  a.k0 = in;
+  a.a0 = {x, x_pitch};
+  a.b0 = {weight, weight_pitch};
+  a.in = {residual, out};
+  a.bias0 = bias;
+  a.act = activation;
+  a.out[0] = y;
+  a.out_pitch = out;
+  return finish(dfa3d::launch_product(a, (cudaStream_t)stream), "dfa3d_linear_act_forward launch");
+}
+
+int dfa3d_linear_act_slope(const void *x, int64_t x_pitch, const void *weight, int64_t weight_pitch, const void *bias,
+                           const void *grad_y, int64_t grad_pitch, int32_t dtype, int64_t rows, int32_t in, int32_t out,
+                           int32_t activation, void *grad_z, void *stream) {
+  if (int rc = check_product(dtype, rows, {in, out}, activation)) return rc;
+  if (int rc = check_elements(dtype, {bias})) return rc;
+  if (rows == 0) return DFA3D_OK;
+  REQUIRE_OPERAND(x, x_pitch, in);
+  REQUIRE_OPERAND(weight, weight_pitch, in);
+  REQUIRE_OPERAND(grad_y, grad_pitch, out);
+  REQUIRE_OPERAND(grad_z, grad_pitch, out);
+  dfa3d::ProductArgs a;
+  a.kind = dfa3d::kSlope;
+  a.dtype = dtype;
+  a.rows = rows;
+  a.n = out;
+  a.k0 = in;
+  a.a0 = {x, x_pitch};
+  a.b0 = {weight, weight_pitch};
+  a.in = {grad_y, grad_pitch};
+  a.bias0 = bias;
+  a.act = activation;
+  a.out[0] = grad_z;
+  a.out_pitch = grad_pitch;
+  return finish(dfa3d::launch_product(a, (cudaStream_t)stream), "dfa3d_linear_act_slope launch");
+}
+
+int dfa3d_linear_input_gradient(const void *grad, const void *grad2, int64_t grad_pitch, const void *weight, const void *weight2,
+                                int64_t weight_pitch, const void *add, int64_t add_pitch, int32_t dtype, int64_t rows, int32_t in,
+                                int32_t out, void *grad_x, void *stream) {
+  if (int rc = check_product(dtype, rows, {in, out}, DFA3D_ROW_NONE)) return rc;
+  if ((grad2 == nullptr) != (weight2 == nullptr))
+    return fail(DFA3D_ERR_INVALID_ARGUMENT, "grad2 and weight2 must be given together or not at all");
+  if (int rc = check_elements(dtype, {grad_x})) return rc;
+  if (rows == 0) return DFA3D_OK;
+  REQUIRE_OPERAND(grad, grad_pitch, out);
+  REQUIRE_OPERAND(weight, weight_pitch, in);
+  if (grad2) {
+    REQUIRE_OPERAND(grad2, grad_pitch, out);
+    REQUIRE_OPERAND(weight2, weight_pitch, in);
+  }
+  if (add) REQUIRE_OPERAND(add, add_pitch, in);
+  REQUIRE_PTR(grad_x);
+  dfa3d::ProductArgs a;
+  a.kind = dfa3d::kInputGrad;
+  a.dtype = dtype;
+  a.rows = rows;
+  a.n = in;
+  a.k0 = out;
+  a.k1 = grad2 ? out : 0;
+  a.a0 = {grad, grad_pitch};
+  a.a1 = {grad2, grad_pitch};
+  a.b0 = {weight, weight_pitch};
+  a.b1 = {weight2, weight_pitch};
+  a.in = {add, add_pitch};
+  a.out[0] = grad_x;
+  a.out_pitch = in;
+  return finish(dfa3d::launch_product(a, (cudaStream_t)stream), "dfa3d_linear_input_gradient launch");
+}
+
+int dfa3d_gated_hidden_forward(const void *x, int64_t x_pitch, const void *weight_gate, const void *weight_up,
+                               int64_t weight_pitch, const void *bias_gate, const void *bias_up, int32_t dtype, int64_t rows,
+                               int32_t in, int32_t hidden, int32_t activation, void *h, int64_t hidden_pitch, void *stream) {
+  if (int rc = check_product(dtype, rows, {in, hidden}, activation)) return rc;
+  if (int rc = check_elements(dtype, {bias_gate, bias_up})) return rc;
+  if (rows == 0) return DFA3D_OK;
+  REQUIRE_OPERAND(x, x_pitch, in);
+  REQUIRE_OPERAND(weight_gate, weight_pitch, in);
+  REQUIRE_OPERAND(weight_up, weight_pitch, in);
+  REQUIRE_OPERAND(h, hidden_pitch, hidden);
+  dfa3d::ProductArgs a;
+  a.kind = dfa3d::kGated;
+  a.dtype = dtype;
+  a.rows = rows;
+  a.n = hidden;
+  a.k0 = in;
+  a.a0 = {x, x_pitch};
+  a.b0 = {weight_gate, weight_pitch};
+  a.b1 = {weight_up, weight_pitch};
+  a.bias0 = bias_gate;
+  a.bias1 = bias_up;
+  a.act = activation;
+  a.out[0] = h;
+  a.out_pitch = hidden_pitch;
+  return finish(dfa3d::launch_product(a, (cudaStream_t)stream), "dfa3d_gated_hidden_forward launch");
+}
+
+int dfa3d_gated_hidden_backward(const void *x, int64_t x_pitch, const void *weight_gate, const void *weight_up,
+                                int64_t weight_pitch, const void *bias_gate, const void *bias_up, const void *grad_y,
+                                int64_t grad_pitch, const void *weight_down, int64_t down_pitch, int32_t dtype, int64_t rows,
+                                int32_t in, int32_t hidden, int32_t out, int32_t activation, void *grad_gate, void *grad_up,
+                                void *h, int64_t hidden_pitch, void *stream) {
+  if (int rc = check_product(dtype, rows, {in, hidden, out}, activation)) return rc;
+  if (int rc = check_elements(dtype, {bias_gate, bias_up})) return rc;
+  if (rows == 0) return DFA3D_OK;
+  REQUIRE_OPERAND(x, x_pitch, in);
+  REQUIRE_OPERAND(weight_gate, weight_pitch, in);
+  REQUIRE_OPERAND(weight_up, weight_pitch, in);
+  REQUIRE_OPERAND(grad_y, grad_pitch, out);
+  REQUIRE_OPERAND(weight_down, down_pitch, hidden);
+  REQUIRE_OPERAND(grad_gate, hidden_pitch, hidden);
+  REQUIRE_OPERAND(grad_up, hidden_pitch, hidden);
+  REQUIRE_OPERAND(h, hidden_pitch, hidden);
+  dfa3d::ProductArgs a;
+  a.kind = dfa3d::kGatedGrad;
+  a.dtype = dtype;
+  a.rows = rows;
+  a.n = hidden;
+  a.k0 = in;
+  a.k1 = out;
+  a.a0 = {x, x_pitch};
+  a.a1 = {grad_y, grad_pitch};
+  a.b0 = {weight_gate, weight_pitch};
+  a.b1 = {weight_up, weight_pitch};
+  a.b2 = {weight_down, down_pitch};
+  a.bias0 = bias_gate;
+  a.bias1 = bias_up;
+  a.act = activation;
+  a.out[0] = grad_gate;
+  a.out[1] = grad_up;
+  a.out[2] = h;
+  a.out_pitch = hidden_pitch;
+  return finish(dfa3d::launch_product(a, (cudaStream_t)stream), "dfa3d_gated_hidden_backward launch");
+}
+
+static int check_weight_gradients(const dfa3d_weight_gradient *w, int32_t count, int64_t rows, dfa3d::WeightProblem *q) {
+  if (count < 1 || count > DFA3D_MAX_WEIGHT_GRADIENTS)
+    return fail(DFA3D_ERR_INVALID_ARGUMENT, "count must be in [1, %d] (got %d)", DFA3D_MAX_WEIGHT_GRADIENTS, count);
+  REQUIRE_PTR(w);
+  int64_t tiles = 0;
+  for (int32_t i = 0; i < count; ++i) {
+    if (int rc = check_product(DFA3D_DTYPE_BF16, rows, {w[i].in, w[i].out}, DFA3D_ROW_NONE)) return rc;
+    tiles += (int64_t)((w[i].out + 127) / 128) * ((w[i].in + 63) / 64);
+    q[i].p = w[i].out;
+    q[i].q = w[i].in;
+  }
+  if (tiles >= (1LL << 26)) return fail(DFA3D_ERR_UNSUPPORTED, "the weight gradients are too large");
+  return DFA3D_OK;
+}
+
+int64_t dfa3d_weight_gradients_workspace(const dfa3d_weight_gradient *w, int32_t count, int64_t rows) {
+  dfa3d::WeightProblem q[DFA3D_MAX_WEIGHT_GRADIENTS];
+  if (int rc = check_weight_gradients(w, count, rows, q)) return rc;
+  return dfa3d::weight_gradient_workspace(rows, q, count);
+}
+
+int dfa3d_weight_gradients(const dfa3d_weight_gradient *w, int32_t count, int32_t dtype, int64_t rows, void *workspace,
+                           int64_t workspace_bytes, void *stream) {
+  dfa3d::WeightProblem q[DFA3D_MAX_WEIGHT_GRADIENTS];
+  if (int rc = check_product(dtype, rows, {}, DFA3D_ROW_NONE)) return rc;
+  if (int rc = check_weight_gradients(w, count, rows, q)) return rc;
+  for (int32_t i = 0; i < count; ++i) {
+    if (int rc = check_elements(dtype, {w[i].grad_weight, w[i].grad_bias})) return rc;
+    REQUIRE_PTR(w[i].grad_weight);
+    if (rows > 0) {
+      REQUIRE_OPERAND(w[i].grad, w[i].grad_pitch, w[i].out);
+      REQUIRE_OPERAND(w[i].x, w[i].x_pitch, w[i].in);
+    }
+    q[i].g = {w[i].grad, w[i].grad_pitch};
+    q[i].x = {w[i].x, w[i].x_pitch};
+    q[i].out = w[i].grad_weight;
+    q[i].bias = w[i].grad_bias;
+  }
+  if (rows == 0) {      // sums over no rows
+    for (int32_t i = 0; i < count; ++i) {
+      cudaError_t rc = cudaMemsetAsync(q[i].out, 0, (size_t)q[i].p * q[i].q * 2, (cudaStream_t)stream);
+      if (rc == cudaSuccess && q[i].bias) rc = cudaMemsetAsync(q[i].bias, 0, (size_t)q[i].p * 2, (cudaStream_t)stream);
+      if (rc != cudaSuccess) return finish(rc, "dfa3d_weight_gradients");
+    }
+    return DFA3D_OK;
+  }
+  REQUIRE_PTR(workspace); REQUIRE_ALIGNED(workspace);
+  const long long need = dfa3d::weight_gradient_workspace(rows, q, count);
+  if (workspace_bytes < need)
+    return fail(DFA3D_ERR_INVALID_ARGUMENT, "workspace of %lld bytes is smaller than the %lld needed", (long long)workspace_bytes,
+                need);
+  return finish(dfa3d::launch_weight_gradient(dtype, rows, q, count, workspace, (cudaStream_t)stream),
+                "dfa3d_weight_gradients launch");
+}
+
+int dfa3d_copy_rows(const dfa3d_row_copy *c, int32_t count, int32_t dtype, void *stream) {
+  if (dtype != DFA3D_DTYPE_BF16 && dtype != DFA3D_DTYPE_F16)
+    return fail(DFA3D_ERR_INVALID_ARGUMENT, "dtype %d is neither DFA3D_DTYPE_BF16 nor DFA3D_DTYPE_F16", dtype);
+  if (count < 1 || count > DFA3D_MAX_ROW_COPIES)
+    return fail(DFA3D_ERR_INVALID_ARGUMENT, "count must be in [1, %d] (got %d)", DFA3D_MAX_ROW_COPIES, count);
+  REQUIRE_PTR(c);
+  dfa3d::RowCopy q[DFA3D_MAX_ROW_COPIES];
+  bool any = false;
+  for (int32_t i = 0; i < count; ++i) {
+    if (c[i].rows < 0 || c[i].cols < 0 || c[i].rows >= (1LL << 31) || c[i].cols >= (1LL << 31) || c[i].src_pitch < c[i].cols ||
+        c[i].dst_pitch < c[i].cols)
+      return fail(DFA3D_ERR_INVALID_ARGUMENT, "copy %d: %lld x %lld with pitches %lld and %lld", i, (long long)c[i].rows,
+                  (long long)c[i].cols, (long long)c[i].src_pitch, (long long)c[i].dst_pitch);
+    if (int rc = check_elements(c[i].wide ? DFA3D_DTYPE_F32 : dtype, {c[i].src})) return rc;
+    if (int rc = check_elements(dtype, {c[i].dst})) return rc;
+    if (c[i].rows > 0 && c[i].cols > 0) {
+      REQUIRE_PTR(c[i].src); REQUIRE_PTR(c[i].dst);
+      any = true;
+    }
+    q[i] = {c[i].src, c[i].dst, c[i].rows, c[i].cols, c[i].src_pitch, c[i].dst_pitch, c[i].wide};
+  }
+  if (!any) return DFA3D_OK;
+  return finish(dfa3d::launch_copy_rows(dtype, q, count, (cudaStream_t)stream), "dfa3d_copy_rows launch");
+}
+
+static int check_compressed(int32_t dtype, int64_t rows, int32_t cols, int32_t format) {
+  if (format != DFA3D_FORMAT_INT8 && format != DFA3D_FORMAT_E4M3)
+    return fail(DFA3D_ERR_INVALID_ARGUMENT, "format %d is not a DFA3D_FORMAT_*", format);
+  if (rows < 0 || cols < 0) return fail(DFA3D_ERR_INVALID_ARGUMENT, "rows and cols must be >= 0 (got %lld, %d)", (long long)rows, cols);
+  if (rows >= (1LL << 40) || cols > (1 << 30)) return fail(DFA3D_ERR_UNSUPPORTED, "%lld x %d is too large", (long long)rows, cols);
+  return check_elements(dtype, {});
+}
+
+int dfa3d_compress8(const void *x, int32_t dtype, int64_t rows, int32_t cols, int32_t format, uint8_t *codes, uint8_t *scales,
+                    void *stream) {
+  if (int rc = check_compressed(dtype, rows, cols, format)) return rc;
+  if (int rc = check_elements(dtype, {x})) return rc;
+  if (rows == 0 || cols == 0) return DFA3D_OK;
+  REQUIRE_PTR(x); REQUIRE_PTR(codes); REQUIRE_PTR(scales);
+  return finish(dfa3d::launch_compress8(x, dtype, rows, cols, format, codes, scales, (cudaStream_t)stream), "dfa3d_compress8 launch");
+}
+
+int dfa3d_decompress8(const uint8_t *codes, const uint8_t *scales, int32_t format, int64_t rows, int32_t cols, int32_t dtype,
+                      void *x, int64_t pitch, void *stream) {
+  if (int rc = check_compressed(dtype, rows, cols, format)) return rc;
+  if (int rc = check_elements(dtype, {x})) return rc;
+  if (pitch < cols || pitch >= (1LL << 38))
+    return fail(DFA3D_ERR_INVALID_ARGUMENT, "pitch must be at least cols (got %lld)", (long long)pitch);
+  if (rows == 0 || cols == 0) return DFA3D_OK;
+  REQUIRE_PTR(x); REQUIRE_PTR(codes); REQUIRE_PTR(scales);
+  return finish(dfa3d::launch_decompress8(codes, scales, format, rows, cols, dtype, x, pitch, (cudaStream_t)stream),
+                "dfa3d_decompress8 launch");
 }
 
 // ---- double precision -------------------------------------------------------------------------

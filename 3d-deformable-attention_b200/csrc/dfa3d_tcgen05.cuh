@@ -1,0 +1,163 @@
+// The sm_100a instructions that the matrix products are made of: barriers in shared memory, tiled copies, tensor-core products whose
+// accumulators live in tensor memory.  Thin wrappers; operand layouts are described where the descriptors are made.
+#pragma once
+#include <cuda.h>
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <stdint.h>
+
+namespace dfa3d {
+namespace tc {
+
+__device__ __forceinline__ uint32_t shared_address(const void *p) { return (uint32_t)__cvta_generic_to_shared(p); }
+
+__device__ __forceinline__ bool one_lane() {
+  uint32_t p;
+  asm volatile("{\n.reg .pred q;\nelect.sync _|q, 0xffffffff;\nselp.u32 %0, 1, 0, q;\n}" : "=r"(p));
+  return p != 0;
+}
+
+// ---- barriers ----------------------------------------------------------------------------------
+__device__ __forceinline__ void barrier_init(uint32_t bar, uint32_t arrivals) {
+  asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(arrivals) : "memory");
+}
+__device__ __forceinline__ void barriers_visible() { asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory"); }
+__device__ __forceinline__ void arrive(uint32_t bar) {
+  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ void arrive_expect(uint32_t bar, uint32_t bytes) {
+  asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ bool try_wait(uint32_t bar, uint32_t parity) {
+  uint32_t done;
+  asm volatile("{\n.reg .pred q;\nmbarrier.try_wait.parity.shared::cta.b64 q, [%1], %2;\nselp.u32 %0, 1, 0, q;\n}"
+               : "=r"(done)
+               : "r"(bar), "r"(parity)
+               : "memory");
+  return done != 0;
+}
+__device__ __forceinline__ uint64_t nanoseconds() {
+  uint64_t t;
+  asm volatile("mov.u64 %0, %globaltimer;" : "=l"(t));
+  return t;
+}
+constexpr uint64_t kPatience = 4000000000ull;      // ns; waits here last microseconds
+
+// Waits for the phase of `parity` to end; false when that took longer than any sound run could.
+static __device__ __noinline__ bool wait_long(uint32_t bar, uint32_t parity) {
+  const uint64_t start = nanoseconds();
+  do {
+    for (int i = 0; i < 64; ++i)
+      if (try_wait(bar, parity)) return true;
+  } while (nanoseconds() - start < kPatience);
+  return false;
+}
+__device__ __forceinline__ bool wait(uint32_t bar, uint32_t parity) {
+  for (int i = 0; i < 16; ++i)
+    if (try_wait(bar, parity)) return true;
+  return wait_long(bar, parity);
+}
+
+// ---- tiled copies ------------------------------------------------------------------------------
+__device__ __forceinline__ void fetch_map(const CUtensorMap *map) {
+  asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory");
+}
+__device__ __forceinline__ void tile_load(uint32_t dst, const CUtensorMap *map, int x, int y, uint32_t bar) {
+  asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(dst),
+               "l"(map), "r"(x), "r"(y), "r"(bar)
+               : "memory");
+}
+__device__ __forceinline__ void tile_store(const CUtensorMap *map, int x, int y, uint32_t src) {
+  asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.tile.bulk_group [%0, {%1, %2}], [%3];" ::"l"(map), "r"(x), "r"(y), "r"(src)
+               : "memory");
+}
+__device__ __forceinline__ void stores_asked() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }
+template <int LEFT> __device__ __forceinline__ void stores_read() {      // all but the last LEFT groups have left shared memory
+  asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(LEFT) : "memory");
+}
+__device__ __forceinline__ void stores_done() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
+// ordinary accesses of shared memory before it, tiled copies and products of it after it
+__device__ __forceinline__ void shared_to_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+
+// ---- tensor memory -----------------------------------------------------------------------------
+template <int COLUMNS> __device__ __forceinline__ void tensor_memory_take(uint32_t where) {      // one whole warp
+  static_assert(COLUMNS >= 32 && COLUMNS <= 512 && (COLUMNS & (COLUMNS - 1)) == 0, "power of two");
+  asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(where), "n"(COLUMNS) : "memory");
+  asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+}
+template <int COLUMNS> __device__ __forceinline__ void tensor_memory_give(uint32_t base) {       // the same warp
+  asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(base), "n"(COLUMNS));
+}
+__device__ __forceinline__ void order_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void order_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+
+// 32 columns of the 32 lanes that this warp may read: thread = lane = row of the accumulator.  Not there before tensor_loads_done().
+__device__ __forceinline__ void tensor_load(float (&v)[32], uint32_t at) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,"
+      "%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,"
+      "%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+      : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7]),
+        "=f"(v[8]), "=f"(v[9]), "=f"(v[10]), "=f"(v[11]), "=f"(v[12]), "=f"(v[13]), "=f"(v[14]), "=f"(v[15]),
+        "=f"(v[16]), "=f"(v[17]), "=f"(v[18]), "=f"(v[19]), "=f"(v[20]), "=f"(v[21]), "=f"(v[22]), "=f"(v[23]),
+        "=f"(v[24]), "=f"(v[25]), "=f"(v[26]), "=f"(v[27]), "=f"(v[28]), "=f"(v[29]), "=f"(v[30]), "=f"(v[31])
+      : "r"(at));
+}
+// The values pass through it, so that nothing that uses them can be moved in front of it.
+__device__ __forceinline__ void tensor_loads_done(float (&v)[32]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+      : "+f"(v[0]), "+f"(v[1]), "+f"(v[2]), "+f"(v[3]), "+f"(v[4]), "+f"(v[5]), "+f"(v[6]), "+f"(v[7]),
+        "+f"(v[8]), "+f"(v[9]), "+f"(v[10]), "+f"(v[11]), "+f"(v[12]), "+f"(v[13]), "+f"(v[14]), "+f"(v[15]),
+        "+f"(v[16]), "+f"(v[17]), "+f"(v[18]), "+f"(v[19]), "+f"(v[20]), "+f"(v[21]), "+f"(v[22]), "+f"(v[23]),
+        "+f"(v[24]), "+f"(v[25]), "+f"(v[26]), "+f"(v[27]), "+f"(v[28]), "+f"(v[29]), "+f"(v[30]), "+f"(v[31])
+      :
+      : "memory");
+}
+
+// ---- products ----------------------------------------------------------------------------------
+// Operand tiles are rows of 128 bytes (64 elements of 16 bits) whose 16-byte pieces are permuted by the low three bits of the row
+// number (the 128-byte swizzle of tiled copies), on a 1024-byte boundary.
+//   k_major:  a row is 64 elements along the summed axis; eight rows, 1024 bytes, further come the next eight of the other axis.  A
+//             step of 16 along the summed axis is 32 bytes.
+//   mn_major: a row is 64 elements along the other axis, one row for each element of the summed one; eight rows, 1024 bytes, further
+//             come the next eight of the summed axis; `group` bytes further the next 64 of the other.  A step of 16 is 2048 bytes.
+constexpr uint64_t kOperandBits = (uint64_t(1) << 46) | (uint64_t(2) << 61) | (uint64_t(1024 >> 4) << 32);
+__device__ __forceinline__ uint64_t k_major(uint32_t at) { return kOperandBits | (uint64_t(1) << 16) | ((at >> 4) & 0x3fff); }
+__device__ __forceinline__ uint64_t mn_major(uint32_t at, uint32_t group) {
+  return kOperandBits | (uint64_t(group >> 4) << 16) | ((at >> 4) & 0x3fff);
+}
+template <typename T> constexpr uint32_t kOperandType = 0;                     // fp16
+template <> inline constexpr uint32_t kOperandType<__nv_bfloat16> = 1;
+// 128 rows, n columns, 32-bit sums
+template <typename T> __host__ __device__ constexpr uint32_t product_shape(int n, bool a_mn_major, bool b_mn_major) {
+  return (1u << 4) | (kOperandType<T> << 7) | (kOperandType<T> << 10) | (uint32_t(a_mn_major) << 15) | (uint32_t(b_mn_major) << 16) |
+         (uint32_t(n / 8) << 17) | (uint32_t(128 / 16) << 24);
+}
+// D (+)= A B over 16 elements of the summed axis; one thread
+__device__ __forceinline__ void product(uint32_t d, uint64_t a, uint64_t b, uint32_t shape, bool add) {
+  asm volatile("{\n.reg .pred q;\nsetp.ne.u32 q, %4, 0;\ntcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, q;\n}" ::"r"(d), "l"(a),
+               "l"(b), "r"(shape), "r"((uint32_t)add)
+               : "memory");
+}
+// The barrier is arrived at when the products that this thread has issued so far are done.
+__device__ __forceinline__ void products_arrive(uint32_t bar) {
+  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+}
+
+// ---- shared memory by address ------------------------------------------------------------------
+__device__ __forceinline__ uint4 read16(uint32_t at) {
+  uint4 w;
+  asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(w.x), "=r"(w.y), "=r"(w.z), "=r"(w.w) : "r"(at) : "memory");
+  return w;
+}
+__device__ __forceinline__ void write16(uint32_t at, uint4 w) {
+  asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(w.x), "r"(w.y), "r"(w.z), "r"(w.w) : "memory");
+}
+__device__ __forceinline__ float4 read_four(uint32_t at) {
+  float4 w;
+  asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(w.x), "=f"(w.y), "=f"(w.z), "=f"(w.w) : "r"(at) : "memory");
+  return w;
+}
+
+}  // namespace tc
+}  // namespace dfa3d

@@ -33,6 +33,19 @@ class Problem(ctypes.Structure):
         super().__init__(*args, **kw)
 
 
+class WeightGradient(ctypes.Structure):
+    """struct dfa3d_weight_gradient."""
+    _fields_ = [("grad", ctypes.c_void_p), ("x", ctypes.c_void_p), ("grad_pitch", ctypes.c_int64), ("x_pitch", ctypes.c_int64),
+                ("grad_weight", ctypes.c_void_p), ("grad_bias", ctypes.c_void_p), ("in_features", ctypes.c_int32),
+                ("out_features", ctypes.c_int32)]
+
+
+class RowCopy(ctypes.Structure):
+    """struct dfa3d_row_copy."""
+    _fields_ = [("src", ctypes.c_void_p), ("dst", ctypes.c_void_p)] + \
+               [(n, ctypes.c_int64) for n in ("rows", "cols", "src_pitch", "dst_pitch")] + [("wide", ctypes.c_int32)]
+
+
 class _I32:
     """An int32 argument.  ctypes.c_int32 would pass the lower half of a number that does not fit."""
 
@@ -112,12 +125,25 @@ PLAIN_ENTRY_POINTS = {
     "dfa3d_group_norm_backward": [_V, _V] + [_I32] * 5 + [_V, _I32, _V, _I32, _V, _V, _I32, _I32] + [_V] * 6 + [_I64, _V],
     "dfa3d_dropout_add_layer_norm_workspace": [_I64, _I32],
     "dfa3d_group_norm_workspace": [_I32] * 6,
+    "dfa3d_linear_act_forward": [_V, _I64, _V, _I64, _V, _V, _I32, _I32, _I64, _I32, _I32, _I32, _V, _V],
+    "dfa3d_linear_act_slope": [_V, _I64, _V, _I64, _V, _V, _I64, _I32, _I64, _I32, _I32, _I32, _V, _V],
+    "dfa3d_linear_input_gradient": [_V, _V, _I64, _V, _V, _I64, _V, _I64, _I32, _I64, _I32, _I32, _V, _V],
+    "dfa3d_gated_hidden_forward": [_V, _I64, _V, _V, _I64, _V, _V, _I32, _I64, _I32, _I32, _I32, _V, _I64, _V],
+    "dfa3d_gated_hidden_backward": [_V, _I64, _V, _V, _I64, _V, _V, _V, _I64, _V, _I64, _I32, _I64] + [_I32] * 4
+                                   + [_V, _V, _V, _I64, _V],
+    "dfa3d_weight_gradients_workspace": [_V, _I32, _I64],
+    "dfa3d_weight_gradients": [_V, _I32, _I32, _I64, _V, _I64, _V],
+    "dfa3d_copy_rows": [_V, _I32, _I32, _V],
+    "dfa3d_compress8": [_V, _I32, _I64, _I32, _I32, _V, _V, _V],
+    "dfa3d_decompress8": [_V, _V, _I32, _I64, _I32, _I32, _V, _I64, _V],
     "dfa3d_zero_two": [ctypes.c_void_p, _I64, ctypes.c_void_p, _I64, ctypes.c_void_p],
 }
 # of these the ones that answer with a number of bytes (or a negative error code)
-SIZE_ENTRY_POINTS = ("dfa3d_dropout_add_layer_norm_workspace", "dfa3d_group_norm_workspace")
+SIZE_ENTRY_POINTS = ("dfa3d_dropout_add_layer_norm_workspace", "dfa3d_group_norm_workspace",
+                     "dfa3d_weight_gradients_workspace")
 ACT_SOFTMAX, ACT_SIGMOID = 0, 1
-ROW_NONE, ROW_RELU, ROW_SILU = 0, 1, 2
+ROW_NONE, ROW_RELU, ROW_SILU, ROW_GELU = 0, 1, 2, 3
+FORMAT_INT8, FORMAT_E4M3 = 0, 1
 
 _lib = None
 _native = None

@@ -413,6 +413,7 @@ int dfa3d_convert_two(int32_t narrow_dtype, int32_t widen, void *narrow0, void *
 #define DFA3D_ROW_NONE 0
 #define DFA3D_ROW_RELU 1
 #define DFA3D_ROW_SILU 2
+#define DFA3D_ROW_GELU 3      /* with erf; the products of a feed-forward block only */
 
 /* y = [residual +] keep * act(x) / (1 - p), n elements; activation DFA3D_ROW_NONE or _RELU; residual may be null.  y may be x. */
 int dfa3d_dropout_forward(const void *x, const void *residual, int32_t dtype, int64_t n, int32_t activation, double p,
@@ -465,6 +466,88 @@ int dfa3d_group_norm_backward(const void *grad_y, const void *x, int32_t dtype, 
                               const float *weight, const float *bias, int32_t weight_rows, int32_t activation,
                               const float *mean, const float *rstd, void *grad_x, float *grad_weight, float *grad_bias,
                               void *workspace, int64_t workspace_bytes, void *stream);
+
+/* ---- products of a feed-forward block -------------------------------------------------------------
+ * Matrix products of bf16 or fp16 matrices on the tensor cores with what follows them: sums, bias, activation, residual and
+ * derivatives in fp32, one rounding at the end.  dtype (of all matrices and vectors unless it is said otherwise):
+ * DFA3D_DTYPE_BF16 or _F16; activation: DFA3D_ROW_*.  Matrices are row-major; an argument with a pitch (elements from row to
+ * row) is an operand of a product or a workspace that becomes one: it begins on a 16-byte boundary and its pitch is a multiple
+ * of 8 (dfa3d_copy_rows makes such a copy; what lies between the columns and the pitch is not looked at).  Matrices without
+ * a pitch are contiguous and may lie anywhere.  0 <= rows < 2^31 - 128, widths from 1 to 2^24.  Results overlap no input. */
+
+/* y (rows, out) = act(x W^T + bias) + residual, x (rows, in), weight (out, in).  bias (out) and residual (rows, out) may be null.
+ * out_dtype (of residual and y): dtype or DFA3D_DTYPE_F32. */
+int dfa3d_linear_act_forward(const void *x, int64_t x_pitch, const void *weight, int64_t weight_pitch, const void *bias,
+                             const void *residual, int32_t dtype, int32_t out_dtype, int64_t rows, int32_t in, int32_t out,
+                             int32_t activation, void *y, void *stream);
+
+/* grad_z (rows, out) = grad_y * act'(x W^T + bias): the product is formed again.  grad_y and grad_z share a pitch. */
+int dfa3d_linear_act_slope(const void *x, int64_t x_pitch, const void *weight, int64_t weight_pitch, const void *bias,
+                           const void *grad_y, int64_t grad_pitch, int32_t dtype, int64_t rows, int32_t in, int32_t out,
+                           int32_t activation, void *grad_z, void *stream);
+
+/* grad_x (rows, in) = grad W [+ grad2 W2] [+ add], grad (rows, out), weight (out, in).  grad2 and weight2, of the same sizes, may
+ * be null together, add (rows, in) by itself. */
+int dfa3d_linear_input_gradient(const void *grad, const void *grad2, int64_t grad_pitch, const void *weight, const void *weight2,
+                                int64_t weight_pitch, const void *add, int64_t add_pitch, int32_t dtype, int64_t rows, int32_t in,
+                                int32_t out, void *grad_x, void *stream);
+
+/* h (rows, hidden) = act(x Wg^T + bg) * (x Wu^T + bu), the first half of a gated feed-forward block; both biases may be null.
+ * weight_pitch is that of both weights. */
+int dfa3d_gated_hidden_forward(const void *x, int64_t x_pitch, const void *weight_gate, const void *weight_up,
+                               int64_t weight_pitch, const void *bias_gate, const void *bias_up, int32_t dtype, int64_t rows,
+                               int32_t in, int32_t hidden, int32_t activation, void *h, int64_t hidden_pitch, void *stream);
+
+/* What the backward of the block needs, from x and the gradient grad_y (rows, out) of h Wd^T: with g, u = the two products again
+ * and d = grad_y Wd, Wd (out, hidden):  grad_gate = d u act'(g), grad_up = d act(g), h = act(g) u.  All three (rows, hidden) with
+ * hidden_pitch. */
+int dfa3d_gated_hidden_backward(const void *x, int64_t x_pitch, const void *weight_gate, const void *weight_up,
+                                int64_t weight_pitch, const void *bias_gate, const void *bias_up, const void *grad_y,
+                                int64_t grad_pitch, const void *weight_down, int64_t down_pitch, int32_t dtype, int64_t rows,
+                                int32_t in, int32_t hidden, int32_t out, int32_t activation, void *grad_gate, void *grad_up,
+                                void *h, int64_t hidden_pitch, void *stream);
+
+/* grad_weight (out, in) = grad^T x over the rows, grad_bias (out) = sum of grad over the rows (null: not wanted), contiguous. */
+typedef struct dfa3d_weight_gradient {
+  const void *grad, *x;            /* (rows, out), (rows, in) */
+  int64_t grad_pitch, x_pitch;
+  void *grad_weight, *grad_bias;
+  int32_t in, out;
+} dfa3d_weight_gradient;
+#define DFA3D_MAX_WEIGHT_GRADIENTS 3
+
+/* Bytes of device memory that a call with these sizes needs (16-byte aligned, contents irrelevant), or a negative error code. */
+int64_t dfa3d_weight_gradients_workspace(const dfa3d_weight_gradient *w, int32_t count, int64_t rows);
+
+/* Up to three of them at once (the table is in HOST memory).  The rows are summed in shares that are added up in a fixed order:
+ * same bits in every run on one device. */
+int dfa3d_weight_gradients(const dfa3d_weight_gradient *w, int32_t count, int32_t dtype, int64_t rows, void *workspace,
+                           int64_t workspace_bytes, void *stream);
+
+/* Copies of matrices of 16-bit elements (wide: of fp32, rounded to dtype), up to eight with one launch; the table is in HOST
+ * memory. */
+typedef struct dfa3d_row_copy {
+  const void *src;
+  void *dst;
+  int64_t rows, cols, src_pitch, dst_pitch;
+  int32_t wide;
+} dfa3d_row_copy;
+#define DFA3D_MAX_ROW_COPIES 8
+int dfa3d_copy_rows(const dfa3d_row_copy *c, int32_t count, int32_t dtype, void *stream);
+
+/* ---- activations in 8 bits -----------------------------------------------------------------------
+ * Blocks of 32 neighbours of a row (the last one of a row may be shorter) under one power of two 2^e, e >= -127 the smallest for
+ * which no element is beyond the format's largest number: 127 (DFA3D_FORMAT_INT8, signed integers) or 448 (DFA3D_FORMAT_E4M3,
+ * sign, 4 bits of exponent, 3 of mantissa).  A code is x / 2^e rounded to nearest even; it stands for code * 2^e, or the largest
+ * finite number of the type where that is beyond it.  codes (rows, cols), scales (rows, ceil(cols / 32)) = e + 127, or 255 for a
+ * block that held an infinity or NaN: all of it comes back as NaN.  x of DFA3D_DTYPE_F32, _BF16 or _F16, anywhere in memory; the
+ * pitch of the second is in elements. */
+#define DFA3D_FORMAT_INT8 0
+#define DFA3D_FORMAT_E4M3 1
+int dfa3d_compress8(const void *x, int32_t dtype, int64_t rows, int32_t cols, int32_t format, uint8_t *codes, uint8_t *scales,
+                    void *stream);
+int dfa3d_decompress8(const uint8_t *codes, const uint8_t *scales, int32_t format, int64_t rows, int32_t cols, int32_t dtype,
+                      void *x, int64_t pitch, void *stream);
 
 #ifdef __cplusplus
 }
