@@ -974,7 +974,7 @@ int dfa3d_linear_act_forward(const void *x, int64_t x_pitch, const void *weight,
   dfa3d::ProductArgs a;
   a.kind = dfa3d::kLinear;
   a.dtype = dtype;
-  a.wide_out = out_dtype == DFA3D_DTYPE_F32;
+  a.wide = out_dtype == DFA3D_DTYPE_F32;
   a.rows = rows;
   a.n = out;
   a.k0 = in;
@@ -989,15 +989,17 @@ int dfa3d_linear_act_forward(const void *x, int64_t x_pitch, const void *weight,
 }
 
 int dfa3d_linear_act_slope(const void *x, int64_t x_pitch, const void *weight, int64_t weight_pitch, const void *bias,
-                           const void *grad_y, int64_t grad_pitch, int32_t dtype, int64_t rows, int32_t in, int32_t out,
-                           int32_t activation, void *grad_z, void *stream) {
+                           const void *grad_y, int64_t grad_pitch, int32_t dtype, int32_t grad_dtype, int64_t rows, int32_t in,
+                           int32_t out, int32_t activation, void *grad_z, int64_t grad_z_pitch, void *stream) {
   if (int rc = check_product(dtype, rows, {in, out}, activation)) return rc;
+  if (grad_dtype != dtype && grad_dtype != DFA3D_DTYPE_F32)
+    return fail(DFA3D_ERR_INVALID_ARGUMENT, "grad_dtype %d is neither dtype nor DFA3D_DTYPE_F32", grad_dtype);
   if (int rc = check_elements(dtype, {bias})) return rc;
   if (rows == 0) return DFA3D_OK;
   REQUIRE_OPERAND(x, x_pitch, in);
   REQUIRE_OPERAND(weight, weight_pitch, in);
   REQUIRE_OPERAND(grad_y, grad_pitch, out);
-  REQUIRE_OPERAND(grad_z, grad_pitch, out);
+  REQUIRE_OPERAND(grad_z, grad_z_pitch, out);
   dfa3d::ProductArgs a;
   a.kind = dfa3d::kSlope;
   a.dtype = dtype;
@@ -1010,7 +1012,8 @@ int dfa3d_linear_act_slope(const void *x, int64_t x_pitch, const void *weight, i
   a.bias0 = bias;
   a.act = activation;
   a.out[0] = grad_z;
-  a.out_pitch = grad_pitch;
+  a.out_pitch = grad_z_pitch;
+  a.wide = grad_dtype == DFA3D_DTYPE_F32;
   return finish(dfa3d::launch_product(a, (cudaStream_t)stream), "dfa3d_linear_act_slope launch");
 }
 

@@ -23,7 +23,7 @@ enum ProductKind {
 struct ProductArgs {
   ProductKind kind;
   int dtype;                // DFA3D_DTYPE_BF16 or _F16
-  bool wide_out = false;    // kLinear: in and out are fp32
+  bool wide = false;        // kLinear: in and out are fp32; kSlope: in is
   long long rows = 0;
   int n = 0, k0 = 0, k1 = 0;
   Operand a0, a1, b0, b1, b2, in;

@@ -58,6 +58,29 @@ __device__ __forceinline__ bool wait(uint32_t bar, uint32_t parity) {
   return wait_long(bar, parity);
 }
 
+// The same for a whole warp, with one answer.
+__device__ __forceinline__ bool wait_warp(uint32_t bar, uint32_t parity) { return __all_sync(0xffffffffu, wait(bar, parity)); }
+
+// ---- pairs of CTAs -----------------------------------------------------------------------------
+__device__ __forceinline__ uint32_t rank_in_pair() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %cluster_ctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ uint32_t address_in(uint32_t at, uint32_t rank) {      // the same place in another CTA's shared memory
+  uint32_t r;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(at), "r"(rank));
+  return r;
+}
+// At an address_in().  It hands over nothing but tensor memory that has been read, which order_before() and order_after() see to:
+// releasing this CTA's writes to the other one as well took 1600 cycles of a warp at each arrival.
+__device__ __forceinline__ void arrive_in(uint32_t bar) {
+  asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ void pair_sync() {      // all threads of both
+  asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+
 // ---- tiled copies ------------------------------------------------------------------------------
 __device__ __forceinline__ void fetch_map(const CUtensorMap *map) {
   asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory");
@@ -66,6 +89,16 @@ __device__ __forceinline__ void tile_load(uint32_t dst, const CUtensorMap *map, 
   asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(dst),
                "l"(map), "r"(x), "r"(y), "r"(bar)
                : "memory");
+}
+// The same for one of a pair, whose barrier may be the other's.
+__device__ __forceinline__ void tile_load_pair(uint32_t dst, const CUtensorMap *map, int x, int y, uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(dst),
+      "l"(map), "r"(x), "r"(y), "r"(bar)
+      : "memory");
+}
+__device__ __forceinline__ void tile_to_l2(const CUtensorMap *map, int x, int y) {
+  asm volatile("cp.async.bulk.prefetch.tensor.2d.L2.global.tile [%0, {%1, %2}];" ::"l"(map), "r"(x), "r"(y) : "memory");
 }
 __device__ __forceinline__ void tile_store(const CUtensorMap *map, int x, int y, uint32_t src) {
   asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.tile.bulk_group [%0, {%1, %2}], [%3];" ::"l"(map), "r"(x), "r"(y), "r"(src)
@@ -80,18 +113,26 @@ __device__ __forceinline__ void stores_done() { asm volatile("cp.async.bulk.wait
 __device__ __forceinline__ void shared_to_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
 // ---- tensor memory -----------------------------------------------------------------------------
-template <int COLUMNS> __device__ __forceinline__ void tensor_memory_take(uint32_t where) {      // one whole warp
+// PAIR: by one warp of each of the pair's CTAs, for products of both.
+template <int COLUMNS, bool PAIR> __device__ __forceinline__ void tensor_memory_take(uint32_t where) {      // one whole warp
   static_assert(COLUMNS >= 32 && COLUMNS <= 512 && (COLUMNS & (COLUMNS - 1)) == 0, "power of two");
-  asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(where), "n"(COLUMNS) : "memory");
-  asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+  if constexpr (PAIR) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(where), "n"(COLUMNS) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;");
+  } else {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(where), "n"(COLUMNS) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+  }
 }
-template <int COLUMNS> __device__ __forceinline__ void tensor_memory_give(uint32_t base) {       // the same warp
-  asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(base), "n"(COLUMNS));
+template <int COLUMNS, bool PAIR> __device__ __forceinline__ void tensor_memory_give(uint32_t base) {       // the same warp
+  if constexpr (PAIR) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(base), "n"(COLUMNS));
+  else asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(base), "n"(COLUMNS));
 }
 __device__ __forceinline__ void order_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void order_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 
-// 32 columns of the 32 lanes that this warp may read: thread = lane = row of the accumulator.  Not there before tensor_loads_done().
+// Columns of the 32 lanes that this warp may read: thread = lane = row of the accumulator.  They are not there before
+// tensor_loads_done(), through which they pass so that nothing that uses them can be moved in front of it.
 __device__ __forceinline__ void tensor_load(float (&v)[32], uint32_t at) {
   asm volatile(
       "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,"
@@ -103,13 +144,26 @@ __device__ __forceinline__ void tensor_load(float (&v)[32], uint32_t at) {
         "=f"(v[24]), "=f"(v[25]), "=f"(v[26]), "=f"(v[27]), "=f"(v[28]), "=f"(v[29]), "=f"(v[30]), "=f"(v[31])
       : "r"(at));
 }
-// The values pass through it, so that nothing that uses them can be moved in front of it.
 __device__ __forceinline__ void tensor_loads_done(float (&v)[32]) {
   asm volatile("tcgen05.wait::ld.sync.aligned;"
       : "+f"(v[0]), "+f"(v[1]), "+f"(v[2]), "+f"(v[3]), "+f"(v[4]), "+f"(v[5]), "+f"(v[6]), "+f"(v[7]),
         "+f"(v[8]), "+f"(v[9]), "+f"(v[10]), "+f"(v[11]), "+f"(v[12]), "+f"(v[13]), "+f"(v[14]), "+f"(v[15]),
         "+f"(v[16]), "+f"(v[17]), "+f"(v[18]), "+f"(v[19]), "+f"(v[20]), "+f"(v[21]), "+f"(v[22]), "+f"(v[23]),
         "+f"(v[24]), "+f"(v[25]), "+f"(v[26]), "+f"(v[27]), "+f"(v[28]), "+f"(v[29]), "+f"(v[30]), "+f"(v[31])
+      :
+      : "memory");
+}
+__device__ __forceinline__ void tensor_load(float (&v)[16], uint32_t at) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+      : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7]),
+        "=f"(v[8]), "=f"(v[9]), "=f"(v[10]), "=f"(v[11]), "=f"(v[12]), "=f"(v[13]), "=f"(v[14]), "=f"(v[15])
+      : "r"(at));
+}
+__device__ __forceinline__ void tensor_loads_done(float (&v)[16]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+      : "+f"(v[0]), "+f"(v[1]), "+f"(v[2]), "+f"(v[3]), "+f"(v[4]), "+f"(v[5]), "+f"(v[6]), "+f"(v[7]),
+        "+f"(v[8]), "+f"(v[9]), "+f"(v[10]), "+f"(v[11]), "+f"(v[12]), "+f"(v[13]), "+f"(v[14]), "+f"(v[15])
       :
       : "memory");
 }
@@ -121,27 +175,40 @@ __device__ __forceinline__ void tensor_loads_done(float (&v)[32]) {
 //             step of 16 along the summed axis is 32 bytes.
 //   mn_major: a row is 64 elements along the other axis, one row for each element of the summed one; eight rows, 1024 bytes, further
 //             come the next eight of the summed axis; `group` bytes further the next 64 of the other.  A step of 16 is 2048 bytes.
+//   mn_major_narrow: the same with rows of 64 bytes, 32 elements, and the 64-byte swizzle.  A step of 16 is 1024 bytes.
 constexpr uint64_t kOperandBits = (uint64_t(1) << 46) | (uint64_t(2) << 61) | (uint64_t(1024 >> 4) << 32);
+constexpr uint64_t kNarrowBits = (uint64_t(1) << 46) | (uint64_t(4) << 61) | (uint64_t(512 >> 4) << 32);
 __device__ __forceinline__ uint64_t k_major(uint32_t at) { return kOperandBits | (uint64_t(1) << 16) | ((at >> 4) & 0x3fff); }
 __device__ __forceinline__ uint64_t mn_major(uint32_t at, uint32_t group) {
   return kOperandBits | (uint64_t(group >> 4) << 16) | ((at >> 4) & 0x3fff);
 }
+__device__ __forceinline__ uint64_t mn_major_narrow(uint32_t at) { return kNarrowBits | (uint64_t(1) << 16) | ((at >> 4) & 0x3fff); }
 template <typename T> constexpr uint32_t kOperandType = 0;                     // fp16
 template <> inline constexpr uint32_t kOperandType<__nv_bfloat16> = 1;
-// 128 rows, n columns, 32-bit sums
-template <typename T> __host__ __device__ constexpr uint32_t product_shape(int n, bool a_mn_major, bool b_mn_major) {
+// 128 rows, or 256 of a pair; n columns; 32-bit sums
+template <typename T> __host__ __device__ constexpr uint32_t product_shape(int rows, int n, bool a_mn_major, bool b_mn_major) {
   return (1u << 4) | (kOperandType<T> << 7) | (kOperandType<T> << 10) | (uint32_t(a_mn_major) << 15) | (uint32_t(b_mn_major) << 16) |
-         (uint32_t(n / 8) << 17) | (uint32_t(128 / 16) << 24);
+         (uint32_t(n / 8) << 17) | (uint32_t(rows / 16) << 24);
 }
-// D (+)= A B over 16 elements of the summed axis; one thread
-__device__ __forceinline__ void product(uint32_t d, uint64_t a, uint64_t b, uint32_t shape, bool add) {
-  asm volatile("{\n.reg .pred q;\nsetp.ne.u32 q, %4, 0;\ntcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, q;\n}" ::"r"(d), "l"(a),
-               "l"(b), "r"(shape), "r"((uint32_t)add)
-               : "memory");
+// D (+)= A B over 16 elements of the summed axis; one thread.  PAIR: of the pair's first CTA; each CTA holds its 128 rows of A and of
+// D and half of B's columns, all at the same places.
+template <bool PAIR> __device__ __forceinline__ void product(uint32_t d, uint64_t a, uint64_t b, uint32_t shape, bool add) {
+  if constexpr (PAIR)
+    asm volatile("{\n.reg .pred q;\nsetp.ne.u32 q, %4, 0;\ntcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, q;\n}" ::"r"(d),
+                 "l"(a), "l"(b), "r"(shape), "r"((uint32_t)add)
+                 : "memory");
+  else
+    asm volatile("{\n.reg .pred q;\nsetp.ne.u32 q, %4, 0;\ntcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, q;\n}" ::"r"(d),
+                 "l"(a), "l"(b), "r"(shape), "r"((uint32_t)add)
+                 : "memory");
 }
-// The barrier is arrived at when the products that this thread has issued so far are done.
-__device__ __forceinline__ void products_arrive(uint32_t bar) {
-  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+// The barrier (PAIR: of both CTAs) is arrived at when the products that this thread has issued so far are done.
+template <bool PAIR> __device__ __forceinline__ void products_arrive(uint32_t bar) {
+  if constexpr (PAIR)
+    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar),
+                 "h"((uint16_t)3)
+                 : "memory");
+  else asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
 }
 
 // ---- shared memory by address ------------------------------------------------------------------
@@ -152,6 +219,16 @@ __device__ __forceinline__ uint4 read16(uint32_t at) {
 }
 __device__ __forceinline__ void write16(uint32_t at, uint4 w) {
   asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(w.x), "r"(w.y), "r"(w.z), "r"(w.w) : "memory");
+}
+template <typename O> __device__ __forceinline__ O read_one(uint32_t at) {
+  O v;
+  if constexpr (sizeof(O) == 4) asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(at) : "memory");
+  else asm volatile("ld.shared.u16 %0, [%1];" : "=h"(reinterpret_cast<uint16_t &>(v)) : "r"(at) : "memory");
+  return v;
+}
+template <typename O> __device__ __forceinline__ void write_one(uint32_t at, O v) {
+  if constexpr (sizeof(O) == 4) asm volatile("st.shared.f32 [%0], %1;" ::"r"(at), "f"(v) : "memory");
+  else asm volatile("st.shared.u16 [%0], %1;" ::"r"(at), "h"(reinterpret_cast<const uint16_t &>(v)) : "memory");
 }
 __device__ __forceinline__ float4 read_four(uint32_t at) {
   float4 w;

@@ -62,7 +62,7 @@ __global__ void __launch_bounds__(kThreads8, 1) weight_gradient_kernel(const __g
     tc::barrier_init(quiet, 1);
     tc::barriers_visible();
   }
-  if (warp == 2) tc::tensor_memory_take<L::memory>(where);
+  if (warp == 2) tc::tensor_memory_take<L::memory, false>(where);
   if (warp >= 4) {      // the same whatever the layout
     const T one = narrow<T>(1.f);
     const uint32_t two = (uint32_t)reinterpret_cast<const uint16_t &>(one) * 0x10001u;
@@ -103,7 +103,7 @@ __global__ void __launch_bounds__(kThreads8, 1) weight_gradient_kernel(const __g
     }
   } else if (warp == 1) {
     if (tc::one_lane()) {
-      constexpr uint32_t shape = tc::product_shape<T>(BN, true, true), shape_ones = tc::product_shape<T>(kOnes, true, false);
+      constexpr uint32_t shape = tc::product_shape<T>(kTileP, BN, true, true), shape_ones = tc::product_shape<T>(kTileP, kOnes, true, false);
       int s = 0;
       uint32_t phase = 0;
       bool ok = true;
@@ -114,17 +114,17 @@ __global__ void __launch_bounds__(kThreads8, 1) weight_gradient_kernel(const __g
 #pragma unroll
         for (int j = 0; j < kDepth / 16; ++j) {
           const uint64_t da = tc::mn_major(a + j * 2048, kDepth * 128);
-          tc::product(memory, da, tc::mn_major(b + j * 2048, kDepth * 128), shape, k > begin || j > 0);
-          if (bias) tc::product(memory + BN, da, tc::k_major(ones), shape_ones, k > begin || j > 0);
+          tc::product<false>(memory, da, tc::mn_major(b + j * 2048, kDepth * 128), shape, k > begin || j > 0);
+          if (bias) tc::product<false>(memory + BN, da, tc::k_major(ones), shape_ones, k > begin || j > 0);
         }
-        tc::products_arrive(empty + s * 8);
+        tc::products_arrive<false>(empty + s * 8);
         if (++s == L::stages) {
           s = 0;
           phase ^= 1;
         }
       }
-      if (ok) tc::products_arrive(done);
-      tc::products_arrive(quiet);
+      if (ok) tc::products_arrive<false>(done);
+      tc::products_arrive<false>(quiet);
       tc::wait(quiet, 0);
     }
   } else if (warp >= 4) {
@@ -153,7 +153,7 @@ __global__ void __launch_bounds__(kThreads8, 1) weight_gradient_kernel(const __g
   __syncthreads();
   if (warp == 2) {
     tc::order_after();
-    tc::tensor_memory_give<L::memory>(memory);
+    tc::tensor_memory_give<L::memory, false>(memory);
   }
 }
 

@@ -126,7 +126,7 @@ PLAIN_ENTRY_POINTS = {
     "dfa3d_dropout_add_layer_norm_workspace": [_I64, _I32],
     "dfa3d_group_norm_workspace": [_I32] * 6,
     "dfa3d_linear_act_forward": [_V, _I64, _V, _I64, _V, _V, _I32, _I32, _I64, _I32, _I32, _I32, _V, _V],
-    "dfa3d_linear_act_slope": [_V, _I64, _V, _I64, _V, _V, _I64, _I32, _I64, _I32, _I32, _I32, _V, _V],
+    "dfa3d_linear_act_slope": [_V, _I64, _V, _I64, _V, _V, _I64, _I32, _I32, _I64, _I32, _I32, _I32, _V, _I64, _V],
     "dfa3d_linear_input_gradient": [_V, _V, _I64, _V, _V, _I64, _V, _I64, _I32, _I64, _I32, _I32, _V, _V],
     "dfa3d_gated_hidden_forward": [_V, _I64, _V, _V, _I64, _V, _V, _I32, _I64, _I32, _I32, _I32, _V, _I64, _V],
     "dfa3d_gated_hidden_backward": [_V, _I64, _V, _V, _I64, _V, _V, _V, _I64, _V, _I64, _I32, _I64] + [_I32] * 4

@@ -172,13 +172,19 @@ class LinearActFunction(Function):
             with torch.cuda.device(grad_y.device):
                 (x, xp), (weight, bias) = _kept_input(ctx)
                 g = grad_y if grad_y.dtype in (ctx.dtype, torch.float32) else grad_y.to(ctx.dtype)
-                (w, wp), (g, gp) = _operands(ctx.dtype, weight, _rows(g))
+                g2, wide = _rows(g).contiguous(), _lib.DTYPE_F32
+                if ctx.act != _lib.ROW_NONE and g2.dtype == torch.float32 and N % 8 == 0 and g2.data_ptr() % 16 == 0:
+                    (w, wp), = _operands(ctx.dtype, weight)           # not rounded before the derivative has been applied
+                    g, gp = g2, N
+                else:
+                    (w, wp), (g, gp) = _operands(ctx.dtype, weight, g2)
+                    wide = _DTYPES[ctx.dtype]
                 st = _stream(g)
                 if ctx.act != _lib.ROW_NONE:
-                    dz, gp2 = _workspace(rows, N, g)
+                    dz, zp = _workspace(rows, N, x)
                     _lib.call_plain("dfa3d_linear_act_slope", x.data_ptr(), xp, w.data_ptr(), wp, _ptr(bias), g.data_ptr(), gp,
-                                    _DTYPES[ctx.dtype], rows, K, N, ctx.act, dz.data_ptr(), st)
-                    g = dz
+                                    _DTYPES[ctx.dtype], wide, rows, K, N, ctx.act, dz.data_ptr(), zp, st)
+                    g, gp = dz, zp
                 if need[0]:
                     grad_x = torch.empty(ctx.x_shape, dtype=ctx.dtype, device=g.device)
                     _lib.call_plain("dfa3d_linear_input_gradient", g.data_ptr(), None, gp, w.data_ptr(), None, wp, None, 0,

@@ -481,10 +481,11 @@ int dfa3d_linear_act_forward(const void *x, int64_t x_pitch, const void *weight,
                              const void *residual, int32_t dtype, int32_t out_dtype, int64_t rows, int32_t in, int32_t out,
                              int32_t activation, void *y, void *stream);
 
-/* grad_z (rows, out) = grad_y * act'(x W^T + bias): the product is formed again.  grad_y and grad_z share a pitch. */
+/* grad_z (rows, out) = grad_y * act'(x W^T + bias): the product is formed again.  grad_dtype (of grad_y): dtype or
+ * DFA3D_DTYPE_F32. */
 int dfa3d_linear_act_slope(const void *x, int64_t x_pitch, const void *weight, int64_t weight_pitch, const void *bias,
-                           const void *grad_y, int64_t grad_pitch, int32_t dtype, int64_t rows, int32_t in, int32_t out,
-                           int32_t activation, void *grad_z, void *stream);
+                           const void *grad_y, int64_t grad_pitch, int32_t dtype, int32_t grad_dtype, int64_t rows, int32_t in,
+                           int32_t out, int32_t activation, void *grad_z, int64_t grad_z_pitch, void *stream);
 
 /* grad_x (rows, in) = grad W [+ grad2 W2] [+ add], grad (rows, out), weight (out, in).  grad2 and weight2, of the same sizes, may
  * be null together, add (rows, in) by itself. */
