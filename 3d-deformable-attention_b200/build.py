@@ -19,7 +19,8 @@ SOURCES = ["dfa3d_forward.cu", "dfa3d_forward_packed.cu", "dfa3d_backward.cu", "
            "dfa3d_checkpoint8.cu", "dfa3d_capi.cu"]
 RATES_SRC = os.path.join(CSRC, "rates", "dfa3d_rates.cu")
 RATES_OUT = os.path.join(HERE, "dfa3d_b200", "libdfa3d_rates.so")
-NATIVE_SRC = [os.path.join(CSRC, "binding", f) for f in ("dfa3d_torch.cpp", "dfa3d_torch_layers.cpp", "dfa3d_torch_rows.cpp")]
+NATIVE_SRC = [os.path.join(CSRC, "binding", f) for f in ("dfa3d_torch.cpp", "dfa3d_torch_layers.cpp", "dfa3d_torch_rows.cpp",
+                                                           "dfa3d_torch_ffn.cpp")]
 NATIVE_OUT = os.path.join(HERE, "dfa3d_b200", "_native.so")
 INCLUDE = os.path.join(HERE, "..", "include")
 NVCC_FLAGS = ["-O3", "-I", INCLUDE, "-std=c++17", "-lineinfo", "-gencode", "arch=compute_100a,code=sm_100a",

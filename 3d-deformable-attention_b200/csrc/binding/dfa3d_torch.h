@@ -1,5 +1,6 @@
 // What the parts of the native host path share: the C ABI's entry points, argument checks and small helpers
-// (dfa3d_torch.cpp: the operator; dfa3d_torch_layers.cpp: the layer around it; dfa3d_torch_rows.cpp: dropout and group norm).
+// (dfa3d_torch.cpp: the operator; dfa3d_torch_layers.cpp: the layer around it; dfa3d_torch_rows.cpp: dropout and group norm;
+// dfa3d_torch_ffn.cpp: the feed-forward block in 16 bits).
 #pragma once
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
@@ -42,7 +43,9 @@ using torch::autograd::variable_list;
   X(dfa3d_dropout_forward) X(dfa3d_dropout_backward) X(dfa3d_dropout_add_layer_norm_forward)             \
   X(dfa3d_dropout_add_layer_norm_workspace) X(dfa3d_dropout_add_layer_norm_backward)                     \
   X(dfa3d_group_norm_workspace) X(dfa3d_group_norm_forward) X(dfa3d_group_norm_backward)                 \
-  X(dfa3d_relu_dropout_backward_column_sum)
+  X(dfa3d_relu_dropout_backward_column_sum) X(dfa3d_linear_act_forward) X(dfa3d_linear_act_slope)        \
+  X(dfa3d_linear_input_gradient) X(dfa3d_gated_hidden_forward) X(dfa3d_gated_hidden_backward)            \
+  X(dfa3d_weight_gradients_workspace) X(dfa3d_weight_gradients) X(dfa3d_copy_rows) X(dfa3d_compress8) X(dfa3d_decompress8)
 
 struct Abi {
 #define X(name) decltype(&::name) name = nullptr;
@@ -316,5 +319,6 @@ constexpr int64_t kSplitRows = 16384, kSplits = 16;
 
 extern PyMethodDef layer_methods[];      // dfa3d_torch_layers.cpp, ends in a null entry
 extern PyMethodDef row_methods[];        // dfa3d_torch_rows.cpp, likewise
+extern PyMethodDef ffn_methods[];        // dfa3d_torch_ffn.cpp, likewise
 
 }  // namespace dfa3d_torch

@@ -12,7 +12,7 @@ namespace dfa3d {
 namespace {
 
 constexpr int kPack = 8, kBlock = 32;      // elements of a thread, of a block (four threads)
-constexpr int kThreads8 = 256, kItems = 2;
+constexpr int kThreads8 = 256, kItems = 4;
 
 // The factor's exponent + 127 for a largest magnitude of `top` (its bits); 255 where that is no number.
 template <int FORMAT> __device__ __forceinline__ uint32_t scale_of(uint32_t top) {
@@ -75,26 +75,42 @@ template <typename T, int FORMAT> __device__ __forceinline__ void decode(uint2 c
   }
 }
 
-// Item = eight elements of a row: (row, piece), four pieces a block, rows of `pieces` pieces.
-template <typename T, int FORMAT, bool WORDS>
+// Item = eight elements of a row: (row, piece), `pieces` a row.  How they lie: kFlat, whole blocks in every row, so that neither rows
+// nor blocks have to be found (a division costs more than the rest of an item); kWords, rows of whole items; kAny.
+enum Lie { kFlat, kWords, kAny };
+template <Lie LIE> struct Items {
+  long long items;
+  int pieces;
+  __device__ __forceinline__ void find(long long item, long long &row, int &col) const {
+    if constexpr (LIE == kFlat) {
+      row = 0;
+      col = 0;
+    } else {
+      row = item >> 31 ? item / pieces : (long long)((uint32_t)item / (uint32_t)pieces);
+      col = (int)(item - row * pieces) * kPack;
+    }
+  }
+};
+
+template <typename T, int FORMAT, Lie LIE>
 __global__ void __launch_bounds__(kThreads8) compress8_kernel(const T *__restrict__ x, long long rows, int cols, uint8_t *__restrict__ codes,
                                                                uint8_t *__restrict__ scales) {
-  const int blocks = (cols + kBlock - 1) / kBlock, pieces = blocks * 4;
-  const long long items = rows * pieces;
-  for (long long first = (long long)blockIdx.x * (kThreads8 * kItems); first < items; first += (long long)gridDim.x * (kThreads8 * kItems)) {
+  const int blocks = (cols + kBlock - 1) / kBlock;
+  const Items<LIE> all{rows * blocks * 4, blocks * 4};
+  for (long long first = (long long)blockIdx.x * (kThreads8 * kItems); first < all.items;
+       first += (long long)gridDim.x * (kThreads8 * kItems)) {
     float f[kItems][kPack];
     long long row[kItems];
     int col[kItems];
 #pragma unroll
     for (int k = 0; k < kItems; ++k) {
       const long long item = first + k * kThreads8 + threadIdx.x;
-      row[k] = item / pieces;
-      col[k] = (int)(item - row[k] * pieces) * kPack;
+      all.find(item, row[k], col[k]);
 #pragma unroll
       for (int i = 0; i < kPack; ++i) f[k][i] = 0.f;
-      if (item >= items) continue;
-      const T *src = x + row[k] * cols + col[k];
-      if constexpr (WORDS) {
+      if (item >= all.items) continue;
+      const T *src = LIE == kFlat ? x + item * kPack : x + row[k] * cols + col[k];
+      if constexpr (LIE != kAny) {
         if (col[k] < cols) {
           constexpr int V = 16 / (int)sizeof(T);
 #pragma unroll
@@ -113,21 +129,26 @@ __global__ void __launch_bounds__(kThreads8) compress8_kernel(const T *__restric
     }
 #pragma unroll
     for (int k = 0; k < kItems; ++k) {
+      const long long item = first + k * kThreads8 + threadIdx.x;
       uint32_t top = 0;
 #pragma unroll
       for (int i = 0; i < kPack; ++i) top = max(top, __float_as_uint(f[k][i]) & 0x7fffffffu);
       top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
       top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
       const uint32_t scale = scale_of<FORMAT>(top);
-      if (row[k] >= rows) continue;
+      if (item >= all.items) continue;
       if (scale == 255) {
 #pragma unroll
         for (int i = 0; i < kPack; ++i) f[k][i] = 0.f;
       }
-      if (col[k] % kBlock == 0) scales[row[k] * blocks + col[k] / kBlock] = (uint8_t)scale;
+      if constexpr (LIE == kFlat) {
+        if (item % 4 == 0) scales[item / 4] = (uint8_t)scale;
+      } else {
+        if (col[k] % kBlock == 0) scales[row[k] * blocks + col[k] / kBlock] = (uint8_t)scale;
+      }
       const uint2 w = encode<FORMAT>(f[k], inverse_of(scale));
-      uint8_t *dst = codes + row[k] * cols + col[k];
-      if constexpr (WORDS) {
+      uint8_t *dst = LIE == kFlat ? codes + item * kPack : codes + row[k] * cols + col[k];
+      if constexpr (LIE != kAny) {
         if (col[k] < cols) *reinterpret_cast<uint2 *>(dst) = w;
       } else {
 #pragma unroll
@@ -138,12 +159,13 @@ __global__ void __launch_bounds__(kThreads8) compress8_kernel(const T *__restric
   }
 }
 
-template <typename T, int FORMAT, bool WORDS>
+template <typename T, int FORMAT, Lie LIE>
 __global__ void __launch_bounds__(kThreads8) decompress8_kernel(const uint8_t *__restrict__ codes, const uint8_t *__restrict__ scales,
                                                                  long long rows, int cols, T *__restrict__ x, long long pitch) {
   const int blocks = (cols + kBlock - 1) / kBlock, pieces = (cols + kPack - 1) / kPack;
-  const long long items = rows * pieces;
-  for (long long first = (long long)blockIdx.x * (kThreads8 * kItems); first < items; first += (long long)gridDim.x * (kThreads8 * kItems)) {
+  const Items<LIE> all{rows * pieces, pieces};
+  for (long long first = (long long)blockIdx.x * (kThreads8 * kItems); first < all.items;
+       first += (long long)gridDim.x * (kThreads8 * kItems)) {
     uint2 w[kItems];
     uint32_t scale[kItems];
     long long row[kItems];
@@ -151,28 +173,28 @@ __global__ void __launch_bounds__(kThreads8) decompress8_kernel(const uint8_t *_
 #pragma unroll
     for (int k = 0; k < kItems; ++k) {
       const long long item = first + k * kThreads8 + threadIdx.x;
-      row[k] = item / pieces;
-      col[k] = (int)(item - row[k] * pieces) * kPack;
+      all.find(item, row[k], col[k]);
       w[k] = make_uint2(0, 0);
       scale[k] = 0;
-      if (item >= items) continue;
-      const uint8_t *src = codes + row[k] * cols + col[k];
-      if constexpr (WORDS) {
+      if (item >= all.items) continue;
+      const uint8_t *src = LIE == kFlat ? codes + item * kPack : codes + row[k] * cols + col[k];
+      if constexpr (LIE != kAny) {
         w[k] = __ldcs(reinterpret_cast<const uint2 *>(src));
       } else {
 #pragma unroll
         for (int i = 0; i < kPack; ++i)
           if (col[k] + i < cols) (i < 4 ? w[k].x : w[k].y) |= (uint32_t)src[i] << (8 * (i & 3));
       }
-      scale[k] = scales[row[k] * blocks + col[k] / kBlock];
+      scale[k] = scales[LIE == kFlat ? item / 4 : row[k] * blocks + col[k] / kBlock];
     }
 #pragma unroll
     for (int k = 0; k < kItems; ++k) {
-      if (row[k] >= rows) continue;
+      const long long item = first + k * kThreads8 + threadIdx.x;
+      if (item >= all.items) continue;
       float f[kPack];
       decode<T, FORMAT>(w[k], scale[k], f);
-      T *dst = x + row[k] * pitch + col[k];
-      if constexpr (WORDS) {
+      T *dst = LIE == kFlat ? x + item * kPack : x + row[k] * pitch + col[k];
+      if constexpr (LIE != kAny) {
         constexpr int V = 16 / (int)sizeof(T);
 #pragma unroll
         for (int i = 0; i < kPack; i += V) {
@@ -201,30 +223,52 @@ template <typename T, int FORMAT>
 void compress_typed(const void *x, long long rows, int cols, uint8_t *codes, uint8_t *scales, cudaStream_t s) {
   const unsigned grid = grid_of(rows * ((cols + kBlock - 1) / kBlock) * 4);
   const T *src = static_cast<const T *>(x);
-  if (cols % kPack == 0 && on_grid(x, 16) && on_grid(codes, 8)) compress8_kernel<T, FORMAT, true><<<grid, kThreads8, 0, s>>>(src, rows, cols, codes, scales);
-  else compress8_kernel<T, FORMAT, false><<<grid, kThreads8, 0, s>>>(src, rows, cols, codes, scales);
+  const bool words = cols % kPack == 0 && on_grid(x, 16) && on_grid(codes, 8);
+  if (words && cols % kBlock == 0) compress8_kernel<T, FORMAT, kFlat><<<grid, kThreads8, 0, s>>>(src, rows, cols, codes, scales);
+  else if (words) compress8_kernel<T, FORMAT, kWords><<<grid, kThreads8, 0, s>>>(src, rows, cols, codes, scales);
+  else compress8_kernel<T, FORMAT, kAny><<<grid, kThreads8, 0, s>>>(src, rows, cols, codes, scales);
 }
 template <typename T, int FORMAT>
 void decompress_typed(const uint8_t *codes, const uint8_t *scales, long long rows, int cols, void *x, long long pitch, cudaStream_t s) {
   const unsigned grid = grid_of(rows * ((cols + kPack - 1) / kPack));
   T *dst = static_cast<T *>(x);
-  if (cols % kPack == 0 && pitch % kPack == 0 && on_grid(x, 16) && on_grid(codes, 8))
-    decompress8_kernel<T, FORMAT, true><<<grid, kThreads8, 0, s>>>(codes, scales, rows, cols, dst, pitch);
-  else decompress8_kernel<T, FORMAT, false><<<grid, kThreads8, 0, s>>>(codes, scales, rows, cols, dst, pitch);
+  const bool words = cols % kPack == 0 && pitch % kPack == 0 && on_grid(x, 16) && on_grid(codes, 8);
+  if (words && cols % kBlock == 0 && pitch == cols)
+    decompress8_kernel<T, FORMAT, kFlat><<<grid, kThreads8, 0, s>>>(codes, scales, rows, cols, dst, pitch);
+  else if (words) decompress8_kernel<T, FORMAT, kWords><<<grid, kThreads8, 0, s>>>(codes, scales, rows, cols, dst, pitch);
+  else decompress8_kernel<T, FORMAT, kAny><<<grid, kThreads8, 0, s>>>(codes, scales, rows, cols, dst, pitch);
 }
 
 // ------------------------------------------------------------------------------------------------
 struct Copies {
   RowCopy of[kMaxRowCopies];
+  int words[kMaxRowCopies];      // eight elements at a time
 };
 template <typename T> __global__ void __launch_bounds__(256) copy_rows_kernel(const __grid_constant__ Copies c) {
   const RowCopy &m = c.of[blockIdx.y];
-  const long long n = m.rows * m.cols;
+  const int each = c.words[blockIdx.y] ? 8 : 1;
+  const long long n = m.rows * m.cols / each, across = m.cols / each;
   T *dst = static_cast<T *>(m.dst);
   for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < n; i += (long long)gridDim.x * 256) {
-    const long long row = i / m.cols, col = i - row * m.cols;
-    if (m.wide) dst[row * m.dst_pitch + col] = narrow<T>(static_cast<const float *>(m.src)[row * m.src_pitch + col]);
-    else dst[row * m.dst_pitch + col] = static_cast<const T *>(m.src)[row * m.src_pitch + col];
+    const long long row = (i | across) >> 31 ? i / across : (long long)((uint32_t)i / (uint32_t)across), col = (i - row * across) * each;
+    T *to = dst + row * m.dst_pitch + col;
+    if (each == 1) {
+      *to = m.wide ? narrow<T>(static_cast<const float *>(m.src)[row * m.src_pitch + col])
+                   : static_cast<const T *>(m.src)[row * m.src_pitch + col];
+    } else if (m.wide) {
+      const float *from = static_cast<const float *>(m.src) + row * m.src_pitch + col;
+      float f[8], a[4], b[4];
+      widen_word<float, 4>(load_once<float, 4>(from), a);
+      widen_word<float, 4>(load_once<float, 4>(from + 4), b);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        f[k] = a[k];
+        f[4 + k] = b[k];
+      }
+      store_word<T, 8>(to, f);
+    } else {
+      *reinterpret_cast<uint4 *>(to) = *reinterpret_cast<const uint4 *>(static_cast<const T *>(m.src) + row * m.src_pitch + col);
+    }
   }
 }
 
@@ -259,9 +303,12 @@ cudaError_t launch_copy_rows(int dtype, const RowCopy *c, int count, cudaStream_
   long long most = 0;
   for (int i = 0; i < count; ++i) {
     m.of[i] = c[i];
-    most = c[i].rows * c[i].cols > most ? c[i].rows * c[i].cols : most;
+    m.words[i] = c[i].cols % 8 == 0 && c[i].src_pitch % (c[i].wide ? 4 : 8) == 0 && c[i].dst_pitch % 8 == 0 && on_grid(c[i].src, 16) &&
+                 on_grid(c[i].dst, 16);
+    const long long n = c[i].rows * c[i].cols / (m.words[i] ? 8 : 1);
+    most = n > most ? n : most;
   }
-  const long long ctas = (most + 1023) / 1024, wave = 8LL * sm_count();
+  const long long ctas = (most + 511) / 512, wave = 8LL * sm_count();
   const dim3 grid((unsigned)(ctas < wave ? ctas : wave), count);
   if (dtype == DFA3D_DTYPE_F16) copy_rows_kernel<__half><<<grid, 256, 0, s>>>(m);
   else copy_rows_kernel<__nv_bfloat16><<<grid, 256, 0, s>>>(m);

@@ -157,37 +157,37 @@ __global__ void __launch_bounds__(kThreads8, 1) weight_gradient_kernel(const __g
   }
 }
 
-// A CTA adds up the shares of 32 columns of a tile, turns them around in shared memory and writes rows of the result.
+// A CTA adds up the shares of eight columns of a tile (a thread four rows of one), turns them around in shared memory and writes rows
+// of the result.  Few columns, so that even one tile has many CTAs: the shares are read one after the other, and what there is to
+// read is little (20 MB at most) but far away.
+constexpr int kSumColumns = 8;
 template <typename T, int BN> __global__ void __launch_bounds__(256) weight_gradient_sum_kernel(const __grid_constant__ Problems w) {
-  __shared__ float turned[32][kTileP + 1];
-  const int tile = blockIdx.x / (BN / 32), c0 = blockIdx.x % (BN / 32) * 32;
+  __shared__ float turned[kSumColumns][kTileP + 1];
+  const int tile = blockIdx.x / (BN / kSumColumns), c0 = blockIdx.x % (BN / kSumColumns) * kSumColumns;
   const Problem &pr = w.of[problem_of(w, tile)];
   const int p0 = (tile - pr.first) / pr.tiles_q * kTileP, q0 = (tile - pr.first) % pr.tiles_q * BN + c0;
   if (q0 >= pr.q) return;
   const long long step = (long long)w.tiles * Grad<BN>::columns * kTileP;
   const float *src = w.partial + (long long)tile * Grad<BN>::columns * kTileP;
-#pragma unroll
-  for (int k = 0; k < 4; ++k) {
-    const int at = (k * 256 + threadIdx.x) * 4;      // of 32 x 128
-    float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-    for (int s = 0; s < w.shares; ++s) {
-      const float4 v = *reinterpret_cast<const float4 *>(src + s * step + c0 * kTileP + at);
-      sum.x += v.x; sum.y += v.y; sum.z += v.z; sum.w += v.w;
-    }
-    float *to = &turned[at / kTileP][at % kTileP];
-    to[0] = sum.x; to[1] = sum.y; to[2] = sum.z; to[3] = sum.w;
+  const int at = threadIdx.x * 4;      // of 8 x 128
+  float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 8
+  for (int s = 0; s < w.shares; ++s) {
+    const float4 v = __ldcs(reinterpret_cast<const float4 *>(src + s * step + c0 * kTileP + at));
+    sum.x += v.x; sum.y += v.y; sum.z += v.z; sum.w += v.w;
   }
+  float *to = &turned[at / kTileP][at % kTileP];
+  to[0] = sum.x; to[1] = sum.y; to[2] = sum.z; to[3] = sum.w;
   if (pr.bias && q0 == 0 && threadIdx.x < kTileP && p0 + threadIdx.x < pr.p) {
-    float sum = 0.f;
-    for (int s = 0; s < w.shares; ++s) sum += src[s * step + BN * kTileP + threadIdx.x];
-    static_cast<T *>(pr.bias)[p0 + threadIdx.x] = narrow<T>(sum);
+    float total = 0.f;
+#pragma unroll 8
+    for (int s = 0; s < w.shares; ++s) total += src[s * step + BN * kTileP + threadIdx.x];
+    static_cast<T *>(pr.bias)[p0 + threadIdx.x] = narrow<T>(total);
   }
   __syncthreads();
-  const int lane = threadIdx.x & 31;
-  for (int r = threadIdx.x >> 5; r < kTileP; r += 8)
-    if (p0 + r < pr.p && q0 + lane < pr.q)
-      static_cast<T *>(pr.out)[(long long)(p0 + r) * pr.q + q0 + lane] = narrow<T>(turned[lane][r]);
+  const int c = threadIdx.x % kSumColumns;
+  for (int r = threadIdx.x / kSumColumns; r < kTileP; r += 256 / kSumColumns)
+    if (p0 + r < pr.p && q0 + c < pr.q) static_cast<T *>(pr.out)[(long long)(p0 + r) * pr.q + q0 + c] = narrow<T>(turned[c][r]);
 }
 
 int width_for(const WeightProblem *w, int count) {
@@ -231,7 +231,7 @@ cudaError_t launch_shares(int dtype, long long rows, const WeightProblem *w, int
   cudaError_t rc = allow_shared<kernel>(L::bytes);
   if (rc != cudaSuccess) return rc;
   kernel<<<q.tiles * q.shares, kThreads8, L::bytes, s>>>(q);
-  weight_gradient_sum_kernel<T, BN><<<q.tiles * (BN / 32), 256, 0, s>>>(q);
+  weight_gradient_sum_kernel<T, BN><<<q.tiles * (BN / kSumColumns), 256, 0, s>>>(q);
   return cudaGetLastError();
 }
 

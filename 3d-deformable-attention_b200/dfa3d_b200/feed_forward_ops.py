@@ -133,6 +133,7 @@ def _weight_gradients(dtype, rows, problems):
     return out
 
 
+@_lib.native_apply("linear_act")
 class LinearActFunction(Function):
     @staticmethod
     def forward(ctx, x, weight, bias, residual, activation, checkpoint):
@@ -195,6 +196,7 @@ class LinearActFunction(Function):
         return grad_x, grad_w, grad_b, (grad_y if ctx.has_residual and need[3] else None), None, None
 
 
+@_lib.native_apply("gated_feed_forward")
 class GatedFeedForwardFunction(Function):
     @staticmethod
     def forward(ctx, x, w_gate, w_up, w_down, b_gate, b_up, b_down, residual, plus_x, activation, checkpoint):
