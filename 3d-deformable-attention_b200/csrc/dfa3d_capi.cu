@@ -1021,10 +1021,10 @@ int dfa3d_linear_input_gradient(const void *grad, const void *grad2, int64_t gra
                                 int64_t weight_pitch, const void *add, int64_t add_pitch, int32_t dtype, int64_t rows, int32_t in,
                                 int32_t out, void *grad_x, void *stream) {
   if (int rc = check_product(dtype, rows, {in, out}, DFA3D_ROW_NONE)) return rc;
+  if (int rc = check_elements(dtype, {grad_x})) return rc;
+  if (rows == 0) return DFA3D_OK;      // an empty matrix may have no address
   if ((grad2 == nullptr) != (weight2 == nullptr))
     return fail(DFA3D_ERR_INVALID_ARGUMENT, "grad2 and weight2 must be given together or not at all");
-  if (int rc = check_elements(dtype, {grad_x})) return rc;
-  if (rows == 0) return DFA3D_OK;
   REQUIRE_OPERAND(grad, grad_pitch, out);
   REQUIRE_OPERAND(weight, weight_pitch, in);
   if (grad2) {

@@ -8,7 +8,7 @@ operators raise.
 from . import _lib, ext  # noqa: F401
 from .dropout_ops import CounterDropout, draw_seed, dropout, dropout_add_layer_norm  # noqa: F401
 from .checkpoint_ops import compress8, decompress8  # noqa: F401
-from .feed_forward_ops import gated_feed_forward, linear_act  # noqa: F401
+from .feed_forward_ops import GatedFeedForward, LinearAct, gated_feed_forward, linear_act  # noqa: F401
 from .group_norm_ops import LevelGroupNorm, group_norm  # noqa: F401
 from .host import HostPipeline  # noqa: F401
 from .functions import (  # noqa: F401
@@ -31,7 +31,7 @@ from .functions import (  # noqa: F401
 __all__ = [
     "ext", "HostPipeline",
     "CounterDropout", "draw_seed", "dropout", "dropout_add_layer_norm", "LevelGroupNorm", "group_norm",
-    "compress8", "decompress8", "linear_act", "gated_feed_forward",
+    "compress8", "decompress8", "linear_act", "gated_feed_forward", "LinearAct", "GatedFeedForward",
     "MultiScaleDepthScoreSampleFunction", "WeightedMultiScaleDeformableAttnFunction",
     "MultiScale3DDeformableAttnFunction",
     "MultiScaleDepthScoreSampleFunction_fp32", "WeightedMultiScaleDeformableAttnFunction_fp32",

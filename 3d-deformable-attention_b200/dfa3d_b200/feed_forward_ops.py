@@ -24,7 +24,8 @@ from torch.autograd.function import Function, once_differentiable
 
 from . import _lib
 from .checkpoint_ops import Compressed8, check_format, compress8, into
-from .dropout_ops import keep, kept
+from .dropout_ops import CounterDropout, keep, kept
+from .layer_ops import runs_forward_only
 
 _DTYPES = {torch.bfloat16: _lib.DTYPE_BF16, torch.float16: _lib.DTYPE_F16}
 _ACTS = {None: _lib.ROW_NONE, "relu": _lib.ROW_RELU, "silu": _lib.ROW_SILU, "gelu": _lib.ROW_GELU}
@@ -41,6 +42,12 @@ def _ptr(t):
 def _check_matrix(t, name, shape, like):
     if t.dtype != like.dtype or t.device != like.device or tuple(t.shape) != shape:
         raise RuntimeError(f"{name} must be {shape} {like.dtype} on {like.device}, got {tuple(t.shape)} {t.dtype} on {t.device}")
+
+
+def _rows_of(t, name):
+    if t.dim() != 2 or t.shape[0] == 0:
+        raise RuntimeError(f"{name} must have two dimensions and at least one row, got {tuple(t.shape)}")
+    return t.shape[0]
 
 
 def _check_input(x, activation, checkpoint):
@@ -139,7 +146,7 @@ class LinearActFunction(Function):
     def forward(ctx, x, weight, bias, residual, activation, checkpoint):
         """act(x W^T + b) + residual."""
         _check_input(x, activation, checkpoint)
-        K, N = x.shape[-1], weight.shape[0]
+        K, N = x.shape[-1], _rows_of(weight, "weight")
         _check_matrix(weight, "weight", (N, K), x)
         if bias is not None:
             _check_matrix(bias, "bias", (N,), x)
@@ -202,7 +209,7 @@ class GatedFeedForwardFunction(Function):
     def forward(ctx, x, w_gate, w_up, w_down, b_gate, b_up, b_down, residual, plus_x, activation, checkpoint):
         """(act(x Wg^T + bg) * (x Wu^T + bu)) Wd^T + bd [+ residual, or + x]."""
         _check_input(x, activation, checkpoint)
-        E, F, N = x.shape[-1], w_gate.shape[0], w_down.shape[0]
+        E, F, N = x.shape[-1], _rows_of(w_gate, "w_gate"), _rows_of(w_down, "w_down")
         _check_matrix(w_gate, "w_gate", (F, E), x)
         _check_matrix(w_up, "w_up", (F, E), x)
         _check_matrix(w_down, "w_down", (N, F), x)
@@ -289,3 +296,61 @@ def gated_feed_forward(x, w_gate, w_up, w_down, b_gate=None, b_up=None, b_down=N
     plus_x = plus_x and x2 is x
     return GatedFeedForwardFunction.apply(x2, w_gate, w_up, w_down, b_gate, b_up, b_down, None if plus_x else residual, plus_x,
                                           activation, checkpoint)
+
+
+class _Computed(nn.Module):
+    """float32 parameters, computed with in 16 bits: x's type where it has one, autocast's under autocast, compute_dtype otherwise."""
+
+    compute_dtype = torch.bfloat16
+
+    def _type(self, x):
+        if torch.is_autocast_enabled("cuda"):
+            return torch.get_autocast_dtype("cuda")
+        return x.dtype if x.dtype in _DTYPES else self.compute_dtype
+
+
+def _to(t, dtype):
+    return None if t is None else t.to(dtype)
+
+
+class LinearAct(nn.Linear, _Computed):
+    """``torch.nn.Linear`` (same parameters and state-dict keys), an activation and a residual on ``linear_act``."""
+
+    def __init__(self, in_features, out_features, bias=True, activation=None, checkpoint=None, compute_dtype=torch.bfloat16):
+        super().__init__(in_features, out_features, bias)
+        self.activation, self.checkpoint, self.compute_dtype = activation, checkpoint, compute_dtype
+
+    def forward(self, x, residual=None):
+        dt = self._type(x)
+        return linear_act(x.to(dt), self.weight.to(dt), _to(self.bias, dt), self.activation, residual, self.checkpoint)
+
+
+class GatedFeedForward(_Computed):
+    """``dropout((act(gate(x)) * up(x)) down) [+ residual]`` on ``gated_feed_forward``.  A float32 residual is added unrounded."""
+
+    def __init__(self, embed_dims, hidden_dims, activation="silu", bias=True, dropout=0.0, counter_dropout=False, checkpoint=None,
+                 compute_dtype=torch.bfloat16):
+        super().__init__()
+        self.gate = nn.Linear(embed_dims, hidden_dims, bias)
+        self.up = nn.Linear(embed_dims, hidden_dims, bias)
+        self.down = nn.Linear(hidden_dims, embed_dims, bias)
+        self.dropout = CounterDropout(dropout) if counter_dropout else nn.Dropout(dropout)
+        self.activation, self.checkpoint, self.compute_dtype = activation, checkpoint, compute_dtype
+
+    def drops(self):
+        """Whether the dropout does anything, so that the residual has to wait for it."""
+        return not runs_forward_only(self.dropout) or (self.dropout.training and self.dropout.p > 0)
+
+    def branch(self, x, residual=None):
+        """The block without its dropout."""
+        dt = self._type(x)
+        narrow = x.to(dt)
+        w = [t for m in (self.gate, self.up, self.down) for t in (m.weight.to(dt), _to(m.bias, dt))]
+        return gated_feed_forward(narrow, w[0], w[2], w[4], w[1], w[3], w[5], self.activation,
+                                  narrow if residual is x and narrow is x else residual, self.checkpoint)
+
+    def forward(self, x, residual=None):
+        if not self.drops():
+            return self.branch(x, residual)
+        y = self.dropout(self.branch(x))
+        return y if residual is None else residual + y

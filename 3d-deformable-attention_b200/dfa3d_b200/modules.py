@@ -24,6 +24,8 @@ The layers' norms are ``layer_ops.AddLayerNorm`` (torch LayerNorm parameters; th
 inside the norm kernel) and the projections ``layer_ops.Linear`` (bias gradient by a column-sum kernel).
 ``counter_dropout=True`` builds the layers with ``CounterDropout`` instead of ``torch.nn.Dropout`` (no stored masks; another
 sequence of them for one torch seed), which the layers then run inside the norm and the feed-forward kernels.
+``gated_feed_forward=True`` (or a dict of ``GatedFeedForward``'s arguments, ``dict(activation="gelu", checkpoint="int8")``) builds the
+layers with the gated block in 16 bits instead of the reference's; its residual stays float32 and is added inside the last product.
 """
 import math
 
@@ -37,6 +39,7 @@ from .functions import (MultiScaleDeformableAttnFunction_fp32,
                         MultiScale3DDeformableAttnRaggedFunction_fp32)
 from . import _lib
 from .dropout_ops import CounterDropout
+from .feed_forward_ops import GatedFeedForward
 from .layer_ops import (AddLayerNorm, Linear, PassSeed, dropout_norm, dropout_sum, joint_linear, linear_relu,
                         linear_relu_dropout, runs_forward_only)
 from .rebatch import (CombineCamerasFunction, GatherQueriesFunction, GatherSharedRowsFunction, RebatchPlan,
@@ -451,7 +454,11 @@ def _run_ffn(ffn, x):
 
 def _ffn_norm(ffn, norm, x, seed):
     """``norm(ffn(x), x)``; where the block is the layers' own with CounterDropouts, the first dropout is run with the first
-    product and the second one inside the norm."""
+    product and the second one inside the norm.  The gated block adds x itself, or leaves it to the norm where a dropout comes first."""
+    if type(ffn) is GatedFeedForward and runs_forward_only(ffn):
+        if not ffn.drops():
+            return norm(ffn.branch(x, x))
+        return dropout_norm(ffn.branch(x).to(x.dtype), x, ffn.dropout, norm, seed, 3)
     if type(ffn) is not nn.Sequential or len(ffn) != 5 or not runs_forward_only(ffn) or type(ffn[2]) is not CounterDropout \
             or type(ffn[4]) is not CounterDropout:
         return norm(_run_ffn(ffn, x), x)
@@ -468,7 +475,10 @@ def _attention_norm(attention, norm, own, seed, site, query, **kw):
     return norm(*attention(query, return_residual=True, **kw))
 
 
-def _ffn(embed_dims, ffn_dims, dropout, counter_dropout):
+def _ffn(embed_dims, ffn_dims, dropout, counter_dropout, gated=False):
+    if gated or isinstance(gated, dict):
+        return GatedFeedForward(embed_dims, ffn_dims, dropout=dropout, counter_dropout=counter_dropout,
+                                **(gated if isinstance(gated, dict) else {}))
     return nn.Sequential(Linear(embed_dims, ffn_dims), nn.ReLU(inplace=True), _dropout_module(dropout, counter_dropout),
                          Linear(ffn_dims, embed_dims), _dropout_module(dropout, counter_dropout))
 
@@ -478,13 +488,13 @@ class SCAEncoderLayer(nn.Module):
     temporal self-attention, which uses a different, 2-D operator)."""
 
     def __init__(self, embed_dims=256, ffn_dims=512, num_cams=6, num_heads=8, num_levels=4, num_points=8,
-                 dropout=0.1, counter_dropout=False):
+                 dropout=0.1, counter_dropout=False, gated_feed_forward=False):
         super().__init__()
         self.cross_attn = SpatialCrossAttention_DFA3D(
             embed_dims, num_cams, dropout,
             MSDeformableAttention3D_DFA3D(embed_dims, num_heads, num_levels, num_points), counter_dropout=counter_dropout)
         self.norm1 = AddLayerNorm(embed_dims)
-        self.ffn = _ffn(embed_dims, ffn_dims, dropout, counter_dropout)
+        self.ffn = _ffn(embed_dims, ffn_dims, dropout, counter_dropout, gated_feed_forward)
         self.norm2 = AddLayerNorm(embed_dims)
 
     def forward(self, query, **kw):
@@ -583,7 +593,7 @@ class BEVFormerEncoderLayer(nn.Module):
     by encoder.py:363-411; post-norm, so every block adds its own input as the residual)."""
 
     def __init__(self, embed_dims=256, ffn_dims=512, num_cams=6, num_heads=8, num_levels=4, num_points=8,
-                 bev_h=200, bev_w=200, dropout=0.1, counter_dropout=False):
+                 bev_h=200, bev_w=200, dropout=0.1, counter_dropout=False, gated_feed_forward=False):
         super().__init__()
         self.bev_h, self.bev_w = bev_h, bev_w
         self._tables = {}
@@ -595,7 +605,7 @@ class BEVFormerEncoderLayer(nn.Module):
             MSDeformableAttention3D_DFA3D(embed_dims, num_heads, num_levels, num_points), bev_h=bev_h,
             bev_w=bev_w, num_head=num_heads, counter_dropout=counter_dropout)
         self.norm1 = AddLayerNorm(embed_dims)
-        self.ffn = _ffn(embed_dims, ffn_dims, dropout, counter_dropout)
+        self.ffn = _ffn(embed_dims, ffn_dims, dropout, counter_dropout, gated_feed_forward)
         self.norm2 = AddLayerNorm(embed_dims)
 
     def _bev_tables(self, device, dtype):
