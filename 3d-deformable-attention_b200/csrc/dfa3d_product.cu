@@ -42,32 +42,34 @@ template <ProductKind KIND, typename I, typename O, int BN, bool RESIDENT> struc
   static constexpr int sums = KIND == kGatedGrad ? BN + BN / 2 : BN;             // accumulator columns
   static constexpr int depth = 512 / sums < 4 ? 512 / sums : 4;                  // accumulators
   static constexpr int memory = depth * sums <= 256 ? 256 : 512;
-  // Epilogue warps: sixteen where a tile is summed quickly; eight, and more operands on their way, where it takes longer; eight
-  // for the three results of kGatedGrad, which need 96 columns in registers and three slabs a warp.
-  static constexpr int groups = KIND == kGatedGrad || !RESIDENT ? 2 : 4, warps = 4 * groups, threads = (4 + warps) * 32;
+  // Epilogue warps: sixteen where a tile is summed quickly; eight, and more operands on their way, where it takes longer.  Two mates
+  // share the chunk of three results of kGatedGrad, whose slabs leave no room for sixteen.
+  static constexpr int groups = KIND == kGatedGrad || RESIDENT ? 4 : 2, warps = 4 * groups, threads = (4 + warps) * 32;
+  static constexpr int mates = KIND == kGatedGrad ? 2 : 1, takers = groups / mates;
   static constexpr bool apart = sizeof(I) != sizeof(O);                          // `in` has a slab of its own
   static constexpr int chunk = KIND == kGatedGrad ? 32 : 128 / (int)sizeof(I);   // columns that a warp takes at a time
   static constexpr int chunks = columns / chunk;
-  static constexpr int turns = chunks < groups ? groups / chunks : 1;            // a warp has a chunk of every so many tiles
+  static constexpr int part = chunk / mates;                                     // of a chunk, columns of a warp
+  static constexpr int turns = chunks < takers ? takers / chunks : 1;            // a warp has a chunk of every so many tiles
   static constexpr int sub = 16;                                                // columns in registers, twice
   static constexpr int in_bytes = chunk * (int)sizeof(I), row_bytes = chunk * (int)sizeof(O);
   static constexpr int slab = 32 * row_bytes, slab_in = apart ? 32 * in_bytes : 0;
-  static constexpr int slabs = warps * (outs * slab + slab_in);
-  static constexpr int bias = warps * chunk * (gated ? 2 : 1) * 4;
+  static constexpr int slabs = warps / mates * (outs * slab + slab_in);
+  static constexpr int bias = warps * part * (gated ? 2 : 1) * 4;
   static constexpr int b_rows = BN / 2, b_bytes = b_rows * kDepth * 2;           // of each CTA
   static constexpr int b_ones = KIND == kInputGrad ? b_rows : BN / 4;            // columns of an mn-major B (kGatedGrad: the second)
-  // About 2400 cycles pass from a product that frees a slot to the one that reads what was loaded into it, and a step of BN = 256 is
-  // summed in 512: the rings have to hold that much.
-  static constexpr int room = 227 * 1024 - 2048 - slabs - bias;
-  static constexpr int both = room / (kOperandA + b_bytes) < 8 ? room / (kOperandA + b_bytes) : 8;
-  static constexpr int slots_a = !RESIDENT ? both : KIND == kGatedGrad ? 8 : 4;
-  static constexpr int most_b = (room - slots_a * kOperandA) / b_bytes;
-  static constexpr int slots_b = most_b < 12 ? most_b : 12;
-  static constexpr int barriers = 2 * slots_a + 2 * slots_b + 2 * depth + warps + 1;
-  static constexpr int bytes = 1024 + slots_a * kOperandA + slots_b * b_bytes + slabs + bias + barriers * 8 + 16;
+  // Steps whose operands share a slot of the ring: waiting for a slot, giving it back and asking for the next cost the one thread that
+  // does each about 400 cycles, and a step of BN = 256 is summed in 512, of 128 in 256.  Without RESIDENT a slot holds A's too.
+  static constexpr int per = BN == 256 ? 1 : RESIDENT && BN == 64 ? 4 : 2;
+  static constexpr int in_slot_b = per * b_bytes, slot = in_slot_b + (RESIDENT ? 0 : per * kOperandA);
+  static constexpr int slots_a = !RESIDENT ? 0 : KIND == kGatedGrad ? 8 : 4;
+  static constexpr int room = 227 * 1024 - 512 - slots_a * kOperandA - slabs - bias;
+  static constexpr int slots = room / slot < 8 ? room / slot : 8;
+  static constexpr int barriers = 2 * slots_a + 2 * slots + 2 * depth + warps + 1;
+  static constexpr int bytes = slots_a * kOperandA + slots * slot + slabs + bias + barriers * 8 + 16;
   // whoever reads an accumulator reads it every time, or it would take one phase of its barrier for another
-  static_assert(depth % turns == 0 && (chunks <= groups ? groups % chunks : chunks % groups) == 0, "turns");
-  static_assert(bytes <= 227 * 1024 && slots_b >= 4 && (row_bytes == 64 || row_bytes == 128) && chunks >= 1, "layout");
+  static_assert(depth % turns == 0 && (chunks <= takers ? takers % chunks : chunks % takers) == 0 && part % sub == 0, "turns");
+  static_assert(bytes <= 227 * 1024 && slots >= 3 && (row_bytes == 64 || row_bytes == 128) && chunks >= 1, "layout");
 };
 
 // The 16-byte piece `piece` of row `row` of a slab as tiled copies lay it out.
@@ -198,12 +200,12 @@ template <ProductKind KIND, typename T, typename I, typename O, int BN, bool RES
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Tile<KIND, I, O, BN, RESIDENT>::threads, 1)
     product_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Extents p) {
   using L = Tile<KIND, I, O, BN, RESIDENT>;
-  extern __shared__ uint8_t raw[];
-  const uint32_t base_a = (tc::shared_address(raw) + 1023) & ~1023u, base_b = base_a + L::slots_a * kOperandA;
-  const uint32_t slabs = base_b + L::slots_b * L::b_bytes, bias_at = slabs + L::slabs;
+  extern __shared__ __align__(1024) uint8_t raw[];      // operand tiles and slabs begin on its grid
+  const uint32_t base_a = tc::shared_address(raw), ring = base_a + L::slots_a * kOperandA;
+  const uint32_t slabs = ring + L::slots * L::slot, bias_at = slabs + L::slabs;
   const uint32_t full_a = bias_at + L::bias, empty_a = full_a + L::slots_a * 8;
-  const uint32_t full_b = empty_a + L::slots_a * 8, empty_b = full_b + L::slots_b * 8;
-  const uint32_t summed = empty_b + L::slots_b * 8, drained = summed + L::depth * 8;
+  const uint32_t full = empty_a + L::slots_a * 8, empty = full + L::slots * 8;
+  const uint32_t summed = empty + L::slots * 8, drained = summed + L::depth * 8;
   const uint32_t in_there = drained + L::depth * 8, quiet = in_there + L::warps * 8, where = quiet + 8;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t rank = tc::rank_in_pair();
@@ -212,9 +214,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Tile<KIND, I, O, BN,
   const int first_tile = (int)((long long)p.tiles * pair / pairs), last_tile = (int)((long long)p.tiles * (pair + 1) / pairs);
 
   if (warp == 1) {
-    for (int i = lane; i < L::barriers; i += 32) {      // all of them lie side by side; only the drained ones have many arrivals
-      const int from = (int)(drained - full_a) / 8;
-      tc::barrier_init(full_a + i * 8, i >= from && i < from + L::depth ? 2 * 4 * L::chunks : 1);
+    for (int i = lane; i < L::barriers; i += 32) {      // all of them lie side by side
+      const uint32_t at = full_a + i * 8;
+      tc::barrier_init(at, at >= drained && at < in_there       ? 2 * 4 * L::chunks * L::mates
+                           : at >= full && at < empty && !RESIDENT ? 2
+                                                                   : 1);
     }
     tc::barriers_visible();
   }
@@ -232,21 +236,20 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Tile<KIND, I, O, BN,
   uint32_t memory;
   asm volatile("ld.shared.u32 %0, [%1];" : "=r"(memory) : "r"(where));
 
-  const int steps = p.steps0 + p.steps1, slots_a = RESIDENT ? steps : L::slots_a;
+  const int steps = p.steps0 + p.steps1;
   if (warp == 0 || warp == 3) {
     // ---- operand tiles: this CTA's, into its shared memory; the first CTA's barriers count those of both.  One warp for each
     // operand: a step of a narrow tile is summed as fast as one thread asks for its operands. ----
     if (tc::one_lane()) {
-      const bool is_a = warp == 3;
-      const uint32_t ring = is_a ? base_a : base_b, full = is_a ? full_a : full_b, empty = is_a ? empty_a : empty_b;
-      const uint32_t first_full = tc::address_in(full, 0), bytes = is_a ? kOperandA : L::b_bytes;
-      const int slots = is_a ? slots_a : L::slots_b;
+      const bool own = RESIDENT && warp == 3;                    // A's slots have barriers of their own
+      const uint32_t there = own ? full_a : full, gone = own ? empty_a : empty, first_there = tc::address_in(there, 0);
+      const int slots = own ? steps : L::slots;
       int slot = 0, asked = 0;      // asked: no more than it takes to go round once
       uint32_t phase = 0;
       bool ok = true;
-      auto take = [&] {             // the next slot, once it is free
-        ok = tc::wait(empty + slot * 8, phase ^ 1);
-        if (ok && rank == 0) tc::arrive_expect(full + slot * 8, 2 * bytes);
+      auto take = [&](uint32_t bytes) {      // the next slot, once it is free
+        ok = tc::wait(gone + slot * 8, phase ^ 1);
+        if (ok && rank == 0) tc::arrive_expect(there + slot * 8, 2 * bytes);
         return ok;
       };
       auto next = [&] {
@@ -259,42 +262,50 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Tile<KIND, I, O, BN,
       Place at_tile = first;
       for (int tile = first_tile; tile < last_tile && ok; ++tile, at_tile.on(1, p.tiles_n)) {
         const int m0 = (at_tile.m * 2 + (int)rank) * kRows, n0 = at_tile.column(p.tiles_n) * L::columns;
-        if (is_a) {
+        if (warp == 3) {
           const bool fresh = tile == first_tile || at_tile.n == 0, look = fresh && tile + p.tiles_n - at_tile.n < last_tile;
           if (RESIDENT && !fresh) continue;
-          for (int k = 0; k < steps; ++k, next()) {
-            const bool second = k >= p.steps0;
-            const CUtensorMap *map = second ? &maps.a1 : &maps.a0;
-            const int at = (second ? k - p.steps0 : k) * kDepth;
-            if (!take()) break;
-            tc::tile_load_pair(ring + slot * kOperandA, map, at, m0, first_full + slot * 8);
-            if (look) tc::tile_to_l2(map, at, m0 + 2 * kRows);
-          }
-        } else if constexpr (KIND == kInputGrad) {
-          constexpr int box = L::b_rows < 64 ? L::b_rows : 64;
-          for (int k = 0; k < steps; ++k, next()) {
-            const bool second = k >= p.steps0;
-            const CUtensorMap *map = second ? &maps.b1 : &maps.b0;
-            const int at = (second ? k - p.steps0 : k) * kDepth;
-            if (!take()) break;
-#pragma unroll
-            for (int i = 0; i < L::b_rows / box; ++i)
-              tc::tile_load_pair(ring + slot * L::b_bytes + i * kDepth * 128, map, n0 + (int)rank * L::b_rows + i * box, at,
-                                 first_full + slot * 8);
+          constexpr int PER = RESIDENT ? 1 : L::per;
+          for (int k = 0; k < steps; k += PER, next()) {
+            const int count = min(PER, steps - k);
+            if (!take(count * kOperandA)) break;
+            uint32_t to = RESIDENT ? base_a + slot * kOperandA : ring + slot * L::slot + L::in_slot_b;
+            for (int j = k; j < k + count; ++j, to += kOperandA) {
+              const bool second = j >= p.steps0;
+              const CUtensorMap *map = second ? &maps.a1 : &maps.a0;
+              const int at = (second ? j - p.steps0 : j) * kDepth;
+              tc::tile_load_pair(to, map, at, m0, first_there + slot * 8);
+              if (look) tc::tile_to_l2(map, at, m0 + 2 * kRows);
+            }
           }
         } else {
-          const CUtensorMap *map = L::gated && rank ? &maps.b1 : &maps.b0;
-          const int y = L::gated ? n0 : n0 + (int)rank * L::b_rows;
-          for (int k = 0; k < p.steps0; ++k, next()) {
-            if (!take()) break;
-            tc::tile_load_pair(ring + slot * L::b_bytes, map, k * kDepth, y, first_full + slot * 8);
+          const int first_steps = KIND == kGatedGrad ? p.steps0 : steps;
+          for (int k = 0; k < first_steps; k += L::per, next()) {
+            const int count = min(L::per, first_steps - k);
+            if (!take(count * L::b_bytes)) break;
+            uint32_t to = ring + slot * L::slot;
+            for (int j = k; j < k + count; ++j, to += L::b_bytes) {
+              if constexpr (KIND == kInputGrad) {
+                const bool second = j >= p.steps0;
+                const CUtensorMap *map = second ? &maps.b1 : &maps.b0;
+                const int at = (second ? j - p.steps0 : j) * kDepth;
+                constexpr int box = L::b_rows < 64 ? L::b_rows : 64;
+#pragma unroll
+                for (int i = 0; i < L::b_rows / box; ++i)
+                  tc::tile_load_pair(to + i * kDepth * 128, map, n0 + (int)rank * L::b_rows + i * box, at, first_there + slot * 8);
+              } else {
+                tc::tile_load_pair(to, L::gated && rank ? &maps.b1 : &maps.b0, j * kDepth, L::gated ? n0 : n0 + (int)rank * L::b_rows,
+                                   first_there + slot * 8);
+              }
+            }
           }
-          if constexpr (KIND == kGatedGrad) {      // half as wide: two steps fill a slot
-            for (int k = 0; k < p.steps1 && ok; k += 2, next()) {
-              if (!take()) break;
-              tc::tile_load_pair(ring + slot * L::b_bytes, &maps.b2, n0 + (int)rank * L::b_ones, k * kDepth, first_full + slot * 8);
-              tc::tile_load_pair(ring + slot * L::b_bytes + L::b_bytes / 2, &maps.b2, n0 + (int)rank * L::b_ones, (k + 1) * kDepth,
-                                 first_full + slot * 8);
+          if constexpr (KIND == kGatedGrad) {      // half as wide, twice as many steps in a slot
+            for (int k = 0; k < p.steps1 && ok; k += 2 * L::per, next()) {
+              const int count = min(2 * L::per, p.steps1 - k);
+              if (!take(count * (L::b_bytes / 2))) break;
+              uint32_t to = ring + slot * L::slot;
+              for (int j = k; j < k + count; ++j, to += L::b_bytes / 2)
+                tc::tile_load_pair(to, &maps.b2, n0 + (int)rank * L::b_ones, j * kDepth, first_there + slot * 8);
             }
           }
         }
@@ -306,7 +317,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Tile<KIND, I, O, BN,
             slot = slots - 1;
             phase ^= 1;
           }
-          tc::wait(full + slot * 8, phase);
+          tc::wait(there + slot * 8, phase);
         }
       }
       if (!ok) __nanosleep(1000000);
@@ -317,8 +328,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Tile<KIND, I, O, BN,
     if (rank == 0) {
       constexpr uint32_t shape = tc::product_shape<T>(2 * kRows, BN, false, KIND == kInputGrad);
       constexpr uint32_t shape_d = tc::product_shape<T>(2 * kRows, BN / 2, false, true);
-      int sa = 0, sb = 0, slot = 0;
-      uint32_t phase_a = 0, phase_b = 0, round = 0;
+      int at_ring = 0, slot = 0;
+      uint32_t phase_a = 0, phase = 0, round = 0;
       bool ok = true;
       Place at_tile = first;
       for (int tile = first_tile; tile < last_tile && ok; ++tile, at_tile.on(1, p.tiles_n)) {
@@ -326,40 +337,38 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Tile<KIND, I, O, BN,
         const bool fresh = tile == first_tile || at_tile.n == 0, last = tile + 1 == last_tile || at_tile.n + 1 == p.tiles_n;
         if (!(ok = tc::wait_warp(drained + slot * 8, round ^ 1))) break;
         tc::order_after();
-        // Steps of one of the two sums of a tile; everything that can be known before is, since a step of a narrow tile is issued
-        // no faster than it is summed.
         auto sum = [&](auto second, int from, int to, uint32_t d) {
           constexpr bool SECOND = decltype(second)::value;      // kGatedGrad: grad_y Wd
           constexpr uint32_t form = SECOND ? shape_d : shape;
-          for (int k = from; k < to; ++k) {
-            const int use = RESIDENT ? k : sa;
-            if (fresh || !RESIDENT) {
-              if (!(ok = tc::wait_warp(full_a + use * 8, phase_a))) return;
-              if (++sa == slots_a) {
-                sa = 0;
-                phase_a ^= 1;
-              }
-            }
-            const bool odd = SECOND && (k - from) % 2 != 0;      // the second half of a slot
-            if (!odd && !(ok = tc::wait_warp(full_b + sb * 8, phase_b))) return;
+          constexpr int PER = SECOND ? 2 * L::per : L::per, bytes_b = SECOND ? L::b_bytes / 2 : L::b_bytes;
+          constexpr bool mn = SECOND || KIND == kInputGrad, narrow_b = mn && L::b_ones < 64;
+          constexpr int step_b = (narrow_b ? 1024 : mn ? 2048 : 32) / 16;
+          for (int k = from; k < to; k += PER) {
+            const int count = min(PER, to - k);
+            if (RESIDENT && fresh)
+              for (int j = 0; j < count; ++j)
+                if (!(ok = tc::wait_warp(full_a + (k + j) * 8, phase_a))) return;
+            if (!(ok = tc::wait_warp(full + at_ring * 8, phase))) return;
             tc::order_after();
-            const uint64_t a = tc::k_major(base_a + use * kOperandA);
-            const uint32_t at_b = base_b + sb * L::b_bytes + (odd ? L::b_bytes / 2 : 0);
-            constexpr bool mn = SECOND || KIND == kInputGrad, narrow_b = mn && L::b_ones < 64;
+            const uint32_t at_b = ring + at_ring * L::slot, at_a = RESIDENT ? base_a + k * kOperandA : at_b + L::in_slot_b;
+            const uint64_t a = tc::k_major(at_a);
             const uint64_t b = narrow_b ? tc::mn_major_narrow(at_b) : mn ? tc::mn_major(at_b, kDepth * 128) : tc::k_major(at_b);
-            constexpr int step_b = (narrow_b ? 1024 : mn ? 2048 : 32) / 16;
-            const bool give_b = !SECOND || odd || k + 1 == to;
             if (tc::one_lane()) {
               tc::product<true>(d, a, b, form, k > from);
 #pragma unroll
-              for (int j = 1; j < kDepth / 16; ++j) tc::product<true>(d, a + j * 2, b + j * step_b, form, true);
-              if (last || !RESIDENT) tc::products_arrive<true>(empty_a + use * 8);
-              if (give_b) tc::products_arrive<true>(empty_b + sb * 8);
+              for (int j = 1; j < PER * (kDepth / 16); ++j) {
+                const int step = j / (kDepth / 16), part = j % (kDepth / 16);
+                if (step < count)
+                  tc::product<true>(d, a + step * (kOperandA / 16) + part * 2, b + step * (bytes_b / 16) + part * step_b, form, true);
+              }
+              if (RESIDENT && last)
+                for (int j = 0; j < count; ++j) tc::products_arrive<true>(empty_a + (k + j) * 8);
+              tc::products_arrive<true>(empty + at_ring * 8);
             }
             __syncwarp();
-            if (give_b && ++sb == L::slots_b) {
-              sb = 0;
-              phase_b ^= 1;
+            if (++at_ring == L::slots) {
+              at_ring = 0;
+              phase ^= 1;
             }
           }
         };
@@ -369,6 +378,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Tile<KIND, I, O, BN,
         } else {
           sum(std::false_type(), 0, steps, acc);
         }
+        if (last) phase_a ^= 1;
         if (ok && tc::one_lane()) tc::products_arrive<true>(summed + slot * 8);
         __syncwarp();
         if (++slot == L::depth) {
@@ -382,15 +392,19 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Tile<KIND, I, O, BN,
     tc::wait_warp(quiet, 0);
   } else if (warp >= 4) {
     // ---- epilogue: a warp has 32 rows; the groups of four warps take a tile's chunks of columns in turn ----
-    const int e = warp - 4, quarter = warp & 3, group = e >> 2;
-    const uint32_t slab_in = slabs + e * (L::outs * L::slab + L::slab_in), slab = slab_in + L::slab_in;
+    const int e = warp - 4, quarter = warp & 3, taker = (e >> 2) / L::mates, mate = (e >> 2) % L::mates;
+    const uint32_t slab_in = slabs + (taker * 4 + quarter) * (L::outs * L::slab + L::slab_in), slab = slab_in + L::slab_in;
+    auto meet = [&] {      // with the mate
+      if constexpr (L::mates == 1) __syncwarp();
+      else asm volatile("bar.sync %0, %1;" ::"r"(1 + taker * 4 + quarter), "n"(32 * L::mates) : "memory");
+    };
     const uint32_t bias = bias_at + e * (L::bias / L::warps), there = in_there + e * 8, first_drained = tc::address_in(drained, 0);
     const bool loads = p.has_in && !p.direct;
     const T *bias0 = static_cast<const T *>(p.bias0), *bias1 = static_cast<const T *>(p.bias1);
     uint32_t in_phase = 0;
     bool ok = true;
 
-    // Chunk number c of this pair: tile first_tile + c / chunks; this warp has c = group, group + groups, ...
+    // Chunk number c of this pair: tile first_tile + c / chunks; this warp has c = taker, taker + takers, ...
     const int all = (last_tile - first_tile) * L::chunks;
     struct Chunk {
       int c, row, column;
@@ -401,13 +415,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Tile<KIND, I, O, BN,
       h.column = h.place.column(p.tiles_n) * L::columns + h.c % L::chunks * L::chunk;
     };
     auto go_on = [&](Chunk &h) {
-      h.place.on((h.c + L::groups) / L::chunks - h.c / L::chunks, p.tiles_n);
-      h.c += L::groups;
+      h.place.on((h.c + L::takers) / L::chunks - h.c / L::chunks, p.tiles_n);
+      h.c += L::takers;
       locate(h);
     };
     auto inside = [&](const Chunk &h) { return h.row < p.rows && h.column < p.n; };
-    Chunk now{group, 0, 0, first};
-    now.place.on(group / L::chunks, p.tiles_n);
+    Chunk now{taker, 0, 0, first};
+    now.place.on(taker / L::chunks, p.tiles_n);
     locate(now);
     Chunk then = now;            // of what is added to a chunk or multiplied by it, the one to ask for next
     auto ask = [&] {
@@ -420,31 +434,34 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Tile<KIND, I, O, BN,
     };
     if (loads && lane == 0) ask();
     // biases of the next chunk are on their way while this one is worked on
-    constexpr int ahead = L::chunk / 32;
+    constexpr int ahead = (L::part + 31) / 32;
     float next0[ahead], next1[ahead];
-    auto ask_bias = [&](int c, int col) {
+    auto ask_bias = [&] {
 #pragma unroll
       for (int i = 0; i < ahead; ++i) {
-        const bool in = c < all && col + i * 32 + lane < p.n;
-        next0[i] = in && bias0 ? wide(bias0[col + i * 32 + lane]) : 0.f;
-        if constexpr (L::gated) next1[i] = in && bias1 ? wide(bias1[col + i * 32 + lane]) : 0.f;
+        const int k = i * 32 + lane, col = now.column + mate * L::part + k;
+        const bool in = now.c < all && k < L::part && col < p.n;
+        next0[i] = in && bias0 ? wide(bias0[col]) : 0.f;
+        if constexpr (L::gated) next1[i] = in && bias1 ? wide(bias1[col]) : 0.f;
       }
     };
-    if constexpr (KIND != kInputGrad) ask_bias(now.c, now.column);
+    if constexpr (KIND != kInputGrad) ask_bias();
 
     while (now.c < all) {
       const int it = now.c / L::chunks, slot = it % L::depth, m0 = now.row, col = now.column;
-      const uint32_t acc = memory + ((uint32_t)quarter << 21) + slot * L::sums + now.c % L::chunks * L::chunk;
+      const uint32_t acc = memory + ((uint32_t)quarter << 21) + slot * L::sums + now.c % L::chunks * L::chunk + mate * L::part;
       const bool some = inside(now);
       const int rows_in = min(32, p.rows - m0), cols_in = min(L::chunk, p.n - col);
       if constexpr (KIND != kInputGrad) {
 #pragma unroll
         for (int i = 0; i < ahead; ++i) {
-          tc::write_one<float>(bias + (i * 32 + lane) * 4, next0[i]);
-          if constexpr (L::gated) tc::write_one<float>(bias + (L::chunk + i * 32 + lane) * 4, next1[i]);
+          const int k = i * 32 + lane;
+          if (k >= L::part) continue;
+          tc::write_one<float>(bias + k * 4, next0[i]);
+          if constexpr (L::gated) tc::write_one<float>(bias + (L::part + k) * 4, next1[i]);
         }
         go_on(now);
-        ask_bias(now.c, now.column);
+        ask_bias();
       } else {
         go_on(now);
       }
@@ -454,10 +471,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Tile<KIND, I, O, BN,
           __syncwarp();
           copy_direct<I, L::in_bytes, false>(static_cast<const I *>(p.in) + m0 * p.in_pitch + col, p.in_pitch, rows_in, cols_in, slab_in,
                                              lane);
-        } else if ((!loads || L::apart) && lane == 0) {
+        } else if ((!loads || L::apart) && lane == 0 && mate == 0) {
           tc::stores_read<0>();
         }
-        __syncwarp();
+        meet();
       }
       if (ok) ok = __all_sync(0xffffffffu, tc::wait(summed + slot * 8, (uint32_t)(it / L::depth) & 1));
       tc::order_after();
@@ -467,7 +484,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Tile<KIND, I, O, BN,
           in_phase ^= 1;
         }
         // columns of the accumulators, the next ones on their way while these are worked on
-        constexpr int sums = KIND == kGatedGrad ? 3 : L::gated ? 2 : 1, turns = L::chunk / L::sub;
+        constexpr int sums = KIND == kGatedGrad ? 3 : L::gated ? 2 : 1, turns = L::part / L::sub;
         float v[2][sums][L::sub];
         auto fetch = [&](int t) {
 #pragma unroll
@@ -476,13 +493,19 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Tile<KIND, I, O, BN,
         fetch(0);
 #pragma unroll
         for (int t = 0; t < turns; ++t) {
-          const int off = t * L::sub, first = off * (int)sizeof(O) / 16;
+          const int off = t * L::sub, first = (mate * L::part + off) * (int)sizeof(O) / 16;
           float(&z)[L::sub] = v[t & 1][0];
 #pragma unroll
           for (int i = 0; i < sums; ++i) tc::tensor_loads_done(v[t & 1][i]);
-          if (t + 1 < turns) fetch(t + 1);
+          if (t + 1 < turns) {
+            fetch(t + 1);
+          } else {      // the accumulator may be summed into again
+            tc::order_before();
+            __syncwarp();
+            if (lane == 0) tc::arrive_in(first_drained + slot * 8);
+          }
           if constexpr (KIND != kInputGrad) add_bias(z, bias + off * 4);
-          if constexpr (L::gated) add_bias(v[t & 1][1], bias + (L::chunk + off) * 4);
+          if constexpr (L::gated) add_bias(v[t & 1][1], bias + (L::part + off) * 4);
           if constexpr (KIND == kGatedGrad) {
             float(&u)[L::sub] = v[t & 1][1], (&d)[L::sub] = v[t & 1][2];
             gate_all(z, u, d, p.act);
@@ -502,14 +525,16 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Tile<KIND, I, O, BN,
           put<O, L::row_bytes>(z, slab, lane, first);
         }
       }
-      tc::order_before();
+      if (!some) {
+        __syncwarp();
+        if (lane == 0) tc::arrive_in(first_drained + slot * 8);
+        continue;
+      }
       if (!p.direct) tc::shared_to_async();
-      __syncwarp();
-      if (lane == 0) tc::arrive_in(first_drained + slot * 8);
-      if (!some) continue;
+      meet();
       if (p.direct) {
         copy_direct<O, L::row_bytes, true>(static_cast<O *>(p.out) + m0 * p.out_pitch + col, p.out_pitch, rows_in, cols_in, slab, lane);
-      } else if (lane == 0) {
+      } else if (lane == 0 && mate == 0) {
 #pragma unroll
         for (int o = 0; o < L::outs; ++o) tc::tile_store(&maps.out[o], col, m0, slab + o * L::slab);
         tc::stores_asked();
