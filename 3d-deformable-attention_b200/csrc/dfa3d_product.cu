@@ -61,6 +61,7 @@ template <ProductKind KIND, typename I, typename O, int BN, bool RESIDENT> struc
   // Steps whose operands share a slot of the ring: waiting for a slot, giving it back and asking for the next cost the one thread that
   // does each about 400 cycles, and a step of BN = 256 is summed in 512, of 128 in 256.  Without RESIDENT a slot holds A's too.
   static constexpr int per = BN == 256 ? 1 : RESIDENT && BN == 64 ? 4 : 2;
+  static constexpr int per_second = RESIDENT ? 2 * per : per;                    // of the second sum of kGatedGrad, half as wide
   static constexpr int in_slot_b = per * b_bytes, slot = in_slot_b + (RESIDENT ? 0 : per * kOperandA);
   static constexpr int slots_a = !RESIDENT ? 0 : KIND == kGatedGrad ? 8 : 4;
   static constexpr int room = 227 * 1024 - 512 - slots_a * kOperandA - slabs - bias;
@@ -224,6 +225,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Tile<KIND, I, O, BN,
   }
   if (warp == 2) tc::tensor_memory_take<L::memory, true>(where);
   const Place first(first_tile, p.tiles_n);
+  tc::let_next_kernel_begin();
+  tc::wait_for_last_kernel();
   if (warp == 0) {      // the first rows and columns come from far away: they are asked for while the CTAs find together
     const int m0 = (first.m * 2 + (int)rank) * kRows;
     if (lane < p.steps0 && lane < 8) tc::tile_to_l2(&maps.a0, lane * kDepth, m0);
@@ -266,8 +269,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Tile<KIND, I, O, BN,
           const bool fresh = tile == first_tile || at_tile.n == 0, look = fresh && tile + p.tiles_n - at_tile.n < last_tile;
           if (RESIDENT && !fresh) continue;
           constexpr int PER = RESIDENT ? 1 : L::per;
-          for (int k = 0; k < steps; k += PER, next()) {
-            const int count = min(PER, steps - k);
+          // the two sums of kGatedGrad share no slot
+          for (int k = 0, count; k < steps; k += count, next()) {
+            count = min(PER, (KIND == kGatedGrad && k < p.steps0 ? p.steps0 : steps) - k);
             if (!take(count * kOperandA)) break;
             uint32_t to = RESIDENT ? base_a + slot * kOperandA : ring + slot * L::slot + L::in_slot_b;
             for (int j = k; j < k + count; ++j, to += kOperandA) {
@@ -299,9 +303,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Tile<KIND, I, O, BN,
               }
             }
           }
-          if constexpr (KIND == kGatedGrad) {      // half as wide, twice as many steps in a slot
-            for (int k = 0; k < p.steps1 && ok; k += 2 * L::per, next()) {
-              const int count = min(2 * L::per, p.steps1 - k);
+          if constexpr (KIND == kGatedGrad) {
+            for (int k = 0; k < p.steps1 && ok; k += L::per_second, next()) {
+              const int count = min(L::per_second, p.steps1 - k);
               if (!take(count * (L::b_bytes / 2))) break;
               uint32_t to = ring + slot * L::slot;
               for (int j = k; j < k + count; ++j, to += L::b_bytes / 2)
@@ -340,7 +344,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Tile<KIND, I, O, BN,
         auto sum = [&](auto second, int from, int to, uint32_t d) {
           constexpr bool SECOND = decltype(second)::value;      // kGatedGrad: grad_y Wd
           constexpr uint32_t form = SECOND ? shape_d : shape;
-          constexpr int PER = SECOND ? 2 * L::per : L::per, bytes_b = SECOND ? L::b_bytes / 2 : L::b_bytes;
+          constexpr int PER = SECOND ? L::per_second : L::per, bytes_b = SECOND ? L::b_bytes / 2 : L::b_bytes;
           constexpr bool mn = SECOND || KIND == kInputGrad, narrow_b = mn && L::b_ones < 64;
           constexpr int step_b = (narrow_b ? 1024 : mn ? 2048 : 32) / 16;
           for (int k = from; k < to; k += PER) {
@@ -601,8 +605,7 @@ cudaError_t launch_as(const ProductArgs &a, cudaStream_t s) {
   cudaError_t rc = allow_shared<kernel>(L::bytes);
   if (rc != cudaSuccess) return rc;
   const int pairs = sm_count() / 2, grid = 2 * (p.tiles < pairs ? p.tiles : pairs);
-  kernel<<<grid, L::threads, L::bytes, s>>>(m, p);
-  return cudaGetLastError();
+  return launch_after(kernel, grid, L::threads, L::bytes, s, m, p);
 }
 
 template <ProductKind KIND, typename T, typename I, typename O, int BN> cudaError_t launch_tiles(const ProductArgs &a, cudaStream_t s) {

@@ -81,6 +81,11 @@ __device__ __forceinline__ void pair_sync() {      // all threads of both
   asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
+// ---- kernels that follow one another -------------------------------------------------------------
+// A kernel launched by launch_after() may begin while the one before it in the stream ends; it reads and writes nothing before this.
+__device__ __forceinline__ void wait_for_last_kernel() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void let_next_kernel_begin() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+
 // ---- tiled copies ------------------------------------------------------------------------------
 __device__ __forceinline__ void fetch_map(const CUtensorMap *map) {
   asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory");

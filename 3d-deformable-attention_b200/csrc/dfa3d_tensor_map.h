@@ -61,4 +61,20 @@ template <auto KERNEL> cudaError_t allow_shared(int bytes) {
   return rc;
 }
 
+// A launch whose CTAs may be set up while the last ones of the kernel before it in the stream end.
+template <typename... P, typename... A>
+cudaError_t launch_after(void (*kernel)(P...), int grid, int threads, int shared, cudaStream_t s, const A &...args) {
+  cudaLaunchConfig_t c{};
+  c.gridDim = dim3(grid);
+  c.blockDim = dim3(threads);
+  c.dynamicSmemBytes = shared;
+  c.stream = s;
+  cudaLaunchAttribute early;
+  early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  early.val.programmaticStreamSerializationAllowed = 1;
+  c.attrs = &early;
+  c.numAttrs = 1;
+  return cudaLaunchKernelEx(&c, kernel, args...);
+}
+
 }  // namespace dfa3d

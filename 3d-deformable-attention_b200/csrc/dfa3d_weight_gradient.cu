@@ -69,6 +69,8 @@ __global__ void __launch_bounds__(kThreads8, 1) weight_gradient_kernel(const __g
     for (int i = threadIdx.x - 128; i < L::ones / 16; i += 256) tc::write16(ones + i * 16, make_uint4(two, two, two, two));
     tc::shared_to_async();
   }
+  tc::let_next_kernel_begin();
+  tc::wait_for_last_kernel();
   tc::order_before();
   __syncthreads();
   tc::order_after();
@@ -163,6 +165,8 @@ __global__ void __launch_bounds__(kThreads8, 1) weight_gradient_kernel(const __g
 constexpr int kSumColumns = 8;
 template <typename T, int BN> __global__ void __launch_bounds__(256) weight_gradient_sum_kernel(const __grid_constant__ Problems w) {
   __shared__ float turned[kSumColumns][kTileP + 1];
+  tc::let_next_kernel_begin();
+  tc::wait_for_last_kernel();
   const int tile = blockIdx.x / (BN / kSumColumns), c0 = blockIdx.x % (BN / kSumColumns) * kSumColumns;
   const Problem &pr = w.of[problem_of(w, tile)];
   const int p0 = (tile - pr.first) / pr.tiles_q * kTileP, q0 = (tile - pr.first) % pr.tiles_q * BN + c0;
@@ -230,9 +234,9 @@ cudaError_t launch_shares(int dtype, long long rows, const WeightProblem *w, int
   constexpr auto kernel = &weight_gradient_kernel<T, BN>;
   cudaError_t rc = allow_shared<kernel>(L::bytes);
   if (rc != cudaSuccess) return rc;
-  kernel<<<q.tiles * q.shares, kThreads8, L::bytes, s>>>(q);
-  weight_gradient_sum_kernel<T, BN><<<q.tiles * (BN / kSumColumns), 256, 0, s>>>(q);
-  return cudaGetLastError();
+  rc = launch_after(kernel, q.tiles * q.shares, kThreads8, L::bytes, s, q);
+  if (rc != cudaSuccess) return rc;
+  return launch_after(&weight_gradient_sum_kernel<T, BN>, q.tiles * (BN / kSumColumns), 256, 0, s, q);
 }
 
 template <typename T>
