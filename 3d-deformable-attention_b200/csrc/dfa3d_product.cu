@@ -28,7 +28,7 @@ struct Maps {
 struct Extents {
   int rows, n, steps0, steps1;      // steps of kDepth
   int tiles, tiles_n;
-  int act, has_in, direct;          // direct: `in` and `out` do not lie as tiled copies need it
+  int act, has_in;
   const void *bias0, *bias1, *in;
   void *out;
   long long in_pitch, out_pitch;
@@ -167,18 +167,48 @@ __device__ __forceinline__ void combine(float (&z)[N], uint32_t slab, int row, i
   }
 }
 
-// What a warp of a direct product does instead of tiled copies: rows between a slab and memory, element by element, neighbours by
-// neighbouring lanes.
-template <typename E, int ROW_BYTES, bool OUT, typename P>
+// What a warp of a direct product does instead of tiled copies: rows between a slab and memory, neighbours by neighbouring lanes, a
+// batch of rows at a time so that their loads are on their way together.
+template <typename E, int SIZE, int ROW_BYTES, bool OUT, typename P>
 __device__ __forceinline__ void copy_direct(P *memory, long long pitch, int rows, int columns, uint32_t slab, int lane) {
-  constexpr int size = (int)sizeof(E);
-  for (int r = 0; r < rows; ++r) {
-    for (int c = lane; c < columns; c += 32) {
-      const uint32_t at = piece_of<ROW_BYTES>(slab, r, c * size / 16) + c * size % 16;
-      if constexpr (OUT) memory[r * pitch + c] = tc::read_one<E>(at);
-      else tc::write_one<E>(at, memory[r * pitch + c]);
+  constexpr int batch = 8;
+  for (int c = lane; c < columns; c += 32) {
+    const int piece = c * SIZE / 16, rest = c * SIZE % 16;
+    for (int r = 0; r < rows; r += batch) {
+      E v[batch];
+#pragma unroll
+      for (int i = 0; i < batch; ++i) {
+        if (r + i >= rows) continue;
+        if constexpr (OUT) v[i] = tc::read_one<E>(piece_of<ROW_BYTES>(slab, r + i, piece) + rest);
+        else v[i] = memory[(r + i) * pitch + c];
+      }
+#pragma unroll
+      for (int i = 0; i < batch; ++i) {
+        if (r + i >= rows) continue;
+        if constexpr (OUT) memory[(r + i) * pitch + c] = v[i];
+        else tc::write_one<E>(piece_of<ROW_BYTES>(slab, r + i, piece) + rest, v[i]);
+      }
     }
   }
+}
+// 16-bit rows that lie on the 4-byte grid go two elements at a time.
+template <typename E, int ROW_BYTES, bool OUT, typename P>
+__device__ __forceinline__ void copy_rows_direct(P *memory, long long pitch, int rows, int columns, uint32_t slab, int lane) {
+  if constexpr (sizeof(E) == 2) {
+    if (((reinterpret_cast<uintptr_t>(memory) | (uintptr_t)(pitch * 2)) & 3) == 0) {
+      using Two = std::conditional_t<OUT, float, const float>;      // two elements as one word; nothing is computed with it
+      copy_direct<float, 4, ROW_BYTES, OUT>(reinterpret_cast<Two *>(memory), pitch / 2, rows, columns / 2, slab, lane);
+      if (columns % 2 == 0) return;
+      const int c = columns - 1;
+      if (lane < rows) {
+        const uint32_t at = piece_of<ROW_BYTES>(slab, lane, c * 2 / 16) + c * 2 % 16;
+        if constexpr (OUT) memory[lane * pitch + c] = tc::read_one<E>(at);
+        else tc::write_one<E>(at, memory[lane * pitch + c]);
+      }
+      return;
+    }
+  }
+  copy_direct<E, (int)sizeof(E), ROW_BYTES, OUT>(memory, pitch, rows, columns, slab, lane);
 }
 
 // A tile by its row and column among the tiles: divided once, then counted, since a division takes a warp a few hundred cycles.  Rows
@@ -197,7 +227,8 @@ struct Place {
   __device__ __forceinline__ int column(int across) const { return n + turn < across ? n + turn : n + turn - across; }
 };
 
-template <ProductKind KIND, typename T, typename I, typename O, int BN, bool RESIDENT>
+// DIRECT: `in` and `out` do not lie as tiled copies need it.  A kernel of its own: that code's registers cost the others a third.
+template <ProductKind KIND, typename T, typename I, typename O, int BN, bool RESIDENT, bool DIRECT>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Tile<KIND, I, O, BN, RESIDENT>::threads, 1)
     product_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Extents p) {
   using L = Tile<KIND, I, O, BN, RESIDENT>;
@@ -403,7 +434,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Tile<KIND, I, O, BN,
       else asm volatile("bar.sync %0, %1;" ::"r"(1 + taker * 4 + quarter), "n"(32 * L::mates) : "memory");
     };
     const uint32_t bias = bias_at + e * (L::bias / L::warps), there = in_there + e * 8, first_drained = tc::address_in(drained, 0);
-    const bool loads = p.has_in && !p.direct;
+    const bool loads = p.has_in && !DIRECT;
     const T *bias0 = static_cast<const T *>(p.bias0), *bias1 = static_cast<const T *>(p.bias1);
     uint32_t in_phase = 0;
     bool ok = true;
@@ -471,10 +502,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Tile<KIND, I, O, BN,
       }
       __syncwarp();
       if (some) {
-        if (p.direct && p.has_in) {
+        if (DIRECT && p.has_in) {
           __syncwarp();
-          copy_direct<I, L::in_bytes, false>(static_cast<const I *>(p.in) + m0 * p.in_pitch + col, p.in_pitch, rows_in, cols_in, slab_in,
-                                             lane);
+          copy_rows_direct<I, L::in_bytes, false>(static_cast<const I *>(p.in) + m0 * p.in_pitch + col, p.in_pitch, rows_in, cols_in,
+                                                  slab_in, lane);
         } else if ((!loads || L::apart) && lane == 0 && mate == 0) {
           tc::stores_read<0>();
         }
@@ -534,10 +565,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Tile<KIND, I, O, BN,
         if (lane == 0) tc::arrive_in(first_drained + slot * 8);
         continue;
       }
-      if (!p.direct) tc::shared_to_async();
+      if (!DIRECT) tc::shared_to_async();
       meet();
-      if (p.direct) {
-        copy_direct<O, L::row_bytes, true>(static_cast<O *>(p.out) + m0 * p.out_pitch + col, p.out_pitch, rows_in, cols_in, slab, lane);
+      if constexpr (DIRECT) {
+        copy_rows_direct<O, L::row_bytes, true>(static_cast<O *>(p.out) + m0 * p.out_pitch + col, p.out_pitch, rows_in, cols_in, slab, lane);
       } else if (lane == 0 && mate == 0) {
 #pragma unroll
         for (int o = 0; o < L::outs; ++o) tc::tile_store(&maps.out[o], col, m0, slab + o * L::slab);
@@ -559,17 +590,19 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Tile<KIND, I, O, BN,
   }
 }
 
-template <ProductKind KIND, typename T, typename I, typename O, int BN, bool RESIDENT>
-cudaError_t launch_as(const ProductArgs &a, cudaStream_t s) {
-  using L = Tile<KIND, I, O, BN, RESIDENT>;
-  auto code = [&](size_t size) { return size == 4 ? DFA3D_DTYPE_F32 : a.dtype; };
+template <typename I, typename O> bool lies_direct(const ProductArgs &a) {
   auto fits = [](const void *q, long long pitch, size_t size) {
     return (reinterpret_cast<uintptr_t>(q) & 15u) == 0 && pitch * size % 16 == 0;
   };
+  return !fits(a.out[0], a.out_pitch, sizeof(O)) || (a.in.data && !fits(a.in.data, a.in.pitch, sizeof(I)));
+}
+
+template <ProductKind KIND, typename T, typename I, typename O, int BN, bool RESIDENT, bool DIRECT>
+cudaError_t launch_as(const ProductArgs &a, cudaStream_t s) {
+  using L = Tile<KIND, I, O, BN, RESIDENT>;
+  auto code = [&](size_t size) { return size == 4 ? DFA3D_DTYPE_F32 : a.dtype; };
   Maps m{};
   Extents p{};
-  p.direct = !fits(a.out[0], a.out_pitch, sizeof(O)) || (a.in.data && !fits(a.in.data, a.in.pitch, sizeof(I)));
-  if (p.direct && KIND != kLinear && KIND != kInputGrad) return cudaErrorInvalidValue;      // their results are workspaces
   constexpr int b_box = KIND == kInputGrad ? (L::b_rows < 64 ? L::b_rows : 64) : L::b_rows;
   bool ok = describe_matrix(m.a0, a.dtype, a.a0.data, a.rows, a.k0, a.a0.pitch, kDepth, kRows);
   if (a.k1 > 0) ok = ok && describe_matrix(m.a1, a.dtype, a.a1.data, a.rows, a.k1, a.a1.pitch, kDepth, kRows);
@@ -581,7 +614,7 @@ cudaError_t launch_as(const ProductArgs &a, cudaStream_t s) {
     if constexpr (L::gated) ok = ok && describe_matrix(m.b1, a.dtype, a.b1.data, a.n, a.k0, a.b1.pitch, kDepth, b_box);
     if constexpr (KIND == kGatedGrad) ok = ok && describe_matrix(m.b2, a.dtype, a.b2.data, a.k1, a.n, a.b2.pitch, L::b_ones, kDepth);
   }
-  if (!p.direct) {
+  if constexpr (!DIRECT) {
     if (a.in.data) ok = ok && describe_matrix(m.in, code(sizeof(I)), a.in.data, a.rows, a.n, a.in.pitch, L::chunk, 32);
     for (int o = 0; o < L::outs; ++o)
       ok = ok && describe_matrix(m.out[o], code(sizeof(O)), a.out[o], a.rows, a.n, a.out_pitch, L::chunk, 32);
@@ -601,17 +634,26 @@ cudaError_t launch_as(const ProductArgs &a, cudaStream_t s) {
   p.in_pitch = a.in.pitch;
   p.out = a.out[0];
   p.out_pitch = a.out_pitch;
-  constexpr auto kernel = &product_kernel<KIND, T, I, O, BN, RESIDENT>;
+  constexpr auto kernel = &product_kernel<KIND, T, I, O, BN, RESIDENT, DIRECT>;
   cudaError_t rc = allow_shared<kernel>(L::bytes);
   if (rc != cudaSuccess) return rc;
   const int pairs = sm_count() / 2, grid = 2 * (p.tiles < pairs ? p.tiles : pairs);
   return launch_after(kernel, grid, L::threads, L::bytes, s, m, p);
 }
 
-template <ProductKind KIND, typename T, typename I, typename O, int BN> cudaError_t launch_tiles(const ProductArgs &a, cudaStream_t s) {
+template <ProductKind KIND, typename T, typename I, typename O, int BN, bool DIRECT = false>
+cudaError_t launch_tiles(const ProductArgs &a, cudaStream_t s) {
   const int steps = (a.k0 + kDepth - 1) / kDepth + (a.k1 + kDepth - 1) / kDepth;
-  return steps <= Tile<KIND, I, O, BN, true>::slots_a ? launch_as<KIND, T, I, O, BN, true>(a, s)
-                                                      : launch_as<KIND, T, I, O, BN, false>(a, s);
+  return steps <= Tile<KIND, I, O, BN, true>::slots_a ? launch_as<KIND, T, I, O, BN, true, DIRECT>(a, s)
+                                                      : launch_as<KIND, T, I, O, BN, false, DIRECT>(a, s);
+}
+
+// Any width for results of the caller, narrow tiles where they lie off the 16-byte grid.
+template <ProductKind KIND, typename T, typename O> cudaError_t launch_widths(const ProductArgs &a, int width, cudaStream_t s) {
+  if (lies_direct<O, O>(a)) return launch_tiles<KIND, T, O, O, 64, true>(a, s);
+  return width == 256   ? launch_tiles<KIND, T, O, O, 256>(a, s)
+         : width == 128 ? launch_tiles<KIND, T, O, O, 128>(a, s)
+                        : launch_tiles<KIND, T, O, O, 64>(a, s);
 }
 
 // The width of tile whose slowest pair has the least to do: a tile costs its columns and, for operands and epilogue, about as much as
@@ -631,16 +673,12 @@ int tile_width(long long rows, int n, int widest) {
 }
 
 template <typename T> cudaError_t launch_typed(const ProductArgs &a, cudaStream_t s) {
+  // the results of the other kinds are workspaces
+  if (a.kind != kLinear && a.kind != kInputGrad && lies_direct<T, T>(a) && !a.wide) return cudaErrorInvalidValue;
   switch (a.kind) {
     case kLinear: {
       const int w = tile_width(a.rows, a.n, 256);
-      if (a.wide)
-        return w == 256   ? launch_tiles<kLinear, T, float, float, 256>(a, s)
-               : w == 128 ? launch_tiles<kLinear, T, float, float, 128>(a, s)
-                          : launch_tiles<kLinear, T, float, float, 64>(a, s);
-      return w == 256   ? launch_tiles<kLinear, T, T, T, 256>(a, s)
-             : w == 128 ? launch_tiles<kLinear, T, T, T, 128>(a, s)
-                        : launch_tiles<kLinear, T, T, T, 64>(a, s);
+      return a.wide ? launch_widths<kLinear, T, float>(a, w, s) : launch_widths<kLinear, T, T>(a, w, s);
     }
     case kSlope: {
       const bool narrow = tile_width(a.rows, a.n, 128) == 64;
@@ -650,12 +688,7 @@ template <typename T> cudaError_t launch_typed(const ProductArgs &a, cudaStream_
     case kGated:
       return tile_width(a.rows, a.n, 128) == 128 ? launch_tiles<kGated, T, T, T, 256>(a, s) : launch_tiles<kGated, T, T, T, 128>(a, s);
     case kGatedGrad: return launch_tiles<kGatedGrad, T, T, T, 128>(a, s);
-    case kInputGrad: {
-      const int w = tile_width(a.rows, a.n, 256);
-      return w == 256   ? launch_tiles<kInputGrad, T, T, T, 256>(a, s)
-             : w == 128 ? launch_tiles<kInputGrad, T, T, T, 128>(a, s)
-                        : launch_tiles<kInputGrad, T, T, T, 64>(a, s);
-    }
+    case kInputGrad: return launch_widths<kInputGrad, T, T>(a, tile_width(a.rows, a.n, 256), s);
   }
   return cudaErrorInvalidValue;
 }

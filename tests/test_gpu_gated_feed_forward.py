@@ -45,7 +45,7 @@ def check(d, act, checkpoint=None):
 
 
 SIZES = [(1, 1, 1, 1), (1, 8, 8, 8), (5, 7, 3, 9), (33, 64, 64, 64), (129, 65, 63, 66), (128, 128, 128, 128), (200, 90, 250, 90),
-         (257, 256, 136, 256), (300, 300, 72, 100), (130, 72, 520, 40)]
+         (257, 256, 136, 256), (300, 300, 72, 100), (130, 72, 520, 40), (200, 300, 72, 310), (200, 330, 140, 700), (140, 64, 60, 600)]
 
 
 @pytest.mark.parametrize("dtype", TYPES)
