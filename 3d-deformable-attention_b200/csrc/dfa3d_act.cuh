@@ -1,6 +1,8 @@
-// Activations that follow a matrix product, and their derivatives, in 32 bits.  An epilogue applies them to every element of a
-// result, so that what they cost in instructions is what many of these products are bound by: exponential and reciprocal are single
-// instructions of a relative error of 2^-22 and 2^-23, far below the 2^-9 or 2^-12 of the result's rounding.
+// Activations that follow a matrix product, and their derivatives, in 32 bits, two elements at a time.  An epilogue applies them to
+// every element of a result, and what they cost in instructions is what many of these products are bound by.  So: products and sums of
+// two elements are one instruction; exponential and reciprocal are single instructions of a relative error of 2^-22 and 2^-23, far
+// below the 2^-9 or 2^-12 of the result's rounding; and since an SM has a quarter as many units for those two, two reciprocals are one,
+// 1 / a = b / (a b).
 #pragma once
 #include "dfa3d_b200.h"
 
@@ -16,52 +18,94 @@ __device__ __forceinline__ float reciprocal(float x) {
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
+__device__ __forceinline__ float no_less(float x, float least) {      // NaN stays
+  float y;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(x), "f"(least));
+  return y;
+}
 
-// 1 / (1 + exp(-z)); far below 0 exp is infinite and the reciprocal 0
-__device__ __forceinline__ float sigmoid(float z) { return reciprocal(1.f + power_of_two(z * -1.4426950408889634f)); }
+struct Two {
+  float x, y;
+};
+__device__ __forceinline__ Two both(float c) { return {c, c}; }
+__device__ __forceinline__ Two operator+(Two a, Two b) {
+  asm("{\n.reg .b64 p, q;\nmov.b64 p, {%0, %1};\nmov.b64 q, {%2, %3};\nadd.rn.f32x2 p, p, q;\nmov.b64 {%0, %1}, p;\n}"
+      : "+f"(a.x), "+f"(a.y)
+      : "f"(b.x), "f"(b.y));
+  return a;
+}
+__device__ __forceinline__ Two operator*(Two a, Two b) {
+  asm("{\n.reg .b64 p, q;\nmov.b64 p, {%0, %1};\nmov.b64 q, {%2, %3};\nmul.rn.f32x2 p, p, q;\nmov.b64 {%0, %1}, p;\n}"
+      : "+f"(a.x), "+f"(a.y)
+      : "f"(b.x), "f"(b.y));
+  return a;
+}
+__device__ __forceinline__ Two times_plus(Two a, Two b, Two c) {      // a b + c
+  asm("{\n.reg .b64 p, q, r;\nmov.b64 p, {%0, %1};\nmov.b64 q, {%2, %3};\nmov.b64 r, {%4, %5};\nfma.rn.f32x2 p, p, q, r;\nmov.b64 {%0, "
+      "%1}, p;\n}"
+      : "+f"(a.x), "+f"(a.y)
+      : "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return a;
+}
+__device__ __forceinline__ Two power_of_two(Two a) { return {power_of_two(a.x), power_of_two(a.y)}; }
+__device__ __forceinline__ Two reciprocal(Two a) {      // of numbers from 1 to 2^61
+  const float r = reciprocal(a.x * a.y);
+  return {r * a.y, r * a.x};
+}
+
+// 1 / (1 + exp(-z)), and 2^-60 below -41.6
+__device__ __forceinline__ Two sigmoid(Two z) {
+  Two q = z * both(-1.4426950408889634f);
+  q = {fminf(q.x, 60.f), fminf(q.y, 60.f)};
+  return reciprocal(power_of_two(q) + both(1.f));
+}
+// where the sigmoid is 2^-60, z as far as it counts: z sigmoid(z) goes to 0 there, and not to -infinity
+__device__ __forceinline__ Two counted(Two z) { return {no_less(z.x, -42.f), no_less(z.y, -42.f)}; }
 
 // The normal distribution's P(X <= z) = erfc(-z / sqrt 2) / 2 and exp(-z^2 / 2).  With t = 1 / (1 + 0.3275911 x),
 // erfc(x) = exp(-x^2) (a1 t + ... + a5 t^5), |error| <= 1.5e-7, for x >= 0 (Abramowitz and Stegun, Handbook of Mathematical
 // Functions, 7.1.26); on the negative side the factor exp(-x^2) keeps the tail's relative error small too.
-__device__ __forceinline__ float normal_cdf(float z, float &bell) {
-  bell = power_of_two(z * z * -0.72134752044448170f);
-  const float t = reciprocal(fmaf(fabsf(z), 0.3275911f * 0.70710678118654752f, 1.f));
-  float w = fmaf(t, 0.5f * 1.061405429f, 0.5f * -1.453152027f);
-  w = fmaf(t, w, 0.5f * 1.421413741f);
-  w = fmaf(t, w, 0.5f * -0.284496736f);
-  w = fmaf(t, w, 0.5f * 0.254829592f);
-  w = w * t * bell;
-  return z < 0.f ? w : 1.f - w;
+__device__ __forceinline__ Two normal_cdf(Two z, Two &bell) {
+  bell = power_of_two(z * z * both(-0.72134752044448170f));
+  const Two far{fminf(fabsf(z.x), 1e8f), fminf(fabsf(z.y), 1e8f)};
+  const Two t = reciprocal(times_plus(far, both(0.3275911f * 0.70710678118654752f), both(1.f)));
+  Two w = times_plus(t, both(0.5f * 1.061405429f), both(0.5f * -1.453152027f));
+  w = times_plus(t, w, both(0.5f * 1.421413741f));
+  w = times_plus(t, w, both(0.5f * -0.284496736f));
+  w = times_plus(t, w, both(0.5f * 0.254829592f));
+  w = w * (t * bell);
+  const Two v = times_plus(w, both(-1.f), both(1.f));
+  return {z.x < 0.f ? w.x : v.x, z.y < 0.f ? w.y : v.y};
 }
 
-template <int ACT> __device__ __forceinline__ float activate(float z) {
-  if constexpr (ACT == DFA3D_ROW_RELU) return z <= 0.f ? 0.f : z;          // NaN stays
-  if constexpr (ACT == DFA3D_ROW_SILU) return z * sigmoid(z);
+template <int ACT> __device__ __forceinline__ Two activate(Two z) {
+  if constexpr (ACT == DFA3D_ROW_RELU) return {z.x <= 0.f ? 0.f : z.x, z.y <= 0.f ? 0.f : z.y};          // NaN stays
+  if constexpr (ACT == DFA3D_ROW_SILU) return counted(z) * sigmoid(z);
   if constexpr (ACT == DFA3D_ROW_GELU) {
-    float bell;
+    Two bell;
     return z * normal_cdf(z, bell);
   }
   return z;
 }
 
 // act(z) and d act / dz
-template <int ACT> __device__ __forceinline__ void activate_both(float z, float &a, float &slope) {
+template <int ACT> __device__ __forceinline__ void activate_both(Two z, Two &a, Two &slope) {
   a = z;
-  slope = 1.f;
+  slope = both(1.f);
   if constexpr (ACT == DFA3D_ROW_RELU) {
-    a = z <= 0.f ? 0.f : z;
-    slope = z <= 0.f ? 0.f : 1.f;
+    a = activate<ACT>(z);
+    slope = {z.x <= 0.f ? 0.f : 1.f, z.y <= 0.f ? 0.f : 1.f};
   }
   if constexpr (ACT == DFA3D_ROW_SILU) {
-    const float s = sigmoid(z);
-    a = z * s;
-    slope = fmaf(a, 1.f - s, s);
+    const Two s = sigmoid(z);
+    a = counted(z) * s;
+    slope = times_plus(a, times_plus(s, both(-1.f), both(1.f)), s);
   }
   if constexpr (ACT == DFA3D_ROW_GELU) {
-    float bell;
-    const float p = normal_cdf(z, bell);
+    Two bell;
+    const Two p = normal_cdf(z, bell);
     a = z * p;
-    slope = fmaf(z * 0.39894228040143268f, bell, p);
+    slope = times_plus(z * both(0.39894228040143268f), bell, p);
   }
 }
 

@@ -81,7 +81,11 @@ template <int ROW_BYTES> __device__ __forceinline__ uint32_t piece_of(uint32_t s
 
 template <int ACT, int N> __device__ __forceinline__ void activate_each(float (&z)[N]) {
 #pragma unroll
-  for (int i = 0; i < N; ++i) z[i] = activate<ACT>(z[i]);
+  for (int i = 0; i < N; i += 2) {
+    const Two a = activate<ACT>(Two{z[i], z[i + 1]});
+    z[i] = a.x;
+    z[i + 1] = a.y;
+  }
 }
 template <int N> __device__ __forceinline__ void activate_all(float (&z)[N], int act) {
   switch (act) {
@@ -93,9 +97,11 @@ template <int N> __device__ __forceinline__ void activate_all(float (&z)[N], int
 }
 template <int ACT, int N> __device__ __forceinline__ void slope_each(float (&z)[N]) {
 #pragma unroll
-  for (int i = 0; i < N; ++i) {
-    float a;
-    activate_both<ACT>(z[i], a, z[i]);
+  for (int i = 0; i < N; i += 2) {
+    Two a, s;
+    activate_both<ACT>(Two{z[i], z[i + 1]}, a, s);
+    z[i] = s.x;
+    z[i + 1] = s.y;
   }
 }
 template <int N> __device__ __forceinline__ void slope_all(float (&z)[N], int act) {
@@ -109,12 +115,17 @@ template <int N> __device__ __forceinline__ void slope_all(float (&z)[N], int ac
 // gate, up, d -> d up act'(gate), d act(gate), act(gate) up
 template <int ACT, int N> __device__ __forceinline__ void gate_each(float (&g)[N], float (&u)[N], float (&d)[N]) {
 #pragma unroll
-  for (int i = 0; i < N; ++i) {
-    float a, s;
-    activate_both<ACT>(g[i], a, s);
-    g[i] = d[i] * u[i] * s;
-    d[i] = d[i] * a;
-    u[i] = a * u[i];
+  for (int i = 0; i < N; i += 2) {
+    const Two up{u[i], u[i + 1]}, through{d[i], d[i + 1]};
+    Two a, s;
+    activate_both<ACT>(Two{g[i], g[i + 1]}, a, s);
+    const Two grad_gate = through * up * s, grad_up = through * a, h = a * up;
+    g[i] = grad_gate.x;
+    g[i + 1] = grad_gate.y;
+    d[i] = grad_up.x;
+    d[i + 1] = grad_up.y;
+    u[i] = h.x;
+    u[i + 1] = h.y;
   }
 }
 template <int N> __device__ __forceinline__ void gate_all(float (&g)[N], float (&u)[N], float (&d)[N], int act) {
@@ -126,18 +137,12 @@ template <int N> __device__ __forceinline__ void gate_all(float (&g)[N], float (
   }
 }
 
-// one instruction for two sums
-__device__ __forceinline__ void add_two(float &a, float &b, float c, float d) {
-  asm("{\n.reg .b64 x, y;\nmov.b64 x, {%0, %1};\nmov.b64 y, {%2, %3};\nadd.rn.f32x2 x, x, y;\nmov.b64 {%0, %1}, x;\n}"
-      : "+f"(a), "+f"(b)
-      : "f"(c), "f"(d));
-}
 template <int N> __device__ __forceinline__ void add_bias(float (&z)[N], uint32_t bias) {
 #pragma unroll
   for (int i = 0; i < N; i += 4) {
     const float4 b = tc::read_four(bias + i * 4);
-    add_two(z[i], z[i + 1], b.x, b.y);
-    add_two(z[i + 2], z[i + 3], b.z, b.w);
+    const Two lo = Two{z[i], z[i + 1]} + Two{b.x, b.y}, hi = Two{z[i + 2], z[i + 3]} + Two{b.z, b.w};
+    z[i] = lo.x; z[i + 1] = lo.y; z[i + 2] = hi.x; z[i + 3] = hi.y;
   }
 }
 
@@ -196,8 +201,8 @@ template <typename E, int ROW_BYTES, bool OUT, typename P>
 __device__ __forceinline__ void copy_rows_direct(P *memory, long long pitch, int rows, int columns, uint32_t slab, int lane) {
   if constexpr (sizeof(E) == 2) {
     if (((reinterpret_cast<uintptr_t>(memory) | (uintptr_t)(pitch * 2)) & 3) == 0) {
-      using Two = std::conditional_t<OUT, float, const float>;      // two elements as one word; nothing is computed with it
-      copy_direct<float, 4, ROW_BYTES, OUT>(reinterpret_cast<Two *>(memory), pitch / 2, rows, columns / 2, slab, lane);
+      using Word = std::conditional_t<OUT, float, const float>;      // two elements; nothing is computed with it
+      copy_direct<float, 4, ROW_BYTES, OUT>(reinterpret_cast<Word *>(memory), pitch / 2, rows, columns / 2, slab, lane);
       if (columns % 2 == 0) return;
       const int c = columns - 1;
       if (lane < rows) {
@@ -550,7 +555,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Tile<KIND, I, O, BN,
           } else if constexpr (KIND == kGated) {
             activate_all(z, p.act);
 #pragma unroll
-            for (int i = 0; i < L::sub; ++i) z[i] *= v[t & 1][1][i];
+            for (int i = 0; i < L::sub; i += 2) {
+              const Two h = Two{z[i], z[i + 1]} * Two{v[t & 1][1][i], v[t & 1][1][i + 1]};
+              z[i] = h.x;
+              z[i + 1] = h.y;
+            }
           } else {
             if constexpr (KIND == kLinear) activate_all(z, p.act);
             if constexpr (KIND == kSlope) slope_all(z, p.act);
