@@ -21,6 +21,7 @@ namespace {
 
 constexpr int kRows = 128, kDepth = 64;          // of a CTA's tile; along the summed axis, 128 bytes
 constexpr int kOperandA = kRows * kDepth * 2;
+constexpr int kAhead = 10;                        // steps between asking for operands into L2 and into shared memory
 
 struct Maps {
   CUtensorMap a0, a1, b0, b1, b2, in, out[3];
@@ -315,7 +316,17 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Tile<KIND, I, O, BN,
               const CUtensorMap *map = second ? &maps.a1 : &maps.a0;
               const int at = (second ? j - p.steps0 : j) * kDepth;
               tc::tile_load_pair(to, map, at, m0, first_there + slot * 8);
-              if (look) tc::tile_to_l2(map, at, m0 + 2 * kRows);
+              if constexpr (RESIDENT) {
+                if (look) tc::tile_to_l2(map, at, m0 + 2 * kRows);
+              } else if (fresh) {
+                // a few steps further, of these rows or of the next: all of a long sum's would push one another out of L2
+                const int then = j + kAhead < steps ? j + kAhead : j + kAhead - steps;
+                const bool here = j + kAhead < steps;
+                if (here || (look && then < steps)) {
+                  const bool other = then >= p.steps0;
+                  tc::tile_to_l2(other ? &maps.a1 : &maps.a0, (other ? then - p.steps0 : then) * kDepth, here ? m0 : m0 + 2 * kRows);
+                }
+              }
             }
           }
         } else {
