@@ -1,6 +1,7 @@
 // Native host path of the feed-forward block in 16 bits: products with bias, activation and residual, the gated block, inputs kept in
 // 8 bits.  Same contract as dfa3d_torch.cpp: NotImplemented means that the Python code has to take the call.
 #include <ATen/cuda/EmptyTensor.h>
+#include <torch/csrc/Dtype.h>
 
 #include "dfa3d_torch.h"
 
@@ -348,6 +349,66 @@ PyObject *run_gated(PyObject *const *a, Py_ssize_t n) {
   return THPVariable_Wrap(y);
 }
 
+// ------------------------------------------------------------------------------------------------
+// 8 bits by themselves
+// ------------------------------------------------------------------------------------------------
+bool format_argument(PyObject *o, int32_t &format) {
+  return o != Py_None && one_of(o, {"int8", "e4m3"}, DFA3D_FORMAT_INT8, -1, format);
+}
+
+PyObject *run_compress8(PyObject *const *a, Py_ssize_t n) {
+  // x, format -> (codes, scales)
+  int32_t format;
+  Tensor x;
+  if (n != 2 || !plain_mode() || !plain_tensor(a[0], x) || !storage_type(x.scalar_type()) || x.dim() < 1 || x.numel() == 0 ||
+      x.size(-1) > (1 << 30) || !format_argument(a[1], format))
+    return not_plain();
+  Tensor codes, scales;
+  {
+    pybind11::gil_scoped_release nogil;
+    c10::cuda::CUDAGuard guard(x.device());
+    const int64_t cols = x.size(-1), rows = x.numel() / cols;
+    codes = fresh({rows, cols}, at::kByte, x);
+    scales = fresh({rows, (cols + 31) / 32}, at::kByte, x);
+    check(lib.dfa3d_compress8(vp(x), dtype_code(x), rows, (int32_t)cols, format, static_cast<uint8_t *>(vpm(codes)),
+                              static_cast<uint8_t *>(vpm(scales)), stream_of(x)),
+          "dfa3d_compress8");
+  }
+  PyObject *t = PyTuple_New(2);
+  PyTuple_SET_ITEM(t, 0, THPVariable_Wrap(codes));
+  PyTuple_SET_ITEM(t, 1, THPVariable_Wrap(scales));
+  return t;
+}
+
+PyObject *run_decompress8(PyObject *const *a, Py_ssize_t n) {
+  // codes, scales, shape, dtype, format
+  int32_t format;
+  Tensor codes, scales;
+  if (n != 5 || !plain_mode() || !plain_tensor(a[0], codes) || !plain_tensor(a[1], scales) || codes.scalar_type() != at::kByte ||
+      scales.scalar_type() != at::kByte || !one_device(codes, scales) || !PyTuple_Check(a[2]) || PyTuple_GET_SIZE(a[2]) < 1 ||
+      !THPDtype_Check(a[3]) || !format_argument(a[4], format))
+    return not_plain();
+  const at::ScalarType type = reinterpret_cast<THPDtype *>(a[3])->scalar_type;
+  std::vector<int64_t> shape((size_t)PyTuple_GET_SIZE(a[2]));
+  int64_t count = 1;
+  for (size_t i = 0; i < shape.size(); ++i)
+    if (!integer(PyTuple_GET_ITEM(a[2], (Py_ssize_t)i), shape[i]) || shape[i] < 1 || shape[i] > codes.numel() ||
+        (count *= shape[i]) > codes.numel())
+      return not_plain();
+  const int64_t cols = shape.back(), rows = count / cols;
+  if (!storage_type(type) || cols > (1 << 30) || codes.numel() != count || scales.numel() != rows * ((cols + 31) / 32)) return not_plain();
+  Tensor x;
+  {
+    pybind11::gil_scoped_release nogil;
+    c10::cuda::CUDAGuard guard(codes.device());
+    x = fresh(shape, type, codes);
+    check(lib.dfa3d_decompress8(static_cast<const uint8_t *>(vp(codes)), static_cast<const uint8_t *>(vp(scales)), format, rows,
+                                (int32_t)cols, dtype_code(x), vpm(x), cols, stream_of(x)),
+          "dfa3d_decompress8");
+  }
+  return THPVariable_Wrap(x);
+}
+
 #define FAST(name, expr)                                                             \
   PyObject *py_##name(PyObject *, PyObject *const *a, Py_ssize_t n) {                 \
     HANDLE_TH_ERRORS                                                                  \
@@ -356,6 +417,8 @@ PyObject *run_gated(PyObject *const *a, Py_ssize_t n) {
   }
 FAST(linear_act, run_linear_act(a, n))
 FAST(gated_feed_forward, run_gated(a, n))
+FAST(compress8, run_compress8(a, n))
+FAST(decompress8, run_decompress8(a, n))
 #undef FAST
 
 }  // namespace
@@ -363,7 +426,7 @@ FAST(gated_feed_forward, run_gated(a, n))
 namespace dfa3d_torch {
 #define FAST(name) {#name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_##name)), METH_FASTCALL, nullptr}
 PyMethodDef ffn_methods[] = {
-    FAST(linear_act), FAST(gated_feed_forward), {nullptr, nullptr, 0, nullptr},
+    FAST(linear_act), FAST(gated_feed_forward), FAST(compress8), FAST(decompress8), {nullptr, nullptr, 0, nullptr},
 };
 #undef FAST
 }  // namespace dfa3d_torch

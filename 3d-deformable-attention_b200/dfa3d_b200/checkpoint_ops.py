@@ -42,6 +42,9 @@ def _stream(t):
 def compress8(x, format="int8"):
     """x (..., cols), float32, bfloat16 or float16 on a CUDA device, in 8 bits."""
     check_format(format)
+    got = _lib.native().compress8(x, format)
+    if got is not NotImplemented:
+        return Compressed8(*got, x.shape, x.dtype, format)
     if not x.is_cuda or x.dtype not in _DTYPES:
         raise RuntimeError(f"x must be a float32, bfloat16 or float16 CUDA tensor, got {x.dtype} on {x.device}")
     if x.dim() == 0:
@@ -72,6 +75,9 @@ def check_compressed(c):
 
 def decompress8(c):
     """What a ``compress8`` stands for, of the shape and type that it was given."""
+    got = _lib.native().decompress8(*c)
+    if got is not NotImplemented:
+        return got
     rows, cols = check_compressed(c)
     out = torch.empty(c.shape, dtype=c.dtype, device=c.codes.device)
     into(c, out, cols)

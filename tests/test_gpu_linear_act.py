@@ -182,3 +182,16 @@ def test_differences():
             # rounding of the gradient: 2^-11 of its terms; curvature: third order in the step
             bound = 3e-3 * (grads[k].double().abs() * (hi[k].double() - lo[k].double()).abs()).sum()
             assert abs(f(hi) - f(lo) - slope) <= bound
+
+
+def test_past_two_to_the_31_elements():
+    """The last rows of x and y lie beyond 32-bit offsets."""
+    import dfa3d_b200 as M
+    rows, K, N = (1 << 25) + 259, 64, 72              # 2.1e9 and 2.4e9 elements, 4.3 and 4.8 GB
+    d = make(300, K, N, torch.bfloat16, seed=15)
+    x = torch.zeros(rows, K, dtype=torch.bfloat16, device="cuda")
+    x[:300], x[-300:] = d["x"], d["x"]
+    want = M.linear_act(d["x"], d["w"], d["b"], "gelu")
+    y = M.linear_act(x, d["w"], d["b"], "gelu")
+    assert torch.equal(y[:300], want) and torch.equal(y[-300:], want)
+    assert torch.equal(y[300:400], M.linear_act(x[300:400], d["w"], d["b"], "gelu"))
