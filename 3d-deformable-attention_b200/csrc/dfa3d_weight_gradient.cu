@@ -238,10 +238,12 @@ int tiles_for(const WeightProblem *w, int count, int width) {
   for (int i = 0; i < count; ++i) n += (w[i].p + 2 * kTileP - 1) / (2 * kTileP) * ((w[i].q + width - 1) / width);
   return n;
 }
-// As many shares of the rows as pairs of SMs allow in one wave, none without rows.
+// As many shares of the rows as pairs of SMs allow in one wave, of four steps at least (what a share leaves behind takes about as long
+// to write and read back as four steps do), none without rows.
 int shares_for(long long rows, int tiles) {
-  const long long steps = (rows + kDepth - 1) / kDepth, pairs = sm_count() / 2, s = tiles < pairs ? pairs / tiles : 1;
-  return (int)(s < steps ? s : steps);
+  const long long steps = (rows + kDepth - 1) / kDepth, pairs = sm_count() / 2, most = tiles < pairs ? pairs / tiles : 1;
+  const long long s = (steps + 3) / 4;
+  return (int)(s < most ? s : most);
 }
 
 template <typename T, int BN>
