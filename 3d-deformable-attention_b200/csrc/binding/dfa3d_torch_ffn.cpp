@@ -145,8 +145,17 @@ struct LinearActFn : torch::autograd::Function<LinearActFn> {
       if (slope || gw || gb) xr = kept_input(*b, v, o);
       const Rows wr = slope || gx ? o.add(w, b->out, b->in) : Rows();
       // a 32-bit gradient is not rounded before the derivative has been applied
-      const bool wide = slope && gt.scalar_type() == at::kFloat && b->out % 8 == 0 && aligned(gt, 16);
-      Rows g = wide ? Rows{gt, b->out} : o.add(gt, b->rows, b->out);
+      const bool wide = slope && gt.scalar_type() == at::kFloat;
+      Rows g;
+      if (!wide) {
+        g = o.add(gt, b->rows, b->out);
+      } else if (b->out % 8 == 0 && aligned(gt, 16)) {
+        g = {gt, b->out};
+      } else {
+        g = {fresh({b->rows, pitch_of(b->out)}, at::kFloat, gt), pitch_of(b->out)};
+        at::NoGradGuard none;
+        g.t.narrow(1, 0, b->out).copy_(gt.view({b->rows, b->out}));
+      }
       o.copy(s);
       if (slope) {
         const Rows z{fresh({b->rows, pitch_of(b->out)}, b->type, w), pitch_of(b->out)};

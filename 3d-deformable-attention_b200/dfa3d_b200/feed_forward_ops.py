@@ -180,13 +180,16 @@ class LinearActFunction(Function):
             with torch.cuda.device(grad_y.device):
                 (x, xp), (weight, bias) = _kept_input(ctx)
                 g = grad_y if grad_y.dtype in (ctx.dtype, torch.float32) else grad_y.to(ctx.dtype)
-                g2, wide = _rows(g).contiguous(), _lib.DTYPE_F32
-                if ctx.act != _lib.ROW_NONE and g2.dtype == torch.float32 and N % 8 == 0 and g2.data_ptr() % 16 == 0:
+                g, wide = _rows(g).contiguous(), _DTYPES[ctx.dtype]
+                if ctx.act != _lib.ROW_NONE and g.dtype == torch.float32:
                     (w, wp), = _operands(ctx.dtype, weight)           # not rounded before the derivative has been applied
-                    g, gp = g2, N
+                    wide, gp = _lib.DTYPE_F32, _pitch(N)
+                    if gp != N or g.data_ptr() % 16:
+                        on_grid = torch.empty((rows, gp), dtype=torch.float32, device=g.device)
+                        on_grid[:, :N].copy_(g)
+                        g = on_grid
                 else:
-                    (w, wp), (g, gp) = _operands(ctx.dtype, weight, g2)
-                    wide = _DTYPES[ctx.dtype]
+                    (w, wp), (g, gp) = _operands(ctx.dtype, weight, g)
                 st = _stream(g)
                 if ctx.act != _lib.ROW_NONE:
                     dz, zp = _workspace(rows, N, x)

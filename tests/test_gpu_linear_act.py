@@ -62,6 +62,12 @@ def test_wide_residual_of_odd_rows(act, N):
     check(make(150, 96, N, torch.bfloat16, True, "wide", seed=2), act)
 
 
+def test_a_wide_gradient_is_rounded_once(lib_built):
+    """Rows off the 16-byte grid too: the derivative is applied to 32 bits."""
+    check(make(1, 256, 393, torch.bfloat16, False, "wide", seed=2368), "silu", "int8")
+    check(make(7, 64, 2051, torch.float16, True, "wide", seed=3), "gelu")
+
+
 @pytest.mark.parametrize("checkpoint", ["int8", "e4m3"])
 @pytest.mark.parametrize("act", [None, "relu", "silu", "gelu"])
 @pytest.mark.parametrize("K", [96, 59])
