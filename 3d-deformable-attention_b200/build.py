@@ -15,7 +15,7 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 OUT = os.path.join(HERE, "dfa3d_b200", "libdfa3d_b200.so")
 SOURCES = ["dfa3d_forward.cu", "dfa3d_forward_packed.cu", "dfa3d_backward.cu", "dfa3d_backward_packed.cu", "dfa3d_rebatch.cu", "dfa3d_dist_producer.cu",
-           "dfa3d_fp64.cu", "dfa3d_layer_ops.cu", "dfa3d_dropout.cu", "dfa3d_group_norm.cu", "dfa3d_product.cu", "dfa3d_weight_gradient.cu",
+           "dfa3d_fp64.cu", "dfa3d_layer_ops.cu", "dfa3d_dropout.cu", "dfa3d_group_norm.cu", "dfa3d_product.cu", "dfa3d_gated_block.cu", "dfa3d_weight_gradient.cu",
            "dfa3d_checkpoint8.cu", "dfa3d_capi.cu"]
 RATES_SRC = os.path.join(CSRC, "rates", "dfa3d_rates.cu")
 RATES_OUT = os.path.join(HERE, "dfa3d_b200", "libdfa3d_rates.so")

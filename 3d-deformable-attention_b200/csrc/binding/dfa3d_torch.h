@@ -45,6 +45,7 @@ using torch::autograd::variable_list;
   X(dfa3d_group_norm_workspace) X(dfa3d_group_norm_forward) X(dfa3d_group_norm_backward)                 \
   X(dfa3d_relu_dropout_backward_column_sum) X(dfa3d_linear_act_forward) X(dfa3d_linear_act_slope)        \
   X(dfa3d_linear_input_gradient) X(dfa3d_gated_hidden_forward) X(dfa3d_gated_hidden_backward)            \
+  X(dfa3d_gated_block_supported) X(dfa3d_gated_block_forward)                                            \
   X(dfa3d_weight_gradients_workspace) X(dfa3d_weight_gradients) X(dfa3d_copy_rows) X(dfa3d_compress8) X(dfa3d_decompress8)
 
 struct Abi {

@@ -253,9 +253,18 @@ Tensor gated_forward(const Block &b, const Tensor &x, const Weights &w, const Te
   Tensor y = fresh(b.shape, res.defined() ? res.scalar_type() : b.type, x);
   Operands o(b.type);
   const Rows xr = o.add(x, b.rows, b.in), wg = o.add(w.gate, b.hidden, b.in), wu = o.add(w.up, b.hidden, b.in),
-             wd = o.add(w.down, b.out, b.hidden), h{fresh({b.rows, pitch_of(b.hidden)}, b.type, x), pitch_of(b.hidden)};
+             wd = o.add(w.down, b.out, b.hidden);
   void *s = stream_of(x);
   o.copy(s);
+  if (lib.dfa3d_gated_block_supported(out_code(b, y), b.rows, (int32_t)b.in, (int32_t)b.hidden, (int32_t)b.out) &&
+      (!res.defined() || aligned(res, 16))) {
+    check(lib.dfa3d_gated_block_forward(xr.data(), xr.pitch, wg.data(), wu.data(), wg.pitch, vp(w.bias_gate), vp(w.bias_up), wd.data(),
+                                        wd.pitch, vp(w.bias_down), vp(res), b.dtype, out_code(b, y), b.rows, (int32_t)b.in,
+                                        (int32_t)b.hidden, (int32_t)b.out, b.act, vpm(y), s),
+          "dfa3d_gated_block_forward");
+    return y;
+  }
+  const Rows h{fresh({b.rows, pitch_of(b.hidden)}, b.type, x), pitch_of(b.hidden)};
   check(lib.dfa3d_gated_hidden_forward(xr.data(), xr.pitch, wg.data(), wu.data(), wg.pitch, vp(w.bias_gate), vp(w.bias_up), b.dtype,
                                        b.rows, (int32_t)b.in, (int32_t)b.hidden, b.act, vpm(h.t), h.pitch, s),
         "dfa3d_gated_hidden_forward");

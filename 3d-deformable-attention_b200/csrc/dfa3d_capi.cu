@@ -1077,6 +1077,54 @@ int dfa3d_gated_hidden_forward(const void *x, int64_t x_pitch, const void *weigh
   return finish(dfa3d::launch_product(a, (cudaStream_t)stream), "dfa3d_gated_hidden_forward launch");
 }
 
+static dfa3d::ProductArgs gated_block_arguments(int32_t dtype, int32_t out_dtype, int64_t rows, int32_t in, int32_t out) {
+  dfa3d::ProductArgs a;
+  a.kind = dfa3d::kGated;
+  a.dtype = dtype;
+  a.wide = out_dtype == DFA3D_DTYPE_F32;
+  a.rows = rows;
+  a.n = out;
+  a.k0 = in;
+  a.out_pitch = out;
+  return a;
+}
+
+int dfa3d_gated_block_supported(int32_t out_dtype, int64_t rows, int32_t in, int32_t hidden, int32_t out) {
+  if (out_dtype != DFA3D_DTYPE_F32 && out_dtype != DFA3D_DTYPE_BF16 && out_dtype != DFA3D_DTYPE_F16) return 0;
+  if (check_product(DFA3D_DTYPE_BF16, rows, {in, hidden, out}, DFA3D_ROW_NONE) != DFA3D_OK) return 0;
+  return dfa3d::gated_block_covers(gated_block_arguments(DFA3D_DTYPE_BF16, out_dtype, rows, in, out), hidden);
+}
+
+int dfa3d_gated_block_forward(const void *x, int64_t x_pitch, const void *weight_gate, const void *weight_up, int64_t weight_pitch,
+                              const void *bias_gate, const void *bias_up, const void *weight_down, int64_t down_pitch,
+                              const void *bias_down, const void *residual, int32_t dtype, int32_t out_dtype, int64_t rows, int32_t in,
+                              int32_t hidden, int32_t out, int32_t activation, void *y, void *stream) {
+  if (int rc = check_product(dtype, rows, {in, hidden, out}, activation)) return rc;
+  if (out_dtype != dtype && out_dtype != DFA3D_DTYPE_F32)
+    return fail(DFA3D_ERR_INVALID_ARGUMENT, "out_dtype %d is neither dtype nor DFA3D_DTYPE_F32", out_dtype);
+  if (int rc = check_elements(dtype, {bias_gate, bias_up, bias_down})) return rc;
+  if (rows == 0) return DFA3D_OK;
+  REQUIRE_OPERAND(x, x_pitch, in);
+  REQUIRE_OPERAND(weight_gate, weight_pitch, in);
+  REQUIRE_OPERAND(weight_up, weight_pitch, in);
+  REQUIRE_OPERAND(weight_down, down_pitch, hidden);
+  REQUIRE_PTR(y); REQUIRE_ALIGNED(y);
+  REQUIRE_ALIGNED(residual);
+  dfa3d::ProductArgs a = gated_block_arguments(dtype, out_dtype, rows, in, out);
+  if (!dfa3d::gated_block_covers(a, hidden))
+    return fail(DFA3D_ERR_UNSUPPORTED, "%lld x %d -> %d -> %d is not for one kernel", (long long)rows, in, hidden, out);
+  a.a0 = {x, x_pitch};
+  a.b0 = {weight_gate, weight_pitch};
+  a.b1 = {weight_up, weight_pitch};
+  a.b2 = {weight_down, down_pitch};
+  a.in = {residual, out};
+  a.bias0 = bias_gate;
+  a.bias1 = bias_up;
+  a.act = activation;
+  a.out[0] = y;
+  return finish(dfa3d::launch_gated_block(a, hidden, bias_down, (cudaStream_t)stream), "dfa3d_gated_block_forward launch");
+}
+
 int dfa3d_gated_hidden_backward(const void *x, int64_t x_pitch, const void *weight_gate, const void *weight_up,
                                 int64_t weight_pitch, const void *bias_gate, const void *bias_up, const void *grad_y,
                                 int64_t grad_pitch, const void *weight_down, int64_t down_pitch, int32_t dtype, int64_t rows,

@@ -34,6 +34,11 @@ struct ProductArgs {
 };
 cudaError_t launch_product(const ProductArgs &a, cudaStream_t s);
 
+// The whole gated block with one kernel (dfa3d_gated_block.cu): a0 = x, b0, b1 = gate and up (hidden, k0), b2 = down (n, hidden), in =
+// residual, out[0]; bias2 of the result.  Where it is the faster one.
+bool gated_block_covers(const ProductArgs &a, int hidden);
+cudaError_t launch_gated_block(const ProductArgs &a, int hidden, const void *bias2, cudaStream_t s);
+
 // out (p, q) = g^T x over the rows of g (rows, p) and x (rows, q), bias (p) = column sums of g (or null); up to three at once.
 struct WeightProblem {
   Operand g, x;

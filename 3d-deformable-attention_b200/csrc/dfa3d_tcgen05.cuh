@@ -77,6 +77,11 @@ __device__ __forceinline__ uint32_t address_in(uint32_t at, uint32_t rank) {    
 __device__ __forceinline__ void arrive_in(uint32_t bar) {
   asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
+// The same behind writes to the own CTA's shared memory that the products of both CTAs read there: shared_to_async() has seen to these,
+// and the other CTA's threads read none of them.
+__device__ __forceinline__ void hand_over_in(uint32_t bar) {
+  asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+}
 __device__ __forceinline__ void pair_sync() {      // all threads of both
   asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }

@@ -129,6 +129,8 @@ PLAIN_ENTRY_POINTS = {
     "dfa3d_linear_act_slope": [_V, _I64, _V, _I64, _V, _V, _I64, _I32, _I32, _I64, _I32, _I32, _I32, _V, _I64, _V],
     "dfa3d_linear_input_gradient": [_V, _V, _I64, _V, _V, _I64, _V, _I64, _I32, _I64, _I32, _I32, _V, _V],
     "dfa3d_gated_hidden_forward": [_V, _I64, _V, _V, _I64, _V, _V, _I32, _I64, _I32, _I32, _I32, _V, _I64, _V],
+    "dfa3d_gated_block_supported": [_I32, _I64, _I32, _I32, _I32],
+    "dfa3d_gated_block_forward": [_V, _I64, _V, _V, _I64, _V, _V, _V, _I64, _V, _V, _I32, _I32, _I64] + [_I32] * 4 + [_V, _V],
     "dfa3d_gated_hidden_backward": [_V, _I64, _V, _V, _I64, _V, _V, _V, _I64, _V, _I64, _I32, _I64] + [_I32] * 4
                                    + [_V, _V, _V, _I64, _V],
     "dfa3d_weight_gradients_workspace": [_V, _I32, _I64],

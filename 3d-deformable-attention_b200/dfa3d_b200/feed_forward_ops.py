@@ -233,12 +233,17 @@ class GatedFeedForwardFunction(Function):
         if y.numel():
             with torch.cuda.device(x.device):
                 (xo, xp), (wg, wp), (wu, _), (wd, dp) = _operands(x.dtype, _rows(x), w_gate, w_up, w_down)
-                h, hp = _workspace(rows, F, x)
-                _lib.call_plain("dfa3d_gated_hidden_forward", xo.data_ptr(), xp, wg.data_ptr(), wu.data_ptr(), wp, _ptr(b_gate),
-                                _ptr(b_up), dt, rows, E, F, _ACTS[activation], h.data_ptr(), hp, _stream(x))
-                _lib.call_plain("dfa3d_linear_act_forward", h.data_ptr(), hp, wd.data_ptr(), dp, _ptr(b_down), _ptr(residual), dt,
-                                _lib.DTYPE_F32 if y.dtype == torch.float32 else dt, rows, F, N, _lib.ROW_NONE, y.data_ptr(),
-                                _stream(x))
+                out, st = _lib.DTYPE_F32 if y.dtype == torch.float32 else dt, _stream(x)
+                if _lib.load().dfa3d_gated_block_supported(out, rows, E, F, N) and (residual is None or residual.data_ptr() % 16 == 0):
+                    _lib.call_plain("dfa3d_gated_block_forward", xo.data_ptr(), xp, wg.data_ptr(), wu.data_ptr(), wp, _ptr(b_gate),
+                                    _ptr(b_up), wd.data_ptr(), dp, _ptr(b_down), _ptr(residual), dt, out, rows, E, F, N,
+                                    _ACTS[activation], y.data_ptr(), st)
+                else:
+                    h, hp = _workspace(rows, F, x)
+                    _lib.call_plain("dfa3d_gated_hidden_forward", xo.data_ptr(), xp, wg.data_ptr(), wu.data_ptr(), wp, _ptr(b_gate),
+                                    _ptr(b_up), dt, rows, E, F, _ACTS[activation], h.data_ptr(), hp, st)
+                    _lib.call_plain("dfa3d_linear_act_forward", h.data_ptr(), hp, wd.data_ptr(), dp, _ptr(b_down), _ptr(residual), dt,
+                                    out, rows, F, N, _lib.ROW_NONE, y.data_ptr(), st)
         if any(ctx.needs_input_grad[:7]):
             _keep_input(ctx, x, checkpoint, w_gate, w_up, w_down, b_gate, b_up)
         ctx.act, ctx.plus_x = _ACTS[activation], plus_x

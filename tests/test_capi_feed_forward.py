@@ -29,12 +29,14 @@ HIDDEN = dict(x=OK, x_pitch=16, weight_gate=OK, weight_up=OK, weight_pitch=16, b
 HIDDEN_BACK = dict(x=OK, x_pitch=16, weight_gate=OK, weight_up=OK, weight_pitch=16, bias_gate=OK, bias_up=OK, grad_y=OK, grad_pitch=32,
                    weight_down=OK, down_pitch=24, dtype=1, rows=4, cols_in=16, hidden=24, out=32, activation=2, grad_gate=OK, grad_up=OK,
                    h=OK, hidden_pitch=24, stream=None)
+BLOCK = dict(x=OK, x_pitch=16, weight_gate=OK, weight_up=OK, weight_pitch=16, bias_gate=OK, bias_up=OK, weight_down=OK, down_pitch=24,
+             bias_down=OK, residual=OK, dtype=1, out_dtype=1, rows=40000, cols_in=16, hidden=24, out=32, activation=2, y=OK, stream=None)
 PACK = dict(x=OK, dtype=1, rows=4, cols=16, format=0, codes=OK, scales=OK, stream=None)
 UNPACK = dict(codes=OK, scales=OK, format=0, rows=4, cols=16, dtype=1, x=OK, pitch=16, stream=None)
 ENTRIES = {"dfa3d_linear_act_forward": LINEAR, "dfa3d_linear_act_slope": SLOPE, "dfa3d_linear_input_gradient": INPUT,
-           "dfa3d_gated_hidden_forward": HIDDEN, "dfa3d_gated_hidden_backward": HIDDEN_BACK, "dfa3d_compress8": PACK,
+           "dfa3d_gated_hidden_forward": HIDDEN, "dfa3d_gated_hidden_backward": HIDDEN_BACK, "dfa3d_gated_block_forward": BLOCK, "dfa3d_compress8": PACK,
            "dfa3d_decompress8": UNPACK}
-PRODUCTS = list(ENTRIES)[:5]
+PRODUCTS = list(ENTRIES)[:6]
 
 
 def call(lib, name, **changed):
@@ -64,8 +66,8 @@ def test_types_widths_and_activations(lib, name):
 def test_operands(lib, name):
     """Null, off the 16-byte grid, pitches that are too short or no multiple of eight."""
     args = ENTRIES[name]
-    direct = {"bias", "residual", "y", "grad_x", "bias_gate", "bias_up", "stream"}
-    optional = {"bias", "residual", "bias_gate", "bias_up", "stream", "add"}
+    direct = {"bias", "grad_x", "bias_gate", "bias_up", "bias_down", "stream"} | (set() if "weight_down" in args else {"residual", "y"})
+    optional = {"bias", "residual", "bias_gate", "bias_up", "bias_down", "stream", "add"}
     for k in [k for k, v in args.items() if v == OK]:
         if k in ("grad2", "weight2"):
             refused(lib, call(lib, name, **{k: None}), b"together")
@@ -90,6 +92,16 @@ def test_mixed_types(lib):
     refused(lib, call(lib, "dfa3d_linear_act_forward", out_dtype=3), b"out_dtype")
     refused(lib, call(lib, "dfa3d_linear_act_slope", grad_dtype=3), b"grad_dtype")
     refused(lib, call(lib, "dfa3d_linear_act_forward", out_dtype=0, residual=OK + 2), b"aligned to its elements")
+
+
+def test_the_block_with_one_kernel(lib):
+    yes = lib.dfa3d_gated_block_supported
+    assert yes(1, 40000, 256, 512, 256) and yes(0, 40000, 8, 1, 4) and yes(3, 40000, 256, 1 << 20, 8)
+    for no in ((1, 900, 256, 512, 256), (1, 40000, 257, 512, 256), (1, 40000, 256, 512, 257), (1, 40000, 256, 512, 36), (0, 40000, 256, 512, 34),
+               (2, 40000, 256, 512, 256), (1, -1, 256, 512, 256), (1, 40000, 0, 512, 256), (1, 40000, 256, 0, 256), (1, 40000, 256, 512, 0)):
+        assert not yes(*no), no
+    refused(lib, call(lib, "dfa3d_gated_block_forward", rows=100), b"not for one kernel", -2)
+    refused(lib, call(lib, "dfa3d_gated_block_forward", out_dtype=3), b"out_dtype")
 
 
 def test_compressed(lib):

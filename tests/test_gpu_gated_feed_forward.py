@@ -140,3 +140,62 @@ def test_not_a_number_stays_in_its_rows():
     assert bad[7] and int(bad.sum()) == 1
     rows = torch.arange(300, device="cuda") != 7
     assert torch.isfinite(grads["x"][rows]).all()
+
+
+ONE_KERNEL = 9473      # rows enough for the kernel that keeps the hidden rows on the SMs (37 of 74 pairs with 256 rows each), one more
+
+
+@pytest.mark.parametrize("E,F,N", [(256, 512, 256), (256, 130, 256), (64, 128, 64), (8, 8, 8), (200, 72, 136), (136, 1000, 24), (96, 200, 248)])
+@pytest.mark.parametrize("residual", [None, "same", "wide"])
+def test_hidden_rows_that_stay_on_the_sms(lib_built, E, F, N, residual):
+    from dfa3d_b200 import _lib
+    assert _lib.load().dfa3d_gated_block_supported(_lib.DTYPE_F32, ONE_KERNEL, E, F, N)
+    d = make(ONE_KERNEL, E, F, N, torch.bfloat16, residual=residual, seed=12)
+    check(d, "gelu")
+
+
+@pytest.mark.parametrize("act", ["relu", "silu", "gelu", None])
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("bias", [True, False])
+def test_one_kernel_and_two_give_the_same_bits(lib_built, act, dtype, bias):
+    """Many rows with one kernel, few with two: a row's result depends on the row alone."""
+    import dfa3d_b200 as M
+    from dfa3d_b200 import _lib
+    d = make(40001, 128, 330, 128, dtype, bias=bias, residual="wide", seed=13)
+    assert not _lib.load().dfa3d_gated_block_supported(_lib.DTYPE_F32, 9000, 128, 330, 128)
+    f = lambda rows: M.gated_feed_forward(d["x"][rows], *(d[k] for k in NAMES[1:]), activation=act, residual=d["r"][rows])
+    whole = f(slice(None))
+    for first in range(0, 40001, 9000):
+        rows = slice(first, min(first + 9000, 40001))
+        assert torch.equal(whole[rows], f(rows))
+
+
+def test_one_kernel_on_two_streams_and_with_no_numbers(lib_built):
+    import dfa3d_b200 as M
+    jobs = [make(20000, 256, 256, 256, torch.bfloat16, residual="x", seed=s) for s in (14, 15)]
+    f = lambda d: M.gated_feed_forward(*(d[k] for k in NAMES), residual=d["x"])
+    want = [f(d) for d in jobs]
+    streams = [torch.cuda.Stream() for _ in jobs]
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream())
+    got = [[], []]
+    for _ in range(6):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i].append(f(jobs[i]))
+    torch.cuda.synchronize()
+    assert all(torch.equal(g, want[i]) for i in range(2) for g in got[i])
+    jobs[0]["x"][777, 5] = float("nan")
+    bad = ~torch.isfinite(f(jobs[0])).all(1)
+    assert bad[777] and int(bad.sum()) == 1
+
+
+@pytest.mark.parametrize("case", ["residual", "x", "weights"])
+def test_one_kernel_and_storage_off_the_grid(lib_built, case):
+    import dfa3d_b200 as M
+    d = make(ONE_KERNEL, 64, 96, 64, torch.bfloat16, residual="same", seed=16)
+    f = lambda e: M.gated_feed_forward(*(e[k] for k in NAMES), residual=e["r"])
+    want = f(d)
+    off = lambda t: torch.empty(t.numel() + 1, dtype=t.dtype, device="cuda")[1:].view_as(t).copy_(t)
+    moved = {"residual": ("r",), "x": ("x",), "weights": NAMES[1:]}[case]
+    assert torch.equal(f(dict(d, **{k: off(d[k]) for k in moved})), want)
