@@ -62,7 +62,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     }
     tc::barriers_visible();
   }
-  if (warp == 2) tc::tensor_memory_take<512, true>(where);
+  if (warp == 2) tc::tensor_memory_take<512>(where);
   tc::let_next_kernel_begin();
   tc::wait_for_last_kernel();
   tc::order_before();
@@ -157,12 +157,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
             tc::order_after();
             const uint64_t a = tc::k_major(base_a + k * kOperandA), b = tc::k_major(ring + slot * L::slot);
             if (tc::one_lane()) {
-              tc::product<true>(memory, a, b, shape, k > 0);
+              tc::product(memory, a, b, shape, k > 0);
 #pragma unroll
-              for (int i = 1; i < 4; ++i) tc::product<true>(memory, a + i * 2, b + i * 2, shape, true);
-              if (j + 1 == p.across) tc::products_arrive<true>(empty_a + k * 8);
-              tc::products_arrive<true>(empty + slot * 8);
-              if (k + 1 == p.steps) tc::products_arrive<true>(summed);
+              for (int i = 1; i < 4; ++i) tc::product(memory, a + i * 2, b + i * 2, shape, true);
+              if (j + 1 == p.across) tc::products_arrive(empty_a + k * 8);
+              tc::products_arrive(empty + slot * 8);
+              if (k + 1 == p.steps) tc::products_arrive(summed);
             }
             __syncwarp();
             next();
@@ -178,13 +178,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
             tc::order_after();
             const uint64_t a = tc::k_major(base_h + k * kOperandA), b = tc::k_major(ring + slot * L::slot);
             if (tc::one_lane()) {
-              tc::product<true>(memory + L::sums_y, a, b, shape_y, last > 0 || k > 0);
+              tc::product(memory + L::sums_y, a, b, shape_y, last > 0 || k > 0);
 #pragma unroll
-              for (int i = 1; i < 4; ++i) tc::product<true>(memory + L::sums_y, a + i * 2, b + i * 2, shape_y, true);
-              tc::products_arrive<true>(empty + slot * 8);
+              for (int i = 1; i < 4; ++i) tc::product(memory + L::sums_y, a + i * 2, b + i * 2, shape_y, true);
+              tc::products_arrive(empty + slot * 8);
               if (k + 1 == kHidden / kDepth) {
-                tc::products_arrive<true>(h_empty);
-                if (last + 1 == p.across) tc::products_arrive<true>(y_full);
+                tc::products_arrive(h_empty);
+                if (last + 1 == p.across) tc::products_arrive(y_full);
               }
             }
             __syncwarp();
@@ -195,7 +195,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         last = j;
         if (++j == p.across) j = 0;
       }
-      if (tc::one_lane()) tc::products_arrive<true>(quiet);
+      if (tc::one_lane()) tc::products_arrive(quiet);
       __syncwarp();
     }
     tc::wait_warp(quiet, 0);
@@ -340,7 +340,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   tc::pair_sync();      // the other CTA's products read this one's shared memory, its warps arrive at this one's barriers
   if (warp == 2) {
     tc::order_after();
-    tc::tensor_memory_give<512, true>(memory);
+    tc::tensor_memory_give<512>(memory);
   }
 }
 

@@ -159,7 +159,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Tile<KIND, I, O, BN,
     }
     tc::barriers_visible();
   }
-  if (warp == 2) tc::tensor_memory_take<L::memory, true>(where);
+  if (warp == 2) tc::tensor_memory_take<L::memory>(where);
   const Place first(first_tile, p.tiles_n);
   tc::let_next_kernel_begin();
   tc::wait_for_last_kernel();
@@ -304,16 +304,16 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Tile<KIND, I, O, BN,
             const uint64_t a = tc::k_major(at_a);
             const uint64_t b = narrow_b ? tc::mn_major_narrow(at_b) : mn ? tc::mn_major(at_b, kDepth * 128) : tc::k_major(at_b);
             if (tc::one_lane()) {
-              tc::product<true>(d, a, b, form, k > from);
+              tc::product(d, a, b, form, k > from);
 #pragma unroll
               for (int j = 1; j < PER * (kDepth / 16); ++j) {
                 const int step = j / (kDepth / 16), part = j % (kDepth / 16);
                 if (step < count)
-                  tc::product<true>(d, a + step * (kOperandA / 16) + part * 2, b + step * (bytes_b / 16) + part * step_b, form, true);
+                  tc::product(d, a + step * (kOperandA / 16) + part * 2, b + step * (bytes_b / 16) + part * step_b, form, true);
               }
               if (RESIDENT && last)
-                for (int j = 0; j < count; ++j) tc::products_arrive<true>(empty_a + (k + j) * 8);
-              tc::products_arrive<true>(empty + at_ring * 8);
+                for (int j = 0; j < count; ++j) tc::products_arrive(empty_a + (k + j) * 8);
+              tc::products_arrive(empty + at_ring * 8);
             }
             __syncwarp();
             if (++at_ring == L::slots) {
@@ -329,14 +329,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Tile<KIND, I, O, BN,
           sum(std::false_type(), 0, steps, acc);
         }
         if (last) phase_a ^= 1;
-        if (ok && tc::one_lane()) tc::products_arrive<true>(summed + slot * 8);
+        if (ok && tc::one_lane()) tc::products_arrive(summed + slot * 8);
         __syncwarp();
         if (++slot == L::depth) {
           slot = 0;
           round ^= 1;
         }
       }
-      if (tc::one_lane()) tc::products_arrive<true>(quiet);
+      if (tc::one_lane()) tc::products_arrive(quiet);
       __syncwarp();
     }
     tc::wait_warp(quiet, 0);
@@ -505,7 +505,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Tile<KIND, I, O, BN,
   tc::pair_sync();      // the other CTA's products read this one's shared memory, its warps arrive at this one's barriers
   if (warp == 2) {
     tc::order_after();
-    tc::tensor_memory_give<L::memory, true>(memory);
+    tc::tensor_memory_give<L::memory>(memory);
   }
 }
 

@@ -92,9 +92,6 @@ __device__ __forceinline__ void wait_for_last_kernel() { asm volatile("griddepco
 __device__ __forceinline__ void let_next_kernel_begin() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 
 // ---- tiled copies ------------------------------------------------------------------------------
-__device__ __forceinline__ void fetch_map(const CUtensorMap *map) {
-  asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory");
-}
 __device__ __forceinline__ void tile_load(uint32_t dst, const CUtensorMap *map, int x, int y, uint32_t bar) {
   asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(dst),
                "l"(map), "r"(x), "r"(y), "r"(bar)
@@ -123,20 +120,14 @@ __device__ __forceinline__ void stores_done() { asm volatile("cp.async.bulk.wait
 __device__ __forceinline__ void shared_to_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
 // ---- tensor memory -----------------------------------------------------------------------------
-// PAIR: by one warp of each of the pair's CTAs, for products of both.
-template <int COLUMNS, bool PAIR> __device__ __forceinline__ void tensor_memory_take(uint32_t where) {      // one whole warp
+// By one warp of each of the pair's CTAs, for products of both.
+template <int COLUMNS> __device__ __forceinline__ void tensor_memory_take(uint32_t where) {
   static_assert(COLUMNS >= 32 && COLUMNS <= 512 && (COLUMNS & (COLUMNS - 1)) == 0, "power of two");
-  if constexpr (PAIR) {
-    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(where), "n"(COLUMNS) : "memory");
-    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;");
-  } else {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(where), "n"(COLUMNS) : "memory");
-    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
-  }
+  asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(where), "n"(COLUMNS) : "memory");
+  asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;");
 }
-template <int COLUMNS, bool PAIR> __device__ __forceinline__ void tensor_memory_give(uint32_t base) {       // the same warp
-  if constexpr (PAIR) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(base), "n"(COLUMNS));
-  else asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(base), "n"(COLUMNS));
+template <int COLUMNS> __device__ __forceinline__ void tensor_memory_give(uint32_t base) {       // the same warp
+  asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(base), "n"(COLUMNS));
 }
 __device__ __forceinline__ void order_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void order_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
@@ -195,30 +186,23 @@ __device__ __forceinline__ uint64_t mn_major(uint32_t at, uint32_t group) {
 __device__ __forceinline__ uint64_t mn_major_narrow(uint32_t at) { return kNarrowBits | (uint64_t(1) << 16) | ((at >> 4) & 0x3fff); }
 template <typename T> constexpr uint32_t kOperandType = 0;                     // fp16
 template <> inline constexpr uint32_t kOperandType<__nv_bfloat16> = 1;
-// 128 rows, or 256 of a pair; n columns; 32-bit sums
+// the pair's 256 rows; n columns; 32-bit sums
 template <typename T> __host__ __device__ constexpr uint32_t product_shape(int rows, int n, bool a_mn_major, bool b_mn_major) {
   return (1u << 4) | (kOperandType<T> << 7) | (kOperandType<T> << 10) | (uint32_t(a_mn_major) << 15) | (uint32_t(b_mn_major) << 16) |
          (uint32_t(n / 8) << 17) | (uint32_t(rows / 16) << 24);
 }
-// D (+)= A B over 16 elements of the summed axis; one thread.  PAIR: of the pair's first CTA; each CTA holds its 128 rows of A and of
-// D and half of B's columns, all at the same places.
-template <bool PAIR> __device__ __forceinline__ void product(uint32_t d, uint64_t a, uint64_t b, uint32_t shape, bool add) {
-  if constexpr (PAIR)
-    asm volatile("{\n.reg .pred q;\nsetp.ne.u32 q, %4, 0;\ntcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, q;\n}" ::"r"(d),
-                 "l"(a), "l"(b), "r"(shape), "r"((uint32_t)add)
-                 : "memory");
-  else
-    asm volatile("{\n.reg .pred q;\nsetp.ne.u32 q, %4, 0;\ntcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, q;\n}" ::"r"(d),
-                 "l"(a), "l"(b), "r"(shape), "r"((uint32_t)add)
-                 : "memory");
+// D (+)= A B over 16 elements of the summed axis; one thread of the pair's first CTA.  Each CTA holds its 128 rows of A and of D and half
+// of B's columns, all at the same places.
+__device__ __forceinline__ void product(uint32_t d, uint64_t a, uint64_t b, uint32_t shape, bool add) {
+  asm volatile("{\n.reg .pred q;\nsetp.ne.u32 q, %4, 0;\ntcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, q;\n}" ::"r"(d), "l"(a),
+               "l"(b), "r"(shape), "r"((uint32_t)add)
+               : "memory");
 }
-// The barrier (PAIR: of both CTAs) is arrived at when the products that this thread has issued so far are done.
-template <bool PAIR> __device__ __forceinline__ void products_arrive(uint32_t bar) {
-  if constexpr (PAIR)
-    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar),
-                 "h"((uint16_t)3)
-                 : "memory");
-  else asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+// The barrier of both CTAs is arrived at when the products that this thread has issued so far are done.
+__device__ __forceinline__ void products_arrive(uint32_t bar) {
+  asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar),
+               "h"((uint16_t)3)
+               : "memory");
 }
 
 // ---- shared memory by address ------------------------------------------------------------------

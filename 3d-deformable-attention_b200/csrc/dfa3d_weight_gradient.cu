@@ -68,7 +68,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads8, 1) weight
     tc::barrier_init(quiet, 1);
     tc::barriers_visible();
   }
-  if (warp == 2) tc::tensor_memory_take<L::memory, true>(where);
+  if (warp == 2) tc::tensor_memory_take<L::memory>(where);
   if (warp >= 4) {      // the same whatever the layout
     const T one = narrow<T>(1.f);
     const uint32_t two = (uint32_t)reinterpret_cast<const uint16_t &>(one) * 0x10001u;
@@ -130,10 +130,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads8, 1) weight
         if (tc::one_lane()) {
 #pragma unroll
           for (int j = 0; j < kDepth / 16; ++j) {
-            tc::product<true>(memory, a + j * (2048 / 16), b + j * step_b, shape, k > begin || j > 0);
-            if (bias) tc::product<true>(memory + BN, a + j * (2048 / 16), tc::k_major(ones), shape_ones, k > begin || j > 0);
+            tc::product(memory, a + j * (2048 / 16), b + j * step_b, shape, k > begin || j > 0);
+            if (bias) tc::product(memory + BN, a + j * (2048 / 16), tc::k_major(ones), shape_ones, k > begin || j > 0);
           }
-          tc::products_arrive<true>(empty + s * 8);
+          tc::products_arrive(empty + s * 8);
         }
         __syncwarp();
         if (++s == L::stages) {
@@ -142,8 +142,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads8, 1) weight
         }
       }
       if (tc::one_lane()) {
-        if (ok) tc::products_arrive<true>(done);
-        tc::products_arrive<true>(quiet);
+        if (ok) tc::products_arrive(done);
+        tc::products_arrive(quiet);
       }
       __syncwarp();
     }
@@ -177,7 +177,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads8, 1) weight
   tc::pair_sync();
   if (warp == 2) {
     tc::order_after();
-    tc::tensor_memory_give<L::memory, true>(memory);
+    tc::tensor_memory_give<L::memory>(memory);
   }
 }
 
