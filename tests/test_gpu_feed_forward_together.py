@@ -302,3 +302,75 @@ def test_activation_checkpoints_of_a_layer(lib_built):
     # the rest of the layer adds up in an order that is not fixed
     for a, b in zip(*results):
         torch.testing.assert_close(a, b, rtol=2e-2, atol=2e-2 * float(b.abs().max()))
+
+
+@pytest.mark.parametrize("kind", KINDS)
+def test_captured_behind_a_join(lib_built, kind):
+    """The kernels may begin before the one in front of them ends: not before either of two that they follow."""
+    f, leaves = call(kind, rows=3000, E=136, F=200)
+    go = torch.randn(f().shape, generator=torch.Generator().manual_seed(9)).to(DEV).to(f().dtype)
+    base = [t.detach().clone() for t in leaves]
+    side = torch.cuda.Stream()
+
+    def run():
+        here = torch.cuda.current_stream()
+        side.wait_stream(here)
+        with torch.no_grad():
+            leaves[0].copy_(base[0] * 2 - base[0])                      # what the call reads, written on both streams
+            with torch.cuda.stream(side):
+                for t, b in zip(leaves[1:], base[1:]):
+                    t.copy_(b * 2 - b)
+        here.wait_stream(side)
+        out = grads_of(f, leaves, go)
+        with torch.no_grad():
+            for t in leaves:                                            # behind it: the call has read all of it
+                t.fill_(float("nan"))
+        return out
+
+    want = run()
+    with torch.no_grad():
+        for t, b in zip(leaves, base):
+            t.copy_(b)
+    assert equal(want, grads_of(f, leaves, go))
+    warm = torch.cuda.Stream()
+    warm.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(warm):
+        run()
+    torch.cuda.current_stream().wait_stream(warm)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = run()
+    for _ in range(5):
+        graph.replay()
+        assert equal(out, want)
+
+
+@BOTH
+def test_shared_and_broadcast_inputs(lib_built, native):
+    """One tensor in several places, and rows that are one row: gradients add up."""
+    g = torch.Generator().manual_seed(4)
+    n = lambda *s: torch.randn(*s, generator=g).bfloat16().to(DEV)
+    row, w, wd, b, go = n(1, 40), n(56, 40), n(40, 56), n(56), n(70, 40)
+    linear, gated = (f if native else _python(f) for f in (LinearActFunction, GatedFeedForwardFunction))
+    leaves = [t.clone().requires_grad_(True) for t in (row, w, wd, b)]
+    x = leaves[0].expand(70, 40)
+    y = gated.apply(x, leaves[1], leaves[1], leaves[2], leaves[3], leaves[3], None, x, False, "silu", None)
+    got = torch.autograd.grad(y, leaves, go)
+    apart = [t.clone().requires_grad_(True) for t in (row.expand(70, 40), w, w, wd, b, b, row.expand(70, 40))]
+    z = gated.apply(*apart[:6], None, apart[6], False, "silu", None)
+    each = torch.autograd.grad(z, apart, go)
+    assert torch.equal(y, z)
+    # two gradients added once in 16 bits; 140 of them added up in 32 and rounded once (2^-8 each, the second of what the first
+    # has rounded)
+    assert torch.equal(got[1], each[1] + each[2]) and torch.equal(got[2], each[3]) and torch.equal(got[3], each[4] + each[5])
+    total = each[0].double() + each[6].double()
+    assert ((got[0].double() - total.sum(0)).abs() <= 1.01 * 2 ** -8 * (total.abs().sum(0) + total.sum(0).abs())).all()
+    square = n(64, 64).requires_grad_(True)
+    y = linear.apply(square, square, None, square, "gelu", None)
+    go = n(64, 64)
+    got, = torch.autograd.grad(y, square, go)
+    three = [square.detach().clone().requires_grad_(True) for _ in range(3)]
+    each = torch.autograd.grad(linear.apply(three[0], three[1], None, three[2], "gelu", None), three, go)
+    total = sum(t.double() for t in each)
+    # two sums in 16 bits, half a step each of at most the terms' magnitudes
+    assert ((got.double() - total).abs() <= 1.01 * 2 * 2 ** -8 * sum(t.double().abs() for t in each)).all()
