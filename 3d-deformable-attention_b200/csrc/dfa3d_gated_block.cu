@@ -6,6 +6,13 @@
 // tensor memory, sixteen warps read them at once, so that the next ones may be summed, and turn them into hidden rows in shared memory,
 // which are the operand of the next product, summed in the other half over all hidden columns.  The products of one item and the sums of
 // the next are issued in turn, so that the tensor cores sum while the warps work; a result is read while the next rows begin.
+//
+// Measured behind a flush of L2, bf16, SiLU, a 16-bit residual, against the two kernels: 40 000 rows 256 -> 512 -> 256 45.1 us to 47.1,
+// 30 000 rows 34.8 to 41.0, 80 000 rows 67.6 to 75.8; 80 000 rows 256 -> 1024 -> 256 119 to 139; on calls that follow one another 38.7 to
+// 42.5, 27.9 to 34.7, 60.8 to 74.4, 106 to 138.  The floor of the first is 31.5 GFLOP, 20 us at 1.6 PFLOP/s.  What binds is the chain
+// of an item -- products, 32 columns of math a warp, hand-over -- of about 3900 cycles, and 5200 between the rows of two tiles, where
+// a warp's chunks of the result go through one slab one after the other: two slabs a warp leave three slots of the ring instead of
+// five, which cost wide blocks 10 %.
 #include "dfa3d_common.cuh"
 #include "dfa3d_epilogue.cuh"
 #include "dfa3d_product.h"
@@ -384,7 +391,12 @@ bool gated_block_covers(const ProductArgs &a, int hidden) {
   const int size = a.wide ? 4 : 2;
   auto fits = [&](const void *q, long long pitch) { return (reinterpret_cast<uintptr_t>(q) & 15u) == 0 && pitch * size % 16 == 0; };
   if (a.k0 > kStepsA * kDepth || a.n > 256 || !fits(a.out[0], a.out_pitch) || (a.in.data && !fits(a.in.data, a.in.pitch))) return false;
-  return (a.rows + 2 * kRows - 1) / (2 * kRows) * 2 >= sm_count() / 2;
+  // What of the time of the busiest pair of SMs the average one has work for: the two kernels' tiles are narrower and divide more evenly.
+  // At 38 row tiles for 74 pairs one kernel takes 0.75 to 0.87 of the two kernels' time up to 512 hidden columns, 0.86 to 0.9 with 1024
+  // and 0.95 to 1.05 with 2048; at 75 tiles 0.93 to 1.0, but with 1024 and 2048, where a tile takes longer, 1.04 to 1.17, at 86 tiles
+  // then 0.9 to 1.1, at 118 0.8 to 0.95.
+  const long long tiles = (a.rows + 2 * kRows - 1) / (2 * kRows), pairs = sm_count() / 2, rounds = (tiles + pairs - 1) / pairs;
+  return tiles * 10 >= rounds * pairs * (rounds > 1 && hidden > 512 ? 6 : 5);
 }
 
 cudaError_t launch_gated_block(const ProductArgs &a, int hidden, const void *bias2, cudaStream_t s) {

@@ -7,6 +7,17 @@
 // along the summed axis (tiled copies into rings), one thread of the pair issues the products, whose 32-bit sums stay in tensor
 // memory, two to four tiles at a time, so that the next tile is summed while the other warps read the last one, apply bias,
 // activation, residual or derivatives in 32 bits, round once and hand rows to tiled stores.
+//
+// Measured on calls that follow one another, bf16, 40 000 rows between 256 and 512 columns (10.5 GFLOP a product, 7 us at 1.6 PFLOP/s;
+// 61 MB, the 41 MB of a result of 512 columns 10.5 us at the 3.9 TB/s at which writes end):
+//   256 -> 512: 15.9 us; with GELU 23.7; its derivative times a gradient 30.9.   512 -> 256: 14.9; with a residual of 16 bits 17.3,
+//   of 32 bits 27.7.   Input gradients: 14.9, of two products at once 30.2.   Gated hidden rows with SiLU 25, with GELU 29; their three
+//   backward results, 123 MB, 45.7 and 50.
+// Without an activation the writes bind; with one the epilogue's instructions (GELU 17.5 cycles a warp and 32 elements, SiLU 12.5),
+// of which a warp scheduler issues on 40 of 100 cycles between its waits for tensor memory and slabs.
+//
+// Gradients are rounded to 16 bits behind an activation's derivative, once: they are operands of the next products, and the bias
+// gradient is the sum of what those read.
 #include <type_traits>
 
 #include "dfa3d_common.cuh"

@@ -502,8 +502,8 @@ int dfa3d_gated_hidden_forward(const void *x, int64_t x_pitch, const void *weigh
 /* The whole gated block with one kernel: y (rows, out) = (act(x Wg^T + bg) * (x Wu^T + bu)) Wd^T + bd + residual, weight_down
  * (out, hidden); any bias and residual may be null.  The hidden rows, rounded to dtype as between the two kernels, do not reach
  * memory.  out_dtype (of residual and y): dtype or DFA3D_DTYPE_F32; both 16-byte aligned.  Only where dfa3d_gated_block_supported() is
- * not 0 (up to 256 columns in and out, rows of a multiple of 16 bytes, rows enough for half of the SMs); others: dfa3d_gated_hidden_forward
- * and dfa3d_linear_act_forward. */
+ * not 0 (up to 256 columns in and out, rows of a multiple of 16 bytes, rows that keep at least half of the SMs busy); others:
+ * dfa3d_gated_hidden_forward and dfa3d_linear_act_forward. */
 int dfa3d_gated_block_supported(int32_t out_dtype, int64_t rows, int32_t in, int32_t hidden, int32_t out);
 int dfa3d_gated_block_forward(const void *x, int64_t x_pitch, const void *weight_gate, const void *weight_up, int64_t weight_pitch,
                               const void *bias_gate, const void *bias_up, const void *weight_down, int64_t down_pitch,

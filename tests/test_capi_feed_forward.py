@@ -187,3 +187,13 @@ def test_python_refuses_other_tensors(lib_built):
     with pytest.raises(RuntimeError, match="on one CUDA device"):
         from dfa3d_b200.checkpoint_ops import Compressed8
         M.decompress8(Compressed8(torch.zeros(4, 16, dtype=torch.uint8), torch.zeros(4, 1, dtype=torch.uint8), x.shape, x.dtype, "int8"))
+
+
+def test_one_kernel_where_its_rows_divide_evenly(lib):
+    """Tiles of 256 rows over pairs of SMs; without a device as many as this GPU has."""
+    yes = lib.dfa3d_gated_block_supported
+    for hidden in (512, 513):
+        for rows in (9473, 18944, 30000, 40000, 80000):
+            assert yes(1, rows, 256, hidden, 256), (rows, hidden)
+        assert not yes(1, 9000, 256, hidden, 256)
+    assert yes(1, 18945, 256, 512, 256) and not yes(1, 18945, 256, 513, 256) and not yes(1, 22000, 256, 513, 256)
