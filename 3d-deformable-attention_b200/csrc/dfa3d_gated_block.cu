@@ -44,7 +44,7 @@ template <typename O, int BN> struct Block {
   static constexpr int sums_y = 2 * kHidden;                                   // tensor memory: gate and up, then the result
   static constexpr int barriers = 2 * kStepsA + 2 * slots + 4 + 2 + kWarps + 1;
   static constexpr int bytes = kStepsA * kOperandA + hidden + slots * slot + kWarps * (slab + bias) + barriers * 8 + 16;
-  static_assert(bytes <= 227 * 1024 && down_bytes <= slot && chunks >= 1, "layout");
+  static_assert(one_an_sm(bytes) && bytes <= 227 * 1024 && down_bytes <= slot && chunks >= 1, "layout");
 };
 
 template <typename T, typename O, int BN>

@@ -80,7 +80,7 @@ template <ProductKind KIND, typename I, typename O, int BN, bool RESIDENT> struc
   static constexpr int bytes = slots_a * kOperandA + slots * slot + slabs + bias + barriers * 8 + 16;
   // whoever reads an accumulator reads it every time, or it would take one phase of its barrier for another
   static_assert(depth % turns == 0 && (chunks <= takers ? takers % chunks : chunks % takers) == 0 && part % sub == 0, "turns");
-  static_assert(bytes <= 227 * 1024 && slots >= 3 && (row_bytes == 64 || row_bytes == 128) && chunks >= 1, "layout");
+  static_assert(one_an_sm(bytes) && bytes <= 227 * 1024 && slots >= 3 && (row_bytes == 64 || row_bytes == 128) && chunks >= 1, "layout");
 };
 
 // What a warp of a direct product does instead of tiled copies: rows between a slab and memory, neighbours by neighbouring lanes, a

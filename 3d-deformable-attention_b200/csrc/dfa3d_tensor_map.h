@@ -48,6 +48,10 @@ inline bool describe_matrix(CUtensorMap &map, int dtype, const void *data, long 
                           CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+// Two CTAs of these kernels on one SM, each of a pair that holds tensor memory on the other one's second SM, would wait for each other:
+// each takes more than half of an SM's shared memory.
+constexpr bool one_an_sm(int bytes) { return 2 * (bytes + 1024) > 228 * 1024; }
+
 // Shared memory beyond 48 KB is a setting of a kernel on a device, made once for each of the first 64.
 template <auto KERNEL> cudaError_t allow_shared(int bytes) {
   static std::atomic<unsigned long long> done{0};

@@ -40,7 +40,7 @@ template <int BN> struct Grad {
   static constexpr int memory = BN == 256 ? 512 : BN == 128 ? 256 : 128;
   static constexpr int bytes = stages * stage + ones + (2 * stages + 2) * 8 + 16;
   static constexpr int columns = BN + 1;
-  static_assert(bytes <= 227 * 1024, "layout");
+  static_assert(one_an_sm(bytes) && bytes <= 227 * 1024, "layout");
 };
 
 __device__ __forceinline__ int problem_of(const Problems &w, int tile) {
