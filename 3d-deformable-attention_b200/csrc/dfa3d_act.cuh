@@ -62,17 +62,21 @@ __device__ __forceinline__ Two sigmoid(Two z) {
 // where the sigmoid is 2^-60, z as far as it counts: z sigmoid(z) goes to 0 there, and not to -infinity
 __device__ __forceinline__ Two counted(Two z) { return {no_less(z.x, -42.f), no_less(z.y, -42.f)}; }
 
-// The normal distribution's P(X <= z) = erfc(-z / sqrt 2) / 2 and exp(-z^2 / 2).  With t = 1 / (1 + 0.3275911 x),
-// erfc(x) = exp(-x^2) (a1 t + ... + a5 t^5), |error| <= 1.5e-7, for x >= 0 (Abramowitz and Stegun, Handbook of Mathematical
-// Functions, 7.1.26); on the negative side the factor exp(-x^2) keeps the tail's relative error small too.
+// The normal distribution's P(X <= z) and exp(-z^2 / 2).  P(X <= -|z|) = exp(-z^2 / 2) R(|z|) with R(|z|) = erfcx(|z| / sqrt 2) / 2, which
+// falls as 1 / |z| and is a polynomial of t = 1 / (1 + 0.365 |z| / sqrt 2) without a constant term: seven terms, fitted to the
+// definition on 0 <= |z| <= 13.5 for the least largest error (a linear program over 1200 points), each error counted against the
+// larger of what 3e-8 of the probability and 2^-18.7 of R are.  So the tail is right relative to itself: with the roundings 4e-6 up
+// to |z| = 6 and 1e-5 up to 13, where 32 bits end; an error bound of the probability alone leaves 1 % at 8.
 __device__ __forceinline__ Two normal_cdf(Two z, Two &bell) {
   bell = power_of_two(z * z * both(-0.72134752044448170f));
   const Two far{fminf(fabsf(z.x), 1e8f), fminf(fabsf(z.y), 1e8f)};
-  const Two t = reciprocal(times_plus(far, both(0.3275911f * 0.70710678118654752f), both(1.f)));
-  Two w = times_plus(t, both(0.5f * 1.061405429f), both(0.5f * -1.453152027f));
-  w = times_plus(t, w, both(0.5f * 1.421413741f));
-  w = times_plus(t, w, both(0.5f * -0.284496736f));
-  w = times_plus(t, w, both(0.5f * 0.254829592f));
+  const Two t = reciprocal(times_plus(far, both(0.365f * 0.70710678118654752f), both(1.f)));
+  Two w = times_plus(t, both(-0.076127111f), both(0.247021068f));
+  w = times_plus(t, w, both(-0.129819675f));
+  w = times_plus(t, w, both(0.181564439f));
+  w = times_plus(t, w, both(0.067287249f));
+  w = times_plus(t, w, both(0.107386443f));
+  w = times_plus(t, w, both(0.102687557f));
   w = w * (t * bell);
   const Two v = times_plus(w, both(-1.f), both(1.f));
   return {z.x < 0.f ? w.x : v.x, z.y < 0.f ? w.y : v.y};
