@@ -53,14 +53,15 @@ __device__ __forceinline__ Two reciprocal(Two a) {      // of numbers from 1 to 
   return {r * a.y, r * a.x};
 }
 
-// 1 / (1 + exp(-z)), and 2^-60 below -41.6
+// e^z / (1 + e^z), 1 from 2^60 on: on the negative side as right relative to itself as e^z is, down to where 32 bits end
 __device__ __forceinline__ Two sigmoid(Two z) {
-  Two q = z * both(-1.4426950408889634f);
+  Two q = z * both(1.4426950408889634f);
   q = {fminf(q.x, 60.f), fminf(q.y, 60.f)};
-  return reciprocal(power_of_two(q) + both(1.f));
+  const Two e = power_of_two(q);
+  return e * reciprocal(e + both(1.f));
 }
-// where the sigmoid is 2^-60, z as far as it counts: z sigmoid(z) goes to 0 there, and not to -infinity
-__device__ __forceinline__ Two counted(Two z) { return {no_less(z.x, -42.f), no_less(z.y, -42.f)}; }
+// z as far as it counts: z sigmoid(z) is 0 at -infinity
+__device__ __forceinline__ Two counted(Two z) { return {no_less(z.x, -1e30f), no_less(z.y, -1e30f)}; }
 
 // The normal distribution's P(X <= z) and exp(-z^2 / 2).  P(X <= -|z|) = exp(-z^2 / 2) R(|z|) with R(|z|) = erfcx(|z| / sqrt 2) / 2, which
 // falls as 1 / |z| and is a polynomial of t = 1 / (1 + 0.365 |z| / sqrt 2) without a constant term: seven terms, fitted to the

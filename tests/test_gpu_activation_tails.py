@@ -3,9 +3,10 @@ the activation's value there, not a number of the same smallness.
 
 z passes through a product with the identity, exactly; with a float32 residual of zeros the activation is seen in 32 bits.
 
-Bounds, relative, with U = 2^-24 the rounding of one operation.  Exponential 2^-22, reciprocal 2^-23.
+Bounds, relative, with U = 2^-24 the rounding of one operation.  SiLU, z e^z / (1 + e^z): the exponent's argument is off by 2 U |A|,
+A = z log2 e, which moves e^z by ln 2 times as much, 2 U |z|; exponential 2^-22, reciprocal 2^-23, six roundings: below 2^-20 in all.
 GELU, z P(X <= z), for z < 0 a factor exp(-z^2 / 2) whose argument is off by 3 U |A|, A = z^2 / 2 log2 e: 1.5 U z^2; a polynomial
-that is fitted to 2^-18, nine of its terms' roundings, exponential and reciprocal: below 2^-17.  Results below 2^-118 come from
+that is fitted to 2^-18, nine of its terms' roundings, exponential and reciprocal as above: below 2^-17.  Results below 2^-118 come from
 an exponential that ends at 2^-126."""
 import math
 
@@ -30,6 +31,12 @@ def numbers(dtype, most):
 def definition(z, act):
     """Value, derivative, and the bounds of both."""
     v = z.double()
+    if act == "silu":
+        s, far = torch.sigmoid(v), 1 / (1 + torch.exp(v))          # far = 1 - s
+        a, d = v * s, s * (1 + v * far)
+        rel = 2.0 ** -20 + 2 * U * v.abs()
+        # the derivative's 1 - s is off by what s is off by
+        return a, d, rel * a.abs() + END, rel * (s + a.abs() * far) + a.abs() * 2.0 ** -21 + END
     p = 0.5 * torch.special.erfc(-v / math.sqrt(2))
     bell = v * torch.exp(-0.5 * v * v) / math.sqrt(2 * math.pi)
     rel = 2.0 ** -17 + 1.5 * U * v * v
@@ -49,7 +56,7 @@ def run(z, act, wide):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
-@pytest.mark.parametrize("act,most", [("gelu", 40.0)])
+@pytest.mark.parametrize("act,most", [("silu", 300.0), ("gelu", 40.0)])
 def test_every_number(lib_built, dtype, act, most):
     z = numbers(dtype, most)
     a, d, ea, ed = definition(z, act)
@@ -62,7 +69,7 @@ def test_every_number(lib_built, dtype, act, most):
     assert_within("16-bit y", y, a.cpu(), stored(a, ea))
 
 
-@pytest.mark.parametrize("act", ["gelu"])
+@pytest.mark.parametrize("act", ["silu", "gelu"])
 def test_far_on_the_negative_side_nothing_is_left(lib_built, act):
     """Where the value is below what 32 bits hold it is 0."""
     z = -torch.logspace(2.5, 30, 64, device="cuda").bfloat16().view(8, 8)
@@ -70,7 +77,7 @@ def test_far_on_the_negative_side_nothing_is_left(lib_built, act):
     assert (y == 0).all() and (g == 0).all()
 
 
-@pytest.mark.parametrize("act", ["gelu"])
+@pytest.mark.parametrize("act", ["silu", "gelu"])
 def test_gate_times_large_up(lib_built, act):
     """A gate far out in the tail closes whatever it stands before: act(gate) up is right relative to itself."""
     import dfa3d_b200 as M
