@@ -454,14 +454,18 @@ def _run_ffn(ffn, x):
 
 def _ffn_norm(ffn, norm, x, seed):
     """``norm(ffn(x), x)``; where the block is the layers' own with CounterDropouts, the first dropout is run with the first
-    product and the second one inside the norm.  The gated block adds x itself, or leaves it to the norm where a dropout comes first."""
+    product and the second one inside the norm.  The gated block adds x itself, or leaves it to the norm where a dropout comes first;
+    with hooks it is called with x as its residual too.  What another block returns in fewer bits than x is widened for the norm."""
     if type(ffn) is GatedFeedForward and runs_forward_only(ffn):
         if not ffn.drops():
             return norm(ffn.branch(x, x))
         return dropout_norm(ffn.branch(x).to(x.dtype), x, ffn.dropout, norm, seed, 3)
+    if isinstance(ffn, GatedFeedForward) and type(ffn).forward is GatedFeedForward.forward and "forward" not in ffn.__dict__:
+        return norm(ffn(x, x))
     if type(ffn) is not nn.Sequential or len(ffn) != 5 or not runs_forward_only(ffn) or type(ffn[2]) is not CounterDropout \
             or type(ffn[4]) is not CounterDropout:
-        return norm(_run_ffn(ffn, x), x)
+        y = _run_ffn(ffn, x)
+        return norm(y.to(torch.promote_types(y.dtype, x.dtype)), x)
     h = linear_relu_dropout(x, ffn[0], ffn[1], ffn[2], seed, 2)
     return dropout_norm(ffn[3](h), x, ffn[4], norm, seed, 3)
 
