@@ -317,6 +317,12 @@ class _Computed(nn.Module):
         return x.dtype if x.dtype in _DTYPES else self.compute_dtype
 
 
+def _plain_product(m):
+    """Whether calling m is a product with its weight and bias and nothing else."""
+    return (type(m).forward is nn.Linear.forward or (type(m).forward is LinearAct.forward and m.activation is None)) \
+        and runs_forward_only(m)
+
+
 def _to(t, dtype):
     return None if t is None else t.to(dtype)
 
@@ -333,15 +339,20 @@ class LinearAct(nn.Linear, _Computed):
         return linear_act(x.to(dt), self.weight.to(dt), _to(self.bias, dt), self.activation, residual, self.checkpoint)
 
 
+_PLAIN_ACTS = {None: lambda z: z, "relu": torch.relu, "silu": nn.functional.silu, "gelu": nn.functional.gelu}
+
+
 class GatedFeedForward(_Computed):
-    """``dropout((act(gate(x)) * up(x)) down) [+ residual]`` on ``gated_feed_forward``.  A float32 residual is added unrounded."""
+    """``dropout((act(gate(x)) * up(x)) down) [+ residual]`` on ``gated_feed_forward``.  A float32 residual is added unrounded.  Where
+    ``gate``, ``up`` or ``down`` is more than a product with its parameters (hooks on it, a module that has replaced it), the three are
+    called one by one instead: their results are rounded in between too, and they keep their inputs whole."""
 
     def __init__(self, embed_dims, hidden_dims, activation="silu", bias=True, dropout=0.0, counter_dropout=False, checkpoint=None,
                  compute_dtype=torch.bfloat16):
         super().__init__()
-        self.gate = nn.Linear(embed_dims, hidden_dims, bias)
-        self.up = nn.Linear(embed_dims, hidden_dims, bias)
-        self.down = nn.Linear(hidden_dims, embed_dims, bias)
+        self.gate = LinearAct(embed_dims, hidden_dims, bias)
+        self.up = LinearAct(embed_dims, hidden_dims, bias)
+        self.down = LinearAct(hidden_dims, embed_dims, bias)
         self.dropout = CounterDropout(dropout) if counter_dropout else nn.Dropout(dropout)
         self.activation, self.checkpoint, self.compute_dtype = activation, checkpoint, compute_dtype
 
@@ -349,10 +360,19 @@ class GatedFeedForward(_Computed):
         """Whether the dropout does anything, so that the residual has to wait for it."""
         return not runs_forward_only(self.dropout) or (self.dropout.training and self.dropout.p > 0)
 
+    def _one_by_one(self, x, residual):
+        if self.activation not in _ACTS:
+            raise ValueError(f"activation must be one of {list(_ACTS)}, got {self.activation!r}")
+        h = _PLAIN_ACTS[self.activation](self.gate(x).float()) * self.up(x).float()
+        y = self.down(h.to(x.dtype))
+        return y if residual is None else residual + y
+
     def branch(self, x, residual=None):
         """The block without its dropout."""
         dt = self._type(x)
         narrow = x.to(dt)
+        if not all(_plain_product(m) for m in (self.gate, self.up, self.down)):
+            return self._one_by_one(narrow, residual)
         w = [t for m in (self.gate, self.up, self.down) for t in (m.weight.to(dt), _to(m.bias, dt))]
         return gated_feed_forward(narrow, w[0], w[2], w[4], w[1], w[3], w[5], self.activation,
                                   narrow if residual is x and narrow is x else residual, self.checkpoint)
