@@ -238,9 +238,15 @@ void keep(AutogradContext *ctx, const c10::intrusive_ptr<X> &x, variable_list te
   ctx->saved_data["x"] = c10::IValue::make_capsule(x);
 }
 
+// What a node keeps beside its tensors, which stay packed.
+template <typename X>
+c10::intrusive_ptr<X> kept_beside(AutogradContext *ctx) {
+  return c10::static_intrusive_pointer_cast<X>(ctx->saved_data.at("x").toCapsule());
+}
+
 template <typename X>
 c10::intrusive_ptr<X> kept(AutogradContext *ctx, variable_list &tensors) {
-  const auto x = c10::static_intrusive_pointer_cast<X>(ctx->saved_data.at("x").toCapsule());
+  const auto x = kept_beside<X>(ctx);
   tensors = ctx->get_saved_variables();
   TORCH_CHECK(tensors.size() == x->was.size(), "saved tensors are missing");
   for (size_t i = 0; i < tensors.size(); ++i) {

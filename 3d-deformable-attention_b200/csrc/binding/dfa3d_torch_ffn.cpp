@@ -45,6 +45,8 @@ struct Block : Kept {
   at::ScalarType type = at::kHalf;
   int32_t dtype = 0, act = 0, format = -1;            // format: how the input is kept; -1 whole
   bool plus_x = false, residual = false;
+  bool reads = false;                                 // whether a gradient may be wanted that reads what is kept
+  bool bias[3] = {false, false, false};               // of a single product: the first
 };
 
 // The input as it is kept for the backward, {x, -} or {codes, scales}.
@@ -125,19 +127,23 @@ struct LinearActFn : torch::autograd::Function<LinearActFn> {
     const Tensor bt = bias ? *bias : Tensor(), rt = res ? *res : Tensor();
     Tensor y = linear_act_forward(*b, x, w, bt, rt);
     variable_list v;
-    keep_input(*b, x, v);
-    keep(ctx, b, {v[0], v[1], w, bt});
+    if (b->reads) {
+      keep_input(*b, x, v);
+      v.insert(v.end(), {w, bt});
+    }
+    keep(ctx, b, std::move(v));
     return y;
   }
   static variable_list backward(AutogradContext *ctx, variable_list grads) {
-    variable_list v;
-    const auto b = kept<Block>(ctx, v);
-    const Tensor &w = v[2], &bias = v[3];
-    c10::cuda::CUDAGuard guard(w.device());
-    void *s = stream_of(w);
-    const bool gx = ctx->needs_input_grad(0), gw = ctx->needs_input_grad(1), gb = bias.defined() && ctx->needs_input_grad(2);
+    const auto b = kept_beside<Block>(ctx);
+    const bool gx = ctx->needs_input_grad(0), gw = ctx->needs_input_grad(1), gb = b->bias[0] && ctx->needs_input_grad(2);
     Tensor grad_x, grad_w, grad_b;
     if (gx || gw || gb) {
+      variable_list v;
+      kept<Block>(ctx, v);
+      const Tensor &w = v[2], &bias = v[3];
+      c10::cuda::CUDAGuard guard(w.device());
+      void *s = stream_of(w);
       const Tensor gt = gradient(grads[0], b->type);
       Operands o(b->type);
       const bool slope = b->act != DFA3D_ROW_NONE;
@@ -175,7 +181,7 @@ struct LinearActFn : torch::autograd::Function<LinearActFn> {
       }
       weight_gradients(*b, {{&g, b->out, &xr, b->in, gw, gb, &grad_w, &grad_b}}, w);
     }
-    return once({grad_x, grad_w, grad_b, b->residual && ctx->needs_input_grad(bias.defined() ? 3 : 2) ? grads[0] : Tensor(), Tensor()},
+    return once({grad_x, grad_w, grad_b, b->residual && ctx->needs_input_grad(b->bias[0] ? 3 : 2) ? grads[0] : Tensor(), Tensor()},
                 grads);
   }
 };
@@ -229,10 +235,12 @@ PyObject *run_linear_act(PyObject *const *a, Py_ssize_t n) {
   b->shape.back() = b->out;
   if (!optional_residual(a[3], res, x, b->shape)) return not_plain();
   b->residual = res.defined();
+  b->bias[0] = bias.defined();
+  b->reads = wants_grad(x, w) || (bias.defined() && wants_grad(bias));
   Tensor y;
   {
     pybind11::gil_scoped_release nogil;
-    if (wants_grad(x, w) || (bias.defined() && wants_grad(bias)) || (res.defined() && wants_grad(res))) {
+    if (b->reads || (res.defined() && wants_grad(res))) {
       y = LinearActFn::apply(x, w, given(bias), given(res), b);
     } else {
       c10::cuda::CUDAGuard guard(x.device());
@@ -282,26 +290,30 @@ struct GatedFn : torch::autograd::Function<GatedFn> {
     const Weights w{gate, up, down, bg ? *bg : Tensor(), bu ? *bu : Tensor(), bd ? *bd : Tensor()};
     Tensor y = gated_forward(*b, x, w, b->plus_x ? x : res ? *res : Tensor());
     variable_list v;
-    keep_input(*b, x, v);
-    keep(ctx, b, {v[0], v[1], w.gate, w.up, w.down, w.bias_gate, w.bias_up, w.bias_down});
+    if (b->reads) {
+      keep_input(*b, x, v);
+      v.insert(v.end(), {w.gate, w.up, w.down, w.bias_gate, w.bias_up});
+    }
+    keep(ctx, b, std::move(v));
     return y;
   }
   static variable_list backward(AutogradContext *ctx, variable_list grads) {
-    variable_list v;
-    const auto b = kept<Block>(ctx, v);
-    const Weights w{v[2], v[3], v[4], v[5], v[6], v[7]};
-    c10::cuda::CUDAGuard guard(w.gate.device());
-    void *s = stream_of(w.gate);
+    const auto b = kept_beside<Block>(ctx);
     bool need[8], any = false;
     size_t edge = 0;      // inputs that are absent have none
     for (int i = 0; i < 8; ++i) {
-      const bool there = i < 4 || (i == 4 ? w.bias_gate.defined() : i == 5 ? w.bias_up.defined() : i == 6 ? w.bias_down.defined() : b->residual);
+      const bool there = i < 4 || (i < 7 ? b->bias[i - 4] : b->residual);
       need[i] = there && ctx->needs_input_grad(edge);
       edge += there;
       if (i < 7) any |= need[i];
     }
     Tensor gx, gg, gu, gd, gbg, gbu, gbd;
     if (any) {
+      variable_list v;
+      kept<Block>(ctx, v);
+      const Weights w{v[2], v[3], v[4], v[5], v[6], Tensor()};
+      c10::cuda::CUDAGuard guard(w.gate.device());
+      void *s = stream_of(w.gate);
       const Tensor gt = gradient(grads[0], b->type);
       Operands o(b->type);
       const Rows xr = kept_input(*b, v, o), wg = o.add(w.gate, b->hidden, b->in), wu = o.add(w.up, b->hidden, b->in),
@@ -355,9 +367,13 @@ PyObject *run_gated(PyObject *const *a, Py_ssize_t n) {
   Tensor y;
   {
     pybind11::gil_scoped_release nogil;
-    bool grad = wants_grad(x, w.gate, w.up, w.down);
-    for (const Tensor *t : {&w.bias_gate, &w.bias_up, &w.bias_down, &res}) grad |= t->defined() && wants_grad(*t);
-    if (grad) {
+    b->reads = wants_grad(x, w.gate, w.up, w.down);
+    const Tensor *biases[3] = {&w.bias_gate, &w.bias_up, &w.bias_down};
+    for (int i = 0; i < 3; ++i) {
+      b->bias[i] = biases[i]->defined();
+      b->reads |= b->bias[i] && wants_grad(*biases[i]);
+    }
+    if (b->reads || (res.defined() && wants_grad(res))) {
       y = GatedFn::apply(x, w.gate, w.up, w.down, given(w.bias_gate), given(w.bias_up), given(w.bias_down), given(res), b);
     } else {
       c10::cuda::CUDAGuard guard(x.device());
