@@ -1,6 +1,7 @@
 // What the epilogues of the feed-forward products do with a row of sums in registers.
 #pragma once
 #include "dfa3d_act.cuh"
+#include "dfa3d_lost.h"
 #include "dfa3d_rowvec.cuh"
 #include "dfa3d_tcgen05.cuh"
 
@@ -10,6 +11,12 @@ namespace dfa3d {
 template <int ROW_BYTES> __device__ __forceinline__ uint32_t piece_of(uint32_t slab, int row, int piece) {
   const int mix = ROW_BYTES == 128 ? row & 7 : (row >> 1) & 3;
   return slab + row * ROW_BYTES + ((piece ^ mix) << 4);
+}
+
+// Row `row` of a slab that a wait was for which has run out.
+template <int ROW_BYTES> __device__ __forceinline__ void lose_row(uint32_t slab, int row) {
+  for (int piece = 0; piece < ROW_BYTES / 16; ++piece)
+    tc::write16(slab + row * ROW_BYTES + piece * 16, make_uint4(kLost, kLost, kLost, kLost));
 }
 
 template <int ACT, int N> __device__ __forceinline__ void activate_each(float (&z)[N]) {

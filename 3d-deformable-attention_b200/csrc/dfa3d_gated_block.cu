@@ -214,10 +214,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     const uint32_t lanes = memory + ((uint32_t)quarter << 21);
     const T *bias_gate = static_cast<const T *>(p.bias_gate), *bias_up = static_cast<const T *>(p.bias_up);
     const T *bias_down = static_cast<const T *>(p.bias_down);
-    const float lost = __int_as_float(0x7fffffff);
     const int y_column = group * L::part;
     uint32_t in_phase = 0;
-    bool ok = true;
+    bool ok = true, comes = true;      // sums and hidden rows; residuals
 
     auto row_of = [&](int tile) { return (tile * 2 + (int)rank) * kRows + quarter * 32; };
     auto inside = [&](int tile, int c) { return row_of(tile) < p.rows && y_column + c * L::chunk < p.n; };
@@ -248,9 +247,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
           }
           if (!p.has_in && lane == 0) tc::stores_read<0>();
           __syncwarp();
-          if (p.has_in) {
-            if (ok) ok = __all_sync(0xffffffffu, tc::wait(there, in_phase));
+          if (p.has_in && comes) {
+            comes = __all_sync(0xffffffffu, tc::wait(there, in_phase));
             in_phase ^= 1;
+            ok = ok && comes;
           }
 #pragma unroll
           for (int off = 0; off < L::chunk; off += 16) {
@@ -259,16 +259,16 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
             tc::tensor_loads_done(z);
             add_bias(z, bias + (64 + off) * 4);
             if (p.has_in) combine<O, 64, false>(z, slab, lane, off * (int)sizeof(O) / 16);
-            if (!ok) z[0] = lost;
             put<O, 64>(z, slab, lane, off * (int)sizeof(O) / 16);
           }
         }
         if (c + 1 == L::chunks) {
           tc::order_before();
           __syncwarp();
-          if (lane == 0) tc::arrive_in(first_y_empty);
+          if (ok && lane == 0) tc::arrive_in(first_y_empty);
         }
         if (!inside(tile, c)) continue;
+        if (!ok) lose_row<64>(slab, lane);
         tc::shared_to_async();
         __syncwarp();
         if (lane == 0) {
@@ -276,7 +276,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
           tc::stores_asked();
           if (p.has_in) {
             tc::stores_read<0>();
-            if (ok) ask();
+            if (comes) ask();
           }
         }
         __syncwarp();
@@ -318,7 +318,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       }
       tc::order_before();
       __syncwarp();
-      if (lane == 0) tc::arrive_in(first_drained);
+      if (ok && lane == 0) tc::arrive_in(first_drained);
 #pragma unroll
       for (int t = 0; t < 2; ++t) {
         add_bias(g[t], bias + t * 64);
@@ -331,15 +331,16 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
           g[t][i + 1] = h.y;
         }
         if (t == 0 && ok) ok = __all_sync(0xffffffffu, tc::wait(h_empty, (uint32_t)(item + 1) & 1));
-        put<T, 128>(g[t], base_h + (group >> 1) * kOperandA + quarter * 32 * 128, lane, (group & 1) * 4 + t * 2);
+        if (ok) put<T, 128>(g[t], base_h + (group >> 1) * kOperandA + quarter * 32 * 128, lane, (group & 1) * 4 + t * 2);
       }
       tc::shared_to_async();
       __syncwarp();
-      if (lane == 0) tc::hand_over_in(first_h_full);
+      if (ok && lane == 0) tc::hand_over_in(first_h_full);
       // the result of the rows before these is there when the first hidden columns of these have been made
       if (begin) result(before, before - first_tile);
     }
     if (items > 0) result(last_tile - 1, last_tile - 1 - first_tile);
+    if (!comes) tc::wait(there, in_phase ^ 1);      // a residual that is late may still be on its way
     if (lane == 0) tc::stores_done();
   }
   tc::order_before();

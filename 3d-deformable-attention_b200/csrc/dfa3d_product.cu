@@ -363,7 +363,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Tile<KIND, I, O, BN,
     const bool loads = p.has_in && !DIRECT;
     const T *bias0 = static_cast<const T *>(p.bias0), *bias1 = static_cast<const T *>(p.bias1);
     uint32_t in_phase = 0;
-    bool ok = true;
+    bool ok = true, comes = true;      // sums; what is added to them or multiplied by them
 
     // Chunk number c of this pair: tile first_tile + c / chunks; this warp has c = taker, taker + takers, ...
     const int all = (last_tile - first_tile) * L::chunks;
@@ -440,9 +440,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Tile<KIND, I, O, BN,
       if (ok) ok = __all_sync(0xffffffffu, tc::wait(summed + slot * 8, (uint32_t)(it / L::depth) & 1));
       tc::order_after();
       if (some) {
-        if (loads) {
-          if (ok) ok = __all_sync(0xffffffffu, tc::wait(there, in_phase));
+        if (loads && comes) {
+          comes = __all_sync(0xffffffffu, tc::wait(there, in_phase));
           in_phase ^= 1;
+          ok = ok && comes;
         }
         // columns of the accumulators, the next ones on their way while these are worked on
         constexpr int sums = KIND == kGatedGrad ? 3 : L::gated ? 2 : 1, turns = L::part / L::sub;
@@ -463,14 +464,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Tile<KIND, I, O, BN,
           } else {      // the accumulator may be summed into again
             tc::order_before();
             __syncwarp();
-            if (lane == 0) tc::arrive_in(first_drained + slot * 8);
+            if (ok && lane == 0) tc::arrive_in(first_drained + slot * 8);
           }
           if constexpr (KIND != kInputGrad) add_bias(z, bias + off * 4);
           if constexpr (L::gated) add_bias(v[t & 1][1], bias + (L::part + off) * 4);
           if constexpr (KIND == kGatedGrad) {
             float(&u)[L::sub] = v[t & 1][1], (&d)[L::sub] = v[t & 1][2];
             gate_all(z, u, d, p.act);
-            if (!ok) z[0] = u[0] = d[0] = __int_as_float(0x7fffffff);
             put<O, L::row_bytes>(d, slab + L::slab, lane, first);
             put<O, L::row_bytes>(u, slab + 2 * L::slab, lane, first);
           } else if constexpr (KIND == kGated) {
@@ -486,15 +486,16 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Tile<KIND, I, O, BN,
             if constexpr (KIND == kSlope) slope_all(z, p.act);
             if (p.has_in) combine<I, L::in_bytes, KIND == kSlope>(z, slab_in, lane, off * (int)sizeof(I) / 16);
           }
-          if (!ok) z[0] = __int_as_float(0x7fffffff);
           put<O, L::row_bytes>(z, slab, lane, first);
         }
       }
       if (!some) {
         __syncwarp();
-        if (lane == 0) tc::arrive_in(first_drained + slot * 8);
+        if (ok && lane == 0) tc::arrive_in(first_drained + slot * 8);
         continue;
       }
+      if (!ok)
+        for (int o = 0; o < L::outs; ++o) lose_row<L::row_bytes>(slab + o * L::slab, lane);
       if (!DIRECT) tc::shared_to_async();
       meet();
       if constexpr (DIRECT) {
@@ -505,10 +506,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Tile<KIND, I, O, BN,
         tc::stores_asked();
         if (loads) {
           if (!L::apart) tc::stores_read<0>();
-          if (ok) ask();
+          if (comes) ask();
         }
       }
     }
+    if (!comes) tc::wait(there, in_phase ^ 1);      // what is late may still be on its way
     if (lane == 0) tc::stores_done();
   }
   tc::order_before();
