@@ -188,7 +188,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads8, 1) weight
 
 // A CTA adds up the shares of four columns of a CTA's tile -- a thread four rows of one column of every other share --, turns them
 // around in shared memory and writes rows of the result.  So few, that even one tile has many CTAs and a thread few loads one after
-// the other: what there is to read is little (20 MB at most) but far away.
+// the other: what there is to read is little (20 MB where the shares fill one wave of pairs; of a result with more tiles
+// than pairs one share, 32 bits an element, 67 MB for 4096 x 4096) but far away.
 constexpr int kSumColumns = 4;
 template <typename T, int BN> __global__ void __launch_bounds__(256) weight_gradient_sum_kernel(const __grid_constant__ Problems w) {
   __shared__ float4 other[kSumColumns * kTileP / 4];
