@@ -77,8 +77,11 @@ __device__ __forceinline__ uint32_t address_in(uint32_t at, uint32_t rank) {    
 __device__ __forceinline__ void arrive_in(uint32_t bar) {
   asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
-// The same behind writes to the own CTA's shared memory that the products of both CTAs read there: shared_to_async() has seen to these,
-// and the other CTA's threads read none of them.
+// The same behind writes to the own CTA's shared memory that the products of both CTAs read there.  An arrival without a scope releases
+// to the own CTA only, while the thread that waits and issues the products may sit in the other one.  That rests on an assumption: no
+// thread of the other CTA reads what was written, the tensor cores of this SM do, through the async proxy, to which shared_to_async() has
+// made it visible before the arrival leaves this SM, and the products that read it are issued when the arrival has been seen.  A
+// release to the pair is what the memory model would ask for besides; it is the one that takes 1600 cycles.
 __device__ __forceinline__ void hand_over_in(uint32_t bar) {
   asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
