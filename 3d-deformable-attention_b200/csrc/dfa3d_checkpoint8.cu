@@ -3,7 +3,7 @@
 // types too (7 or 4 bits behind the factor), so that the products of a backward read exactly what the codes stand for.
 //
 // HBM binds: bytes of both sides are all there is.  Measured: bf16 184 950 x 256 to e4m3 (144 MB, 22 us at 6.55 TB/s) 28 us in, 21
-// out; fp32 40 000 x 512 to int8 (103 MB, 16 us) 17 in, 25 out, whose 82 MB of results end at the 3.9 TB/s of writes (21 us).  A
+// out; fp32 40 000 x 512 to int8 (103 MB, 16 us) 17 in, 25 out (82 MB of it written, which a fill does in 14).  A
 // thread has four items, whose loads are on their way together.
 #include <cuda_fp8.h>
 

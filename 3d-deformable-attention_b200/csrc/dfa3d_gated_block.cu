@@ -1,18 +1,21 @@
 // The gated feed-forward block with one kernel: y = (act(x Wg^T + bg) * (x Wu^T + bu)) Wd^T + bd + residual, whose hidden rows never leave
-// the SMs.  Written to memory and read again they are most of what the two kernels of dfa3d_product.cu move (82 of 102 bytes an element
-// of x at 256 -> 512 -> 256), and writes end at 3.9 TB/s.
+// the SMs.  Written to memory and read again they are most of what the two kernels of dfa3d_product.cu move (82 of 123 MB for 40 000 rows
+// 256 -> 512 -> 256 with a 16-bit residual that is x).
 //
 // A pair of CTAs takes 256 rows, which stay (64 KB each), and walks over 128 hidden columns at a time: gate and up are summed in half of
 // tensor memory, sixteen warps read them at once, so that the next ones may be summed, and turn them into hidden rows in shared memory,
 // which are the operand of the next product, summed in the other half over all hidden columns.  The products of one item and the sums of
 // the next are issued in turn, so that the tensor cores sum while the warps work; a result is read while the next rows begin.
 //
-// Measured behind a flush of L2, bf16, SiLU, a 16-bit residual, against the two kernels: 40 000 rows 256 -> 512 -> 256 45.1 us to 47.1,
-// 30 000 rows 34.8 to 41.0, 80 000 rows 67.6 to 75.8; 80 000 rows 256 -> 1024 -> 256 119 to 139; on calls that follow one another 38.7 to
-// 42.5, 27.9 to 34.7, 60.8 to 74.4, 106 to 138.  The floor of the first is 31.5 GFLOP, 20 us at 1.6 PFLOP/s.  What binds is the chain
-// of an item -- products, 32 columns of math a warp, hand-over -- of about 3900 cycles, and 5200 between the rows of two tiles, where
-// a warp's chunks of the result go through one slab one after the other: two slabs a warp leave three slots of the ring instead of
-// five, which cost wide blocks 10 %.
+// Measured against the two kernels, us, bf16, SiLU, behind a flush of L2 / on calls that follow one another:
+//   16-bit residual: 256 -> 512 -> 256, 30 000 rows 36.9 to 42.0 / 28.2 to 35.1, 40 000 rows 47.1 to 48.2 / 39.3 to 43.0, 80 000 rows 69.6
+//   to 78.8 / 61.9 to 74.1; 256 -> 1024 -> 256, 80 000 rows 115 to 136 / 107 to 133.
+//   32-bit residual: 45.1 to 48.1 / 33.2 to 43.9, 59.4 to 56.4 / 50.2 to 51.0, 90.1 to 93.2 / 81.6 to 89.2; 144 to 161 / 135 to 155.  The
+//   result's chunks, twice as many, take most of what the hidden rows save; at 40 000 rows all of it.
+// The floor of 40 000 rows is 31.5 GFLOP, 20 us at 1.6 PFLOP/s.  What binds is the chain of an item -- products, 32 columns of math a warp,
+// hand-over -- of about 3900 cycles, and 5200 between the rows of two tiles, where a warp's chunks of the result go through one slab
+// one after the other: two slabs a warp leave three slots of the ring instead of five, which cost wide blocks 10 %.  157 tiles of rows
+// over 74 pairs are three rounds for 2.1 rounds of work.
 #include "dfa3d_common.cuh"
 #include "dfa3d_epilogue.cuh"
 #include "dfa3d_product.h"
@@ -395,7 +398,8 @@ bool gated_block_covers(const ProductArgs &a, int hidden) {
   // What of the time of the busiest pair of SMs the average one has work for: the two kernels' tiles are narrower and divide more evenly.
   // At 38 row tiles for 74 pairs one kernel takes 0.75 to 0.87 of the two kernels' time up to 512 hidden columns, 0.86 to 0.9 with 1024
   // and 0.95 to 1.05 with 2048; at 75 tiles 0.93 to 1.0, but with 1024 and 2048, where a tile takes longer, 1.04 to 1.17, at 86 tiles
-  // then 0.9 to 1.1, at 118 0.8 to 0.95.
+  // then 0.9 to 1.1, at 118 0.8 to 0.95.  Measured with 16-bit residuals; with 32-bit ones 0.75 to 1.02, and behind a flush of L2
+  // 1.05 at 157 tiles of 512 hidden columns.
   const long long tiles = (a.rows + 2 * kRows - 1) / (2 * kRows), pairs = sm_count() / 2, rounds = (tiles + pairs - 1) / pairs;
   return tiles * 10 >= rounds * pairs * (rounds > 1 && hidden > 512 ? 6 : 5);
 }

@@ -9,12 +9,15 @@
 // activation, residual or derivatives in 32 bits, round once and hand rows to tiled stores.
 //
 // Measured on calls that follow one another, bf16, 40 000 rows between 256 and 512 columns (10.5 GFLOP a product, 7 us at 1.6 PFLOP/s;
-// 61 MB, the 41 MB of a result of 512 columns 10.5 us at the 3.9 TB/s at which writes end):
-//   256 -> 512: 15.9 us; with GELU 23.7; its derivative times a gradient 30.9.   512 -> 256: 14.9; with a residual of 16 bits 17.3,
-//   of 32 bits 27.7.   Input gradients: 14.9, of two products at once 30.2.   Gated hidden rows with SiLU 25, with GELU 29; their three
-//   backward results, 123 MB, 45.7 and 50.
-// Without an activation the writes bind; with one the epilogue's instructions (GELU 17.5 cycles a warp and 32 elements, SiLU 12.5),
-// of which a warp scheduler issues on 40 of 100 cycles between its waits for tensor memory and slabs.
+// 61 MB, 9.4 us at 6.5 TB/s):
+//   256 -> 512: 15.8 us; with SiLU 20.2, with GELU 25.4; GELU's derivative times a gradient 32.3.   512 -> 256: 14.8; with a residual
+//   of 16 bits 17.5, of 32 bits 28.   Input gradients: 14.8, of two products at once 30.2.   Gated hidden rows with SiLU 24.5, with GELU
+//   28.5; their three backward results, 123 MB, 45.7 and 48.3.
+// An activation's instructions (GELU 19.6 cycles of a scheduler for a warp's 32 elements, SiLU 13.4: 11 and 7.5 us of these calls) come
+// almost whole on top of the rest: where a tile has as many chunks as there are takers, all epilogue warps read the same sums, compute
+// and store at the same time, and issue on 37 to 42 of 100 cycles.  Without one neither HBM (results of this size stay in L2, 0 to 2 MB
+// are written out while a kernel runs) nor the tensor cores (15 to 30 % of the cycles) are near their rates; what is left is the way from L2 into
+// shared memory, uneven last rounds of tiles and about 4 us of setting up and ending.
 //
 // Gradients are rounded to 16 bits behind an activation's derivative, once: they are operands of the next products, and the bias
 // gradient is the sum of what those read.

@@ -81,7 +81,8 @@ __device__ __forceinline__ void arrive_in(uint32_t bar) {
 // to the own CTA only, while the thread that waits and issues the products may sit in the other one.  That rests on an assumption: no
 // thread of the other CTA reads what was written, the tensor cores of this SM do, through the async proxy, to which shared_to_async() has
 // made it visible before the arrival leaves this SM, and the products that read it are issued when the arrival has been seen.  A
-// release to the pair is what the memory model would ask for besides; it is the one that takes 1600 cycles.
+// release to the pair is what the memory model would ask for besides; with it the gated block's forward takes 42 us for 35.7 (40 000 rows,
+// 256 -> 512 -> 256, no activation).
 __device__ __forceinline__ void hand_over_in(uint32_t bar) {
   asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }

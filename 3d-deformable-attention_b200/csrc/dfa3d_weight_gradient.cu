@@ -4,9 +4,9 @@
 // once.  The bias gradient is one more operand of the product, columns of ones.  A step of 64 rows is summed in 512 cycles and brings
 // 32 KB into each SM: the way from L2 (about 45 bytes a cycle and SM while all read) binds, and without pairs it would be 48 KB.
 //
-// Measured with the sum kernel on calls that follow one another, bf16: 40 000 x 512 by 256 23.9 us (61 MB, 9.6 us at 6.4 TB/s; the
-// partial sums, 19 MB written and read again, are most of the rest), the three gradients of a gated block 256 -> 512 -> 256 41, of 80 000
-// rows 256 -> 1024 -> 256 120.  One launch for all gradients of a block: a product of its own has too few tiles for 74 pairs, and
+// Measured with the sum kernel on calls that follow one another, bf16: 40 000 x 512 by 256 22.4 us (61 MB, 9.4 us at 6.5 TB/s; the
+// partial sums, 19 MB written and read again, are most of the rest), the three gradients of a gated block 256 -> 512 -> 256 40, of 80 000
+// rows 256 -> 1024 -> 256 112.  One launch for all gradients of a block: a product of its own has too few tiles for 74 pairs, and
 // more shares instead would leave more partial sums behind.
 #include "dfa3d_common.cuh"
 #include "dfa3d_product.h"

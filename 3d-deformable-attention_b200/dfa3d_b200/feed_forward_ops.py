@@ -328,7 +328,8 @@ def _to(t, dtype):
 
 
 class LinearAct(nn.Linear, _Computed):
-    """``torch.nn.Linear`` (same parameters and state-dict keys), an activation and a residual on ``linear_act``."""
+    """``torch.nn.Linear`` (same parameters and state-dict keys), an activation and a residual on ``linear_act``.  Unlike it, a float32 x
+    without a residual gives a result of compute_dtype: a float32 result takes a float32 residual."""
 
     def __init__(self, in_features, out_features, bias=True, activation=None, checkpoint=None, compute_dtype=torch.bfloat16):
         super().__init__(in_features, out_features, bias)

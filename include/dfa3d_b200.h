@@ -473,7 +473,8 @@ int dfa3d_group_norm_backward(const void *grad_y, const void *x, int32_t dtype, 
  * DFA3D_DTYPE_BF16 or _F16; activation: DFA3D_ROW_*.  Matrices are row-major; an argument with a pitch (elements from row to
  * row) is an operand of a product or a workspace that becomes one: it begins on a 16-byte boundary and its pitch is a multiple
  * of 8 (dfa3d_copy_rows makes such a copy; what lies between the columns and the pitch is not looked at).  Matrices without
- * a pitch are contiguous and may lie anywhere.  0 <= rows < 2^31 - 128, widths from 1 to 2^24.  Results overlap no input. */
+ * a pitch are contiguous and may lie anywhere.  0 <= rows < 2^31 - 128, widths from 1 to 2^24.  Results overlap no input.
+ * Waits inside these kernels end after 4 s, which no sound run reaches: what was to come is then NaN, and no error is reported. */
 
 /* y (rows, out) = act(x W^T + bias) + residual, x (rows, in), weight (out, in).  bias (out) and residual (rows, out) may be null.
  * out_dtype (of residual and y): dtype or DFA3D_DTYPE_F32. */
