@@ -65,9 +65,9 @@ __device__ __forceinline__ Two counted(Two z) { return {no_less(z.x, -1e30f), no
 
 // The normal distribution's P(X <= z) and exp(-z^2 / 2).  P(X <= -|z|) = exp(-z^2 / 2) R(|z|) with R(|z|) = erfcx(|z| / sqrt 2) / 2, which
 // falls as 1 / |z| and is a polynomial of t = 1 / (1 + 0.365 |z| / sqrt 2) without a constant term: seven terms, fitted to the
-// definition on 0 <= |z| <= 13.5 for the least largest error (a linear program over 1200 points), each error counted against the
-// larger of what 3e-8 of the probability and 2^-18.7 of R are.  So the tail is right relative to itself: with the roundings 4e-6 up
-// to |z| = 6 and 1e-5 up to 13, where 32 bits end; an error bound of the probability alone leaves 1 % at 8.
+// definition on 0 <= |z| <= 13.5 by a linear program over 1200 points so that the probability is off by at most 3e-8 and by at most
+// 2^-18.7 of itself.  So the tail is right too: with the roundings to 4e-6 of itself up to |z| = 6 and to 1e-5 up to 13, where 32 bits
+// end; a bound of the first kind alone leaves 1 % at 8.
 __device__ __forceinline__ Two normal_cdf(Two z, Two &bell) {
   bell = power_of_two(z * z * both(-0.72134752044448170f));
   const Two far{fminf(fabsf(z.x), 1e8f), fminf(fabsf(z.y), 1e8f)};
